@@ -317,6 +317,114 @@ int omx_gdn_qkv_conv_proj(const void* x, const void* w, const float* conv_w, voi
 int omx_gdn_ab_proj(const void* x, const void* w_a, const void* w_b, void* a, void* b,
                     int64_t M, int64_t D, int64_t Hv, void* stream);
 
+/*
+ * Causal softmax attention over packed prompts: the token mixer of the decoder's full-attention
+ * layers (omegalax/models/qwen3_5/attention.py:115-119, between its projections, norms, rotary
+ * embedding and output gate), with the packed sequences of omx_gdn_prefill.
+ *   o[i] = sum_j softmax_j(scale q[i] . k[j]) v[j] over the keys j <= i of i's sequence.
+ *
+ *   q            [B, T, Hq, D] bf16, token stride q_ld elements (heads side by side, the rows of
+ *                a batch T q_ld apart), so that q, k and v may be columns of one projection
+ *   k, v         [B, T, Hkv, D] bf16, token strides k_ld, v_ld; query head h reads key head
+ *                h / (Hq / Hkv), Hq / Hkv <= 32
+ *   cu_seqlens   as for omx_gdn_chunk_fwd (N sequences, B = 1), or NULL (N = B)
+ *   o            [B, T, Hq, D] bf16
+ *   lse          [B, T, Hq] f32 or NULL: log sum_j exp(scale q . k), for omx_gdn_attn_bwd
+ *   scale        positive
+ * D is a multiple of 8, at most 256 (compiled for 64, 128 and 256; others run zero-filled at the
+ * next).  Strides are multiples of 8 and at most 2^22, q, k, v and o 16-byte aligned.  Scores,
+ * softmax and sums are fp32; the weights are rounded to bf16 for their product with v.  A row's
+ * values are those of its own sequence alone, whatever lies beside it.
+ */
+int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld,
+                     int64_t v_ld, const int32_t* cu_seqlens, int64_t N, void* o, float* lse,
+                     int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, float scale,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace omx_gdn_attn_fwd needs (16-byte aligned): the tile list of more than
+ * 64 packed sequences; none for fewer, or without cu_seqlens (N = 0). */
+size_t omx_gdn_attn_fwd_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64_t N);
+
+/*
+ * Backward pass (VJP) of omx_gdn_attn_fwd, for the cotangent d_o of o.  Inputs as there; o and
+ * lse are what it wrote.
+ *   d_o          [B, T, Hq, D] bf16
+ *   dq           [B, T, Hq, D], dk, dv [B, T, Hkv, D] bf16, dense; dk and dv are summed over each
+ *                key head's query heads.  No sum depends on the order of execution.
+ */
+int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld,
+                     int64_t v_ld, const int32_t* cu_seqlens, int64_t N, const void* o,
+                     const float* lse, const void* d_o, void* dq, void* dk, void* dv, int64_t B,
+                     int64_t T, int64_t Hq, int64_t Hkv, int64_t D, float scale, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace omx_gdn_attn_bwd needs (16-byte aligned; N = 0 without cu_seqlens). */
+size_t omx_gdn_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                       int64_t N);
+
+/*
+ * The paged key-value cache, which the next three entry points share.
+ *   k_pages, v_pages  [n_pages, page_size, Hkv, D] bf16, 16-byte aligned; D 64, 128 or 256,
+ *                page_size a multiple of 16 up to 65536.  Slots that no token was written to may
+ *                hold anything.
+ *   block_table  int32 [N, table_width]: page of tokens i page_size .. of each sequence.  Entries
+ *                outside [0, n_pages) are no page: nothing is written there, and their tokens
+ *                are left out of every softmax.
+ *   lengths      int32 [N]: tokens each sequence held before this call.  They are not advanced.
+ *                A negative length marks a sequence that takes no part: nothing is written for
+ *                it, and its outputs are zeros.
+ * Tokens past table_width * page_size have no place: they are not written, and not attended.  A
+ * page that is written to belongs to one sequence; others may be shared.
+ *
+ * omx_gdn_kv_write appends the keys and values of new tokens: token i of sequence n goes to
+ * position lengths[n] + i.  k, v, their strides and cu_seqlens as for omx_gdn_attn_fwd.
+ */
+int omx_gdn_kv_write(const void* k, const void* v, int64_t k_ld, int64_t v_ld,
+                     const int32_t* cu_seqlens, int64_t N, void* k_pages, void* v_pages,
+                     int64_t n_pages, int64_t page_size, const int32_t* block_table,
+                     int64_t table_width, const int32_t* lengths, int64_t B, int64_t T,
+                     int64_t Hkv, int64_t D, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* Bytes of device workspace omx_gdn_kv_write needs (N = 0 without cu_seqlens). */
+size_t omx_gdn_kv_write_workspace_size(int64_t T, int64_t N);
+
+/*
+ * Attention of new tokens over the cache that omx_gdn_kv_write has put them into: query i of
+ * sequence n attends positions 0 .. lengths[n] + i.  A prompt in pieces, a turn continued from
+ * its cache.  q, cu_seqlens, o, scale as for omx_gdn_attn_fwd.  A query that no key is left for
+ * gives zeros.
+ */
+int omx_gdn_attn_paged(const void* q, int64_t q_ld, const int32_t* cu_seqlens, int64_t N,
+                       const void* k_pages, const void* v_pages, int64_t n_pages,
+                       int64_t page_size, const int32_t* block_table, int64_t table_width,
+                       const int32_t* lengths, void* o, int64_t B, int64_t T, int64_t Hq,
+                       int64_t Hkv, int64_t D, float scale, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace omx_gdn_attn_paged needs (16-byte aligned): the tile list, and the
+ * partial sums of a cache that is read in shares.  packed: whether cu_seqlens is given. */
+size_t omx_gdn_attn_paged_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                         int64_t N, int packed, int64_t page_size,
+                                         int64_t table_width);
+
+/*
+ * The decode step: one new token per sequence.  Writes its key and value to position lengths[b]
+ * and attends positions 0 .. lengths[b].
+ *   q [B, Hq, D], k, v [B, Hkv, D] bf16, row strides q_ld, k_ld, v_ld;  out [B, Hq, D] bf16
+ */
+int omx_gdn_attn_decode_step(const void* q, const void* k, const void* v, int64_t q_ld,
+                             int64_t k_ld, int64_t v_ld, void* k_pages, void* v_pages,
+                             int64_t n_pages, int64_t page_size, const int32_t* block_table,
+                             int64_t table_width, const int32_t* lengths, void* out, int64_t B,
+                             int64_t Hq, int64_t Hkv, int64_t D, float scale, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace omx_gdn_attn_decode_step needs (16-byte aligned): the partial sums of
+ * a cache that is read in shares. */
+size_t omx_gdn_attn_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                          int64_t page_size, int64_t table_width);
+
 #ifdef __cplusplus
 }
 #endif

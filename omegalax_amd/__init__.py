@@ -4,6 +4,10 @@ The compute lives in libomx_gdn.so (HIP kernels behind the C ABI of
 include/omx_gdn.h); this package is the Python host side that mirrors the
 reference's interface (omegalax/models/qwen3_5/deltanet.py).
 """
+from .attention import (  # noqa: F401
+    attention_decode_step, attention_prefill, attention_prefill_bwd, attention_prefill_paged,
+    kv_pages_write,
+)
 from .deltanet import (  # noqa: F401
     GDNError, chunk_gated_delta_rule, chunk_gated_delta_rule_bwd, gdn_ab_projections,
     gdn_decode_step, gdn_prefill, gdn_prefill_bwd, qkv_conv_projection,

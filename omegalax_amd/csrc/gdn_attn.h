@@ -1,0 +1,201 @@
+// Softmax attention: what its kernels share.
+//
+// Rows.  A key head's g = Hq / Hkv query heads see the same keys, so their queries are one
+// matrix: row r of a tile that starts at token t0 is token t0 + r / g, head r % g.  A tile of R
+// rows takes the whole tokens that fit, R / g, and leaves the rest of its rows idle.  A tile
+// then reads its keys once for all g heads, and the gradients of a key head sum over its query
+// heads inside one product.
+//
+// Fragments.  All products are v_mfma_f32_32x32x16_bf16 with, for l the lane, h = l / 32 and
+// c = l % 32 (verified on MI355X by products of small integers):
+//   A[c][8h .. 8h+7],  B[8h .. 8h+7][c],  C[8 (i / 4) + 4h + i % 4][c], i = 0..15
+// A product that leaves its result C[key][row] feeds the next one, whose contraction runs over
+// the keys, without exchanging lanes: elements 8s .. 8s+7 of a lane's C are the keys 16s + 4h +
+// {0..3, 8..11}, and taking them as the B operand of step s only asks that the A operand lists
+// its keys in the same order, which two transposed LDS reads of 4 keys each do.
+#pragma once
+
+#include "gdn_common.h"
+#include "gdn_kernels.h"
+#include "gdn_mfma.h"
+
+namespace omx {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) bf16_t lds_bf16;
+typedef __attribute__((address_space(1))) void glob_void;
+
+// C += A(32x16) B(16x32)
+__device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                 __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// elements 8s .. 8s+7 of a C fragment as a B operand (see the top of this file)
+__device__ __forceinline__ u32x4 pack8_of(const f32x16& c, int s) {
+  return u32x4{pack_bf16(c[8 * s], c[8 * s + 1]), pack_bf16(c[8 * s + 2], c[8 * s + 3]),
+               pack_bf16(c[8 * s + 4], c[8 * s + 5]), pack_bf16(c[8 * s + 6], c[8 * s + 7])};
+}
+
+// value of the lane 32 away combined with the lane's own
+__device__ __forceinline__ float max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Rows of DP bf16 in LDS without padding, in 16-byte segments: segment s of row r lies at
+// s ^ swz(r).  One pass of a 16-byte read serves lanes {0-3, 12-15, 20-27} (and the rest of
+// each half), whose rows' images must differ in the 16 segments that the 64 banks hold; one
+// pass of a transposed 8-byte read serves four neighbouring rows' four neighbouring segments,
+// which must lie in different quarters.  The row's low bits go to the segment's high ones and
+// the other way round, which gives both.  Rows of 64 elements fill the banks two by two.
+template <int DP>
+__device__ __forceinline__ int attn_swz(int r) {
+  return DP == 64 ? ((((r >> 1) & 1) << 2) | ((r >> 2) & 3)) : (((r & 3) << 2) | ((r >> 2) & 3));
+}
+
+// A operand (32 rows row0 .. +31, elements 16 step .. +15) of a [row][DP] LDS tile
+template <int DP>
+__device__ __forceinline__ u32x4 attn_frag(const bf16_t* base, int row0, int step) {
+  const int l = lane_id(), h = l >> 5, c = l & 31;
+  return *(const u32x4*)(base + (row0 + c) * DP + (((2 * step + h) ^ attn_swz<DP>(c)) << 3));
+}
+
+// A operand whose rows are the tile's columns 32 cb .. +31 and whose contraction runs over its
+// rows row0 + {4h .. +3, 8 + 4h .. +3}: the order of pack8_of
+template <int DP>
+__device__ __forceinline__ u32x4 attn_frag_tr(const bf16_t* base, int row0, int cb) {
+  const int l = lane_id(), h = l >> 5, s = l & 15;
+  const int col = 32 * cb + 16 * ((l >> 4) & 1) + 4 * (s & 3);
+  const int r0 = row0 + 4 * h + (s >> 2), r1 = r0 + 8;
+  const u32x2 a = ds_read_tr(base + r0 * DP + (((col >> 3) ^ attn_swz<DP>(r0)) << 3) + (col & 7));
+  const u32x2 b = ds_read_tr(base + r1 * DP + (((col >> 3) ^ attn_swz<DP>(r1)) << 3) + (col & 7));
+  return u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// One staging instruction writes 1 KiB of LDS, 64 / (DP / 8) rows.  Of a tile's instructions a
+// wavefront takes w, w + NW, ...: row of lane l in its j-th, and the segment it fetches.
+template <int DP, int NW>
+__device__ __forceinline__ int stage_row(int w, int j) {
+  constexpr int CH = DP / 8;
+  return (64 / CH) * (w + NW * j) + lane_id() / CH;
+}
+template <int DP>
+__device__ __forceinline__ int stage_seg(int row) {
+  return (lane_id() % (DP / 8)) ^ attn_swz<DP>(row);
+}
+
+// Which tile a workgroup takes: sequence `seq` of tokens start .. start + len, tile `tile` of
+// `tiles`.
+struct AttnTile {
+  int seq, len, tile, tiles;
+  long long start;
+};
+
+// Tile of rank `rank` of sequences packed by cu, those with most keys first (a tile's work
+// grows with its index), found by every wavefront for itself when there are at most 64
+// sequences: lane n holds sequence n.  The offsets are read as their ordered repair.
+__device__ __forceinline__ bool packed_tile(const int32_t* cu, int N, int T, int per, int rank,
+                                            AttnTile& it) {
+  const int n = lane_id();
+  int end = n + 1 < N ? cu[n + 1] : T;
+  end = end < 0 ? 0 : (end > T ? T : end);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(end, o, 64);
+    if (n >= o && x > end) end = x;
+  }
+  const int prev = __shfl_up(end, 1, 64);
+  const int start = n == 0 ? 0 : prev;
+  const int len = n < N ? end - start : 0, nt = (len + per - 1) / per;
+  // at(j): tiles of index j and more
+  auto at = [&](int j) {
+    int v = nt > j ? nt - j : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+  };
+  if (rank >= at(0)) return false;
+  int lo = 0, hi = (T + per - 1) / per;  // at(lo) > rank >= at(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (at(mid) > rank) lo = mid; else hi = mid;
+  }
+  const int k = rank - at(lo + 1);  // the k-th of the sequences that have a tile lo
+  const unsigned long long have = __ballot(nt > lo);
+  const unsigned long long below = have & ((1ull << n) - 1);
+  const unsigned long long mine = __ballot(nt > lo && __popcll(below) == k);
+  const int s = __ffsll(mine) - 1;
+  it.seq = __builtin_amdgcn_readfirstlane(s);
+  it.start = __builtin_amdgcn_readlane(start, it.seq);
+  it.len = __builtin_amdgcn_readlane(len, it.seq);
+  it.tile = __builtin_amdgcn_readfirstlane(lo);
+  it.tiles = __builtin_amdgcn_readlane(nt, it.seq);
+  return true;
+}
+
+// Tile of rank `rank` of sequence or packed row `row`; false past the last one.
+__device__ __forceinline__ bool attn_tile(const AttnParams& p, int row, int rank, int per,
+                                          AttnTile& it) {
+  if (!p.cu) {
+    it.seq = row;
+    it.len = p.T;
+    it.start = (long long)row * p.T;
+    it.tiles = (p.T + per - 1) / per;
+    it.tile = it.tiles - 1 - rank;
+    return it.tile >= 0;
+  }
+  if (!p.plan) return packed_tile(p.cu, p.N, p.T, per, rank, it);
+  // more than 64 sequences: the plan kernel's list (count, then sequence and tile per rank)
+  const int32_t* plan = p.plan;
+  if (rank >= plan[0]) return false;
+  it.seq = plan[2 + 2 * (long long)rank];
+  it.tile = plan[3 + 2 * (long long)rank];
+  it.start = p.cu_plan[it.seq];
+  it.len = p.cu_plan[it.seq + 1] - p.cu_plan[it.seq];
+  it.tiles = (it.len + per - 1) / per;
+  return true;
+}
+
+// Order of the workgroups: (unit, rank) of workgroup `bid`, with units (a sequence's or packed
+// row's key head) kept on few of the 8 XCDs, whose L2s then hold that head's keys and values.
+// Consecutive workgroups go to consecutive XCDs.  The grid is attn_grid() workgroups; ranks
+// past a unit's last tile have nothing to do.
+__device__ __forceinline__ void attn_place(int bid, int units, int ranks, int& unit, int& rank) {
+  if (units % 8 == 0) {
+    const int x = bid & 7, j = bid >> 3;
+    unit = x + 8 * (j / ranks);
+    rank = j % ranks;
+  } else if (8 % units == 0) {
+    const int x = bid & 7, j = bid >> 3, r = 8 / units;
+    unit = x / r;
+    rank = j * r + x % r;
+  } else {
+    unit = bid % units;
+    rank = bid / units;
+  }
+}
+inline long long attn_grid(long long units, long long ranks) {
+  if (units % 8 != 0 && 8 % units == 0) {
+    const long long r = 8 / units;
+    return 8 * ((ranks + r - 1) / r);
+  }
+  return units * ranks;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+}  // namespace omx

@@ -1,0 +1,432 @@
+// Causal softmax attention of whole prompts and of new tokens over a paged cache.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij - lse_i),  s_ij = scale q_i . k_j,  j <= i
+//
+// One workgroup takes a tile of 128 rows (token, query head of one key head) and passes over the
+// keys once, 64 at a time, with the running maximum and sum of each row's softmax.  The keys' and
+// values' tiles go from memory to LDS without passing through registers, one tile ahead.  A
+// wavefront owns 32 rows and forms S^T = K Q^T, whose fragment holds one row per lane: maximum
+// and sum are sums within a lane and one exchange of halves, and P^T is the B operand of
+// O^T += V^T P^T as it stands.
+#include "gdn_attn.h"
+
+namespace omx {
+namespace {
+
+constexpr int kBM = 128, kBN = 64, kNW = 4, kNT = 64 * kNW;
+
+// m starts here: below any score, and finite, so that rows which have seen no key stay at 0
+constexpr float kLow = -1e30f;
+
+template <int DP, bool PAGED>
+__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
+void attn_fwd_kernel(AttnParams p, int ranks) {
+  constexpr int KS = DP / 16, DB = DP / 32;      // steps of a score, blocks of an output row
+  constexpr int NJ = kBN * DP / 8 / 64 / kNW;    // staging instructions per wavefront and tile
+  __shared__ __align__(16) bf16_t sK0[kBN * DP], sK1[kBN * DP], sV0[kBN * DP], sV1[kBN * DP];
+
+  const int tid = threadIdx.x, l = tid & 63, h = l >> 5, c = l & 31;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = p.G, D = p.D, Hkv = p.Hkv, per = kBM / G;
+
+  int unit, rank;
+  const int units = (p.cu ? 1 : p.N) * Hkv;
+  attn_place((int)blockIdx.x, units, ranks, unit, rank);
+  if (rank >= ranks) return;
+  const int split = (int)blockIdx.y;
+  const int hk = unit % Hkv;
+  AttnTile it;
+  if (!attn_tile(p, unit / Hkv, rank, per, it)) return;
+  const int t0 = it.tile * per;                                   // first token of the tile
+  const int nt = it.len - t0 < per ? it.len - t0 : per;           // its tokens
+  int held = 0;
+  bool idle = false;
+  if constexpr (PAGED) {
+    held = __builtin_amdgcn_readfirstlane(p.held[it.seq]);
+    idle = held < 0;  // a sequence that takes no part: zeros
+    held = held < 0 ? 0 : (held > p.table_w * p.page ? p.table_w * p.page : held);
+  }
+
+  // this lane's row
+  const int row = 32 * w + c, rt = row / G, rg = row - rt * G;
+  const bool live = rt < nt;
+  const long long tok = it.start + t0 + rt;
+  const int pos = held + t0 + rt;                                 // its last key
+  const int w_lo = held + t0 + (32 * w) / G;                      // the wavefront's first row's
+  const int w_hi = held + t0 + (32 * w + 31) / G;                 //   and last row's last key
+
+  u32x4 q[KS];
+  {
+    const bf16_t* qp = (const bf16_t*)p.q + tok * p.q_ld + (long long)(hk * G + rg) * D;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = 16 * s + 8 * h;
+      q[s] = u32x4{0, 0, 0, 0};
+      if (live && d < D) q[s] = *(const u32x4*)(qp + d);
+    }
+  }
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o[d] = zero16();
+  float m = kLow, lsum = 0.f;
+  const float cs = p.scale * kLog2e;
+
+  // the tile's keys: 0 .. last, in tiles of kBN, of which this split takes [kt0, kt1)
+  const int keys = held + t0 + nt;
+  int kt0 = 0, kt1 = (keys + kBN - 1) / kBN;
+  if (PAGED && p.splits > 1) {
+    const int each = (kt1 + p.splits - 1) / p.splits;
+    kt0 = split * each < kt1 ? split * each : kt1;
+    kt1 = kt0 + each < kt1 ? kt0 + each : kt1;
+  }
+  if (idle) kt1 = kt0;
+
+  // ---------------------------------------------------------------- staging
+  int srow[NJ], sseg[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    srow[j] = stage_row<DP, kNW>(w, j);
+    sseg[j] = stage_seg<DP>(srow[j]);
+  }
+  const unsigned kld2 = PAGED ? (unsigned)(Hkv * D * 2) : (unsigned)(p.k_ld * 2);
+  const unsigned vld2 = PAGED ? (unsigned)(Hkv * D * 2) : (unsigned)(p.v_ld * 2);
+  // the cache: page slot and offset of the next tile to stage, and the pages of its four groups
+  // of 16 keys (a page is a multiple of 16 tokens), read one tile before they are used
+  int slot = 0, off = 0, pid[4], poff[4];
+  // (read through the scalar cache: its wait does not touch the staging loads' counter)
+  typedef const __attribute__((address_space(4))) int32_t const_i32;
+  const_i32* table = PAGED ? (const_i32*)(p.table + (long long)it.seq * p.table_w) : nullptr;
+  auto look = [&](int kt) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const bool in = kt * kBN + 16 * g < keys && slot < p.table_w;
+      int id = in ? table[slot] : -1;
+      id = id >= p.n_pages ? -1 : id;
+      pid[g] = __builtin_amdgcn_readfirstlane(id);
+      poff[g] = off;
+      off += 16;
+      if (off >= p.page) { off = 0; ++slot; }
+    }
+  };
+  // groups of a staged tile that hold keys
+  auto stage = [&](int kt, bf16_t* sk, bf16_t* sv) -> unsigned {
+    unsigned have = 15;
+    if constexpr (PAGED) {
+      have = 0;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) have |= pid[g] >= 0 ? 1u << g : 0u;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int g0 = (64 / (DP / 8)) * kNW * j / 16;  // the group of row stage_row(0, j)
+        int id = pid[g0], of = poff[g0];
+        if (DP == 64 && w >= 2) { id = pid[g0 + 1]; of = poff[g0 + 1]; }
+        if (id >= 0) {
+          const long long at = ((long long)id * p.page + of) * Hkv * D + hk * D;
+          const unsigned lo = (unsigned)(srow[j] & 15) * kld2 + 16u * (unsigned)sseg[j];
+          const int i = w + kNW * j;
+          __builtin_amdgcn_global_load_lds((glob_void*)((const char*)((const bf16_t*)p.k_pages + at) + lo),
+                                           (lds_void*)(sk + 512 * i), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds((glob_void*)((const char*)((const bf16_t*)p.v_pages + at) + lo),
+                                           (lds_void*)(sv + 512 * i), 16, 0, 0);
+        }
+      }
+    } else {
+      const int left = it.len - kt * kBN, n = left < kBN ? left : kBN;  // rows past the sequence
+      const long long at = it.start + (long long)kt * kBN;              //   read as zeros
+      const auto kr = buf_rsrc((const bf16_t*)p.k + at * p.k_ld + hk * D, (unsigned)(n - 1) * kld2 + 2u * D);
+      const auto vr = buf_rsrc((const bf16_t*)p.v + at * p.v_ld + hk * D, (unsigned)(n - 1) * vld2 + 2u * D);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int i = w + kNW * j;
+        const bool in = 8 * sseg[j] < D;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            kr, (lds_void*)(sk + 512 * i), 16,
+            in ? (unsigned)srow[j] * kld2 + 16u * (unsigned)sseg[j] : kDropOffset, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            vr, (lds_void*)(sv + 512 * i), 16,
+            in ? (unsigned)srow[j] * vld2 + 16u * (unsigned)sseg[j] : kDropOffset, 0, 0, 0);
+      }
+    }
+    return have;
+  };
+
+  // ---------------------------------------------------------------- one tile of keys
+  auto compute = [&](int kt, const bf16_t* sk, const bf16_t* sv, unsigned have) {
+    const int key0 = kt * kBN;
+    if (key0 > w_hi) return;  // uniform in the wavefront: no row of it sees these keys
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = zero16();
+#pragma unroll
+      for (int k = 0; k < KS; ++k) s[b] = mma32(attn_frag<DP>(sk, 32 * b, k), q[k], s[b]);
+    }
+    if (key0 + kBN - 1 > w_lo || have != 15) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = key0 + 32 * b + 8 * (i / 4) + 4 * h + i % 4;
+          if (key > pos || (PAGED && !((have >> (2 * b + i / 8)) & 1))) s[b][i] = -INFINITY;
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+    mx = max_halves(mx);
+    // the maximum is only raised, and what is summed so far scaled down, when some row's grew
+    // by more than 2^8: the weights stay below that, far inside bf16 and fp32
+    if (__any((mx - m) * cs > 8.f)) {
+      const float mn = fmaxf(m, mx);
+      const float a = __builtin_amdgcn_exp2f((m - mn) * cs);
+      m = mn;
+      lsum *= a;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= a;
+    }
+    const float mc = m * cs;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], cs, -mc));
+        sum[i & 3] += s[b][i];
+      }
+    lsum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const u32x4 pb = pack8_of(s[b], k);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+          o[d] = mma32(attn_frag_tr<DP>(sv, 32 * b + 16 * k, d), pb, o[d]);
+      }
+  };
+
+  // rows of a staged tile that hold no key are cleared: a weight of zero does not clear them
+  // of a NaN
+  auto clear = [&](int kt, bf16_t* sv, unsigned have) {
+    for (int i = tid; i < kBN * DP / 8; i += kNT) {
+      const int r = i / (DP / 8);
+      if (kt * kBN + r >= keys || !((have >> (r / 16)) & 1)) *(u32x4*)(sv + 8 * i) = u32x4{0, 0, 0, 0};
+    }
+  };
+  auto arrived = [&](int kt, bf16_t* sv, unsigned have) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of the tile
+    lds_barrier();                       // everyone's; and the other buffers are free
+    if constexpr (PAGED) {
+      if (have != 15 || (kt + 1) * kBN > keys) {  // uniform in the workgroup
+        clear(kt, sv, have);
+        lds_barrier();
+      }
+    }
+  };
+
+  if (kt0 < kt1) {
+    if constexpr (PAGED) {
+      slot = kt0 * kBN / p.page;
+      off = kt0 * kBN - slot * p.page;
+      look(kt0);
+    }
+    unsigned have0 = stage(kt0, sK0, sV0), have1 = 15;
+    if constexpr (PAGED) look(kt0 + 1);
+    for (int kt = kt0; kt < kt1; kt += 2) {
+      arrived(kt, sV0, have0);
+      if (kt + 1 < kt1) have1 = stage(kt + 1, sK1, sV1);
+      if constexpr (PAGED) look(kt + 2);
+      compute(kt, sK0, sV0, have0);
+      if (kt + 1 >= kt1) break;
+      arrived(kt + 1, sV1, have1);
+      if (kt + 2 < kt1) have0 = stage(kt + 2, sK0, sV0);
+      if constexpr (PAGED) look(kt + 3);
+      compute(kt + 1, sK1, sV1, have1);
+    }
+  }
+
+  // ---------------------------------------------------------------- output
+  lsum = sum_halves(lsum);
+  if (!live) return;
+  const int Hq = Hkv * G, head = hk * G + rg;
+  if (PAGED && p.splits > 1) {
+    const long long at = ((long long)split * p.tokens + tok) * Hq + head;
+    float* po = p.part_o + at * DP;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(f32x4*)(po + 32 * d + 8 * g + 4 * h) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+    if (h == 0) {
+      p.part_ml[2 * at] = m * cs;
+      p.part_ml[2 * at + 1] = lsum;
+    }
+    return;
+  }
+  const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);  // a NaN stays
+  bf16_t* op = (bf16_t*)p.o + (tok * Hq + head) * D;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+      // the halves exchange 4-element pieces so that each stores 8 neighbours
+      const auto x = __builtin_amdgcn_permlane32_swap(pack_bf16(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
+                                                      pack_bf16(o[d][4 * g + 4] * inv, o[d][4 * g + 5] * inv), false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(pack_bf16(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv),
+                                                      pack_bf16(o[d][4 * g + 6] * inv, o[d][4 * g + 7] * inv), false, false);
+      const int col = 32 * d + 8 * g + 8 * h;
+      if (col < D) *(u32x4*)(op + col) = u32x4{x[0], y[0], x[1], y[1]};
+    }
+  if (p.lse && h == 0) p.lse[tok * Hq + head] = lsum > 0.f ? m * p.scale + __logf(lsum) : (lsum == 0.f ? -INFINITY : lsum);
+}
+
+// Joins the splits of a row: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, one wavefront a
+// row.  Bound by its reads, 4 (DP + 2) bytes a split and row.
+template <int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
+  constexpr int E = DP / 64;
+  typedef float fE __attribute__((ext_vector_type(E)));
+  const int l = threadIdx.x & 63;
+  const long long rows = p.tokens * p.Hkv * p.G, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  float M = kLow * kLog2e;
+  for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[2 * (s * rows + row)]);
+  float acc[E], den = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const long long at = s * rows + row;
+    const float a = __builtin_amdgcn_exp2f(p.part_ml[2 * at] - M), ls = p.part_ml[2 * at + 1];
+    if (ls == 0.f) continue;  // a split without keys
+    den += a * ls;
+    const fE x = *(const fE*)(p.part_o + at * DP + E * l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += a * x[e];
+  }
+  const float inv = den > 0.f ? 1.f / den : (den == 0.f ? 0.f : den);
+  bf16_t* op = (bf16_t*)p.o + row * DP + E * l;
+#pragma unroll
+  for (int e = 0; e < E; ++e) op[e] = f2bf(acc[e] * inv);
+}
+
+// The tile list of more than 64 packed sequences, and their repaired offsets: one workgroup.
+// plan: [count, 0, (sequence, tile) by rank], tiles with most keys first.  Tiles are counted by
+// index in kBuckets buckets of equal width, then placed bucket by bucket from the last; within a
+// bucket the order is of no consequence.
+constexpr int kPlanNT = 1024, kBuckets = 2048;
+__global__ __launch_bounds__(kPlanNT) void attn_plan_kernel(const int32_t* cu, int32_t* plan,
+                                                            int32_t* out, int N, int T, int per) {
+  __shared__ int sScan[kPlanNT], sCount[kBuckets];
+  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+  int shift = 0;
+  while (((T + per - 1) / per) >> shift >= kBuckets) ++shift;
+  for (int i = tid; i < kBuckets; i += kPlanNT) sCount[i] = 0;
+  // the ordered repair: a running maximum of the clamped offsets
+  int carry = 0;
+  for (int n0 = 0; n0 < N; n0 += kPlanNT) {
+    const int n = n0 + tid;
+    int e = n + 1 < N ? cu[n + 1] : T;
+    e = e < 0 ? 0 : (e > T ? T : e);
+    sScan[tid] = e > carry ? e : carry;
+    __syncthreads();
+    for (int o = 1; o < kPlanNT; o <<= 1) {
+      const int x = tid >= o ? sScan[tid - o] : 0;
+      __syncthreads();
+      if (x > sScan[tid]) sScan[tid] = x;
+      __syncthreads();
+    }
+    if (n < N) out[n + 1] = sScan[tid];
+    carry = sScan[kPlanNT - 1];
+    __syncthreads();
+  }
+  if (tid == 0) out[0] = 0;
+  __syncthreads();  // out is read below by other threads of this workgroup
+  for (int n = w; n < N; n += kPlanNT / 64) {
+    const int nt = (out[n + 1] - out[n] + per - 1) / per;
+    for (int j = l; j < nt; j += 64) atomicAdd(&sCount[j >> shift], 1);
+  }
+  __syncthreads();
+  // where each bucket starts: the tiles of later buckets come first
+  if (tid == 0) {
+    int at = 0;
+    for (int b = kBuckets - 1; b >= 0; --b) {
+      const int x = sCount[b];
+      sCount[b] = at;
+      at += x;
+    }
+    plan[0] = at;
+    plan[1] = 0;
+  }
+  __syncthreads();
+  for (int n = w; n < N; n += kPlanNT / 64) {
+    const int nt = (out[n + 1] - out[n] + per - 1) / per;
+    for (int j = l; j < nt; j += 64) {
+      const int at = atomicAdd(&sCount[j >> shift], 1);
+      plan[2 + 2 * (long long)at] = n;
+      plan[3 + 2 * (long long)at] = j;
+    }
+  }
+}
+
+int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
+
+}  // namespace
+
+int attn_tile_tokens(int G) { return kBM / G; }
+
+long long attn_ranks(const AttnParams& p, int per) {
+  const long long tiles = ((long long)p.T + per - 1) / per;
+  if (!p.cu) return tiles;
+  const long long most = tiles + p.N;  // a sequence adds at most one partial tile
+  return most < p.T ? most : p.T;
+}
+
+size_t attn_plan_words(long long T, long long N, int per) {
+  if (N <= 64) return 0;
+  return (size_t)(2 + 2 * ((T + per - 1) / per + N));
+}
+
+hipError_t launch_attn_plan(const AttnParams& p, int per, hipStream_t stream) {
+  attn_plan_kernel<<<1, kPlanNT, 0, stream>>>(p.cu, p.plan, p.cu_plan, p.N, p.T, per);
+  return hipGetLastError();
+}
+
+hipError_t launch_attn_fwd(const AttnParams& p, hipStream_t stream) {
+  const int per = attn_tile_tokens(p.G);
+  const long long ranks = attn_ranks(p, per), units = (long long)(p.cu ? 1 : p.N) * p.Hkv;
+  const bool paged = p.k_pages != nullptr;
+  const dim3 grid((unsigned)attn_grid(units, ranks), paged ? (unsigned)p.splits : 1u);
+  switch (padded_dim(p.D)) {
+#define OMX_FWD(DP)                                                                   \
+  case DP:                                                                            \
+    if (paged)                                                                        \
+      attn_fwd_kernel<DP, true><<<grid, kNT, 0, stream>>>(p, (int)ranks);             \
+    else                                                                              \
+      attn_fwd_kernel<DP, false><<<grid, kNT, 0, stream>>>(p, (int)ranks);            \
+    break;
+    OMX_FWD(64)
+    OMX_FWD(128)
+    OMX_FWD(256)
+#undef OMX_FWD
+  }
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !paged || p.splits == 1) return e;
+  return launch_attn_join(p, stream);
+}
+
+hipError_t launch_attn_join(const AttnParams& p, hipStream_t stream) {
+  const unsigned grid = (unsigned)((p.tokens * p.Hkv * p.G + 3) / 4);
+  switch (padded_dim(p.D)) {
+    case 64: attn_join_kernel<64><<<grid, 256, 0, stream>>>(p); break;
+    case 128: attn_join_kernel<128><<<grid, 256, 0, stream>>>(p); break;
+    default: attn_join_kernel<256><<<grid, 256, 0, stream>>>(p); break;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace omx

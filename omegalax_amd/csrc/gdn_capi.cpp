@@ -15,11 +15,16 @@
 #include <mutex>
 #include <string>
 
+#include "gdn_capi.h"
 #include "gdn_kernels.h"
 
 namespace {
 
 thread_local std::string g_last_error;
+
+}  // namespace
+
+namespace omx {
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -41,14 +46,16 @@ int launch_status(hipError_t e, const char* what) {
   return ok();
 }
 
-bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+}  // namespace omx
+
+namespace {
+
+using omx::aligned;
+using omx::fail;
+using omx::launch_status;
+using omx::ok;
 
 size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
-
-#define REQUIRE(cond, ...) \
-  do {                     \
-    if (!(cond)) return fail(OMX_GDN_EINVAL, __VA_ARGS__); \
-  } while (0)
 
 // Workspace of the chunked prefill, offsets aligned to 256 bytes: the records of
 // the preparation kernel (one per chunk slot and value head; a sequence adds at

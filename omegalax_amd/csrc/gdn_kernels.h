@@ -262,4 +262,53 @@ int qkv_proj_tile_depth();
 hipError_t launch_ab_proj(const void* x, const void* wa, const void* wb, void* a, void* b,
                           long long M, int D, int Hv, hipStream_t stream);
 
+// Causal softmax attention (gdn_attn.hip, gdn_attn_bwd.hip, gdn_paged.hip).  Query head h reads
+// key head h / G, G = Hq / Hkv.  Tokens are packed by `cu` (N sequences over T tokens), or form N
+// rows of T tokens each (cu null).  Strides *_ld are elements from token to token; heads lie side
+// by side.  With pages (k_pages not null) the keys and values are those of a paged cache that
+// held `held[n]` tokens of sequence n before the new ones.
+struct AttnParams {
+  const void *q, *k, *v;
+  void* o;
+  float* lse;                  // [tokens, Hq], natural logarithm; may be null
+  long long q_ld, k_ld, v_ld;
+  const int32_t* cu;
+  int32_t* plan;               // more than 64 packed sequences: the tile list and the repaired
+  int32_t* cu_plan;            //   offsets, written by launch_attn_plan
+  int N, T, Hkv, G, D;
+  long long tokens;            // T packed tokens, or N T
+  float scale;
+  // the paged cache
+  void *k_pages, *v_pages;     // [n_pages, page, Hkv, D]
+  const int32_t* table;        // [N, table_w]
+  const int32_t* held;         // [N]
+  int table_w, page, n_pages;
+  // work split over the keys: partial sums, joined by launch_attn_join
+  int splits;
+  float *part_o, *part_ml;
+  // backward
+  const void* dout;
+  float* delta;                // [tokens, Hq] sum of dout * o
+  void *dq, *dk, *dv;
+};
+constexpr int kAttnMaxG = 32, kAttnMaxD = 256;
+// tokens per tile of the forward, tiles of a row at most, and int32 words of the plan
+int attn_tile_tokens(int G);
+long long attn_ranks(const AttnParams& p, int per);
+size_t attn_plan_words(long long T, long long N, int per);
+hipError_t launch_attn_plan(const AttnParams& p, int per, hipStream_t stream);
+hipError_t launch_attn_fwd(const AttnParams& p, hipStream_t stream);
+hipError_t launch_attn_join(const AttnParams& p, hipStream_t stream);
+
+// the backward: dq and delta, then dk and dv (keys per tile of the second: its plan's tokens)
+int attn_dkv_tile_tokens();
+hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream);
+hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream);
+// the cache's entry points: head dims, append, decode step (splits of the keys by the number of
+// (sequence, key head) pairs and the tokens a table has room for)
+bool paged_dims_supported(int D);
+hipError_t launch_kv_write(const AttnParams& p, hipStream_t stream);
+int decode_splits(long long units, long long capacity);
+hipError_t launch_attn_decode(const AttnParams& p, hipStream_t stream);
+
 }  // namespace omx

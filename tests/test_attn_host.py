@@ -1,0 +1,123 @@
+"""Refusals of the attention entry points, on any machine: every bad argument is turned into an
+error before the first HIP call."""
+import os
+
+import pytest
+
+from omegalax_amd import _lib
+
+pytestmark = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH),
+                                reason="libomx_gdn.so not built (python -m omegalax_amd.build)")
+
+
+def _run(fn, args, over):
+    a = dict(args, **over)
+    L = _lib.lib()
+    rc = getattr(L, fn)(*a.values())
+    return rc, L.omx_gdn_last_error().decode()
+
+
+FWD = dict(q=16, k=16, v=16, q_ld=512, k_ld=256, v_ld=256, cu=None, N=2, o=16, lse=None, B=2, T=100, Hq=4, Hkv=2,
+           D=128, scale=0.1, ws=None, ws_bytes=0, stream=None)
+BWD = dict(q=16, k=16, v=16, q_ld=512, k_ld=256, v_ld=256, cu=None, N=2, o=16, lse=16, do=16, dq=16, dk=16, dv=16,
+           B=2, T=100, Hq=4, Hkv=2, D=128, scale=0.1, ws=256, ws_bytes=1 << 20, stream=None)
+SHAPES = [
+    (dict(Hq=5), _lib.EINVAL, "multiple of key heads"), (dict(Hkv=0), _lib.EINVAL, "positive"),
+    (dict(D=12), _lib.EINVAL, "multiple of 8"), (dict(D=0), _lib.EINVAL, "multiple of 8"),
+    (dict(D=264, q_ld=2048, k_ld=2048, v_ld=2048), _lib.EUNSUPPORTED, "above 256"),
+    (dict(Hq=66, q_ld=66 * 128), _lib.EUNSUPPORTED, "above 32"), (dict(B=-1, N=-1), _lib.EINVAL, "negative"),
+    (dict(T=1 << 31), _lib.EINVAL, "too many tokens"), (dict(N=3), _lib.EINVAL, "N must equal B"),
+    (dict(cu=16), _lib.EINVAL, "batch 1"), (dict(cu=16, B=1, N=0), _lib.EINVAL, "sequence count"),
+    (dict(q_ld=504), _lib.EINVAL, "q_ld"), (dict(k_ld=260), _lib.EINVAL, "k_ld"), (dict(v_ld=1 << 23), _lib.EINVAL, "v_ld"),
+    (dict(scale=0.0), _lib.EINVAL, "scale"), (dict(scale=float("nan")), _lib.EINVAL, "scale"),
+    (dict(scale=-1.0), _lib.EINVAL, "scale"), (dict(q=None), _lib.EINVAL, "NULL"), (dict(o=None), _lib.EINVAL, "NULL"),
+    (dict(v=24), _lib.EINVAL, "aligned"),
+]
+
+
+@pytest.mark.parametrize("over,code,msg", SHAPES)
+def test_forward_refuses(over, code, msg):
+    rc, err = _run("omx_gdn_attn_fwd", FWD, over)
+    assert rc == code and msg in err
+
+
+@pytest.mark.parametrize("over,code,msg", SHAPES + [
+    (dict(lse=None), _lib.EINVAL, "NULL"), (dict(dv=None), _lib.EINVAL, "NULL"), (dict(dk=8), _lib.EINVAL, "aligned"),
+    (dict(ws=None), _lib.EINVAL, "workspace"), (dict(ws=8), _lib.EINVAL, "aligned"), (dict(ws_bytes=100), _lib.EINVAL, "workspace"),
+])
+def test_backward_refuses(over, code, msg):
+    rc, err = _run("omx_gdn_attn_bwd", BWD, over)
+    assert rc == code and msg in err
+
+
+def test_many_packed_sequences_need_their_plan():
+    L = _lib.lib()
+    assert L.omx_gdn_attn_fwd_workspace_size(5000, 4, 2, 64) == 0
+    need = L.omx_gdn_attn_fwd_workspace_size(5000, 4, 2, 65)
+    assert need > 0
+    for ws, n in ((256, need - 1), (None, need), (8, need)):
+        rc, err = _run("omx_gdn_attn_fwd", FWD, dict(cu=16, B=1, T=5000, N=65, ws=ws, ws_bytes=n))
+        assert rc == _lib.EINVAL and "workspace" in err
+
+
+CACHE = dict(k_pages=16, v_pages=16, n_pages=10, page=16, table=16, width=10, lengths=16)
+WRITE = dict(k=16, v=16, k_ld=256, v_ld=256, cu=None, N=2, **CACHE, B=2, T=3, Hkv=2, D=128, ws=None, ws_bytes=0, stream=None)
+PAGED = dict(q=16, q_ld=512, cu=None, N=2, **CACHE, o=16, B=2, T=3, Hq=4, Hkv=2, D=128, scale=0.1, ws=None, ws_bytes=0,
+             stream=None)
+DECODE = dict(q=16, k=16, v=16, q_ld=512, k_ld=256, v_ld=256, **CACHE, out=16, B=2, Hq=4, Hkv=2, D=128, scale=0.1, ws=None,
+              ws_bytes=0, stream=None)
+BAD_CACHE = [
+    (dict(page=8), _lib.EINVAL, "page size"), (dict(page=24), _lib.EINVAL, "page size"), (dict(page=1 << 17), _lib.EINVAL, "page size"),
+    (dict(n_pages=-1), _lib.EINVAL, "page count"), (dict(width=-1), _lib.EINVAL, "block table"),
+    (dict(width=1 << 30), _lib.EINVAL, "block table"), (dict(k_pages=None), _lib.EINVAL, "NULL"),
+    (dict(table=None), _lib.EINVAL, "NULL"), (dict(lengths=None), _lib.EINVAL, "NULL"), (dict(v_pages=8), _lib.EINVAL, "aligned"),
+    (dict(D=96), _lib.EUNSUPPORTED, "not compiled"), (dict(D=100), _lib.EINVAL, "multiple of 8"),
+]
+
+
+@pytest.mark.parametrize("over,code,msg", BAD_CACHE + [
+    (dict(k=None), _lib.EINVAL, "NULL"), (dict(k=8), _lib.EINVAL, "aligned"), (dict(v_ld=128), _lib.EINVAL, "v_ld"),
+    (dict(N=1), _lib.EINVAL, "N must equal B"),
+])
+def test_append_refuses(over, code, msg):
+    rc, err = _run("omx_gdn_kv_write", WRITE, over)
+    assert rc == code and msg in err
+
+
+@pytest.mark.parametrize("over,code,msg", BAD_CACHE + [
+    (dict(q=None), _lib.EINVAL, "NULL"), (dict(o=8), _lib.EINVAL, "aligned"), (dict(q_ld=128), _lib.EINVAL, "q_ld"),
+    (dict(scale=0.0), _lib.EINVAL, "scale"), (dict(Hq=3), _lib.EINVAL, "multiple of key heads"),
+    (dict(width=100, page=64), _lib.EINVAL, "workspace"),
+])
+def test_paged_attention_refuses(over, code, msg):
+    rc, err = _run("omx_gdn_attn_paged", PAGED, over)
+    assert rc == code and msg in err
+
+
+@pytest.mark.parametrize("over,code,msg", BAD_CACHE + [
+    (dict(q=None), _lib.EINVAL, "NULL"), (dict(out=8), _lib.EINVAL, "aligned"), (dict(k_ld=128), _lib.EINVAL, "k_ld"),
+    (dict(scale=float("inf")), _lib.EINVAL, "scale"), (dict(B=-1), _lib.EINVAL, "negative"),
+    (dict(width=100, page=64), _lib.EINVAL, "workspace"),
+])
+def test_decode_refuses(over, code, msg):
+    rc, err = _run("omx_gdn_attn_decode_step", DECODE, over)
+    assert rc == code and msg in err
+
+
+def test_empty_calls_are_no_ops():
+    assert _run("omx_gdn_attn_fwd", FWD, dict(T=0, q=None, o=None))[0] == _lib.OK
+    assert _run("omx_gdn_attn_bwd", BWD, dict(B=0, N=0, q=None))[0] == _lib.OK
+    assert _run("omx_gdn_kv_write", WRITE, dict(T=0, k=None))[0] == _lib.OK
+    assert _run("omx_gdn_attn_paged", PAGED, dict(T=0, q=None))[0] == _lib.OK
+    assert _run("omx_gdn_attn_decode_step", DECODE, dict(B=0, q=None))[0] == _lib.OK
+
+
+def test_python_checks_before_the_library():
+    torch = pytest.importorskip("torch")
+    import omegalax_amd as om
+    q = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="GPU"):
+        om.attention_prefill(q, q, q)
+    with pytest.raises(ValueError, match="GPU"):
+        om.attention_decode_step(q[0], q[0], q[0], q, q, torch.zeros(4, 1, dtype=torch.int32),
+                                 torch.zeros(4, dtype=torch.int32))
