@@ -330,6 +330,7 @@ int omx_gdn_ab_proj(const void* x, const void* w_a, const void* w_b, void* a, vo
  *   cu_seqlens   as for omx_gdn_chunk_fwd (N sequences, B = 1), or NULL (N = B)
  *   o            [B, T, Hq, D] bf16
  *   lse          [B, T, Hq] f32 or NULL: log sum_j exp(scale q . k), for omx_gdn_attn_bwd
+ *   o_rest       [B, T, Hq, D] bf16 or NULL: what the rounding of o left, for omx_gdn_attn_bwd
  *   scale        positive
  * D is a multiple of 8, at most 256 (compiled for 64, 128 and 256; others run zero-filled at the
  * next).  Strides are multiples of 8 and at most 2^22, q, k, v and o 16-byte aligned.  Scores,
@@ -338,7 +339,7 @@ int omx_gdn_ab_proj(const void* x, const void* w_a, const void* w_b, void* a, vo
  */
 int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld,
                      int64_t v_ld, const int32_t* cu_seqlens, int64_t N, void* o, float* lse,
-                     int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, float scale,
+                     void* o_rest, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, float scale,
                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* Bytes of device workspace omx_gdn_attn_fwd needs (16-byte aligned): the tile list of more than
@@ -346,15 +347,17 @@ int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, 
 size_t omx_gdn_attn_fwd_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64_t N);
 
 /*
- * Backward pass (VJP) of omx_gdn_attn_fwd, for the cotangent d_o of o.  Inputs as there; o and
- * lse are what it wrote.
+ * Backward pass (VJP) of omx_gdn_attn_fwd, for the cotangent d_o of o.  Inputs as there; o,
+ * lse and o_rest are what it wrote.
+ *   o_rest       may be NULL: the sums of d_o * o, which every gradient of a row's scores has
+ *                subtracted, are then those of the rounded o (dq and dk about 6% less exact)
  *   d_o          [B, T, Hq, D] bf16
  *   dq           [B, T, Hq, D], dk, dv [B, T, Hkv, D] bf16, dense; dk and dv are summed over each
  *                key head's query heads.  No sum depends on the order of execution.
  */
 int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld,
                      int64_t v_ld, const int32_t* cu_seqlens, int64_t N, const void* o,
-                     const float* lse, const void* d_o, void* dq, void* dk, void* dv, int64_t B,
+                     const float* lse, const void* o_rest, const void* d_o, void* dq, void* dk, void* dv, int64_t B,
                      int64_t T, int64_t Hq, int64_t Hkv, int64_t D, float scale, void* workspace,
                      size_t workspace_bytes, void* stream);
 

@@ -51,9 +51,9 @@ SIGNATURES = {
                                  _i64, _i64, _p, _sz, _p]),
     "omx_gdn_prefill_bwd_workspace_size": (_sz, [_i64] * 7),
     "omx_gdn_ab_proj": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _p]),
-    "omx_gdn_attn_fwd": (_i, [_p] * 3 + [_i64] * 3 + [_p, _i64, _p, _p] + [_i64] * 5 + [_f, _p, _sz, _p]),
+    "omx_gdn_attn_fwd": (_i, [_p] * 3 + [_i64] * 3 + [_p, _i64, _p, _p, _p] + [_i64] * 5 + [_f, _p, _sz, _p]),
     "omx_gdn_attn_fwd_workspace_size": (_sz, [_i64] * 4),
-    "omx_gdn_attn_bwd": (_i, [_p] * 3 + [_i64] * 3 + [_p, _i64] + [_p] * 6 + [_i64] * 5 + [_f, _p, _sz, _p]),
+    "omx_gdn_attn_bwd": (_i, [_p] * 3 + [_i64] * 3 + [_p, _i64] + [_p] * 7 + [_i64] * 5 + [_f, _p, _sz, _p]),
     "omx_gdn_attn_bwd_workspace_size": (_sz, [_i64] * 6),
     "omx_gdn_kv_write": (_i, [_p, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _i64, _p]
                          + [_i64] * 4 + [_p, _sz, _p]),

@@ -55,6 +55,23 @@ __device__ __forceinline__ float sum_halves(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// four-element pieces of a C fragment's column, scaled, rounded and exchanged between the halves
+// of the wavefront so that each lane stores 8 neighbours of its row
+template <int DB>
+__device__ __forceinline__ void store_rows(bf16_t* row, const f32x16 (&x)[DB], float f, int D, int h) {
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+      const auto a = __builtin_amdgcn_permlane32_swap(pack_bf16(x[d][4 * g] * f, x[d][4 * g + 1] * f),
+                                                      pack_bf16(x[d][4 * g + 4] * f, x[d][4 * g + 5] * f), false, false);
+      const auto b = __builtin_amdgcn_permlane32_swap(pack_bf16(x[d][4 * g + 2] * f, x[d][4 * g + 3] * f),
+                                                      pack_bf16(x[d][4 * g + 6] * f, x[d][4 * g + 7] * f), false, false);
+      const int col = 32 * d + 8 * g + 8 * h;
+      if (col < D) *(u32x4*)(row + col) = u32x4{a[0], b[0], a[1], b[1]};
+    }
+}
+
 // Rows of DP bf16 in LDS without padding, in 16-byte segments: segment s of row r lies at
 // s ^ swz(r).  One pass of a 16-byte read serves lanes {0-3, 12-15, 20-27} (and the rest of
 // each half), whose rows' images must differ in the 16 segments that the 64 banks hold; one

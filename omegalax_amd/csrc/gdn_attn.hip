@@ -269,45 +269,86 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     return;
   }
   const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);  // a NaN stays
-  bf16_t* op = (bf16_t*)p.o + (tok * Hq + head) * D;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int g = 0; g < 4; g += 2) {
-      // the halves exchange 4-element pieces so that each stores 8 neighbours
-      const auto x = __builtin_amdgcn_permlane32_swap(pack_bf16(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
-                                                      pack_bf16(o[d][4 * g + 4] * inv, o[d][4 * g + 5] * inv), false, false);
-      const auto y = __builtin_amdgcn_permlane32_swap(pack_bf16(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv),
-                                                      pack_bf16(o[d][4 * g + 6] * inv, o[d][4 * g + 7] * inv), false, false);
-      const int col = 32 * d + 8 * g + 8 * h;
-      if (col < D) *(u32x4*)(op + col) = u32x4{x[0], y[0], x[1], y[1]};
-    }
+    for (int i = 0; i < 16; ++i) o[d][i] *= inv;
+  store_rows<DB>((bf16_t*)p.o + (tok * Hq + head) * D, o, 1.f, D, h);
+  if (p.o_rest) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = lo_part(o[d][i]);
+    store_rows<DB>((bf16_t*)p.o_rest + (tok * Hq + head) * D, o, 1.f, D, h);
+  }
   if (p.lse && h == 0) p.lse[tok * Hq + head] = lsum > 0.f ? m * p.scale + __logf(lsum) : (lsum == 0.f ? -INFINITY : lsum);
 }
 
-// Joins the splits of a row: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, one wavefront a
-// row.  Bound by its reads, 4 (DP + 2) bytes a split and row.
-template <int DP>
+// Joins the shares of a row: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, with W of a
+// workgroup's four wavefronts on one row, each lane E columns.  The weights are formed once, a
+// share a lane.  Bound by its reads, 4 (DP + 2) bytes a share and row, and for few rows by the
+// latency of a wavefront's chain of reads, which the four cut short.
+template <int DP, int W>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   constexpr int E = DP / 64;
   typedef float fE __attribute__((ext_vector_type(E)));
-  const int l = threadIdx.x & 63;
-  const long long rows = p.tokens * p.Hkv * p.G, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  float M = kLow * kLog2e;
-  for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[2 * (s * rows + row)]);
-  float acc[E], den = 0.f;
+  __shared__ float sAcc[4][DP];
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, part = w % W;
+  const long long rows = p.tokens * p.Hkv * p.G, row = (long long)blockIdx.x * (4 / W) + w / W;
+  const bool live = row < rows;
+  float a[4], M = kLow * kLog2e, den = 0.f;  // splits <= 256
+  float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const long long at = s * rows + row;
-    const float a = __builtin_amdgcn_exp2f(p.part_ml[2 * at] - M), ls = p.part_ml[2 * at + 1];
-    if (ls == 0.f) continue;  // a split without keys
-    den += a * ls;
-    const fE x = *(const fE*)(p.part_o + at * DP + E * l);
+  if (live) {
+    float ls[4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += a * x[e];
+    for (int r = 0; r < 4; ++r) {
+      const int s = 64 * r + l;
+      const bool in = s < p.splits;
+      a[r] = in ? p.part_ml[2 * (s * rows + row)] : kLow * kLog2e;
+      ls[r] = in ? p.part_ml[2 * (s * rows + row) + 1] : 0.f;
+      M = fmaxf(M, a[r]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      a[r] = ls[r] == 0.f ? 0.f : __builtin_amdgcn_exp2f(a[r] - M);
+      den += a[r] * ls[r];
+    }
+    den = wave_sum(den);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int s1 = p.splits - 64 * r < 64 ? p.splits - 64 * r : 64;
+      for (int s = part; s < s1; s += 8 * W) {  // eight reads in flight
+        fE x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int su = s + W * u < s1 ? s + W * u : s1 - 1;
+          x[u] = *(const fE*)(p.part_o + ((64 * r + su) * rows + row) * DP + E * l);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float as = __shfl(a[r], s + W * u, 64);
+          const float f = s + W * u < s1 ? as : 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += f * x[u][e];
+        }
+      }
+    }
   }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) sAcc[w][E * l + e] = acc[e];
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int x = 1; x < W; ++x) acc[e] += sAcc[w + x][E * l + e];
+  }
+  if (!live) return;
   const float inv = den > 0.f ? 1.f / den : (den == 0.f ? 0.f : den);
   bf16_t* op = (bf16_t*)p.o + row * DP + E * l;
 #pragma unroll
@@ -419,12 +460,20 @@ hipError_t launch_attn_fwd(const AttnParams& p, hipStream_t stream) {
   return launch_attn_join(p, stream);
 }
 
+template <int DP>
+static void join(const AttnParams& p, hipStream_t stream) {
+  const long long rows = p.tokens * p.Hkv * p.G;
+  if (p.splits > 8)
+    attn_join_kernel<DP, 4><<<(unsigned)rows, 256, 0, stream>>>(p);
+  else
+    attn_join_kernel<DP, 1><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(p);
+}
+
 hipError_t launch_attn_join(const AttnParams& p, hipStream_t stream) {
-  const unsigned grid = (unsigned)((p.tokens * p.Hkv * p.G + 3) / 4);
   switch (padded_dim(p.D)) {
-    case 64: attn_join_kernel<64><<<grid, 256, 0, stream>>>(p); break;
-    case 128: attn_join_kernel<128><<<grid, 256, 0, stream>>>(p); break;
-    default: attn_join_kernel<256><<<grid, 256, 0, stream>>>(p); break;
+    case 64: join<64>(p, stream); break;
+    case 128: join<128>(p, stream); break;
+    default: join<256>(p, stream); break;
   }
   return hipGetLastError();
 }

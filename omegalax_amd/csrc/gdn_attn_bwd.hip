@@ -14,20 +14,15 @@ namespace {
 
 constexpr int kNW = 4, kNT = 64 * kNW, kBM = 128, kBN = 64;
 
-// four-element pieces of a C fragment's column, scaled, rounded and exchanged between the halves
-// of the wavefront so that each lane stores 8 neighbours of its row
+// the same column in fp32, as one of the shares of a sum
 template <int DB>
-__device__ __forceinline__ void store_rows(bf16_t* row, const f32x16 (&x)[DB], float f, int D, int h) {
+__device__ __forceinline__ void store_part(float* row, const f32x16 (&x)[DB], float f, int D, int h) {
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int g = 0; g < 4; g += 2) {
-      const auto a = __builtin_amdgcn_permlane32_swap(pack_bf16(x[d][4 * g] * f, x[d][4 * g + 1] * f),
-                                                      pack_bf16(x[d][4 * g + 4] * f, x[d][4 * g + 5] * f), false, false);
-      const auto b = __builtin_amdgcn_permlane32_swap(pack_bf16(x[d][4 * g + 2] * f, x[d][4 * g + 3] * f),
-                                                      pack_bf16(x[d][4 * g + 6] * f, x[d][4 * g + 7] * f), false, false);
-      const int col = 32 * d + 8 * g + 8 * h;
-      if (col < D) *(u32x4*)(row + col) = u32x4{a[0], b[0], a[1], b[1]};
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * d + 8 * g + 4 * h;
+      if (col < D) *(f32x4*)(row + col) = f32x4{x[d][4 * g] * f, x[d][4 * g + 1] * f, x[d][4 * g + 2] * f, x[d][4 * g + 3] * f};
     }
 }
 
@@ -76,6 +71,7 @@ void attn_dq_kernel(AttnParams p, int ranks) {
       q[s] = *(const u32x4*)((const bf16_t*)p.q + tok * p.q_ld + (long long)(hk * G + rg) * D + d);
       dout[s] = *(const u32x4*)((const bf16_t*)p.dout + at * D + d);
       delta += dot8(dout[s], *(const u32x4*)((const bf16_t*)p.o + at * D + d));
+      if (p.o_rest) delta += dot8(dout[s], *(const u32x4*)((const bf16_t*)p.o_rest + at * D + d));
     }
   }
   delta = sum_halves(delta);
@@ -158,8 +154,8 @@ void attn_dq_kernel(AttnParams p, int ranks) {
 constexpr int kKeys = 32 * kNW;  // keys of a workgroup's tile
 constexpr int kRows = 64;        // rows of a stage
 
-template <int DP>
-__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(1, 1)))
+template <int DP, bool DK, bool DV>
+__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 || (DK && DV) ? 1 : 2)))
 void attn_dkv_kernel(AttnParams p, int ranks) {
   constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int NJ = kRows * DP / 8 / 64 / kNW;
@@ -178,6 +174,14 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
   if (!attn_tile(p, unit / Hkv, rank, kKeys, it)) return;
   // the first tiles' keys are seen by most rows: those first
   const int k0 = (it.tiles - 1 - it.tile) * kKeys;
+  // this share's rows: tokens [ta, tb) in whole stages
+  int ta = k0, tb = it.len;
+  if (p.splits > 1) {
+    const int n = (it.len - k0 + per - 1) / per, each = (n + p.splits - 1) / p.splits;
+    const int first = (int)blockIdx.y * each;
+    ta = first < n ? k0 + first * per : it.len;
+    tb = first + each < n ? ta + each * per : it.len;
+  }
   const int key = k0 + 32 * w + c;
   const bool live = key < it.len;
   const long long tok = it.start + key;
@@ -189,7 +193,7 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
     kf[s] = vf[s] = u32x4{0, 0, 0, 0};
     if (live && d < D) {
       kf[s] = *(const u32x4*)((const bf16_t*)p.k + tok * p.k_ld + hk * D + d);
-      vf[s] = *(const u32x4*)((const bf16_t*)p.v + tok * p.v_ld + hk * D + d);
+      if constexpr (DK) vf[s] = *(const u32x4*)((const bf16_t*)p.v + tok * p.v_ld + hk * D + d);
     }
   }
   f32x16 dk[DB], dv[DB];
@@ -235,7 +239,8 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
 #pragma unroll
       for (int k = 0; k < KS; ++k) s = mma32(attn_frag<DP>(sq, 32 * rb, k), kf[k], s);
 #pragma unroll
-      for (int k = 0; k < KS; ++k) dp = mma32(attn_frag<DP>(so, 32 * rb, k), vf[k], dp);
+      for (int k = 0; k < KS; ++k)
+        if constexpr (DK) dp = mma32(attn_frag<DP>(so, 32 * rb, k), vf[k], dp);
       if (t < kw + 31) {  // row r is token t + r / G: before the key if r < (key - t) G
         const int first = (key - t) * G;
 #pragma unroll
@@ -258,29 +263,63 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
         const u32x4 pb = pack8_of(s, k), db = pack8_of(ds, k);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          dv[d] = mma32(attn_frag_tr<DP>(so, 32 * rb + 16 * k, d), pb, dv[d]);
-          dk[d] = mma32(attn_frag_tr<DP>(sq, 32 * rb + 16 * k, d), db, dk[d]);
+          if constexpr (DV) dv[d] = mma32(attn_frag_tr<DP>(so, 32 * rb + 16 * k, d), pb, dv[d]);
+          if constexpr (DK) dk[d] = mma32(attn_frag_tr<DP>(sq, 32 * rb + 16 * k, d), db, dk[d]);
         }
       }
     }
   };
-  stage(k0, sQ0, sO0, sS0);
-  for (int t = k0; t < it.len; t += 2 * per) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    lds_barrier();
-    if (t + per < it.len) stage(t + per, sQ1, sO1, sS1);
-    compute(t, sQ0, sO0, sS0);
-    if (t + per >= it.len) break;
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    lds_barrier();
-    if (t + 2 * per < it.len) stage(t + 2 * per, sQ0, sO0, sS0);
-    compute(t + per, sQ1, sO1, sS1);
+  // from the last stage to the first: a unit's workgroups, which start together and see different
+  // numbers of rows, then read the same rows at the same time, and its XCD's L2 serves most of them
+  if (ta < tb) {
+    int t = ta + (tb - ta - 1) / per * per;
+    stage(t, sQ0, sO0, sS0);
+    for (; t >= ta; t -= 2 * per) {
+      __builtin_amdgcn_s_waitcnt(0x0F70);
+      lds_barrier();
+      if (t - per >= ta) stage(t - per, sQ1, sO1, sS1);
+      compute(t, sQ0, sO0, sS0);
+      if (t - per < ta) break;
+      __builtin_amdgcn_s_waitcnt(0x0F70);
+      lds_barrier();
+      if (t - 2 * per >= ta) stage(t - 2 * per, sQ0, sO0, sS0);
+      compute(t - per, sQ1, sO1, sS1);
+    }
   }
-  if (live) {
-    const long long at = (tok * Hkv + hk) * D;
-    store_rows<DB>((bf16_t*)p.dk + at, dk, p.scale, D, h);
-    store_rows<DB>((bf16_t*)p.dv + at, dv, 1.f, D, h);
+  if (!live) return;
+  const long long at = (tok * Hkv + hk) * D;
+  if (p.splits > 1) {
+    const long long ps = (long long)blockIdx.y * p.tokens * Hkv * D + at;
+    if constexpr (DK) store_part<DB>(p.part_k + ps, dk, p.scale, D, h);
+    if constexpr (DV) store_part<DB>(p.part_v + ps, dv, 1.f, D, h);
+  } else {
+    if constexpr (DK) store_rows<DB>((bf16_t*)p.dk + at, dk, p.scale, D, h);
+    if constexpr (DV) store_rows<DB>((bf16_t*)p.dv + at, dv, 1.f, D, h);
   }
+}
+
+// The shares' sums, 8 elements a thread.  Bound by its bytes: 4 a share and 2 out.
+__global__ __launch_bounds__(256) void attn_dkv_sum_kernel(const float* pk, const float* pv, bf16_t* dk,
+                                                           bf16_t* dv, int splits, long long n) {
+  const long long i = 8 * ((long long)blockIdx.x * 256 + threadIdx.x);
+  if (i >= n) return;
+  const float* src = blockIdx.y ? pv : pk;
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x4 y = *(const f32x4*)(src + s * n + i + 4 * j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * j + e] += y[e];
+    }
+  *(u32x4*)((blockIdx.y ? dv : dk) + i) =
+      u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+}
+
+template <int DP>
+void dkv(const AttnParams& p, int ranks, dim3 grid, hipStream_t stream) {
+  attn_dkv_kernel<DP, false, true><<<grid, kNT, 0, stream>>>(p, ranks);
+  attn_dkv_kernel<DP, true, false><<<grid, kNT, 0, stream>>>(p, ranks);
 }
 
 }  // namespace
@@ -296,12 +335,26 @@ hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
+int attn_dkv_splits(long long units, long long T, long long N, int G) {
+  // two workgroups for each compute unit, and no share below eight stages of rows on average
+  const long long tiles = units * ((T + kKeys - 1) / kKeys + (N > 0 ? N - 1 : 0));
+  const long long most = T / (N > 0 ? N : 1) * G / (8 * kRows);
+  long long s = 512 / (tiles > 0 ? tiles : 1);
+  s = s < most ? s : most;
+  return (int)(s < 1 ? 1 : (s > 8 ? 8 : s));
+}
+
 hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream) {
   const long long ranks = attn_ranks(p, kKeys), units = (long long)(p.cu ? 1 : p.N) * p.Hkv;
-  const unsigned grid = (unsigned)attn_grid(units, ranks);
-  if (p.D <= 64) attn_dkv_kernel<64><<<grid, kNT, 0, stream>>>(p, (int)ranks);
-  else if (p.D <= 128) attn_dkv_kernel<128><<<grid, kNT, 0, stream>>>(p, (int)ranks);
-  else attn_dkv_kernel<256><<<grid, kNT, 0, stream>>>(p, (int)ranks);
+  const dim3 grid((unsigned)attn_grid(units, ranks), (unsigned)p.splits);
+  if (p.D <= 64) dkv<64>(p, (int)ranks, grid, stream);
+  else if (p.D <= 128) dkv<128>(p, (int)ranks, grid, stream);
+  else dkv<256>(p, (int)ranks, grid, stream);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.splits == 1) return e;
+  const long long n = p.tokens * p.Hkv * p.D;
+  attn_dkv_sum_kernel<<<dim3((unsigned)((n + 2047) / 2048), 2), 256, 0, stream>>>(
+      p.part_k, p.part_v, (bf16_t*)p.dk, (bf16_t*)p.dv, p.splits, n);
   return hipGetLastError();
 }
 

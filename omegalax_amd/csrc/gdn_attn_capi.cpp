@@ -145,8 +145,9 @@ size_t omx_gdn_attn_fwd_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64
 }
 
 int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
-                     const int32_t* cu_seqlens, int64_t N, void* o, float* lse, int64_t B, int64_t T, int64_t Hq,
-                     int64_t Hkv, int64_t D, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+                     const int32_t* cu_seqlens, int64_t N, void* o, float* lse, void* o_rest, int64_t B, int64_t T,
+                     int64_t Hq, int64_t Hkv, int64_t D, float scale, void* workspace, size_t workspace_bytes,
+                     void* stream) {
   const char* fn = "omx_gdn_attn_fwd";
   const Shape s{N, B, T, Hq, Hkv, D, cu_seqlens != nullptr};
   int rc = check_shape(fn, s);
@@ -162,10 +163,11 @@ int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, 
           workspace_bytes, ws.total);
   if (B * T == 0) return ok();
   REQUIRE(q && k && v && o, "%s: a required pointer is NULL", fn);
-  REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(o, 16), "%s: q, k, v, o must be 16-byte aligned", fn);
+  REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(o, 16) && aligned(o_rest, 16),
+          "%s: q, k, v, o, o_rest must be 16-byte aligned", fn);
   REQUIRE(ws.total == 0 || (workspace && aligned(workspace, 16)), "%s: workspace must be non-NULL and 16-byte aligned", fn);
   omx::AttnParams p = params(s, scale);
-  p.q = q; p.k = k; p.v = v; p.o = o; p.lse = lse;
+  p.q = q; p.k = k; p.v = v; p.o = o; p.o_rest = o_rest; p.lse = lse;
   p.q_ld = q_ld; p.k_ld = k_ld; p.v_ld = v_ld; p.cu = cu_seqlens;
   hipError_t e = use_plan(p, ws, workspace, per, (hipStream_t)stream);
   if (e == hipSuccess) e = omx::launch_attn_fwd(p, (hipStream_t)stream);
@@ -173,30 +175,38 @@ int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, 
 }
 
 namespace {
-// delta, then the plans of the two kernels' tiles
+// delta, the plans of the two kernels' tiles, dk and dv in shares
 struct AttnBwdWs {
   size_t delta;
   PlanWs rows, keys;
-  size_t total;
+  int splits;
+  size_t part_k, part_v, total;
 };
-AttnBwdWs attn_bwd_ws(int64_t tokens, int64_t T, int64_t Hq, int64_t Hkv, int64_t N) {
+AttnBwdWs attn_bwd_ws(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N) {
   AttnBwdWs w{};
-  w.rows = plan_ws(align_up((size_t)(tokens * Hq) * 4), T, N, omx::attn_tile_tokens((int)(Hq / Hkv)));
-  w.keys = plan_ws(w.rows.total, T, N, omx::attn_dkv_tile_tokens());
-  w.total = w.keys.total;
+  const int per = omx::attn_dkv_tile_tokens();
+  w.rows = plan_ws(align_up((size_t)(B * T * Hq) * 4), T, N, omx::attn_tile_tokens((int)(Hq / Hkv)));
+  w.keys = plan_ws(w.rows.total, T, N, per);
+  w.splits = omx::attn_dkv_splits(B * Hkv, T, N, (int)(Hq / Hkv));
+  w.part_k = w.part_v = w.total = w.keys.total;
+  if (w.splits > 1) {
+    const size_t one = align_up((size_t)w.splits * B * T * Hkv * D * 4);
+    w.part_v = w.part_k + one;
+    w.total = w.part_v + one;
+  }
   return w;
 }
 }  // namespace
 
 size_t omx_gdn_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N) {
   if (B < 0 || T < 0 || D < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq / Hkv > omx::kAttnMaxG || N < 0) return 0;
-  return attn_bwd_ws(B * T, T, Hq, Hkv, N).total;
+  return attn_bwd_ws(B, T, Hq, Hkv, D, N).total;
 }
 
 int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
-                     const int32_t* cu_seqlens, int64_t N, const void* o, const float* lse, const void* d_o, void* dq,
-                     void* dk, void* dv, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, float scale,
-                     void* workspace, size_t workspace_bytes, void* stream) {
+                     const int32_t* cu_seqlens, int64_t N, const void* o, const float* lse, const void* o_rest, const void* d_o,
+                     void* dq, void* dk, void* dv, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                     float scale, void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "omx_gdn_attn_bwd";
   const Shape s{N, B, T, Hq, Hkv, D, cu_seqlens != nullptr};
   int rc = check_shape(fn, s);
@@ -207,20 +217,24 @@ int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, 
   const int per = rc ? 1 : omx::attn_tile_tokens((int)(Hq / Hkv));
   if (!rc) rc = check_grid(fn, s, per, 1);
   if (rc) return rc;
-  const AttnBwdWs ws = attn_bwd_ws(B * T, T, Hq, Hkv, s.packed ? N : 0);
+  const AttnBwdWs ws = attn_bwd_ws(B, T, Hq, Hkv, D, s.packed ? N : 0);
   REQUIRE(workspace_bytes >= ws.total, "%s: workspace of %zu bytes is smaller than the %zu needed", fn,
           workspace_bytes, ws.total);
   if (B * T == 0) return ok();
   REQUIRE(q && k && v && o && lse && d_o && dq && dk && dv, "%s: a required pointer is NULL", fn);
-  REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(o, 16) && aligned(d_o, 16) && aligned(dq, 16) &&
+  REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(o, 16) && aligned(o_rest, 16) && aligned(d_o, 16) && aligned(dq, 16) &&
               aligned(dk, 16) && aligned(dv, 16),
-          "%s: q, k, v, o, d_o, dq, dk, dv must be 16-byte aligned", fn);
+          "%s: q, k, v, o, o_rest, d_o, dq, dk, dv must be 16-byte aligned", fn);
   REQUIRE(workspace && aligned(workspace, 16), "%s: workspace must be non-NULL and 16-byte aligned", fn);
   omx::AttnParams p = params(s, scale);
   p.q = q; p.k = k; p.v = v; p.o = const_cast<void*>(o); p.lse = const_cast<float*>(lse); p.dout = d_o;
+  p.o_rest = const_cast<void*>(o_rest);
   p.q_ld = q_ld; p.k_ld = k_ld; p.v_ld = v_ld; p.cu = cu_seqlens;
   p.dq = dq; p.dk = dk; p.dv = dv;
   p.delta = (float*)((char*)workspace + ws.delta);
+  p.part_k = (float*)((char*)workspace + ws.part_k);
+  p.part_v = (float*)((char*)workspace + ws.part_v);
+  p.splits = ws.splits;
   const hipStream_t st = (hipStream_t)stream;
   hipError_t e = use_plan(p, ws.rows, workspace, per, st);
   if (e == hipSuccess) e = omx::launch_attn_dq(p, st);

@@ -270,6 +270,7 @@ hipError_t launch_ab_proj(const void* x, const void* wa, const void* wb, void* a
 struct AttnParams {
   const void *q, *k, *v;
   void* o;
+  void* o_rest;                // what o's rounding left, bf16 as o; may be null
   float* lse;                  // [tokens, Hq], natural logarithm; may be null
   long long q_ld, k_ld, v_ld;
   const int32_t* cu;
@@ -290,6 +291,7 @@ struct AttnParams {
   const void* dout;
   float* delta;                // [tokens, Hq] sum of dout * o
   void *dq, *dk, *dv;
+  float *part_k, *part_v;      // dk and dv in shares of the rows, when there are `splits` of them
 };
 constexpr int kAttnMaxG = 32, kAttnMaxD = 256;
 // tokens per tile of the forward, tiles of a row at most, and int32 words of the plan
@@ -302,6 +304,7 @@ hipError_t launch_attn_join(const AttnParams& p, hipStream_t stream);
 
 // the backward: dq and delta, then dk and dv (keys per tile of the second: its plan's tokens)
 int attn_dkv_tile_tokens();
+int attn_dkv_splits(long long units, long long T, long long N, int G);
 hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream);
 hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream);
 // the cache's entry points: head dims, append, decode step (splits of the keys by the number of

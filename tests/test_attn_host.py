@@ -17,9 +17,10 @@ def _run(fn, args, over):
     return rc, L.omx_gdn_last_error().decode()
 
 
-FWD = dict(q=16, k=16, v=16, q_ld=512, k_ld=256, v_ld=256, cu=None, N=2, o=16, lse=None, B=2, T=100, Hq=4, Hkv=2,
-           D=128, scale=0.1, ws=None, ws_bytes=0, stream=None)
-BWD = dict(q=16, k=16, v=16, q_ld=512, k_ld=256, v_ld=256, cu=None, N=2, o=16, lse=16, do=16, dq=16, dk=16, dv=16,
+FWD = dict(q=16, k=16, v=16, q_ld=512, k_ld=256, v_ld=256, cu=None, N=2, o=16, lse=None, o_rest=None, B=2, T=100, Hq=4,
+           Hkv=2, D=128, scale=0.1, ws=None, ws_bytes=0, stream=None)
+BWD = dict(q=16, k=16, v=16, q_ld=512, k_ld=256, v_ld=256, cu=None, N=2, o=16, lse=16, o_rest=None, do=16, dq=16, dk=16,
+           dv=16,
            B=2, T=100, Hq=4, Hkv=2, D=128, scale=0.1, ws=256, ws_bytes=1 << 20, stream=None)
 SHAPES = [
     (dict(Hq=5), _lib.EINVAL, "multiple of key heads"), (dict(Hkv=0), _lib.EINVAL, "positive"),
