@@ -72,6 +72,18 @@ __device__ __forceinline__ void store_rows(bf16_t* row, const f32x16 (&x)[DB], f
     }
 }
 
+// the same column in fp32, as one of the shares of a sum
+template <int DB>
+__device__ __forceinline__ void store_part(float* row, const f32x16 (&x)[DB], float f, int D, int h) {
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = 32 * d + 8 * g + 4 * h;
+      if (col < D) *(f32x4*)(row + col) = f32x4{x[d][4 * g] * f, x[d][4 * g + 1] * f, x[d][4 * g + 2] * f, x[d][4 * g + 3] * f};
+    }
+}
+
 // Rows of DP bf16 in LDS without padding, in 16-byte segments: segment s of row r lies at
 // s ^ swz(r).  One pass of a 16-byte read serves lanes {0-3, 12-15, 20-27} (and the rest of
 // each half), whose rows' images must differ in the 16 segments that the 64 banks hold; one
@@ -83,23 +95,68 @@ __device__ __forceinline__ int attn_swz(int r) {
   return DP == 64 ? ((((r >> 1) & 1) << 2) | ((r >> 2) & 3)) : (((r & 3) << 2) | ((r >> 2) & 3));
 }
 
+// A lane's byte offsets in such a tile, for the two kinds of fragments: step and column block
+// only flip bits of the segment.
+struct AttnLane {
+  unsigned f, t;
+};
+template <int DP>
+__device__ __forceinline__ AttnLane attn_lane() {
+  const int l = lane_id(), h = l >> 5, c = l & 31, s = l & 15, r = 4 * h + (s >> 2);
+  return {(unsigned)(c * DP * 2 + ((h ^ attn_swz<DP>(c)) << 4)),
+          (unsigned)(r * DP * 2 + (((2 * ((l >> 4) & 1) + ((s >> 1) & 1)) ^ attn_swz<DP>(r)) << 4) + 8 * (s & 1))};
+}
+// the same, recomputed from here on: keeps the compiler from holding every offset in a register
+__device__ __forceinline__ AttnLane fresh(AttnLane ln) {
+  asm volatile("" : "+v"(ln.f), "+v"(ln.t));
+  return ln;
+}
+
 // A operand (32 rows row0 .. +31, elements 16 step .. +15) of a [row][DP] LDS tile
 template <int DP>
-__device__ __forceinline__ u32x4 attn_frag(const bf16_t* base, int row0, int step) {
-  const int l = lane_id(), h = l >> 5, c = l & 31;
-  return *(const u32x4*)(base + (row0 + c) * DP + (((2 * step + h) ^ attn_swz<DP>(c)) << 3));
+__device__ __forceinline__ u32x4 attn_frag(const bf16_t* base, AttnLane ln, int row0, int step) {
+  return *(const u32x4*)((const char*)(base + row0 * DP) + (ln.f ^ (unsigned)(step << 5)));
 }
 
 // A operand whose rows are the tile's columns 32 cb .. +31 and whose contraction runs over its
-// rows row0 + {4h .. +3, 8 + 4h .. +3}: the order of pack8_of
+// rows row0 + {4h .. +3, 8 + 4h .. +3}: the order of pack8_of (row0 a multiple of 16; eight rows
+// on, the swizzle differs in bit 1)
 template <int DP>
-__device__ __forceinline__ u32x4 attn_frag_tr(const bf16_t* base, int row0, int cb) {
-  const int l = lane_id(), h = l >> 5, s = l & 15;
-  const int col = 32 * cb + 16 * ((l >> 4) & 1) + 4 * (s & 3);
-  const int r0 = row0 + 4 * h + (s >> 2), r1 = r0 + 8;
-  const u32x2 a = ds_read_tr(base + r0 * DP + (((col >> 3) ^ attn_swz<DP>(r0)) << 3) + (col & 7));
-  const u32x2 b = ds_read_tr(base + r1 * DP + (((col >> 3) ^ attn_swz<DP>(r1)) << 3) + (col & 7));
+__device__ __forceinline__ u32x4 attn_frag_tr(const bf16_t* base, AttnLane ln, int row0, int cb) {
+  const unsigned at = ln.t ^ (unsigned)(cb << 6);
+  const u32x2 a = ds_read_tr((const bf16_t*)((const char*)(base + row0 * DP) + at));
+  const u32x2 b = ds_read_tr((const bf16_t*)((const char*)(base + (row0 + 8) * DP) + (at ^ 32u)));
   return u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// Loads of 16 (or 4) bytes a lane into LDS at `lds` + 16 (4) lane, past the compiler's book of
+// outstanding loads: with the builtin it put a wait for all of them before reads of buffers that
+// they do not touch.  Whoever reads the bytes waits for them with wait_loads.
+// (The resource's words are uniform; readfirstlane also puts one there that the compiler keeps in
+// a vector register, and five wait states then lie between that write and the load.)
+__device__ __forceinline__ u32x4 rsrc_words(const void* p, unsigned bytes) {
+  const unsigned long long a = (unsigned long long)p;
+  return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((unsigned)a),
+               (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffffu),
+               (unsigned)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(unsigned long long)(const __attribute__((address_space(3))) char*)p;
+}
+__device__ __forceinline__ void load_to_lds16(u32x4 rsrc, unsigned lds, unsigned off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory");
+}
+__device__ __forceinline__ void load_to_lds4(u32x4 rsrc, unsigned lds, unsigned off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory");
+}
+
+// waits until at most N of the wavefront's vector memory operations are outstanding
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "the counter's range");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
 // One staging instruction writes 1 KiB of LDS, 64 / (DP / 8) rows.  Of a tile's instructions a
@@ -177,11 +234,12 @@ __device__ __forceinline__ bool attn_tile(const AttnParams& p, int row, int rank
   if (!p.plan) return packed_tile(p.cu, p.N, p.T, per, rank, it);
   // more than 64 sequences: the plan kernel's list (count, then sequence and tile per rank)
   const int32_t* plan = p.plan;
-  if (rank >= plan[0]) return false;
-  it.seq = plan[2 + 2 * (long long)rank];
-  it.tile = plan[3 + 2 * (long long)rank];
-  it.start = p.cu_plan[it.seq];
-  it.len = p.cu_plan[it.seq + 1] - p.cu_plan[it.seq];
+  if (rank >= __builtin_amdgcn_readfirstlane(plan[0])) return false;
+  it.seq = __builtin_amdgcn_readfirstlane(plan[2 + 2 * (long long)rank]);
+  it.tile = __builtin_amdgcn_readfirstlane(plan[3 + 2 * (long long)rank]);
+  const int start = __builtin_amdgcn_readfirstlane(p.cu_plan[it.seq]);
+  it.start = start;
+  it.len = __builtin_amdgcn_readfirstlane(p.cu_plan[it.seq + 1]) - start;
   it.tiles = (it.len + per - 1) / per;
   return true;
 }
@@ -192,9 +250,9 @@ __device__ __forceinline__ bool attn_tile(const AttnParams& p, int row, int rank
 // past a unit's last tile have nothing to do.
 __device__ __forceinline__ void attn_place(int bid, int units, int ranks, int& unit, int& rank) {
   if (units % 8 == 0) {
-    const int x = bid & 7, j = bid >> 3;
-    unit = x + 8 * (j / ranks);
-    rank = j % ranks;
+    const int x = bid & 7, j = bid >> 3, each = units / 8;
+    unit = x + 8 * (j % each);
+    rank = j / each;
   } else if (8 % units == 0) {
     const int x = bid & 7, j = bid >> 3, r = 8 / units;
     unit = x / r;
@@ -211,6 +269,9 @@ inline long long attn_grid(long long units, long long ranks) {
   }
   return units * ranks;
 }
+
+// keys of a workgroup's tile of the kernels that sum dk and dv
+constexpr int kDkvKeys = 128;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

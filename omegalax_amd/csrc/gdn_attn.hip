@@ -10,6 +10,9 @@
 // O^T += V^T P^T as it stands.
 #include "gdn_attn.h"
 
+#ifndef FRESH
+#define FRESH fresh
+#endif
 namespace omx {
 namespace {
 
@@ -27,6 +30,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
 
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5, c = l & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const AttnLane lane = attn_lane<DP>();
   const int G = p.G, D = p.D, Hkv = p.Hkv, per = kBM / G;
 
   int unit, rank;
@@ -155,12 +159,13 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   auto compute = [&](int kt, const bf16_t* sk, const bf16_t* sv, unsigned have) {
     const int key0 = kt * kBN;
     if (key0 > w_hi) return;  // uniform in the wavefront: no row of it sees these keys
+    const AttnLane ln = FRESH(lane);
     f32x16 s[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       s[b] = zero16();
 #pragma unroll
-      for (int k = 0; k < KS; ++k) s[b] = mma32(attn_frag<DP>(sk, 32 * b, k), q[k], s[b]);
+      for (int k = 0; k < KS; ++k) s[b] = mma32(attn_frag<DP>(sk, ln, 32 * b, k), q[k], s[b]);
     }
     if (key0 + kBN - 1 > w_lo || have != 15) {
 #pragma unroll
@@ -206,7 +211,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
         const u32x4 pb = pack8_of(s[b], k);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
-          o[d] = mma32(attn_frag_tr<DP>(sv, 32 * b + 16 * k, d), pb, o[d]);
+          o[d] = mma32(attn_frag_tr<DP>(sv, ln, 32 * b + 16 * k, d), pb, o[d]);
       }
   };
 

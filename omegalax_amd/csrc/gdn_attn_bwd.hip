@@ -9,22 +9,13 @@
 // tile of keys (dk, dv).  The scores and do . v are formed in both, 7 products in place of 5.
 #include "gdn_attn.h"
 
+#ifndef FRESH
+#define FRESH fresh
+#endif
 namespace omx {
 namespace {
 
 constexpr int kNW = 4, kNT = 64 * kNW, kBM = 128, kBN = 64;
-
-// the same column in fp32, as one of the shares of a sum
-template <int DB>
-__device__ __forceinline__ void store_part(float* row, const f32x16 (&x)[DB], float f, int D, int h) {
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int col = 32 * d + 8 * g + 4 * h;
-      if (col < D) *(f32x4*)(row + col) = f32x4{x[d][4 * g] * f, x[d][4 * g + 1] * f, x[d][4 * g + 2] * f, x[d][4 * g + 3] * f};
-    }
-}
 
 // sum of the products of two rows' 8 bf16 elements
 __device__ __forceinline__ float dot8(u32x4 a, u32x4 b) {
@@ -46,6 +37,7 @@ void attn_dq_kernel(AttnParams p, int ranks) {
 
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5, c = l & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const AttnLane lane = attn_lane<DP>();
   const int G = p.G, D = p.D, Hkv = p.Hkv, Hq = Hkv * G, per = kBM / G;
 
   int unit, rank;
@@ -76,7 +68,11 @@ void attn_dq_kernel(AttnParams p, int ranks) {
   }
   delta = sum_halves(delta);
   const float lse2 = live ? p.lse[at] * kLog2e : INFINITY;  // idle rows: weights of 0
-  if (live && h == 0) p.delta[at] = delta;
+  if (live && h == 0) {
+    float* st = p.stats + 2 * (tok * Hq + hk * G) + rg;
+    st[0] = lse2;
+    st[G] = -delta;
+  }
 
   f32x16 dq[DB];
 #pragma unroll
@@ -112,11 +108,12 @@ void attn_dq_kernel(AttnParams p, int ranks) {
     if (key0 > w_hi) return;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
+      const AttnLane ln = FRESH(lane);
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-      for (int k = 0; k < KS; ++k) s = mma32(attn_frag<DP>(sk, 32 * b, k), q[k], s);
+      for (int k = 0; k < KS; ++k) s = mma32(attn_frag<DP>(sk, ln, 32 * b, k), q[k], s);
 #pragma unroll
-      for (int k = 0; k < KS; ++k) dp = mma32(attn_frag<DP>(sv, 32 * b, k), dout[k], dp);
+      for (int k = 0; k < KS; ++k) dp = mma32(attn_frag<DP>(sv, ln, 32 * b, k), dout[k], dp);
       if (key0 + 32 * b + 31 > w_lo) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -131,7 +128,7 @@ void attn_dq_kernel(AttnParams p, int ranks) {
       for (int k = 0; k < 2; ++k) {
         const u32x4 ds = pack8_of(s, k);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) dq[d] = mma32(attn_frag_tr<DP>(sk, 32 * b + 16 * k, d), ds, dq[d]);
+        for (int d = 0; d < DB; ++d) dq[d] = mma32(attn_frag_tr<DP>(sk, ln, 32 * b + 16 * k, d), ds, dq[d]);
       }
     }
   };
@@ -150,26 +147,26 @@ void attn_dq_kernel(AttnParams p, int ranks) {
   if (live) store_rows<DB>((bf16_t*)p.dq + at * D, dq, p.scale, D, h);
 }
 
-// ------------------------------------------------------------------------------------ dk, dv
-constexpr int kKeys = 32 * kNW;  // keys of a workgroup's tile
-constexpr int kRows = 64;        // rows of a stage
-
-template <int DP, bool DK, bool DV>
-__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 || (DK && DV) ? 1 : 2)))
-void attn_dkv_kernel(AttnParams p, int ranks) {
+// The same for heads of 256, ...
+constexpr int kWideRows = 64;
+template <int DP, int KB, bool DK, bool DV>
+__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 || (DK && DV) || KB > 1 ? 1 : 2)))
+void attn_dkv_wide_kernel(AttnParams p, int ranks) {
   constexpr int KS = DP / 16, DB = DP / 32;
-  constexpr int NJ = kRows * DP / 8 / 64 / kNW;
-  __shared__ __align__(16) bf16_t sQ0[kRows * DP], sQ1[kRows * DP], sO0[kRows * DP], sO1[kRows * DP];
-  __shared__ __align__(16) float sS0[2 * kRows], sS1[2 * kRows];  // lse and delta of a stage's rows
+  constexpr int NJ = kWideRows * DP / 8 / 64 / kNW;
+  __shared__ __align__(16) bf16_t sQ0[kWideRows * DP], sQ1[kWideRows * DP], sO0[kWideRows * DP], sO1[kWideRows * DP];
+  __shared__ __align__(16) float sS0[2 * kWideRows], sS1[2 * kWideRows];  // lse and delta of a stage's rows
 
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5, c = l & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = p.G, D = p.D, Hkv = p.Hkv, Hq = Hkv * G, per = kRows / G;
+  const AttnLane lane = attn_lane<DP>();
+  const int G = p.G, D = p.D, Hkv = p.Hkv, Hq = Hkv * G, per = kWideRows / G;
 
   int unit, rank;
   attn_place((int)blockIdx.x, (p.cu ? 1 : p.N) * Hkv, ranks, unit, rank);
   if (rank >= ranks) return;
   const int hk = unit % Hkv;
+  constexpr int kKeys = kDkvKeys;
   AttnTile it;
   if (!attn_tile(p, unit / Hkv, rank, kKeys, it)) return;
   // the first tiles' keys are seen by most rows: those first
@@ -182,23 +179,32 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
     ta = first < n ? k0 + first * per : it.len;
     tb = first + each < n ? ta + each * per : it.len;
   }
-  const int key = k0 + 32 * w + c;
-  const bool live = key < it.len;
-  const long long tok = it.start + key;
+  const int kw = k0 + 32 * KB * w;  // the wavefront's first key
 
-  u32x4 kf[KS], vf[KS];
+  // with two blocks of keys a wavefront, v stays in LDS: its fragments would not fit beside the
+  // sums, and two blocks a read of q and do leave the LDS time for them
+  constexpr bool VL = KB == 2 && DP == 128;
+  __shared__ __align__(16) bf16_t sV[VL ? kKeys * DP : 8];
+  u32x4 kf[KB][KS], vf[KB][KS];
+  f32x16 dk[KB][DB], dv[KB][DB];
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int d = 16 * s + 8 * h;
-    kf[s] = vf[s] = u32x4{0, 0, 0, 0};
-    if (live && d < D) {
-      kf[s] = *(const u32x4*)((const bf16_t*)p.k + tok * p.k_ld + hk * D + d);
-      if constexpr (DK) vf[s] = *(const u32x4*)((const bf16_t*)p.v + tok * p.v_ld + hk * D + d);
+  for (int b = 0; b < KB; ++b) {
+    const int key = kw + 32 * b + c;
+    const long long tok = it.start + key;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = 16 * s + 8 * h;
+      kf[b][s] = vf[b][s] = u32x4{0, 0, 0, 0};
+      if (key < it.len && d < D) {
+        kf[b][s] = *(const u32x4*)((const bf16_t*)p.k + tok * p.k_ld + hk * D + d);
+        if constexpr (DK) vf[b][s] = *(const u32x4*)((const bf16_t*)p.v + tok * p.v_ld + hk * D + d);
+      }
+      if constexpr (VL)  // read back by this wavefront alone
+        *(u32x4*)(sV + (32 * (KB * w + b) + c) * DP + (((2 * s + h) ^ attn_swz<DP>(c)) << 3)) = vf[b][s];
     }
-  }
-  f32x16 dk[DB], dv[DB];
 #pragma unroll
-  for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
+    for (int d = 0; d < DB; ++d) dk[b][d] = dv[b][d] = zero16();
+  }
   const float cs = p.scale * kLog2e;
 
   const unsigned qld2 = (unsigned)(p.q_ld * 2), old2 = (unsigned)(Hq * D * 2);
@@ -211,7 +217,7 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
     qoff[j] = in ? (unsigned)t * qld2 + x : kDropOffset;
     ooff[j] = in ? (unsigned)t * old2 + x : kDropOffset;
   }
-  const unsigned soff = l / G < per ? (unsigned)(l / G) * 4u * Hq + 4u * (unsigned)(l % G) : kDropOffset;
+  const unsigned soff = l / G < per ? (unsigned)(l / G) * 8u * Hq + 4u * (unsigned)(l % G) : kDropOffset;
   auto stage = [&](int t, bf16_t* sq, bf16_t* so, float* ss) {
     const int left = it.len - t, n = left < per ? left : per;  // rows past the sequence read as
     const long long a = it.start + t;                          //   zeros: they add nothing
@@ -226,45 +232,80 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(dr, (lds_void*)(so + 512 * i), 16, y, 0, 0, 0);
     }
     if (w < 2) {
-      const auto sr = buf_rsrc((w ? p.delta : p.lse) + a * Hq + hk * G, (unsigned)(n - 1) * 4u * Hq + 4u * G);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_void*)(ss + kRows * w), 4, soff, 0, 0, 0);
+      const auto sr = buf_rsrc(p.stats + 2 * (a * Hq + hk * G) + w * G, (unsigned)(n - 1) * 8u * Hq + 4u * G);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_void*)(ss + kWideRows * w), 4, soff, 0, 0, 0);
     }
   };
   auto compute = [&](int t, const bf16_t* sq, const bf16_t* so, const float* ss) {
-    const int kw = k0 + 32 * w;
     if (t + per <= kw) return;  // every row is before every key of the wavefront
+#ifdef U1
+#pragma unroll 1
+#else
 #pragma unroll
-    for (int rb = 0; rb < kRows / 32; ++rb) {
-      f32x16 s = zero16(), dp = zero16();
+#endif
+    for (int rb = 0; rb < kWideRows / 32; ++rb) {
+      const AttnLane ln = FRESH(lane);
+      f32x16 s[KB], dp[KB];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) s = mma32(attn_frag<DP>(sq, 32 * rb, k), kf[k], s);
+      for (int b = 0; b < KB; ++b) s[b] = dp[b] = zero16();
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
-        if constexpr (DK) dp = mma32(attn_frag<DP>(so, 32 * rb, k), vf[k], dp);
-      if (t < kw + 31) {  // row r is token t + r / G: before the key if r < (key - t) G
-        const int first = (key - t) * G;
+      for (int k = 0; k < KS; ++k) {
+        const u32x4 a = attn_frag<DP>(sq, ln, 32 * rb, k);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (32 * rb + 8 * (i / 4) + 4 * h + i % 4 < first) s[i] = -INFINITY;
+        for (int b = 0; b < KB; ++b) s[b] = mma32(a, kf[b][k], s[b]);
       }
-      f32x16 ds;
+      if constexpr (DK) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const u32x4 a = attn_frag<DP>(so, ln, 32 * rb, k);
+#pragma unroll
+          for (int b = 0; b < KB; ++b)
+            dp[b] = mma32(a, VL ? attn_frag<DP>(sV, ln, 32 * (KB * w + b), k) : vf[b][k], dp[b]);
+        }
+      }
+      if (t < kw + 32 * KB - 1) {  // row r is token t + r / G: before the key if r < (key - t) G
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          const int first = (kw + 32 * b + c - t) * G;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * rb + 8 * (i / 4) + 4 * h + i % 4 < first) s[b][i] = -INFINITY;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const f32x4 lse = *(const f32x4*)(ss + 32 * rb + 8 * j + 4 * h);
-        const f32x4 del = *(const f32x4*)(ss + kRows + 32 * rb + 8 * j + 4 * h);
+        const f32x4 del = *(const f32x4*)(ss + kWideRows + 32 * rb + 8 * j + 4 * h);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], cs, -lse[i] * kLog2e));
-          ds[4 * j + i] = s[4 * j + i] * (dp[4 * j + i] - del[i]);
+          const float l2 = lse[i];
+#pragma unroll
+          for (int b = 0; b < KB; ++b) {
+            s[b][4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[b][4 * j + i], cs, -l2));
+            if constexpr (DK) dp[b][4 * j + i] = s[b][4 * j + i] * (dp[b][4 * j + i] + del[i]);
+          }
         }
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const u32x4 pb = pack8_of(s, k), db = pack8_of(ds, k);
+        u32x4 pb[KB], db[KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          if constexpr (DV) pb[b] = pack8_of(s[b], k);
+          if constexpr (DK) db[b] = pack8_of(dp[b], k);
+        }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          if constexpr (DV) dv[d] = mma32(attn_frag_tr<DP>(so, 32 * rb + 16 * k, d), pb, dv[d]);
-          if constexpr (DK) dk[d] = mma32(attn_frag_tr<DP>(sq, 32 * rb + 16 * k, d), db, dk[d]);
+          if constexpr (DV) {
+            const u32x4 a = attn_frag_tr<DP>(so, ln, 32 * rb + 16 * k, d);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) dv[b][d] = mma32(a, pb[b], dv[b][d]);
+          }
+          if constexpr (DK) {
+            const u32x4 a = attn_frag_tr<DP>(sq, ln, 32 * rb + 16 * k, d);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) dk[b][d] = mma32(a, db[b], dk[b][d]);
+          }
         }
       }
     }
@@ -286,15 +327,19 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
       compute(t - per, sQ1, sO1, sS1);
     }
   }
-  if (!live) return;
-  const long long at = (tok * Hkv + hk) * D;
-  if (p.splits > 1) {
-    const long long ps = (long long)blockIdx.y * p.tokens * Hkv * D + at;
-    if constexpr (DK) store_part<DB>(p.part_k + ps, dk, p.scale, D, h);
-    if constexpr (DV) store_part<DB>(p.part_v + ps, dv, 1.f, D, h);
-  } else {
-    if constexpr (DK) store_rows<DB>((bf16_t*)p.dk + at, dk, p.scale, D, h);
-    if constexpr (DV) store_rows<DB>((bf16_t*)p.dv + at, dv, 1.f, D, h);
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    const int key = kw + 32 * b + c;
+    if (key >= it.len) continue;
+    const long long at = ((it.start + key) * Hkv + hk) * D;
+    if (p.splits > 1) {
+      const long long ps = (long long)blockIdx.y * p.tokens * Hkv * D + at;
+      if constexpr (DK) store_part<DB>(p.part_k + ps, dk[b], p.scale, D, h);
+      if constexpr (DV) store_part<DB>(p.part_v + ps, dv[b], 1.f, D, h);
+    } else {
+      if constexpr (DK) store_rows<DB>((bf16_t*)p.dk + at, dk[b], p.scale, D, h);
+      if constexpr (DV) store_rows<DB>((bf16_t*)p.dv + at, dv[b], 1.f, D, h);
+    }
   }
 }
 
@@ -316,15 +361,9 @@ __global__ __launch_bounds__(256) void attn_dkv_sum_kernel(const float* pk, cons
       u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
 }
 
-template <int DP>
-void dkv(const AttnParams& p, int ranks, dim3 grid, hipStream_t stream) {
-  attn_dkv_kernel<DP, false, true><<<grid, kNT, 0, stream>>>(p, ranks);
-  attn_dkv_kernel<DP, true, false><<<grid, kNT, 0, stream>>>(p, ranks);
-}
-
 }  // namespace
 
-int attn_dkv_tile_tokens() { return kKeys; }
+int attn_dkv_tile_tokens() { return kDkvKeys; }
 
 hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream) {
   const long long ranks = attn_ranks(p, kBM / p.G), units = (long long)(p.cu ? 1 : p.N) * p.Hkv;
@@ -337,19 +376,20 @@ hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream) {
 
 int attn_dkv_splits(long long units, long long T, long long N, int G) {
   // two workgroups for each compute unit, and no share below eight stages of rows on average
-  const long long tiles = units * ((T + kKeys - 1) / kKeys + (N > 0 ? N - 1 : 0));
-  const long long most = T / (N > 0 ? N : 1) * G / (8 * kRows);
+  const long long tiles = units * ((T + kDkvKeys - 1) / kDkvKeys + (N > 0 ? N - 1 : 0));
+  const long long most = T / (N > 0 ? N : 1) * G / (8 * kWideRows);
   long long s = 512 / (tiles > 0 ? tiles : 1);
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 8 ? 8 : s));
 }
 
 hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream) {
-  const long long ranks = attn_ranks(p, kKeys), units = (long long)(p.cu ? 1 : p.N) * p.Hkv;
+  const long long ranks = attn_ranks(p, kDkvKeys), units = (long long)(p.cu ? 1 : p.N) * p.Hkv;
   const dim3 grid((unsigned)attn_grid(units, ranks), (unsigned)p.splits);
-  if (p.D <= 64) dkv<64>(p, (int)ranks, grid, stream);
-  else if (p.D <= 128) dkv<128>(p, (int)ranks, grid, stream);
-  else dkv<256>(p, (int)ranks, grid, stream);
+  if (p.D <= 128)
+    launch_attn_dkv_narrow(p, grid, (int)ranks, stream);
+  else
+    attn_dkv_wide_kernel<256, 1, true, true><<<grid, kNT, 0, stream>>>(p, (int)ranks);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   const long long n = p.tokens * p.Hkv * p.D;

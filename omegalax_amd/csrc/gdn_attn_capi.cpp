@@ -175,9 +175,9 @@ int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, 
 }
 
 namespace {
-// delta, the plans of the two kernels' tiles, dk and dv in shares
+// the rows' lse and delta, the plans of the two kernels' tiles, dk and dv in shares
 struct AttnBwdWs {
-  size_t delta;
+  size_t stats;
   PlanWs rows, keys;
   int splits;
   size_t part_k, part_v, total;
@@ -185,7 +185,7 @@ struct AttnBwdWs {
 AttnBwdWs attn_bwd_ws(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N) {
   AttnBwdWs w{};
   const int per = omx::attn_dkv_tile_tokens();
-  w.rows = plan_ws(align_up((size_t)(B * T * Hq) * 4), T, N, omx::attn_tile_tokens((int)(Hq / Hkv)));
+  w.rows = plan_ws(align_up((size_t)(B * T * Hq) * 8), T, N, omx::attn_tile_tokens((int)(Hq / Hkv)));
   w.keys = plan_ws(w.rows.total, T, N, per);
   w.splits = omx::attn_dkv_splits(B * Hkv, T, N, (int)(Hq / Hkv));
   w.part_k = w.part_v = w.total = w.keys.total;
@@ -231,7 +231,7 @@ int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, 
   p.o_rest = const_cast<void*>(o_rest);
   p.q_ld = q_ld; p.k_ld = k_ld; p.v_ld = v_ld; p.cu = cu_seqlens;
   p.dq = dq; p.dk = dk; p.dv = dv;
-  p.delta = (float*)((char*)workspace + ws.delta);
+  p.stats = (float*)((char*)workspace + ws.stats);
   p.part_k = (float*)((char*)workspace + ws.part_k);
   p.part_v = (float*)((char*)workspace + ws.part_v);
   p.splits = ws.splits;

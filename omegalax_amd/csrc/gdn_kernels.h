@@ -289,7 +289,7 @@ struct AttnParams {
   float *part_o, *part_ml;
   // backward
   const void* dout;
-  float* delta;                // [tokens, Hq] sum of dout * o
+  float* stats;                // [tokens, Hkv, 2, G]: lse / ln 2, and minus the sum of dout * o
   void *dq, *dk, *dv;
   float *part_k, *part_v;      // dk and dv in shares of the rows, when there are `splits` of them
 };
@@ -306,6 +306,7 @@ hipError_t launch_attn_join(const AttnParams& p, hipStream_t stream);
 int attn_dkv_tile_tokens();
 int attn_dkv_splits(long long units, long long T, long long N, int G);
 hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream);
+void launch_attn_dkv_narrow(const AttnParams& p, dim3 grid, int ranks, hipStream_t stream);  // D <= 128
 hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream);
 // the cache's entry points: head dims, append, decode step (splits of the keys by the number of
 // (sequence, key head) pairs and the tokens a table has room for)
