@@ -15,6 +15,8 @@ one ``attention_decode_step``.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -22,6 +24,15 @@ from .deltanet import _cu_seqlens, _ptr, _stream, _workspace
 
 __all__ = ["attention_prefill", "attention_prefill_bwd", "attention_prefill_paged",
            "attention_decode_step", "kv_pages_write"]
+
+
+_BF16 = torch.bfloat16
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, *dims):
+    """A workspace size, which depends on the arguments alone."""
+    return getattr(_lib.lib(), name)(*dims)
 
 
 def _call(dev, name, *args):
@@ -49,19 +60,20 @@ def _device(*ts):
 def _tokens(name, t, dims):
     """A bf16 tensor of token rows [..., heads, D] whose heads lie side by side, with any token
     stride the kernels take (columns of one projection); another layout is copied."""
-    if t.dim() != dims or t.dtype != torch.bfloat16:
-        raise ValueError(f"{name} must be bf16 with {dims} dimensions (got {t.dtype}, {tuple(t.shape)})")
-    H, D = t.shape[-2:]
-    if t.numel() == 0:
-        return t.contiguous(), H * D
+    shape = t.shape
+    if len(shape) != dims or t.dtype is not _BF16:
+        raise ValueError(f"{name} must be bf16 with {dims} dimensions (got {t.dtype}, {tuple(shape)})")
+    H, D = shape[-2:]
+    if t.is_contiguous():
+        return (t if t.data_ptr() % 16 == 0 else t.clone()), H * D
     st = t.stride()
     # stride of a dimension of one is of no consequence
-    ld = st[-3] if t.shape[-3] > 1 else H * D
-    if dims == 4 and t.shape[1] == 1 and t.shape[0] > 1:
+    ld = st[-3] if shape[-3] > 1 else H * D
+    if dims == 4 and shape[1] == 1 and shape[0] > 1:
         ld = st[0]
     ok = (D == 1 or st[-1] == 1) and (H == 1 or st[-2] == D) and H * D <= ld <= 1 << 22
-    if dims == 4 and t.shape[0] > 1:
-        ok = ok and st[0] == t.shape[1] * ld
+    if dims == 4 and shape[0] > 1:
+        ok = ok and st[0] == shape[1] * ld
     if not (ok and ld % 8 == 0 and t.data_ptr() % 16 == 0):
         t, ld = t.contiguous(), H * D
         if t.data_ptr() % 16 != 0:
@@ -98,7 +110,7 @@ def _prefill_fwd(q, k, v, cu_seqlens, scale, with_lse, with_rest):
     o = torch.empty((B, T, Hq, D), dtype=torch.bfloat16, device=dev)
     lse = torch.empty((B, T, Hq), dtype=torch.float32, device=dev) if with_lse else None
     rest = torch.empty_like(o) if with_rest else None
-    ws_bytes = _lib.lib().omx_gdn_attn_fwd_workspace_size(T, Hq, Hkv, 0 if cu is None else N)
+    ws_bytes = _workspace_bytes("omx_gdn_attn_fwd_workspace_size", T, Hq, Hkv, 0 if cu is None else N)
     ws = _workspace(ws_bytes, dev)
     _call(dev, "omx_gdn_attn_fwd", _ptr(q), _ptr(k), _ptr(v), q_ld, k_ld, v_ld, _ptr(cu), N, _ptr(o),
           _ptr(lse), _ptr(rest), B, T, Hq, Hkv, D, _scale(scale, D), _ptr(ws), ws_bytes)
@@ -126,7 +138,7 @@ def attention_prefill_bwd(q, k, v, o, lse, do, *, o_rest=None, cu_seqlens=None, 
     dq = torch.empty((B, T, Hq, D), dtype=torch.bfloat16, device=dev)
     dk = torch.empty((B, T, Hkv, D), dtype=torch.bfloat16, device=dev)
     dv = torch.empty_like(dk)
-    ws_bytes = _lib.lib().omx_gdn_attn_bwd_workspace_size(B, T, Hq, Hkv, D, 0 if cu is None else N)
+    ws_bytes = _workspace_bytes("omx_gdn_attn_bwd_workspace_size", B, T, Hq, Hkv, D, 0 if cu is None else N)
     ws = _workspace(ws_bytes, dev)
     _call(dev, "omx_gdn_attn_bwd", _ptr(q), _ptr(k), _ptr(v), q_ld, k_ld, v_ld, _ptr(cu), N, _ptr(o),
           _ptr(lse), _ptr(o_rest), _ptr(do), _ptr(dq), _ptr(dk), _ptr(dv), B, T, Hq, Hkv, D, _scale(scale, D),
@@ -176,28 +188,29 @@ def attention_prefill(q, k, v, *, cu_seqlens=None, scale=None, output_lse=False)
 
 def _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D):
     """Checks of the cache's tensors, which are used where they lie."""
-    _device(k_pages, v_pages, block_table, lengths)
-    if k_pages.device != dev:
-        raise ValueError(f"tensors on different devices: {dev} vs {k_pages.device}")
+    for t in (k_pages, v_pages, block_table, lengths):
+        if t.device != dev:
+            _device(t)
+            raise ValueError(f"tensors on different devices: {dev} vs {t.device}")
+    shape = k_pages.shape
+    if v_pages.shape != shape or len(shape) != 4 or shape[2] != Hkv or shape[3] != D:
+        raise ValueError(f"k_pages and v_pages must both be [pages, page_size, {Hkv}, {D}] "
+                         f"(got {tuple(shape)}, {tuple(v_pages.shape)})")
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.dtype != torch.bfloat16 or t.dim() != 4 or tuple(t.shape[2:]) != (Hkv, D):
-            raise ValueError(f"{name} must be bf16 [pages, page_size, {Hkv}, {D}] "
-                             f"(got {t.dtype}, {tuple(t.shape)})")
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-    if k_pages.shape != v_pages.shape:
-        raise ValueError(f"k_pages and v_pages differ: {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != N:
+        if t.dtype is not _BF16 or not t.is_contiguous():
+            raise ValueError(f"{name} must be bf16 and contiguous (got {t.dtype})")
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != N:
         raise ValueError(f"block_table must be int32 [{N}, width] (got {block_table.dtype}, "
                          f"{tuple(block_table.shape)})")
-    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (N,):
+    if lengths.dtype is not torch.int32 or lengths.dim() != 1 or lengths.shape[0] != N:
         raise ValueError(f"lengths must be int32 [{N}] (got {lengths.dtype}, {tuple(lengths.shape)})")
-    return block_table.contiguous(), lengths.contiguous(), k_pages.shape[0], k_pages.shape[1]
+    return block_table.contiguous(), lengths.contiguous(), shape[0], shape[1]
 
 
 def _no_grad_only(name, *ts):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise ValueError(f"{name}: gradients through the cache are not supported")
+    for t in ts:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name}: gradients through the cache are not supported")
 
 
 def kv_pages_write(k, v, k_pages, v_pages, block_table, lengths, *, cu_seqlens=None):
@@ -208,10 +221,14 @@ def kv_pages_write(k, v, k_pages, v_pages, block_table, lengths, *, cu_seqlens=N
     left out.
     """
     _no_grad_only("kv_pages_write", k, v, k_pages, v_pages)
-    dev, _, k, v, _, k_ld, v_ld, cu, N = _qkv(k, k, v, cu_seqlens)
+    dev = _device(k, v)
+    (k, k_ld), (v, v_ld) = _tokens("k", k, 4), _tokens("v", v, 4)
+    if k.shape != v.shape:
+        raise ValueError(f"shape mismatch: k{tuple(k.shape)} v{tuple(v.shape)}")
     B, T, Hkv, D = k.shape
+    cu, N = (None, B) if cu_seqlens is None else _cu_seqlens(cu_seqlens, B, T, dev)
     table, lengths, pages, page = _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D)
-    ws_bytes = _lib.lib().omx_gdn_kv_write_workspace_size(T, 0 if cu is None else N)
+    ws_bytes = _workspace_bytes("omx_gdn_kv_write_workspace_size", T, 0 if cu is None else N)
     ws = _workspace(ws_bytes, dev)
     _call(dev, "omx_gdn_kv_write", _ptr(k), _ptr(v), k_ld, v_ld, _ptr(cu), N, _ptr(k_pages), _ptr(v_pages),
           pages, page, _ptr(table), table.shape[1], _ptr(lengths), B, T, Hkv, D, _ptr(ws), ws_bytes)
@@ -234,7 +251,7 @@ def attention_prefill_paged(q, k_pages, v_pages, block_table, lengths, *, cu_seq
     Hkv = k_pages.shape[2] if k_pages.dim() == 4 else 0
     table, lengths, pages, page = _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D)
     o = torch.empty((B, T, Hq, D), dtype=torch.bfloat16, device=dev)
-    ws_bytes = _lib.lib().omx_gdn_attn_paged_workspace_size(B, T, Hq, Hkv, D, N, int(cu_seqlens is not None),
+    ws_bytes = _workspace_bytes("omx_gdn_attn_paged_workspace_size", B, T, Hq, Hkv, D, N, int(cu_seqlens is not None),
                                                             page, table.shape[1])
     ws = _workspace(ws_bytes, dev)
     _call(dev, "omx_gdn_attn_paged", _ptr(q), q_ld, _ptr(cu_seqlens), N, _ptr(k_pages), _ptr(v_pages), pages,
@@ -255,7 +272,7 @@ def attention_decode_step(q, k, v, k_pages, v_pages, block_table, lengths, *, sc
     Hkv = k.shape[1]
     table, lengths, pages, page = _cache(dev, k_pages, v_pages, block_table, lengths, B, Hkv, D)
     out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=dev)
-    ws_bytes = _lib.lib().omx_gdn_attn_decode_workspace_size(B, Hq, Hkv, D, page, table.shape[1])
+    ws_bytes = _workspace_bytes("omx_gdn_attn_decode_workspace_size", B, Hq, Hkv, D, page, table.shape[1])
     ws = _workspace(ws_bytes, dev)
     _call(dev, "omx_gdn_attn_decode_step", _ptr(q), _ptr(k), _ptr(v), q_ld, k_ld, v_ld, _ptr(k_pages),
           _ptr(v_pages), pages, page, _ptr(table), table.shape[1], _ptr(lengths), _ptr(out), B, Hq, Hkv, D,

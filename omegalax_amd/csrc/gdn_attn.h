@@ -147,6 +147,15 @@ __device__ __forceinline__ void load_to_lds16(u32x4 rsrc, unsigned lds, unsigned
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory");
 }
+// two of them, the second 4 KiB on in LDS (a workgroup of four wavefronts takes turns); or one
+__device__ __forceinline__ void loads_to_lds16(u32x4 rsrc, unsigned lds, const unsigned (&off)[2]) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+               "s_add_u32 m0, m0, 4096\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off[0]), "v"(off[1]), "s"(rsrc) : "memory", "scc");
+}
+__device__ __forceinline__ void loads_to_lds16(u32x4 rsrc, unsigned lds, const unsigned (&off)[1]) {
+  load_to_lds16(rsrc, lds, off[0]);
+}
 __device__ __forceinline__ void load_to_lds4(u32x4 rsrc, unsigned lds, unsigned off) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory");

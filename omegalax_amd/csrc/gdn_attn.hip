@@ -10,26 +10,33 @@
 // O^T += V^T P^T as it stands.
 #include "gdn_attn.h"
 
-#ifndef FRESH
-#define FRESH fresh
-#endif
 namespace omx {
 namespace {
 
-constexpr int kBM = 128, kBN = 64, kNW = 4, kNT = 64 * kNW;
+constexpr int kBM = 128, kBN = 64;
 
 // m starts here: below any score, and finite, so that rows which have seen no key stay at 0
 constexpr float kLow = -1e30f;
 
+// Heads of 256 leave room for one such workgroup on a compute unit.  It then has eight wavefronts,
+// KG = 2 to each 32 rows, which take the two halves of each tile's keys and join their sums at the
+// end: two wavefronts a SIMD hide each other's latencies, as two workgroups do for smaller heads.
+constexpr int PF = 4;  // fragments read ahead of their products
+template <int DP> constexpr int kKG = DP == 256 ? 2 : 1;
+template <int DP> constexpr int kFwdNT = 256 * kKG<DP>;
+
 template <int DP, bool PAGED>
-__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
+__global__ __launch_bounds__(kFwdNT<DP>) __attribute__((amdgpu_waves_per_eu(2)))
 void attn_fwd_kernel(AttnParams p, int ranks) {
+  constexpr int KG = kKG<DP>, kNW = 4 * KG, kNT = 64 * kNW;
   constexpr int KS = DP / 16, DB = DP / 32;      // steps of a score, blocks of an output row
+  constexpr int NB = 2 / KG;                     // blocks of 32 keys that a wavefront takes of a tile
   constexpr int NJ = kBN * DP / 8 / 64 / kNW;    // staging instructions per wavefront and tile
   __shared__ __align__(16) bf16_t sK0[kBN * DP], sK1[kBN * DP], sV0[kBN * DP], sV1[kBN * DP];
 
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5, c = l & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = w & 3, b0 = (w >> 2) * NB;  // its 32 rows, its first block of keys
   const AttnLane lane = attn_lane<DP>();
   const int G = p.G, D = p.D, Hkv = p.Hkv, per = kBM / G;
 
@@ -52,12 +59,12 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   }
 
   // this lane's row
-  const int row = 32 * w + c, rt = row / G, rg = row - rt * G;
+  const int row = 32 * wr + c, rt = row / G, rg = row - rt * G;
   const bool live = rt < nt;
   const long long tok = it.start + t0 + rt;
   const int pos = held + t0 + rt;                                 // its last key
-  const int w_lo = held + t0 + (32 * w) / G;                      // the wavefront's first row's
-  const int w_hi = held + t0 + (32 * w + 31) / G;                 //   and last row's last key
+  const int w_lo = held + t0 + (32 * wr) / G;                      // the wavefront's first row's
+  const int w_hi = held + t0 + (32 * wr + 31) / G;                 //   and last row's last key
 
   u32x4 q[KS];
   {
@@ -87,14 +94,16 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   if (idle) kt1 = kt0;
 
   // ---------------------------------------------------------------- staging
-  int srow[NJ], sseg[NJ];
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    srow[j] = stage_row<DP, kNW>(w, j);
-    sseg[j] = stage_seg<DP>(srow[j]);
-  }
+  // a lane's place in a wavefront's instructions: kStep rows lie between them, over which the
+  // swizzle repeats
+  constexpr int kStep = 64 / (DP / 8) * kNW;
+  static_assert(kStep % 16 == 0, "rows whose swizzle repeats");
+  const int srow = stage_row<DP, kNW>(w, 0), sseg = stage_seg<DP>(srow);
   const unsigned kld2 = PAGED ? (unsigned)(Hkv * D * 2) : (unsigned)(p.k_ld * 2);
   const unsigned vld2 = PAGED ? (unsigned)(Hkv * D * 2) : (unsigned)(p.v_ld * 2);
+  const bool in = 8 * sseg < D;
+  const unsigned koff = in ? (unsigned)(PAGED ? srow & 15 : srow) * kld2 + 16u * (unsigned)sseg : kDropOffset;
+  const unsigned voff = in ? (unsigned)(PAGED ? srow & 15 : srow) * vld2 + 16u * (unsigned)sseg : kDropOffset;
   // the cache: page slot and offset of the next tile to stage, and the pages of its four groups
   // of 16 keys (a page is a multiple of 16 tokens), read one tile before they are used
   int slot = 0, off = 0, pid[4], poff[4];
@@ -122,34 +131,36 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       for (int g = 0; g < 4; ++g) have |= pid[g] >= 0 ? 1u << g : 0u;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const int g0 = (64 / (DP / 8)) * kNW * j / 16;  // the group of row stage_row(0, j)
+        // the group of the instruction's rows: 64 / (DP / 8) rows each, and kNW instructions a j
+        const int g0 = (64 / (DP / 8)) * kNW * j / 16;
         int id = pid[g0], of = poff[g0];
         if (DP == 64 && w >= 2) { id = pid[g0 + 1]; of = poff[g0 + 1]; }
         if (id >= 0) {
           const long long at = ((long long)id * p.page + of) * Hkv * D + hk * D;
-          const unsigned lo = (unsigned)(srow[j] & 15) * kld2 + 16u * (unsigned)sseg[j];
           const int i = w + kNW * j;
-          __builtin_amdgcn_global_load_lds((glob_void*)((const char*)((const bf16_t*)p.k_pages + at) + lo),
+          __builtin_amdgcn_global_load_lds((glob_void*)((const char*)((const bf16_t*)p.k_pages + at) + koff),
                                            (lds_void*)(sk + 512 * i), 16, 0, 0);
-          __builtin_amdgcn_global_load_lds((glob_void*)((const char*)((const bf16_t*)p.v_pages + at) + lo),
+          __builtin_amdgcn_global_load_lds((glob_void*)((const char*)((const bf16_t*)p.v_pages + at) + voff),
                                            (lds_void*)(sv + 512 * i), 16, 0, 0);
         }
       }
     } else {
-      const int left = it.len - kt * kBN, n = left < kBN ? left : kBN;  // rows past the sequence
-      const long long at = it.start + (long long)kt * kBN;              //   read as zeros
-      const auto kr = buf_rsrc((const bf16_t*)p.k + at * p.k_ld + hk * D, (unsigned)(n - 1) * kld2 + 2u * D);
-      const auto vr = buf_rsrc((const bf16_t*)p.v + at * p.v_ld + hk * D, (unsigned)(n - 1) * vld2 + 2u * D);
+      const long long at = it.start + (long long)kt * kBN;
+      const bf16_t* ka = (const bf16_t*)p.k + at * p.k_ld + hk * D;
+      const bf16_t* va = (const bf16_t*)p.v + at * p.v_ld + hk * D;
+      int left = it.len - kt * kBN;  // rows past the sequence read as zeros
+      left = left < kBN ? left : kBN;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int i = w + kNW * j;
-        const bool in = 8 * sseg[j] < D;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            kr, (lds_void*)(sk + 512 * i), 16,
-            in ? (unsigned)srow[j] * kld2 + 16u * (unsigned)sseg[j] : kDropOffset, 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            vr, (lds_void*)(sv + 512 * i), 16,
-            in ? (unsigned)srow[j] * vld2 + 16u * (unsigned)sseg[j] : kDropOffset, 0, 0, 0);
+        const auto kr = buf_rsrc(ka, left > 0 ? (unsigned)(left - 1) * kld2 + 2u * D : 0);
+        const auto vr = buf_rsrc(va, left > 0 ? (unsigned)(left - 1) * vld2 + 2u * D : 0);
+        const unsigned x = koff, y = voff;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void*)(sk + 512 * i), 16, x, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void*)(sv + 512 * i), 16, y, 0, 0, 0);
+        ka += kStep * p.k_ld;
+        va += kStep * p.v_ld;
+        left -= kStep;
       }
     }
     return have;
@@ -157,28 +168,37 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
 
   // ---------------------------------------------------------------- one tile of keys
   auto compute = [&](int kt, const bf16_t* sk, const bf16_t* sv, unsigned have) {
-    const int key0 = kt * kBN;
+    const int key0 = kt * kBN + 32 * b0;
     if (key0 > w_hi) return;  // uniform in the wavefront: no row of it sees these keys
-    const AttnLane ln = FRESH(lane);
-    f32x16 s[2];
+    const AttnLane ln = fresh(lane);
+    f32x16 s[NB];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      s[b] = zero16();
+    for (int b = 0; b < NB; ++b) s[b] = zero16();
+    u32x4 f[PF];
+    auto kfrag = [&](int t) { return attn_frag<DP>(sk, ln, 32 * (b0 + t % NB), t / NB); };
 #pragma unroll
-      for (int k = 0; k < KS; ++k) s[b] = mma32(attn_frag<DP>(sk, ln, 32 * b, k), q[k], s[b]);
+    for (int t = 0; t < PF; ++t) f[t] = kfrag(t);
+#pragma unroll
+    for (int t = 0; t < NB * KS; ++t) {
+      s[t % NB] = mma32(f[t % PF], q[t / NB], s[t % NB]);
+      if (t + PF < NB * KS) f[t % PF] = kfrag(t + PF);
     }
-    if (key0 + kBN - 1 > w_lo || have != 15) {
+    // the first of v's fragments arrive during the softmax
+    auto vfrag = [&](int t) { return attn_frag_tr<DP>(sv, ln, 32 * b0 + 16 * (t / DB), t % DB); };
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+    for (int t = 0; t < PF; ++t) f[t] = vfrag(t);
+    if (key0 + 32 * NB - 1 > w_lo || have != 15) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int key = key0 + 32 * b + 8 * (i / 4) + 4 * h + i % 4;
-          if (key > pos || (PAGED && !((have >> (2 * b + i / 8)) & 1))) s[b][i] = -INFINITY;
+          if (key > pos || (PAGED && !((have >> (2 * (b0 + b) + i / 8)) & 1))) s[b][i] = -INFINITY;
         }
     }
     float mx = s[0][0];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
     mx = max_halves(mx);
@@ -197,7 +217,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     const float mc = m * cs;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], cs, -mc));
@@ -205,14 +225,15 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       }
     lsum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int x = 0; x < 2 * NB; ++x) {
+      const u32x4 pb = pack8_of(s[x / 2], x % 2);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const u32x4 pb = pack8_of(s[b], k);
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-          o[d] = mma32(attn_frag_tr<DP>(sv, ln, 32 * b + 16 * k, d), pb, o[d]);
-      }
+      for (int d = 0; d < DB; ++d) {
+        const int t = x * DB + d;
+        o[d] = mma32(f[t % PF], pb, o[d]);
+        if (t + PF < 2 * NB * DB) f[t % PF] = vfrag(t + PF);
+        }
+    }
   };
 
   // rows of a staged tile that hold no key are cleared: a weight of zero does not clear them
@@ -257,6 +278,39 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
 
   // ---------------------------------------------------------------- output
   lsum = sum_halves(lsum);
+  if constexpr (KG == 2) {
+    // the second wavefront of each 32 rows hands its sums over in the buffers, 32 KiB each, an
+    // element's 16-byte pieces a lane apart
+    __shared__ float sML[2][4][32];
+    __syncthreads();
+    float* xs = (float*)(wr == 0 ? sK0 : (wr == 1 ? sK1 : (wr == 2 ? sV0 : sV1)));
+    if (w >= 4) {
+      if (h == 0) {
+        sML[0][wr][c] = m;
+        sML[1][wr][c] = lsum;
+      }
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(f32x4*)(xs + (4 * d + g) * 256 + 4 * l) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+    }
+    __syncthreads();
+    if (w >= 4) return;
+    const float m2 = sML[0][wr][c], l2 = sML[1][wr][c], mn = fmaxf(m, m2);
+    const float a1 = __builtin_amdgcn_exp2f((m - mn) * cs), a2 = __builtin_amdgcn_exp2f((m2 - mn) * cs);
+    m = mn;
+    lsum = lsum * a1 + l2 * a2;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = *(const f32x4*)(xs + (4 * d + g) * 256 + 4 * l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][4 * g + i] = o[d][4 * g + i] * a1 + x[i] * a2;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  }
   if (!live) return;
   const int Hq = Hkv * G, head = hk * G + rg;
   if (PAGED && p.splits > 1) {
@@ -451,9 +505,9 @@ hipError_t launch_attn_fwd(const AttnParams& p, hipStream_t stream) {
 #define OMX_FWD(DP)                                                                   \
   case DP:                                                                            \
     if (paged)                                                                        \
-      attn_fwd_kernel<DP, true><<<grid, kNT, 0, stream>>>(p, (int)ranks);             \
+      attn_fwd_kernel<DP, true><<<grid, kFwdNT<DP>, 0, stream>>>(p, (int)ranks);             \
     else                                                                              \
-      attn_fwd_kernel<DP, false><<<grid, kNT, 0, stream>>>(p, (int)ranks);            \
+      attn_fwd_kernel<DP, false><<<grid, kFwdNT<DP>, 0, stream>>>(p, (int)ranks);            \
     break;
     OMX_FWD(64)
     OMX_FWD(128)

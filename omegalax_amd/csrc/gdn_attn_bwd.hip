@@ -375,10 +375,10 @@ hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream) {
 }
 
 int attn_dkv_splits(long long units, long long T, long long N, int G) {
-  // two workgroups for each compute unit, and no share below eight stages of rows on average
+  // a workgroup for each compute unit, and no share below eight stages of rows on average
   const long long tiles = units * ((T + kDkvKeys - 1) / kDkvKeys + (N > 0 ? N - 1 : 0));
   const long long most = T / (N > 0 ? N : 1) * G / (8 * kWideRows);
-  long long s = 512 / (tiles > 0 ? tiles : 1);
+  long long s = 256 / (tiles > 0 ? tiles : 1);
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 8 ? 8 : s));
 }

@@ -339,10 +339,17 @@ int omx_gdn_attn_paged(const void* q, int64_t q_ld, const int32_t* cu_seqlens, i
   return launch_status(e, fn);
 }
 
+namespace {
+SplitWs decode_ws(int splits, int64_t B, int64_t Hq, int64_t D) {
+  // (one count of splits + B segments, of one row a head each)
+  return splits > 1 ? split_ws(0, splits + (int)B, Hq, D) : split_ws(0, 1, 0, D);
+}
+}  // namespace
+
 size_t omx_gdn_attn_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t page_size,
                                           int64_t table_width) {
-  if (B < 0 || Hq < 1 || Hkv < 1 || D < 1 || page_size < 1 || table_width < 0) return 0;
-  return split_ws(0, B == 0 ? 1 : omx::decode_splits(B * Hkv, page_size * table_width), B * Hq, D).total;
+  if (B < 1 || Hq < 1 || Hkv < 1 || D < 1 || page_size < 1 || table_width < 0) return 0;
+  return decode_ws(omx::decode_splits(B, Hkv, D, page_size * table_width), B, Hq, D).total;
 }
 
 int omx_gdn_attn_decode_step(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
@@ -358,12 +365,12 @@ int omx_gdn_attn_decode_step(const void* q, const void* k, const void* v, int64_
   if (!rc) rc = check_ld(fn, "v_ld", v_ld, Hkv * D);
   if (!rc) rc = check_scale(fn, scale);
   if (rc) return rc;
-  REQUIRE(B <= 65535 * 16, "%s: batch %lld out of range", fn, (long long)B);
+  REQUIRE(B <= 65535 * 16 && B * Hq <= INT_MAX / 4, "%s: batch %lld out of range", fn, (long long)B);
   if (B == 0) return ok();
   rc = check_cache(fn, k_pages, v_pages, n_pages, page_size, block_table, table_width, lengths, D, Hkv);
   if (rc) return rc;
-  const int splits = omx::decode_splits(B * Hkv, page_size * table_width);
-  const SplitWs ws = split_ws(0, splits, B * Hq, D);
+  const int splits = omx::decode_splits(B, Hkv, D, page_size * table_width);
+  const SplitWs ws = decode_ws(splits, B, Hq, D);
   REQUIRE(workspace_bytes >= ws.total, "%s: workspace of %zu bytes is smaller than the %zu needed", fn,
           workspace_bytes, ws.total);
   REQUIRE(q && k && v && out, "%s: a required pointer is NULL", fn);

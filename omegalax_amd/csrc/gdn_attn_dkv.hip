@@ -105,11 +105,11 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
   unsigned o_range = n > 0 ? (unsigned)(m0 - 1) * old2 + 2u * D * G : 0;
   unsigned s_range = n > 0 ? (unsigned)(m0 - 1) * 8u * Hq + 8u * G : 0;
   const unsigned lds0 = lds_address(ring);
-  auto stage_q = [&](int slot, int j) {
-    load_to_lds16(rsrc_words(q_at, q_range), lds0 + 2u * kSlot * (unsigned)slot + 1024u * (unsigned)(w + kNW * j), qoff[j]);
+  auto stage_q = [&](int slot) {
+    loads_to_lds16(rsrc_words(q_at, q_range), lds0 + 2u * kSlot * (unsigned)slot + 1024u * (unsigned)w, qoff);
   };
-  auto stage_o = [&](int slot, int j) {
-    load_to_lds16(rsrc_words(o_at, o_range), lds0 + 2u * (kSlot * (unsigned)slot + kDo) + 1024u * (unsigned)(w + kNW * j), ooff[j]);
+  auto stage_o = [&](int slot) {
+    loads_to_lds16(rsrc_words(o_at, o_range), lds0 + 2u * (kSlot * (unsigned)slot + kDo) + 1024u * (unsigned)w, ooff);
   };
   auto stage_s = [&](int slot) { load_to_lds4(rsrc_words(s_at, s_range), lds0 + 2u * (kSlot * (unsigned)slot + kStats), soff); };
   auto stage_next = [&](bool more) {
@@ -121,11 +121,8 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
     s_range = more ? s_all : 0;
   };
   auto stage = [&](bool more, int slot) {
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      stage_q(slot, j);
-      stage_o(slot, j);
-    }
+    stage_q(slot);
+    stage_o(slot);
     stage_s(slot);
     stage_next(more);
   };
@@ -185,11 +182,10 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
         fq[g / 2] = attn_frag<DP>(st2, lane, 0, g / 2);
       if (g % (NG / 4) == 0) row_lse(st1, g / (NG / 4));
       if (g % (NG / 4) == 1) row_delta(dp, st2, g / (NG / 4));
-      if (g < 2 * NJ) {
-        if (g & 1) stage_o(fetch, g / 2); else stage_q(fetch, g / 2);
-      }
-      if (g == 2 * NJ) stage_s(fetch);
-      if (g == 2 * NJ + 1) stage_next(more);
+      if (g == 0) stage_q(fetch);
+      if (g == 3) stage_o(fetch);
+      if (g == 6) stage_s(fetch);
+      if (g == 7) stage_next(more);
       __builtin_amdgcn_sched_barrier(0);
     }
   };

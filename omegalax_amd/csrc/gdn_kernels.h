@@ -308,11 +308,11 @@ int attn_dkv_splits(long long units, long long T, long long N, int G);
 hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream);
 void launch_attn_dkv_narrow(const AttnParams& p, dim3 grid, int ranks, hipStream_t stream);  // D <= 128
 hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream);
-// the cache's entry points: head dims, append, decode step (splits of the keys by the number of
-// (sequence, key head) pairs and the tokens a table has room for)
+// the cache's entry points: head dims, append, decode step (`splits` workgroups a key head share
+// the keys, by the tokens a table has room for; its partial sums are of splits + N segments)
 bool paged_dims_supported(int D);
 hipError_t launch_kv_write(const AttnParams& p, hipStream_t stream);
-int decode_splits(long long units, long long capacity);
+int decode_splits(long long N, long long Hkv, long long D, long long capacity);
 hipError_t launch_attn_decode(const AttnParams& p, hipStream_t stream);
 
 }  // namespace omx

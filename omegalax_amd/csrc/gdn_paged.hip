@@ -1,4 +1,6 @@
 // The paged key-value cache: the append of new tokens and the decode step of one token a sequence.
+#include <climits>
+
 #include "gdn_attn.h"
 
 namespace omx {
@@ -71,13 +73,48 @@ __global__ __launch_bounds__(256) void kv_write_kernel(AttnParams p) {
 }
 
 // ------------------------------------------------------------------------------------ decode
-// One workgroup takes a sequence's key head, or a share of its keys (`splits` of them); its four
-// wavefronts take turns at stages of 8192 / DP keys... each with its own LDS buffers and no
-// barrier between stages.  Keys and values go from memory to LDS without passing registers, two
-// stages deep (128 KiB in flight a compute unit), and are read once for all query heads, which
-// are the columns of 16x16 products: S^T = K Q^T, O^T += V^T P^T.
+// A workgroup's four wavefronts take turns at stages of a sequence's keys, each with its own LDS
+// buffers and no barrier between stages.  Keys and values go from memory to LDS without passing
+// registers, two stages deep (128 KiB in flight a compute unit), and are read once for all query
+// heads of a key head, which are the columns of 16x16 products: S^T = K Q^T, O^T += V^T P^T.
+// Bound by reading the cache.
+//
+// With `splits` = 1 a workgroup takes one sequence's key head.  Otherwise each key head has `splits`
+// workgroups, and the sequences' stages, laid end to end, are cut into as many equal ranges: lengths
+// may differ as they like, and all workgroups still end together.  A range's part of one sequence
+// is a segment; workgroup w's of sequence b is kept at w + b (a staircase: each next segment has
+// the next w or the next b), and the join adds up a sequence's.  A sequence in one segment needs none.
 constexpr int kDecNW = 4;
 template <int DP> constexpr int kStageKeys = 4096 / DP;  // 64, 32, 16 keys: 8 KiB of each of K, V
+
+// stages of a sequence, one at least: it writes the output
+__device__ __forceinline__ int stages_of(int held, int cap, int sk) {
+  const int keys = held < 0 ? 0 : (held < cap ? held + 1 : cap);
+  const int n = (keys + sk - 1) / sk;
+  return n < 1 ? 1 : n;
+}
+
+// inclusive sum over the lanes
+__device__ __forceinline__ int wave_scan(int v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(v, o, 64);
+    if (lane_id() >= o) v += x;
+  }
+  return v;
+}
+
+// stages of each range: equal shares, but no less than two stages a wavefront
+__device__ __forceinline__ int range_stages(int all, int splits) {
+  const int per = (all + splits - 1) / splits;
+  return per > 2 * kDecNW ? per : 2 * kDecNW;
+}
+
+__device__ __forceinline__ int wave_total(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return __builtin_amdgcn_readfirstlane(v);
+}
 
 template <int DP, int NQ>
 __global__ __launch_bounds__(64 * kDecNW) __attribute__((amdgpu_waves_per_eu(1)))
@@ -93,15 +130,44 @@ void attn_decode_kernel(AttnParams p) {
   const int tid = threadIdx.x, l = tid & 63, g4 = l >> 4, r = l & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.G, Hkv = p.Hkv, Hq = Hkv * G;
-  const int b = (int)blockIdx.x / Hkv, hk = (int)blockIdx.x % Hkv, split = (int)blockIdx.y;
+  const int hk = (int)blockIdx.x % Hkv, wg = (int)blockIdx.x / Hkv;
   const int cap = p.table_w * p.page;
+
+  // the range: stages [x, x1) of all sequences', from stage st0 of sequence b on
+  int b = wg, st0 = 0, x = 0, x1 = INT_MAX;
+  if (p.splits > 1) {
+    // lane n holds the stages of sequence n, n + 64, ..: the first 64 are read once
+    const int v0 = l < p.N ? stages_of(p.held[l], cap, SK) : 0;
+    int v = v0;
+    for (int n = l + 64; n < p.N; n += 64) v += stages_of(p.held[n], cap, SK);
+    const int all = wave_total(v), per = range_stages(all, p.splits);
+    if ((long long)wg * per >= all) return;
+    x = wg * per;
+    x1 = x + per < all ? x + per : all;
+    v = v0;
+    for (int n0 = 0, base = 0;;) {  // x < all: some 64 sequences hold it
+      const int upto = base + wave_scan(v);
+      const unsigned long long past = __ballot(upto > x);
+      if (past) {
+        const int s = __ffsll(past) - 1;
+        b = n0 + s;
+        st0 = x - __builtin_amdgcn_readlane(upto - v, s);
+        break;
+      }
+      base = __builtin_amdgcn_readlane(upto, 63);
+      n0 += 64;
+      v = n0 + l < p.N ? stages_of(p.held[n0 + l], cap, SK) : 0;
+    }
+  }
+
+  for (;;) {  // a segment a turn
   const_i32* table = (const_i32*)(p.table + (long long)b * p.table_w);
   const int held = ((const_i32*)p.held)[b];
   // keys: those held and the new one, at position `held`; past the table there is no room for it
   const int keys = held < 0 ? 0 : (held < cap ? held + 1 : cap);
-  const int nst = (keys + SK - 1) / SK, each = (nst + p.splits - 1) / p.splits;
-  const int st0 = split * each < nst ? split * each : nst;
-  const int st1 = st0 + each < nst ? st0 + each : nst;
+  const int nst = stages_of(held, cap, SK);
+  const int st1 = nst - st0 < x1 - x ? nst : st0 + (x1 - x);
+  const bool alone = st0 == 0 && st1 == nst;
 
   u32x4 q[NQ][KS];
 #pragma unroll
@@ -316,8 +382,8 @@ void attn_decode_kernel(AttnParams p) {
         acc += a * *(const f32x4*)(src + row * (DP / 2) + (col % (DP / 2)));
       }
       const long long at = (long long)b * Hq + hk * G + 16 * n + row;
-      if (p.splits > 1) {
-        const long long ps = (long long)split * p.tokens * Hq + at;
+      if (!alone) {
+        const long long ps = (long long)(wg + b) * Hq + hk * G + 16 * n + row;
         *(f32x4*)(p.part_o + ps * DP + col) = acc;
         if (col == 0) {
           p.part_ml[2 * ps] = M;
@@ -329,17 +395,101 @@ void attn_decode_kernel(AttnParams p) {
             u32x2{pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
       }
     }
-    if (n + 1 < NQ) __syncthreads();
+    __syncthreads();
   }
+  x += st1 - st0;
+  if (p.splits == 1 || x >= x1) return;
+  st0 = 0;
+  ++b;
+  }
+}
+
+// Joins a row's segments, with W of a workgroup's four wavefronts on one row.
+template <int DP, int W>
+__global__ __launch_bounds__(256) void decode_join_kernel(AttnParams p) {
+  constexpr int E = DP / 64, SK = kStageKeys<DP>;
+  typedef float fE __attribute__((ext_vector_type(E)));
+  __shared__ float sAcc[4][DP];
+  const int l = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % W;
+  const int Hq = p.Hkv * p.G;
+  const int rows = p.N * Hq, row = (int)blockIdx.x * (4 / W) + w / W;
+  const bool live = row < rows;
+  const int b = live ? row / Hq : 0, head = live ? row % Hq : 0;
+  const int cap = p.table_w * p.page, nst = stages_of(p.held[b], cap, SK);
+  int v = 0, y = 0;
+  for (int n = l; n < p.N; n += 64) {
+    const int x = stages_of(p.held[n], cap, SK);
+    v += x;
+    if (n < b) y += x;
+  }
+  const int before = wave_total(y), per = range_stages(wave_total(v), p.splits);
+  const int w0 = before / per, segs = live ? (before + nst - 1) / per - w0 + 1 : 1;
+  if (segs == 1 && W == 1) return;  // written already (with W > 1 a whole workgroup agrees on it below)
+  float M = -3e38f, den = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  if (segs > 1) {
+    for (int s = l; s < segs; s += 64) M = fmaxf(M, p.part_ml[2 * ((long long)(w0 + s + b) * Hq + head)]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    for (int s0 = 0; s0 < segs; s0 += 64) {  // weights a lane, then the sums, eight reads in flight
+      const int n = segs - s0 < 64 ? segs - s0 : 64;
+      float a = 0.f;
+      if (l < n) {
+        const long long at = (long long)(w0 + s0 + l + b) * Hq + head;
+        const float ls = p.part_ml[2 * at + 1];
+        a = ls == 0.f ? 0.f : __builtin_amdgcn_exp2f(p.part_ml[2 * at] - M);
+        den += a * ls;
+      }
+      for (int s = part; s < n; s += 8 * W) {
+        fE v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int su = s + W * u < n ? s + W * u : n - 1;
+          v[u] = *(const fE*)(p.part_o + ((long long)(w0 + s0 + su + b) * Hq + head) * DP + E * l);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float as = __shfl(a, (s + W * u) & 63, 64);
+          const float f = s + W * u < n ? as : 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += f * v[u][e];
+        }
+      }
+    }
+    den = wave_sum(den);
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) sAcc[w][E * l + e] = acc[e];
+    __syncthreads();
+    if (part != 0 || segs == 1) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int u = 1; u < W; ++u) acc[e] += sAcc[w + u][E * l + e];
+  }
+  const float inv = den > 0.f ? 1.f / den : (den == 0.f ? 0.f : den);
+  bf16_t* op = (bf16_t*)p.o + (long long)row * DP + E * l;
+#pragma unroll
+  for (int e = 0; e < E; ++e) op[e] = f2bf(acc[e] * inv);
 }
 
 template <int DP>
 void decode_dp(const AttnParams& p, hipStream_t stream) {
-  const dim3 grid((unsigned)(p.N * p.Hkv), (unsigned)p.splits);
+  const unsigned grid = (unsigned)((p.splits > 1 ? p.splits : p.N) * p.Hkv);
   if (p.G <= 16)
     attn_decode_kernel<DP, 1><<<grid, 64 * kDecNW, 0, stream>>>(p);
   else
     attn_decode_kernel<DP, 2><<<grid, 64 * kDecNW, 0, stream>>>(p);
+  if (p.splits == 1) return;
+  // a row has at most as many segments as its key head has workgroups; four wavefronts share a row
+  // where there are few rows
+  const unsigned rows = (unsigned)(p.N * p.Hkv * p.G);
+  if (rows <= 512)
+    decode_join_kernel<DP, 4><<<rows, 256, 0, stream>>>(p);
+  else
+    decode_join_kernel<DP, 1><<<(rows + 3) / 4, 256, 0, stream>>>(p);
 }
 
 }  // namespace
@@ -352,21 +502,23 @@ hipError_t launch_kv_write(const AttnParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-int decode_splits(long long units, long long capacity) {
-  // two workgroups' worth of keys for each compute unit, none below 256 keys
-  long long s = (512 + units - 1) / units;
-  const long long most = (capacity + 255) / 256;
-  s = s < most ? s : most;
-  return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
+int decode_splits(long long N, long long Hkv, long long D, long long capacity) {
+  // One workgroup a sequence and key head where that is enough for the chip twice over, or where a
+  // sequence is so short that the join costs more than it saves (B=1, 4 key heads of 128, 611 keys:
+  // 12.7 us in one launch, 16.8 in two; at 1,500 keys 18.9 and 16.8).  Otherwise one for each
+  // compute unit: their buffers allow no second (64 ragged sequences of 2 heads of 256: 119.6 us
+  // with two rounds of workgroups, 115.4 with one).
+  if (N * Hkv >= 512 || capacity * D <= (1 << 17)) return 1;
+  if (N * (capacity / 16 + 1) > INT_MAX) return 1;  // stages are counted in 32 bits
+  const long long s = 256 / Hkv;
+  return (int)(s < 2 ? 1 : s);
 }
 
 hipError_t launch_attn_decode(const AttnParams& p, hipStream_t stream) {
   if (p.D == 64) decode_dp<64>(p, stream);
   else if (p.D == 128) decode_dp<128>(p, stream);
   else decode_dp<256>(p, stream);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.splits == 1) return e;
-  return launch_attn_join(p, stream);
+  return hipGetLastError();
 }
 
 }  // namespace omx
