@@ -84,6 +84,15 @@ __device__ __forceinline__ void store_part(float* row, const f32x16 (&x)[DB], fl
     }
 }
 
+// s + the products of two rows' 8 bf16 elements
+__device__ __forceinline__ float dot8(u32x4 a, u32x4 b, float s) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, (uint32_t)a[i]),
+                                        __builtin_bit_cast(bf16x2_t, (uint32_t)b[i]), s, false);
+  return s;
+}
+
 // Rows of DP bf16 in LDS without padding, in 16-byte segments: segment s of row r lies at
 // s ^ swz(r).  One pass of a 16-byte read serves lanes {0-3, 12-15, 20-27} (and the rest of
 // each half), whose rows' images must differ in the 16 segments that the 64 banks hold; one
@@ -180,6 +189,34 @@ __device__ __forceinline__ int stage_seg(int row) {
   return (lane_id() % (DP / 8)) ^ attn_swz<DP>(row);
 }
 
+// Inclusive sum and maximum over the lanes of non-negative integers, by lane shifts within rows of
+// 16 and two broadcasts of a row's last lane (a few cycles each, where an exchange through LDS
+// takes a hundred), and the total.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_i(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v += dpp_i<0x111, 0xf>(v);
+  v += dpp_i<0x112, 0xf>(v);
+  v += dpp_i<0x114, 0xf>(v);
+  v += dpp_i<0x118, 0xf>(v);
+  v += dpp_i<0x142, 0xa>(v);
+  v += dpp_i<0x143, 0xc>(v);
+  return v;
+}
+__device__ __forceinline__ int wave_scan_max(int v) {
+  auto up = [&](int x) { v = x > v ? x : v; };
+  up(dpp_i<0x111, 0xf>(v));
+  up(dpp_i<0x112, 0xf>(v));
+  up(dpp_i<0x114, 0xf>(v));
+  up(dpp_i<0x118, 0xf>(v));
+  up(dpp_i<0x142, 0xa>(v));
+  up(dpp_i<0x143, 0xc>(v));
+  return v;
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
 // Which tile a workgroup takes: sequence `seq` of tokens start .. start + len, tile `tile` of
 // `tiles`.
 struct AttnTile {
@@ -187,44 +224,47 @@ struct AttnTile {
   long long start;
 };
 
-// Tile of rank `rank` of sequences packed by cu, those with most keys first (a tile's work
-// grows with its index), found by every wavefront for itself when there are at most 64
-// sequences: lane n holds sequence n.  The offsets are read as their ordered repair.
-__device__ __forceinline__ bool packed_tile(const int32_t* cu, int N, int T, int per, int rank,
-                                            AttnTile& it) {
+// Tokens a sequence has before its first tile's, in tiles: its tiles' places in the order of work.
+__device__ __forceinline__ int tiles_held(const int32_t* held, int n, int cap, int per) {
+  if (!held) return 0;
+  const int x = held[n];
+  return (x < 0 ? 0 : (x < cap ? x : cap)) / per;
+}
+
+// Tile of rank `rank` of sequences packed by cu, those with most keys first (a tile's work grows
+// with its index, from what a cache held on), found by every wavefront for itself when there are
+// at most 64 sequences: lane n holds sequence n.  The offsets are read as their ordered repair.
+__device__ __forceinline__ bool packed_tile(const int32_t* cu, const int32_t* held, int cap, int N, int T, int per,
+                                            int rank, AttnTile& it) {
   const int n = lane_id();
   int end = n + 1 < N ? cu[n + 1] : T;
   end = end < 0 ? 0 : (end > T ? T : end);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(end, o, 64);
-    if (n >= o && x > end) end = x;
-  }
+  end = wave_scan_max(end);
   const int prev = __shfl_up(end, 1, 64);
   const int start = n == 0 ? 0 : prev;
   const int len = n < N ? end - start : 0, nt = (len + per - 1) / per;
-  // at(j): tiles of index j and more
+  const int first = n < N ? tiles_held(held, n, cap, per) : 0;
+  // at(j): tiles of place j and more
   auto at = [&](int j) {
-    int v = nt > j ? nt - j : 0;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    int v = first + nt - j;
+    return wave_total(v < 0 ? 0 : (v > nt ? nt : v));
   };
   if (rank >= at(0)) return false;
-  int lo = 0, hi = (T + per - 1) / per;  // at(lo) > rank >= at(hi)
+  int lo = 0, hi = (T + per - 1) / per + (held ? cap / per : 0);  // at(lo) > rank >= at(hi)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (at(mid) > rank) lo = mid; else hi = mid;
   }
-  const int k = rank - at(lo + 1);  // the k-th of the sequences that have a tile lo
-  const unsigned long long have = __ballot(nt > lo);
+  const int k = rank - at(lo + 1);  // the k-th of the sequences that have a tile at place lo
+  const bool has = first <= lo && lo < first + nt;
+  const unsigned long long have = __ballot(has);
   const unsigned long long below = have & ((1ull << n) - 1);
-  const unsigned long long mine = __ballot(nt > lo && __popcll(below) == k);
+  const unsigned long long mine = __ballot(has && __popcll(below) == k);
   const int s = __ffsll(mine) - 1;
   it.seq = __builtin_amdgcn_readfirstlane(s);
   it.start = __builtin_amdgcn_readlane(start, it.seq);
   it.len = __builtin_amdgcn_readlane(len, it.seq);
-  it.tile = __builtin_amdgcn_readfirstlane(lo);
+  it.tile = lo - __builtin_amdgcn_readlane(first, it.seq);
   it.tiles = __builtin_amdgcn_readlane(nt, it.seq);
   return true;
 }
@@ -240,7 +280,7 @@ __device__ __forceinline__ bool attn_tile(const AttnParams& p, int row, int rank
     it.tile = it.tiles - 1 - rank;
     return it.tile >= 0;
   }
-  if (!p.plan) return packed_tile(p.cu, p.N, p.T, per, rank, it);
+  if (!p.plan) return packed_tile(p.cu, p.held, p.table_w * p.page, p.N, p.T, per, rank, it);
   // more than 64 sequences: the plan kernel's list (count, then sequence and tile per rank)
   const int32_t* plan = p.plan;
   if (rank >= __builtin_amdgcn_readfirstlane(plan[0])) return false;

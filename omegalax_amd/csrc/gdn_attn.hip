@@ -33,6 +33,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   constexpr int NB = 2 / KG;                     // blocks of 32 keys that a wavefront takes of a tile
   constexpr int NJ = kBN * DP / 8 / 64 / kNW;    // staging instructions per wavefront and tile
   __shared__ __align__(16) bf16_t sK0[kBN * DP], sK1[kBN * DP], sV0[kBN * DP], sV1[kBN * DP];
+  __shared__ float sRow[kNW][DP];  // of a row that is summed again
 
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5, c = l & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -276,6 +277,67 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     }
   }
 
+  // A weight of zero does not keep a NaN or an infinity among a tile's values from the rows that do
+  // not see it.  Rows whose sums are not finite though their weights are, are summed again over
+  // the keys that they see, one row at a time: slow, and only for values that are not finite.
+  {
+    float z = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) z = fmaf(o[d][i], 0.f, z);
+    unsigned long long bad = __ballot(live && z != 0.f && sum_halves(lsum) < INFINITY);
+    bad = (bad | bad >> 32) & 0xffffffffu;
+    while (bad) {
+      const int r = __ffsll(bad) - 1;
+      bad &= bad - 1;
+      const int row1 = 32 * wr + r, pos1 = held + t0 + row1 / G;
+      const bf16_t* q1 = (const bf16_t*)p.q + (it.start + t0 + row1 / G) * p.q_ld + (long long)(hk * G + row1 % G) * D;
+      const float m1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), r)) * cs;
+      float acc[DP / 64];
+#pragma unroll
+      for (int e = 0; e < DP / 64; ++e) acc[e] = 0.f;
+      const int last = kt1 * kBN - 1 < pos1 ? kt1 * kBN - 1 : pos1;
+      for (int k0 = kt0 * kBN; k0 <= last; k0 += 64) {  // a key a lane
+        const int key = k0 + l;
+        bool see = key <= last && (KG == 1 || ((l >> 5) & 1) == w >> 2);
+        long long at = (it.start + key) * p.k_ld + hk * D, av = (it.start + key) * p.v_ld + hk * D;
+        if constexpr (PAGED) {
+          const int sl = key / p.page;
+          const int id = see && sl < p.table_w ? table[sl] : -1;
+          see = id >= 0 && id < p.n_pages;
+          at = av = ((long long)id * p.page + (key - sl * p.page)) * Hkv * D + hk * D;
+        }
+        float s1 = 0.f;
+        if (see)
+          for (int d = 0; d < D; d += 8)
+            s1 = dot8(*(const u32x4*)(q1 + d), *(const u32x4*)((const bf16_t*)(PAGED ? p.k_pages : p.k) + at + d), s1);
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s1, cs, -m1));
+        unsigned long long seen = __ballot(see);
+        while (seen) {
+          const int j = __ffsll(seen) - 1;
+          seen &= seen - 1;
+          const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p1), j));
+          const bf16_t* vj = (const bf16_t*)(PAGED ? p.v_pages : p.v) + __shfl(av, j, 64);
+#pragma unroll
+          for (int e = 0; e < DP / 64; ++e)
+            if (64 * e + l < D) acc[e] = fmaf(pj, bf2f(vj[64 * e + l]), acc[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < DP / 64; ++e) sRow[w][64 * e + l] = acc[e];
+      wave_lds_fence();
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = sRow[w][32 * d + 8 * (i / 4) + 4 * h + i % 4];
+          o[d][i] = c == r ? x : o[d][i];
+        }
+      wave_lds_fence();
+    }
+  }
+
   // ---------------------------------------------------------------- output
   lsum = sum_halves(lsum);
   if constexpr (KG == 2) {
@@ -416,15 +478,15 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
 
 // The tile list of more than 64 packed sequences, and their repaired offsets: one workgroup.
 // plan: [count, 0, (sequence, tile) by rank], tiles with most keys first.  Tiles are counted by
-// index in kBuckets buckets of equal width, then placed bucket by bucket from the last; within a
+// place in kBuckets buckets of equal width, then placed bucket by bucket from the last; within a
 // bucket the order is of no consequence.
 constexpr int kPlanNT = 1024, kBuckets = 2048;
-__global__ __launch_bounds__(kPlanNT) void attn_plan_kernel(const int32_t* cu, int32_t* plan,
-                                                            int32_t* out, int N, int T, int per) {
+__global__ __launch_bounds__(kPlanNT) void attn_plan_kernel(const int32_t* cu, const int32_t* held, int cap,
+                                                            int32_t* plan, int32_t* out, int N, int T, int per) {
   __shared__ int sScan[kPlanNT], sCount[kBuckets];
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
   int shift = 0;
-  while (((T + per - 1) / per) >> shift >= kBuckets) ++shift;
+  while (((T + per - 1) / per + (held ? cap / per : 0)) >> shift >= kBuckets) ++shift;
   for (int i = tid; i < kBuckets; i += kPlanNT) sCount[i] = 0;
   // the ordered repair: a running maximum of the clamped offsets
   int carry = 0;
@@ -447,8 +509,8 @@ __global__ __launch_bounds__(kPlanNT) void attn_plan_kernel(const int32_t* cu, i
   if (tid == 0) out[0] = 0;
   __syncthreads();  // out is read below by other threads of this workgroup
   for (int n = w; n < N; n += kPlanNT / 64) {
-    const int nt = (out[n + 1] - out[n] + per - 1) / per;
-    for (int j = l; j < nt; j += 64) atomicAdd(&sCount[j >> shift], 1);
+    const int nt = (out[n + 1] - out[n] + per - 1) / per, first = tiles_held(held, n, cap, per);
+    for (int j = l; j < nt; j += 64) atomicAdd(&sCount[(first + j) >> shift], 1);
   }
   __syncthreads();
   // where each bucket starts: the tiles of later buckets come first
@@ -464,9 +526,9 @@ __global__ __launch_bounds__(kPlanNT) void attn_plan_kernel(const int32_t* cu, i
   }
   __syncthreads();
   for (int n = w; n < N; n += kPlanNT / 64) {
-    const int nt = (out[n + 1] - out[n] + per - 1) / per;
+    const int nt = (out[n + 1] - out[n] + per - 1) / per, first = tiles_held(held, n, cap, per);
     for (int j = l; j < nt; j += 64) {
-      const int at = atomicAdd(&sCount[j >> shift], 1);
+      const int at = atomicAdd(&sCount[(first + j) >> shift], 1);
       plan[2 + 2 * (long long)at] = n;
       plan[3 + 2 * (long long)at] = j;
     }
@@ -492,7 +554,8 @@ size_t attn_plan_words(long long T, long long N, int per) {
 }
 
 hipError_t launch_attn_plan(const AttnParams& p, int per, hipStream_t stream) {
-  attn_plan_kernel<<<1, kPlanNT, 0, stream>>>(p.cu, p.plan, p.cu_plan, p.N, p.T, per);
+  attn_plan_kernel<<<1, kPlanNT, 0, stream>>>(p.cu, p.held, p.table_w * p.page, p.plan, p.cu_plan, p.N,
+                                                    p.T, per);
   return hipGetLastError();
 }
 

@@ -17,16 +17,6 @@ namespace {
 
 constexpr int kNW = 4, kNT = 64 * kNW, kBM = 128, kBN = 64;
 
-// sum of the products of two rows' 8 bf16 elements
-__device__ __forceinline__ float dot8(u32x4 a, u32x4 b) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, (uint32_t)a[i]),
-                                        __builtin_bit_cast(bf16x2_t, (uint32_t)b[i]), s, false);
-  return s;
-}
-
 // ------------------------------------------------------------------------------------ dq
 template <int DP>
 __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
@@ -62,8 +52,8 @@ void attn_dq_kernel(AttnParams p, int ranks) {
     if (live && d < D) {
       q[s] = *(const u32x4*)((const bf16_t*)p.q + tok * p.q_ld + (long long)(hk * G + rg) * D + d);
       dout[s] = *(const u32x4*)((const bf16_t*)p.dout + at * D + d);
-      delta += dot8(dout[s], *(const u32x4*)((const bf16_t*)p.o + at * D + d));
-      if (p.o_rest) delta += dot8(dout[s], *(const u32x4*)((const bf16_t*)p.o_rest + at * D + d));
+      delta = dot8(dout[s], *(const u32x4*)((const bf16_t*)p.o + at * D + d), delta);
+      if (p.o_rest) delta = dot8(dout[s], *(const u32x4*)((const bf16_t*)p.o_rest + at * D + d), delta);
     }
   }
   delta = sum_halves(delta);

@@ -103,7 +103,7 @@ int paged_splits(int64_t N, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t cap
   const int64_t per = omx::attn_tile_tokens((int)(Hq / Hkv));
   const int64_t tiles = ((tokens + per - 1) / per + N - 1) * Hkv;
   int64_t s = tiles > 0 ? 512 / tiles : 1;
-  const int64_t most = capacity / 256;
+  const int64_t most = capacity / 128;
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 32 ? 32 : s));
 }

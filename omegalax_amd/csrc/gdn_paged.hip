@@ -27,11 +27,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(AttnParams p) {
   if (lanes) {
     end = l + 1 < p.N ? p.cu[l + 1] : p.T;
     end = end < 0 ? 0 : (end > p.T ? p.T : end);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(end, o, 64);
-      if (l >= o && x > end) end = x;
-    }
+    end = wave_scan_max(end);
   }
 #pragma unroll 1
   for (int i = 0; i < kWriteTokens; ++i) {
@@ -94,26 +90,10 @@ __device__ __forceinline__ int stages_of(int held, int cap, int sk) {
   return n < 1 ? 1 : n;
 }
 
-// inclusive sum over the lanes
-__device__ __forceinline__ int wave_scan(int v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(v, o, 64);
-    if (lane_id() >= o) v += x;
-  }
-  return v;
-}
-
 // stages of each range: equal shares, but no less than two stages a wavefront
 __device__ __forceinline__ int range_stages(int all, int splits) {
   const int per = (all + splits - 1) / splits;
   return per > 2 * kDecNW ? per : 2 * kDecNW;
-}
-
-__device__ __forceinline__ int wave_total(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return __builtin_amdgcn_readfirstlane(v);
 }
 
 template <int DP, int NQ>

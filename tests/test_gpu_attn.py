@@ -167,6 +167,34 @@ def test_a_sequence_keeps_its_infinities_to_itself():
     assert bool(outs[1][0][:, cu[1]:cu[2]].isnan().all())
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,T,at", [(4, 2, 128, 300, 170), (2, 2, 64, 130, 64), (8, 1, 256, 90, 33),
+                                           (3, 1, 80, 200, 199), (6, 2, 128, 70, 1)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_rows_before_a_token_do_not_see_its_infinities(Hq, Hkv, D, T, at, bad):
+    """Keys and values that are not finite, from one token on (a padded row's, say): the rows before
+    are those of the sequence cut off there, and the rows from there on are not finite where a
+    value is not."""
+    say(f"not finite from {at} of {T}, Hq={Hq} D={D}, {bad}")
+    q, k, v = draw(1, 1, T, Hq, D), draw(2, 1, T, Hkv, D), draw(3, 1, T, Hkv, D)
+    for keys in (False, True):
+        kb, vb = k.clone(), v.clone()
+        if keys:
+            kb[:, at:] = float("nan")
+            vb[:, at:] = bad
+        else:
+            vb[:, at:, :, 1::3] = bad  # some columns only: the others stay as they are
+        o = om.attention_prefill(q, kb, vb)
+        val, tol = one_sequence(*(t[0, :at].double() for t in (q, k, v)), 0)
+        check("rows before", o[0, :at], val["o"], tol["o"])
+        if keys:
+            assert bool(o[:, at:].isnan().all())
+        else:
+            assert not bool(o[:, at:, :, 1::3].isfinite().any())
+            val, tol = one_sequence(*(t[0].double() for t in (q, k, v)), 0)
+            for c in (0, 2):
+                check("other columns", o[0, at:, :, c::3], val["o"][at:, :, c::3], tol["o"][at:, :, c::3])
+
+
 def test_large_scores_and_scale():
     """Scores far from zero in both directions, so that the running maximum moves by a lot."""
     T, D = 300, 64

@@ -250,6 +250,22 @@ def test_pools_larger_than_32_bit_offsets():
     assert not bool(big[0][:pool - n].any())
 
 
+@pytest.mark.parametrize("held,new,D", [(0, 70, 128), (3000, 20, 64), (200, 90, 256)])
+def test_queries_before_a_token_do_not_see_its_infinities(held, new, D):
+    """The last new tokens' values are not finite; the queries before them are unharmed, over a
+    cache read at once and one read in shares."""
+    c = Cache([held], [new], 16, 2, D)
+    q, k, v = draw(1, 1, new, 4, D), draw(2, 1, new, 2, D), draw(3, 1, new, 2, D)
+    cut = new - 5
+    k[:, cut:], v[:, cut:] = NAN, float("inf")
+    om.kv_pages_write(k, v, *c.args())
+    o = om.attention_prefill_paged(q, *c.args())
+    val, tol = one_sequence(q[0, :cut].double(), torch.cat([c.keys[0], k[0, :cut]]).double(),
+                            torch.cat([c.values[0], v[0, :cut]]).double(), held)
+    check("queries before", o[0, :cut], val["o"], tol["o"])
+    assert bool(o[:, cut:].isnan().all())
+
+
 def test_shared_pages():
     """Two sequences with the same first pages."""
     c = Cache([64, 64], [5, 5], 32, 2, 64)
