@@ -156,7 +156,23 @@ __device__ __forceinline__ void load_to_lds16(u32x4 rsrc, unsigned lds, unsigned
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory");
 }
-// two of them, the second 4 KiB on in LDS (a workgroup of four wavefronts takes turns); or one
+// (from a uniform base address and a lane's offset, without a range)
+__device__ __forceinline__ void load_to_lds16(const void* base, unsigned lds, unsigned off) {
+  const unsigned long long a = (unsigned long long)base;
+  const unsigned long long u = (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)a) |
+                               (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32)) << 32;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(u) : "memory");
+}
+// several of them, each 4 KiB further in LDS: a workgroup of four wavefronts takes turns
+__device__ __forceinline__ void loads_to_lds16(u32x4 rsrc, unsigned lds, const unsigned (&off)[4]) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
+               "s_add_u32 m0, m0, 4096\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %5, 0 offen lds\n\t"
+               "s_add_u32 m0, m0, 4096\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %5, 0 offen lds\n\t"
+               "s_add_u32 m0, m0, 4096\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %5, 0 offen lds"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]),
+                  "s"(rsrc) : "memory", "scc");
+}
 __device__ __forceinline__ void loads_to_lds16(u32x4 rsrc, unsigned lds, const unsigned (&off)[2]) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
                "s_add_u32 m0, m0, 4096\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"

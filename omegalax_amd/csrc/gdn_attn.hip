@@ -18,26 +18,25 @@ constexpr int kBM = 128, kBN = 64;
 // m starts here: below any score, and finite, so that rows which have seen no key stay at 0
 constexpr float kLow = -1e30f;
 
-// Heads of 256 leave room for one such workgroup on a compute unit.  It then has eight wavefronts,
-// KG = 2 to each 32 rows, which take the two halves of each tile's keys and join their sums at the
-// end: two wavefronts a SIMD hide each other's latencies, as two workgroups do for smaller heads.
-constexpr int PF = 4;  // fragments read ahead of their products
-template <int DP> constexpr int kKG = DP == 256 ? 2 : 1;
-template <int DP> constexpr int kFwdNT = 256 * kKG<DP>;
+constexpr int kNW = 4, kNT = 64 * kNW;
+
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 
 template <int DP, bool PAGED>
-__global__ __launch_bounds__(kFwdNT<DP>) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
 void attn_fwd_kernel(AttnParams p, int ranks) {
-  constexpr int KG = kKG<DP>, kNW = 4 * KG, kNT = 64 * kNW;
   constexpr int KS = DP / 16, DB = DP / 32;      // steps of a score, blocks of an output row
-  constexpr int NB = 2 / KG;                     // blocks of 32 keys that a wavefront takes of a tile
+  constexpr int NG = 2 * KS, EG = 32 / NG;       // products of a tile's scores (and of its values)
+  constexpr int PF = 4;                          // fragments read ahead of their products
   constexpr int NJ = kBN * DP / 8 / 64 / kNW;    // staging instructions per wavefront and tile
-  __shared__ __align__(16) bf16_t sK0[kBN * DP], sK1[kBN * DP], sV0[kBN * DP], sV1[kBN * DP];
+  constexpr int kTile = kBN * DP;
+  __shared__ __align__(16) bf16_t sK[2 * kTile], sV[2 * kTile];  // two tiles each, by their parity
   __shared__ float sRow[kNW][DP];  // of a row that is summed again
 
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5, c = l & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wr = w & 3, b0 = (w >> 2) * NB;  // its 32 rows, its first block of keys
   const AttnLane lane = attn_lane<DP>();
   const int G = p.G, D = p.D, Hkv = p.Hkv, per = kBM / G;
 
@@ -60,12 +59,12 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   }
 
   // this lane's row
-  const int row = 32 * wr + c, rt = row / G, rg = row - rt * G;
+  const int row = 32 * w + c, rt = row / G, rg = row - rt * G;
   const bool live = rt < nt;
   const long long tok = it.start + t0 + rt;
   const int pos = held + t0 + rt;                                 // its last key
-  const int w_lo = held + t0 + (32 * wr) / G;                      // the wavefront's first row's
-  const int w_hi = held + t0 + (32 * wr + 31) / G;                 //   and last row's last key
+  const int w_lo = held + t0 + (32 * w) / G;                      // the wavefront's first row's
+  const int w_hi = held + t0 + (32 * w + 31) / G;                 //   and last row's last key
 
   u32x4 q[KS];
   {
@@ -95,113 +94,111 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   if (idle) kt1 = kt0;
 
   // ---------------------------------------------------------------- staging
-  // a lane's place in a wavefront's instructions: kStep rows lie between them, over which the
-  // swizzle repeats
-  constexpr int kStep = 64 / (DP / 8) * kNW;
-  static_assert(kStep % 16 == 0, "rows whose swizzle repeats");
-  const int srow = stage_row<DP, kNW>(w, 0), sseg = stage_seg<DP>(srow);
+  // a lane's place in a wavefront's instructions: kStep rows lie between them, and after NO of them
+  // (16 rows, or a multiple) the swizzle repeats
+  constexpr int kStep = 64 / (DP / 8) * kNW, NO = kStep % 16 ? 2 : 1;
+  static_assert(NO * kStep % 16 == 0, "rows whose swizzle repeats");
   const unsigned kld2 = PAGED ? (unsigned)(Hkv * D * 2) : (unsigned)(p.k_ld * 2);
   const unsigned vld2 = PAGED ? (unsigned)(Hkv * D * 2) : (unsigned)(p.v_ld * 2);
-  const bool in = 8 * sseg < D;
-  const unsigned koff = in ? (unsigned)(PAGED ? srow & 15 : srow) * kld2 + 16u * (unsigned)sseg : kDropOffset;
-  const unsigned voff = in ? (unsigned)(PAGED ? srow & 15 : srow) * vld2 + 16u * (unsigned)sseg : kDropOffset;
-  // the cache: page slot and offset of the next tile to stage, and the pages of its four groups
-  // of 16 keys (a page is a multiple of 16 tokens), read one tile before they are used
-  int slot = 0, off = 0, pid[4], poff[4];
-  // (read through the scalar cache: its wait does not touch the staging loads' counter)
+  unsigned koff[NO], voff[NO];
+#pragma unroll
+  for (int n = 0; n < NO; ++n) {
+    const int row = stage_row<DP, kNW>(w, n), seg = stage_seg<DP>(row), r = PAGED ? row & 15 : row;
+    koff[n] = 8 * seg < D ? (unsigned)r * kld2 + 16u * (unsigned)seg : kDropOffset;
+    voff[n] = 8 * seg < D ? (unsigned)r * vld2 + 16u * (unsigned)seg : kDropOffset;
+  }
+  // The cache: page slot and offset of the next tile to look up, and a tile's pages, one for each
+  // of its four groups of 16 keys (a page is a multiple of 16 tokens), -1 where there is none.
+  // They are read a tile before they are used, through the scalar cache, whose wait does not touch
+  // the staging loads' counter.
   typedef const __attribute__((address_space(4))) int32_t const_i32;
   const_i32* table = PAGED ? (const_i32*)(p.table + (long long)it.seq * p.table_w) : nullptr;
+  int slot = 0, off = 0;
+  struct Pages { int id[4], off[4]; unsigned have; };
   auto look = [&](int kt) {
+    Pages x;
+    x.have = 0;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const bool in = kt * kBN + 16 * g < keys && slot < p.table_w;
       int id = in ? table[slot] : -1;
       id = id >= p.n_pages ? -1 : id;
-      pid[g] = __builtin_amdgcn_readfirstlane(id);
-      poff[g] = off;
+      x.id[g] = __builtin_amdgcn_readfirstlane(id);
+      x.off[g] = off;
+      x.have |= x.id[g] >= 0 ? 1u << g : 0u;
       off += 16;
       if (off >= p.page) { off = 0; ++slot; }
     }
+    return x;
   };
-  // groups of a staged tile that hold keys
-  auto stage = [&](int kt, bf16_t* sk, bf16_t* sv) -> unsigned {
-    unsigned have = 15;
+  // fetches a tile of keys (or values) into LDS
+  auto stage = [&](int kt, const Pages& x, const void* pool, const void* rows, long long ld, unsigned ld2,
+                   const unsigned (&lane_off)[NO], const bf16_t* dst) {
+    const unsigned lds = lds_address(dst + (kt & 1) * kTile) + 1024u * (unsigned)w;
     if constexpr (PAGED) {
-      have = 0;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) have |= pid[g] >= 0 ? 1u << g : 0u;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        // the group of the instruction's rows: 64 / (DP / 8) rows each, and kNW instructions a j
-        const int g0 = (64 / (DP / 8)) * kNW * j / 16;
-        int id = pid[g0], of = poff[g0];
-        if (DP == 64 && w >= 2) { id = pid[g0 + 1]; of = poff[g0 + 1]; }
+        const int g0 = kStep * j / 16;  // the group of the instruction's rows
+        int id = x.id[g0], of = x.off[g0];
+        if (DP == 64 && w >= 2) { id = x.id[g0 + 1]; of = x.off[g0 + 1]; }
         if (id >= 0) {
           const long long at = ((long long)id * p.page + of) * Hkv * D + hk * D;
-          const int i = w + kNW * j;
-          __builtin_amdgcn_global_load_lds((glob_void*)((const char*)((const bf16_t*)p.k_pages + at) + koff),
-                                           (lds_void*)(sk + 512 * i), 16, 0, 0);
-          __builtin_amdgcn_global_load_lds((glob_void*)((const char*)((const bf16_t*)p.v_pages + at) + voff),
-                                           (lds_void*)(sv + 512 * i), 16, 0, 0);
+          load_to_lds16((const bf16_t*)pool + at, lds + 1024u * kNW * j, lane_off[j % NO]);
         }
       }
     } else {
-      const long long at = it.start + (long long)kt * kBN;
-      const bf16_t* ka = (const bf16_t*)p.k + at * p.k_ld + hk * D;
-      const bf16_t* va = (const bf16_t*)p.v + at * p.v_ld + hk * D;
       int left = it.len - kt * kBN;  // rows past the sequence read as zeros
       left = left < kBN ? left : kBN;
+      const u32x4 r = rsrc_words((const bf16_t*)rows + (it.start + (long long)kt * kBN) * ld + hk * D,
+                                 (unsigned)(left - 1) * ld2 + 2u * D);
+      constexpr int NL = NJ < 4 ? NJ : 4;  // instructions that follow each other closely
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int i = w + kNW * j;
-        const auto kr = buf_rsrc(ka, left > 0 ? (unsigned)(left - 1) * kld2 + 2u * D : 0);
-        const auto vr = buf_rsrc(va, left > 0 ? (unsigned)(left - 1) * vld2 + 2u * D : 0);
-        const unsigned x = koff, y = voff;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void*)(sk + 512 * i), 16, x, 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void*)(sv + 512 * i), 16, y, 0, 0, 0);
-        ka += kStep * p.k_ld;
-        va += kStep * p.v_ld;
-        left -= kStep;
+      for (int j0 = 0; j0 < NJ; j0 += NL) {
+        unsigned at[NL];
+#pragma unroll
+        for (int j = 0; j < NL; ++j) at[j] = lane_off[(j0 + j) % NO] + (unsigned)((j0 + j) / NO * NO * kStep) * ld2;
+        loads_to_lds16(r, lds + 1024u * kNW * j0, at);
       }
     }
-    return have;
   };
+  auto stage_k = [&](int kt, const Pages& x) { stage(kt, x, p.k_pages, p.k, p.k_ld, kld2, koff, sK); };
+  auto stage_v = [&](int kt, const Pages& x) { stage(kt, x, p.v_pages, p.v, p.v_ld, vld2, voff, sV); };
 
   // ---------------------------------------------------------------- one tile of keys
-  auto compute = [&](int kt, const bf16_t* sk, const bf16_t* sv, unsigned have) {
-    const int key0 = kt * kBN + 32 * b0;
-    if (key0 > w_hi) return;  // uniform in the wavefront: no row of it sees these keys
+  // A wavefront's tiles go through two phases, in which its instructions are laid out group by
+  // group, one product to each with the loads and arithmetic that run beside it:
+  //   1: scores of the next tile  | weights and their sum of this one | reads of k, then of v
+  //   2: weighted values of this  | maximum of the next one's scores  | reads of v
+  u32x4 f[PF], pb[4];
+  float mx = 0.f;
+  auto kfrag = [&](const bf16_t* sk, AttnLane ln, int t) { return attn_frag<DP>(sk, ln, 32 * (t & 1), t / 2); };
+  auto vfrag = [&](const bf16_t* sv, AttnLane ln, int t) { return attn_frag_tr<DP>(sv, ln, 16 * (t / DB), t % DB); };
+  auto first = [&](const bf16_t* sk, f32x16 (&s)[2]) {
     const AttnLane ln = fresh(lane);
-    f32x16 s[NB];
+    s[0] = s[1] = zero16();
 #pragma unroll
-    for (int b = 0; b < NB; ++b) s[b] = zero16();
-    u32x4 f[PF];
-    auto kfrag = [&](int t) { return attn_frag<DP>(sk, ln, 32 * (b0 + t % NB), t / NB); };
+    for (int t = 0; t < NG; ++t) s[t & 1] = mma32(kfrag(sk, ln, t), q[t / 2], s[t & 1]);
+    mx = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < PF; ++t) f[t] = kfrag(t);
+    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[e / 16][e % 16]);
+  };
+  auto mask = [&](int kt, f32x16 (&s)[2], unsigned have) {
+    mx = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < NB * KS; ++t) {
-      s[t % NB] = mma32(f[t % PF], q[t / NB], s[t % NB]);
-      if (t + PF < NB * KS) f[t % PF] = kfrag(t + PF);
+    for (int e = 0; e < 32; ++e) {
+      const int key = kt * kBN + 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * h + e % 4;
+      if (key > pos || (PAGED && !((have >> (e / 8)) & 1))) s[e / 16][e % 16] = -INFINITY;
+      mx = fmaxf(mx, s[e / 16][e % 16]);
     }
-    // the first of v's fragments arrive during the softmax
-    auto vfrag = [&](int t) { return attn_frag_tr<DP>(sv, ln, 32 * b0 + 16 * (t / DB), t % DB); };
+  };
+  auto phase1 = [&](auto more, f32x16 (&s)[2], f32x16 (&sn)[2], const bf16_t* sk, const bf16_t* sv) {
+    constexpr bool kMore = decltype(more)::value;
+    const AttnLane ln = fresh(lane);
+    if constexpr (kMore) {
 #pragma unroll
-    for (int t = 0; t < PF; ++t) f[t] = vfrag(t);
-    if (key0 + 32 * NB - 1 > w_lo || have != 15) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = key0 + 32 * b + 8 * (i / 4) + 4 * h + i % 4;
-          if (key > pos || (PAGED && !((have >> (2 * (b0 + b) + i / 8)) & 1))) s[b][i] = -INFINITY;
-        }
+      for (int t = 0; t < PF; ++t) f[t] = kfrag(sk, ln, t);
+      sn[0] = sn[1] = zero16();
     }
-    float mx = s[0][0];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
     mx = max_halves(mx);
     // the maximum is only raised, and what is summed so far scaled down, when some row's grew
     // by more than 2^8: the weights stay below that, far inside bf16 and fp32
@@ -218,22 +215,33 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     const float mc = m * cs;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int t = 0; t < NG; ++t) {
+      if constexpr (kMore) sn[t & 1] = mma32(f[t % PF], q[t / 2], sn[t & 1]);
+      if (kMore && t + PF < NG) f[t % PF] = kfrag(sk, ln, t + PF);
+      if (t + PF >= NG) f[t % PF] = vfrag(sv, ln, t + PF - NG);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int e = EG * t; e < EG * (t + 1); ++e) {
+        const int b = e / 16, i = e % 16;
         s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], cs, -mc));
-        sum[i & 3] += s[b][i];
+        sum[e & 3] += s[b][i];
+        if (e & 1) pb[e / 8][e / 2 % 4] = pack_bf16(s[b][i - 1], s[b][i]);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
     lsum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  };
+  auto phase2 = [&](auto more, f32x16 (&sn)[2], const bf16_t* sv) {
+    const AttnLane ln = fresh(lane);
+    mx = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < 2 * NB; ++x) {
-      const u32x4 pb = pack8_of(s[x / 2], x % 2);
+    for (int t = 0; t < NG; ++t) {
+      o[t % DB] = mma32(f[t % PF], pb[t / DB], o[t % DB]);
+      if (t + PF < NG) f[t % PF] = vfrag(sv, ln, t + PF);
+      if constexpr (decltype(more)::value) {
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const int t = x * DB + d;
-        o[d] = mma32(f[t % PF], pb, o[d]);
-        if (t + PF < 2 * NB * DB) f[t % PF] = vfrag(t + PF);
-        }
+        for (int e = EG * t; e < EG * (t + 1); ++e) mx = fmaxf(mx, sn[e / 16][e % 16]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -245,35 +253,72 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       if (kt * kBN + r >= keys || !((have >> (r / 16)) & 1)) *(u32x4*)(sv + 8 * i) = u32x4{0, 0, 0, 0};
     }
   };
-  auto arrived = [&](int kt, bf16_t* sv, unsigned have) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of the tile
-    lds_barrier();                       // everyone's; and the other buffers are free
+  Pages pn, pk;  // of the tile whose values come next, and of the one after, whose keys do
+  unsigned have = 15;
+  // tile kt's values and the next one's keys are there; fetches what comes next
+  auto enter = [&](int kt) {
+    wait_loads<0>();  // this wavefront's part of the tiles
+    lds_barrier();    // everyone's; and the other buffers are free
     if constexpr (PAGED) {
       if (have != 15 || (kt + 1) * kBN > keys) {  // uniform in the workgroup
-        clear(kt, sv, have);
+        clear(kt, sV + (kt & 1) * kTile, have);
         lds_barrier();
       }
     }
+    if (kt + 1 < kt1) stage_v(kt + 1, pn);
+    if (kt + 2 < kt1) stage_k(kt + 2, pk);
   };
-
+  auto leave = [&](int kt) {
+    if constexpr (PAGED) {
+      have = pn.have;
+      pn = pk;
+      pk = look(kt + 3);
+    }
+  };
   if (kt0 < kt1) {
+    Pages p0;
+    p0.have = pn.have = pk.have = 15;
     if constexpr (PAGED) {
       slot = kt0 * kBN / p.page;
       off = kt0 * kBN - slot * p.page;
-      look(kt0);
+      p0 = look(kt0);
+      pn = look(kt0 + 1);
+      pk = look(kt0 + 2);
+      have = p0.have;
     }
-    unsigned have0 = stage(kt0, sK0, sV0), have1 = 15;
-    if constexpr (PAGED) look(kt0 + 1);
-    for (int kt = kt0; kt < kt1; kt += 2) {
-      arrived(kt, sV0, have0);
-      if (kt + 1 < kt1) have1 = stage(kt + 1, sK1, sV1);
-      if constexpr (PAGED) look(kt + 2);
-      compute(kt, sK0, sV0, have0);
-      if (kt + 1 >= kt1) break;
-      arrived(kt + 1, sV1, have1);
-      if (kt + 2 < kt1) have0 = stage(kt + 2, sK0, sV0);
-      if constexpr (PAGED) look(kt + 3);
-      compute(kt + 1, sK1, sV1, have1);
+    stage_k(kt0, p0);
+    stage_v(kt0, p0);
+    if (kt0 + 1 < kt1) stage_k(kt0 + 1, pn);
+    wait_loads<0>();
+    lds_barrier();
+    // the wavefront's own last tile: rows of it see no keys of later ones
+    const int last_kt = w_hi / kBN < kt1 - 1 ? w_hi / kBN : kt1 - 1;
+    int kt = kt0;
+    if (kt <= last_kt) {
+      f32x16 s0[2], s1[2];
+      auto turn = [&](auto more, f32x16 (&s)[2], f32x16 (&sn)[2]) {
+        enter(kt);
+        if (kt * kBN + kBN - 1 > w_lo || have != 15) mask(kt, s, have);
+        phase1(more, s, sn, sK + ((kt + 1) & 1) * kTile, sV + (kt & 1) * kTile);
+        phase2(more, sn, sV + (kt & 1) * kTile);
+        leave(kt);
+        ++kt;
+      };
+      first(sK + (kt & 1) * kTile, s0);
+      while (kt + 1 < last_kt) {
+        turn(Yes(), s0, s1);
+        turn(Yes(), s1, s0);
+      }
+      if (kt < last_kt) {
+        turn(Yes(), s0, s1);
+        s0[0] = s1[0];
+        s0[1] = s1[1];
+      }
+      turn(No(), s0, s1);
+    }
+    for (; kt < kt1; ++kt) {  // other wavefronts' tiles: its part of the loads
+      enter(kt);
+      leave(kt);
     }
   }
 
@@ -291,7 +336,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     while (bad) {
       const int r = __ffsll(bad) - 1;
       bad &= bad - 1;
-      const int row1 = 32 * wr + r, pos1 = held + t0 + row1 / G;
+      const int row1 = 32 * w + r, pos1 = held + t0 + row1 / G;
       const bf16_t* q1 = (const bf16_t*)p.q + (it.start + t0 + row1 / G) * p.q_ld + (long long)(hk * G + row1 % G) * D;
       const float m1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), r)) * cs;
       float acc[DP / 64];
@@ -300,7 +345,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       const int last = kt1 * kBN - 1 < pos1 ? kt1 * kBN - 1 : pos1;
       for (int k0 = kt0 * kBN; k0 <= last; k0 += 64) {  // a key a lane
         const int key = k0 + l;
-        bool see = key <= last && (KG == 1 || ((l >> 5) & 1) == w >> 2);
+        bool see = key <= last;
         long long at = (it.start + key) * p.k_ld + hk * D, av = (it.start + key) * p.v_ld + hk * D;
         if constexpr (PAGED) {
           const int sl = key / p.page;
@@ -340,39 +385,6 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
 
   // ---------------------------------------------------------------- output
   lsum = sum_halves(lsum);
-  if constexpr (KG == 2) {
-    // the second wavefront of each 32 rows hands its sums over in the buffers, 32 KiB each, an
-    // element's 16-byte pieces a lane apart
-    __shared__ float sML[2][4][32];
-    __syncthreads();
-    float* xs = (float*)(wr == 0 ? sK0 : (wr == 1 ? sK1 : (wr == 2 ? sV0 : sV1)));
-    if (w >= 4) {
-      if (h == 0) {
-        sML[0][wr][c] = m;
-        sML[1][wr][c] = lsum;
-      }
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *(f32x4*)(xs + (4 * d + g) * 256 + 4 * l) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-    }
-    __syncthreads();
-    if (w >= 4) return;
-    const float m2 = sML[0][wr][c], l2 = sML[1][wr][c], mn = fmaxf(m, m2);
-    const float a1 = __builtin_amdgcn_exp2f((m - mn) * cs), a2 = __builtin_amdgcn_exp2f((m2 - mn) * cs);
-    m = mn;
-    lsum = lsum * a1 + l2 * a2;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 x = *(const f32x4*)(xs + (4 * d + g) * 256 + 4 * l);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[d][4 * g + i] = o[d][4 * g + i] * a1 + x[i] * a2;
-        __builtin_amdgcn_sched_barrier(0);
-      }
-  }
   if (!live) return;
   const int Hq = Hkv * G, head = hk * G + rg;
   if (PAGED && p.splits > 1) {
@@ -568,9 +580,9 @@ hipError_t launch_attn_fwd(const AttnParams& p, hipStream_t stream) {
 #define OMX_FWD(DP)                                                                   \
   case DP:                                                                            \
     if (paged)                                                                        \
-      attn_fwd_kernel<DP, true><<<grid, kFwdNT<DP>, 0, stream>>>(p, (int)ranks);             \
+      attn_fwd_kernel<DP, true><<<grid, kNT, 0, stream>>>(p, (int)ranks);             \
     else                                                                              \
-      attn_fwd_kernel<DP, false><<<grid, kFwdNT<DP>, 0, stream>>>(p, (int)ranks);            \
+      attn_fwd_kernel<DP, false><<<grid, kNT, 0, stream>>>(p, (int)ranks);            \
     break;
     OMX_FWD(64)
     OMX_FWD(128)
