@@ -131,44 +131,44 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     }
     return x;
   };
-  // fetches a tile of keys (or values) into LDS
-  auto stage = [&](int kt, const Pages& x, const void* pool, const void* rows, long long ld, unsigned ld2,
-                   const unsigned (&lane_off)[NO], const bf16_t* dst) {
+  // Fetches a share of a tile of keys (or values) into LDS: NL instructions from the j0-th on.  They
+  // are spread over a tile's products (all at once they hold a wavefront up for as long as its
+  // memory path takes them in: 1,000 of 4,000 cycles a tile of heads of 256).  Tiles past the last
+  // one have an empty range.
+  constexpr int NL = 2, NF = NJ / NL;
+  auto fetch = [&](int kt, const Pages& x, const void* pool, const void* rows, long long ld, unsigned ld2,
+                   const unsigned (&lane_off)[NO], const bf16_t* dst, int j0) {
     const unsigned lds = lds_address(dst + (kt & 1) * kTile) + 1024u * (unsigned)w;
     if constexpr (PAGED) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
+      for (int j = j0; j < j0 + NL; ++j) {
         const int g0 = kStep * j / 16;  // the group of the instruction's rows
         int id = x.id[g0], of = x.off[g0];
         if (DP == 64 && w >= 2) { id = x.id[g0 + 1]; of = x.off[g0 + 1]; }
-        if (id >= 0) {
-          const long long at = ((long long)id * p.page + of) * Hkv * D + hk * D;
-          load_to_lds16((const bf16_t*)pool + at, lds + 1024u * kNW * j, lane_off[j % NO]);
-        }
+        const long long at = ((long long)(id < 0 ? 0 : id) * p.page + of) * Hkv * D + hk * D;
+        load_to_lds16(rsrc_words((const bf16_t*)pool + at, id < 0 || kt >= kt1 ? 0 : 16u * ld2),
+                      lds + 1024u * kNW * j, lane_off[j % NO]);
       }
     } else {
       int left = it.len - kt * kBN;  // rows past the sequence read as zeros
       left = left < kBN ? left : kBN;
-      const u32x4 r = rsrc_words((const bf16_t*)rows + (it.start + (long long)kt * kBN) * ld + hk * D,
-                                 (unsigned)(left - 1) * ld2 + 2u * D);
-      constexpr int NL = NJ < 4 ? NJ : 4;  // instructions that follow each other closely
+      unsigned at[NL];
 #pragma unroll
-      for (int j0 = 0; j0 < NJ; j0 += NL) {
-        unsigned at[NL];
-#pragma unroll
-        for (int j = 0; j < NL; ++j) at[j] = lane_off[(j0 + j) % NO] + (unsigned)((j0 + j) / NO * NO * kStep) * ld2;
-        loads_to_lds16(r, lds + 1024u * kNW * j0, at);
-      }
+      for (int j = 0; j < NL; ++j) at[j] = lane_off[(j0 + j) % NO] + (unsigned)((j0 + j) / NO * NO * kStep) * ld2;
+      loads_to_lds16(rsrc_words((const bf16_t*)rows + (it.start + (long long)kt * kBN) * ld + hk * D,
+                                kt < kt1 ? (unsigned)(left - 1) * ld2 + 2u * D : 0),
+                     lds + 1024u * kNW * j0, at);
     }
   };
-  auto stage_k = [&](int kt, const Pages& x) { stage(kt, x, p.k_pages, p.k, p.k_ld, kld2, koff, sK); };
-  auto stage_v = [&](int kt, const Pages& x) { stage(kt, x, p.v_pages, p.v, p.v_ld, vld2, voff, sV); };
+  auto fetch_k = [&](int kt, const Pages& x, int j) { fetch(kt, x, p.k_pages, p.k, p.k_ld, kld2, koff, sK, NL * j); };
+  auto fetch_v = [&](int kt, const Pages& x, int j) { fetch(kt, x, p.v_pages, p.v, p.v_ld, vld2, voff, sV, NL * j); };
 
   // ---------------------------------------------------------------- one tile of keys
   // A wavefront's tiles go through two phases, in which its instructions are laid out group by
   // group, one product to each with the loads and arithmetic that run beside it:
   //   1: scores of the next tile  | weights and their sum of this one | reads of k, then of v
   //   2: weighted values of this  | maximum of the next one's scores  | reads of v
+  Pages pn, pk;  // of the tile whose values come next, and of the one after, whose keys do
   u32x4 f[PF], pb[4];
   float mx = 0.f;
   auto kfrag = [&](const bf16_t* sk, AttnLane ln, int t) { return attn_frag<DP>(sk, ln, 32 * (t & 1), t / 2); };
@@ -191,7 +191,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       mx = fmaxf(mx, s[e / 16][e % 16]);
     }
   };
-  auto phase1 = [&](auto more, f32x16 (&s)[2], f32x16 (&sn)[2], const bf16_t* sk, const bf16_t* sv) {
+  auto phase1 = [&](auto more, f32x16 (&s)[2], f32x16 (&sn)[2], const bf16_t* sk, const bf16_t* sv, int kt) {
     constexpr bool kMore = decltype(more)::value;
     const AttnLane ln = fresh(lane);
     if constexpr (kMore) {
@@ -226,11 +226,12 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
         sum[e & 3] += s[b][i];
         if (e & 1) pb[e / 8][e / 2 % 4] = pack_bf16(s[b][i - 1], s[b][i]);
       }
+      if (t % (NG / NF) == 0) fetch_v(kt + 1, pn, t / (NG / NF));
       __builtin_amdgcn_sched_barrier(0);
     }
     lsum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
   };
-  auto phase2 = [&](auto more, f32x16 (&sn)[2], const bf16_t* sv) {
+  auto phase2 = [&](auto more, f32x16 (&sn)[2], const bf16_t* sv, int kt) {
     const AttnLane ln = fresh(lane);
     mx = -INFINITY;
 #pragma unroll
@@ -241,6 +242,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
 #pragma unroll
         for (int e = EG * t; e < EG * (t + 1); ++e) mx = fmaxf(mx, sn[e / 16][e % 16]);
       }
+      if (t % (NG / 2 / NF) == 0 && t < NG / 2) fetch_k(kt + 2, pk, t / (NG / 2 / NF));
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -253,9 +255,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       if (kt * kBN + r >= keys || !((have >> (r / 16)) & 1)) *(u32x4*)(sv + 8 * i) = u32x4{0, 0, 0, 0};
     }
   };
-  Pages pn, pk;  // of the tile whose values come next, and of the one after, whose keys do
   unsigned have = 15;
-  // tile kt's values and the next one's keys are there; fetches what comes next
+  // tile kt's values and the next one's keys are there
   auto enter = [&](int kt) {
     wait_loads<0>();  // this wavefront's part of the tiles
     lds_barrier();    // everyone's; and the other buffers are free
@@ -265,8 +266,6 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
         lds_barrier();
       }
     }
-    if (kt + 1 < kt1) stage_v(kt + 1, pn);
-    if (kt + 2 < kt1) stage_k(kt + 2, pk);
   };
   auto leave = [&](int kt) {
     if constexpr (PAGED) {
@@ -286,9 +285,12 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       pk = look(kt0 + 2);
       have = p0.have;
     }
-    stage_k(kt0, p0);
-    stage_v(kt0, p0);
-    if (kt0 + 1 < kt1) stage_k(kt0 + 1, pn);
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+      fetch_k(kt0, p0, j);
+      fetch_v(kt0, p0, j);
+      fetch_k(kt0 + 1, pn, j);
+    }
     wait_loads<0>();
     lds_barrier();
     // the wavefront's own last tile: rows of it see no keys of later ones
@@ -299,8 +301,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       auto turn = [&](auto more, f32x16 (&s)[2], f32x16 (&sn)[2]) {
         enter(kt);
         if (kt * kBN + kBN - 1 > w_lo || have != 15) mask(kt, s, have);
-        phase1(more, s, sn, sK + ((kt + 1) & 1) * kTile, sV + (kt & 1) * kTile);
-        phase2(more, sn, sV + (kt & 1) * kTile);
+        phase1(more, s, sn, sK + ((kt + 1) & 1) * kTile, sV + (kt & 1) * kTile, kt);
+        phase2(more, sn, sV + (kt & 1) * kTile, kt);
         leave(kt);
         ++kt;
       };
@@ -318,9 +320,15 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     }
     for (; kt < kt1; ++kt) {  // other wavefronts' tiles: its part of the loads
       enter(kt);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) {
+        fetch_v(kt + 1, pn, j);
+        fetch_k(kt + 2, pk, j);
+      }
       leave(kt);
     }
   }
+  wait_loads<0>();
 
   // A weight of zero does not keep a NaN or an infinity among a tile's values from the rows that do
   // not see it.  Rows whose sums are not finite though their weights are, are summed again over
