@@ -17,126 +17,6 @@ namespace {
 
 constexpr int kNW = 4, kNT = 64 * kNW, kBM = 128, kBN = 64;
 
-// ------------------------------------------------------------------------------------ dq
-template <int DP>
-__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
-void attn_dq_kernel(AttnParams p, int ranks) {
-  constexpr int KS = DP / 16, DB = DP / 32;
-  constexpr int NJ = kBN * DP / 8 / 64 / kNW;
-  __shared__ __align__(16) bf16_t sK0[kBN * DP], sK1[kBN * DP], sV0[kBN * DP], sV1[kBN * DP];
-
-  const int tid = threadIdx.x, l = tid & 63, h = l >> 5, c = l & 31;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const AttnLane lane = attn_lane<DP>();
-  const int G = p.G, D = p.D, Hkv = p.Hkv, Hq = Hkv * G, per = kBM / G;
-
-  int unit, rank;
-  attn_place((int)blockIdx.x, (p.cu ? 1 : p.N) * Hkv, ranks, unit, rank);
-  if (rank >= ranks) return;
-  const int hk = unit % Hkv;
-  AttnTile it;
-  if (!attn_tile(p, unit / Hkv, rank, per, it)) return;
-  const int t0 = it.tile * per, nt = it.len - t0 < per ? it.len - t0 : per;
-
-  const int row = 32 * w + c, rt = row / G, rg = row - rt * G;
-  const bool live = rt < nt;
-  const long long tok = it.start + t0 + rt, at = tok * Hq + hk * G + rg;
-  const int pos = t0 + rt, w_lo = t0 + (32 * w) / G, w_hi = t0 + (32 * w + 31) / G;
-
-  u32x4 q[KS], dout[KS];
-  float delta = 0.f;
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int d = 16 * s + 8 * h;
-    q[s] = dout[s] = u32x4{0, 0, 0, 0};
-    if (live && d < D) {
-      q[s] = *(const u32x4*)((const bf16_t*)p.q + tok * p.q_ld + (long long)(hk * G + rg) * D + d);
-      dout[s] = *(const u32x4*)((const bf16_t*)p.dout + at * D + d);
-      delta = dot8(dout[s], *(const u32x4*)((const bf16_t*)p.o + at * D + d), delta);
-      if (p.o_rest) delta = dot8(dout[s], *(const u32x4*)((const bf16_t*)p.o_rest + at * D + d), delta);
-    }
-  }
-  delta = sum_halves(delta);
-  const float lse2 = live ? p.lse[at] * kLog2e : INFINITY;  // idle rows: weights of 0
-  if (live && h == 0) {
-    float* st = p.stats + 2 * (tok * Hq + hk * G) + rg;
-    st[0] = lse2;
-    st[G] = -delta;
-  }
-
-  f32x16 dq[DB];
-#pragma unroll
-  for (int d = 0; d < DB; ++d) dq[d] = zero16();
-  const float cs = p.scale * kLog2e;
-  const int nkt = (t0 + nt + kBN - 1) / kBN;
-
-  int srow[NJ], sseg[NJ];
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    srow[j] = stage_row<DP, kNW>(w, j);
-    sseg[j] = stage_seg<DP>(srow[j]);
-  }
-  const unsigned kld2 = (unsigned)(p.k_ld * 2), vld2 = (unsigned)(p.v_ld * 2);
-  auto stage = [&](int kt, bf16_t* sk, bf16_t* sv) {
-    const int left = it.len - kt * kBN, n = left < kBN ? left : kBN;  // rows past the sequence
-    const long long a = it.start + (long long)kt * kBN;               //   read as zeros
-    const auto kr = buf_rsrc((const bf16_t*)p.k + a * p.k_ld + hk * D, (unsigned)(n - 1) * kld2 + 2u * D);
-    const auto vr = buf_rsrc((const bf16_t*)p.v + a * p.v_ld + hk * D, (unsigned)(n - 1) * vld2 + 2u * D);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int i = w + kNW * j;
-      const bool in = 8 * sseg[j] < D;
-      const unsigned so = 16u * (unsigned)sseg[j];
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void*)(sk + 512 * i), 16,
-                                               in ? (unsigned)srow[j] * kld2 + so : kDropOffset, 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void*)(sv + 512 * i), 16,
-                                               in ? (unsigned)srow[j] * vld2 + so : kDropOffset, 0, 0, 0);
-    }
-  };
-  auto compute = [&](int kt, const bf16_t* sk, const bf16_t* sv) {
-    const int key0 = kt * kBN;
-    if (key0 > w_hi) return;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const AttnLane ln = FRESH(lane);
-      f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-      for (int k = 0; k < KS; ++k) s = mma32(attn_frag<DP>(sk, ln, 32 * b, k), q[k], s);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) dp = mma32(attn_frag<DP>(sv, ln, 32 * b, k), dout[k], dp);
-      if (key0 + 32 * b + 31 > w_lo) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (key0 + 32 * b + 8 * (i / 4) + 4 * h + i % 4 > pos) s[i] = -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[i], cs, -lse2));
-        s[i] = x * (dp[i] - delta);
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const u32x4 ds = pack8_of(s, k);
-#pragma unroll
-        for (int d = 0; d < DB; ++d) dq[d] = mma32(attn_frag_tr<DP>(sk, ln, 32 * b + 16 * k, d), ds, dq[d]);
-      }
-    }
-  };
-  stage(0, sK0, sV0);
-  for (int kt = 0; kt < nkt; kt += 2) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    lds_barrier();
-    if (kt + 1 < nkt) stage(kt + 1, sK1, sV1);
-    compute(kt, sK0, sV0);
-    if (kt + 1 >= nkt) break;
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    lds_barrier();
-    if (kt + 2 < nkt) stage(kt + 2, sK0, sV0);
-    compute(kt + 1, sK1, sV1);
-  }
-  if (live) store_rows<DB>((bf16_t*)p.dq + at * D, dq, p.scale, D, h);
-}
-
 // The same for heads of 256, ...
 constexpr int kWideRows = 64;
 template <int DP, int KB, bool DK, bool DV>
@@ -354,15 +234,6 @@ __global__ __launch_bounds__(256) void attn_dkv_sum_kernel(const float* pk, cons
 }  // namespace
 
 int attn_dkv_tile_tokens() { return kDkvKeys; }
-
-hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream) {
-  const long long ranks = attn_ranks(p, kBM / p.G), units = (long long)(p.cu ? 1 : p.N) * p.Hkv;
-  const unsigned grid = (unsigned)attn_grid(units, ranks);
-  if (p.D <= 64) attn_dq_kernel<64><<<grid, kNT, 0, stream>>>(p, (int)ranks);
-  else if (p.D <= 128) attn_dq_kernel<128><<<grid, kNT, 0, stream>>>(p, (int)ranks);
-  else attn_dq_kernel<256><<<grid, kNT, 0, stream>>>(p, (int)ranks);
-  return hipGetLastError();
-}
 
 int attn_dkv_splits(long long units, long long T, long long N, int G) {
   // a workgroup for each compute unit, and no share below eight stages of rows on average
