@@ -247,18 +247,26 @@ __device__ __forceinline__ int tiles_held(const int32_t* held, int n, int cap, i
   return (x < 0 ? 0 : (x < cap ? x : cap)) / per;
 }
 
-// Tile of rank `rank` of sequences packed by cu, those with most keys first (a tile's work grows
-// with its index, from what a cache held on), found by every wavefront for itself when there are
-// at most 64 sequences: lane n holds sequence n.  The offsets are read as their ordered repair.
-__device__ __forceinline__ bool packed_tile(const int32_t* cu, const int32_t* held, int cap, int N, int T, int per,
-                                            int rank, AttnTile& it) {
+// Tokens of sequence n of at most 64 in lane n; the offsets are read as their ordered repair.
+__device__ __forceinline__ void packed_span(const int32_t* cu, int N, int T, int& start, int& len) {
   const int n = lane_id();
   int end = n + 1 < N ? cu[n + 1] : T;
   end = end < 0 ? 0 : (end > T ? T : end);
   end = wave_scan_max(end);
   const int prev = __shfl_up(end, 1, 64);
-  const int start = n == 0 ? 0 : prev;
-  const int len = n < N ? end - start : 0, nt = (len + per - 1) / per;
+  start = n == 0 ? 0 : prev;
+  len = n < N ? end - start : 0;
+}
+
+// Tile of rank `rank` of sequences packed by cu, those with most keys first (a tile's work grows
+// with its index, from what a cache held on), found by every wavefront for itself when there are
+// at most 64 sequences: lane n holds sequence n.
+__device__ __forceinline__ bool packed_tile(const int32_t* cu, const int32_t* held, int cap, int N, int T, int per,
+                                            int rank, AttnTile& it) {
+  const int n = lane_id();
+  int start, len;
+  packed_span(cu, N, T, start, len);
+  const int nt = (len + per - 1) / per;
   const int first = n < N ? tiles_held(held, n, cap, per) : 0;
   // at(j): tiles of place j and more
   auto at = [&](int j) {
@@ -337,6 +345,55 @@ inline long long attn_grid(long long units, long long ranks) {
 
 // keys of a workgroup's tile of the kernels that sum dk and dv
 constexpr int kDkvKeys = 128;
+
+// The rows that see a tile's keys are shared by workgroups when there are few tiles: every share of
+// a call's tiles is of as many tokens as the longest tile's are, so that shares are alike and a short
+// tile has fewer.  Tokens [ta, tb), whole stages of `per`, are for the keys from k0 on.
+struct DkvShare {
+  int len, k0, ta, tb, share, shares;
+  long long start;
+};
+
+// Share of rank `rank` of sequence or packed row `row`, false past the last.  Shares that are alike
+// need no order; whole tiles go longest first (the first keys are seen by most rows).
+__device__ __forceinline__ bool dkv_share(const AttnParams& p, int row, int rank, int per, DkvShare& it) {
+  int len, k0 = 0, each = INT32_MAX, share = 0, shares = 1;
+  long long start;
+  if (p.splits == 1) {
+    AttnTile t;
+    if (!attn_tile(p, row, rank, kDkvKeys, t)) return false;
+    start = t.start;
+    len = t.len;
+    k0 = (t.tiles - 1 - t.tile) * kDkvKeys;
+  } else {
+    int first = 0, n = lane_id() == 0 ? p.T : 0;  // lane i: sequence i, of at most 64
+    if (p.cu) packed_span(p.cu, p.N, p.T, first, n);
+    const int tiles = __builtin_amdgcn_readlane(wave_scan_max((n + kDkvKeys - 1) / kDkvKeys), 63);
+    each = ((tiles * kDkvKeys + per - 1) / per + p.splits - 1) / p.splits * per;
+    int mine = 0;
+    for (int k = 0; k < n; k += kDkvKeys) mine += (n - k + each - 1) / each;
+    const int end = wave_scan(mine);
+    const unsigned long long past = __ballot(end > rank);
+    if (!past) return false;
+    const int s = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+    start = (p.cu ? 0 : (long long)row * p.T) + __builtin_amdgcn_readlane(first, s);
+    len = __builtin_amdgcn_readlane(n, s);
+    share = rank - (__builtin_amdgcn_readlane(end, s) - __builtin_amdgcn_readlane(mine, s));
+    for (;; k0 += kDkvKeys) {  // the share is below the sequence's sum, so it ends in time
+      shares = (len - k0 + each - 1) / each;
+      if (share < shares || k0 + kDkvKeys >= len) break;
+      share -= shares;
+    }
+  }
+  it.start = start;
+  it.len = len;
+  it.k0 = k0;
+  it.share = share;
+  it.shares = shares;
+  it.ta = k0 + (shares > 1 ? share * each : 0);
+  it.tb = len - it.ta > each ? it.ta + each : len;
+  return true;
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

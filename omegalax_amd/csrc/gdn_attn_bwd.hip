@@ -9,225 +9,219 @@
 // tile of keys (dk, dv).  The scores and do . v are formed in both, 7 products in place of 5.
 #include "gdn_attn.h"
 
-#ifndef FRESH
-#define FRESH fresh
-#endif
 namespace omx {
 namespace {
 
-constexpr int kNW = 4, kNT = 64 * kNW, kBM = 128, kBN = 64;
+constexpr int kNW = 4, kNT = 64 * kNW;
+constexpr int kRows = 32, kRing = 4;  // a stage's rows, stages in LDS
 
-// The same for heads of 256, ...
-constexpr int kWideRows = 64;
-template <int DP, int KB, bool DK, bool DV>
-__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 || (DK && DV) || KB > 1 ? 1 : 2)))
+// dk and dv for heads of more than 128.  A wavefront's 32 keys, of the workgroup's 128, stay with
+// their sums in registers (k and v 128, dk and dv 256 of a lane's 512, so one wavefront a SIMD);
+// stages of 32 rows go past them through a ring in LDS.  A stage is four phases, one product after
+// the other with the loads and arithmetic that run beside it:
+//   S = Q K^T | dP = dO V^T, P = exp(S - lse) | dV^T += dO^T P, dS = P (dP - delta) | dK^T += Q^T dS
+template <int DP>
+__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(1)))
 void attn_dkv_wide_kernel(AttnParams p, int ranks) {
-  constexpr int KS = DP / 16, DB = DP / 32;
-  constexpr int NJ = kWideRows * DP / 8 / 64 / kNW;
-  __shared__ __align__(16) bf16_t sQ0[kWideRows * DP], sQ1[kWideRows * DP], sO0[kWideRows * DP], sO1[kWideRows * DP];
-  __shared__ __align__(16) float sS0[2 * kWideRows], sS1[2 * kWideRows];  // lse and delta of a stage's rows
+  constexpr int KS = DP / 16, DB = DP / 32, PF = 4;
+  constexpr int NJ = kRows * DP / 8 / 64 / kNW, kLoads = 2 * NJ + 1;  // a wavefront's loads, a stage
+  constexpr int kSlot = 2 * kRows * DP;                               // of a slot: q, then do
+  static_assert(KS == 16, "one element of the scores beside each product");
+  __shared__ __align__(16) bf16_t ring[kRing * kSlot];
+  __shared__ __align__(16) float stats[kRing * 128];  // a stage's lse, its delta from 64 on
+  __shared__ __align__(16) u32x4 offs[2][kNT];
+  __shared__ unsigned soffs[kNT];
 
   const int tid = threadIdx.x, l = tid & 63, h = l >> 5, c = l & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const AttnLane lane = attn_lane<DP>();
-  const int G = p.G, D = p.D, Hkv = p.Hkv, Hq = Hkv * G, per = kWideRows / G;
+  const int G = p.G, D = p.D, Hkv = p.Hkv, Hq = Hkv * G, per = kRows / G;
 
   int unit, rank;
   attn_place((int)blockIdx.x, (p.cu ? 1 : p.N) * Hkv, ranks, unit, rank);
   if (rank >= ranks) return;
   const int hk = unit % Hkv;
-  constexpr int kKeys = kDkvKeys;
-  AttnTile it;
-  if (!attn_tile(p, unit / Hkv, rank, kKeys, it)) return;
-  // the first tiles' keys are seen by most rows: those first
-  const int k0 = (it.tiles - 1 - it.tile) * kKeys;
-  // this share's rows: tokens [ta, tb) in whole stages
-  int ta = k0, tb = it.len;
-  if (p.splits > 1) {
-    const int n = (it.len - k0 + per - 1) / per, each = (n + p.splits - 1) / p.splits;
-    const int first = (int)blockIdx.y * each;
-    ta = first < n ? k0 + first * per : it.len;
-    tb = first + each < n ? ta + each * per : it.len;
-  }
-  const int kw = k0 + 32 * KB * w;  // the wavefront's first key
+  DkvShare it;
+  if (!dkv_share(p, unit / Hkv, rank, per, it)) return;
+  const int kw = it.k0 + 32 * w, key = kw + c;  // the wavefront's first key, the lane's
 
-  // with two blocks of keys a wavefront, v stays in LDS: its fragments would not fit beside the
-  // sums, and two blocks a read of q and do leave the LDS time for them
-  constexpr bool VL = KB == 2 && DP == 128;
-  __shared__ __align__(16) bf16_t sV[VL ? kKeys * DP : 8];
-  u32x4 kf[KB][KS], vf[KB][KS];
-  f32x16 dk[KB][DB], dv[KB][DB];
-#pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    const int key = kw + 32 * b + c;
-    const long long tok = it.start + key;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d = 16 * s + 8 * h;
-      kf[b][s] = vf[b][s] = u32x4{0, 0, 0, 0};
-      if (key < it.len && d < D) {
-        kf[b][s] = *(const u32x4*)((const bf16_t*)p.k + tok * p.k_ld + hk * D + d);
-        if constexpr (DK) vf[b][s] = *(const u32x4*)((const bf16_t*)p.v + tok * p.v_ld + hk * D + d);
-      }
-      if constexpr (VL)  // read back by this wavefront alone
-        *(u32x4*)(sV + (32 * (KB * w + b) + c) * DP + (((2 * s + h) ^ attn_swz<DP>(c)) << 3)) = vf[b][s];
-    }
-#pragma unroll
-    for (int d = 0; d < DB; ++d) dk[b][d] = dv[b][d] = zero16();
-  }
-  const float cs = p.scale * kLog2e;
+  // stages from the last to the first: a unit's workgroups, which start together and see different
+  // numbers of rows, then read the same rows at the same time, and its XCD's L2 serves most of them
+  const int n = (it.tb - it.ta + per - 1) / per, t_last = it.ta + (n - 1) * per;
+  // of these the wavefront's keys are seen by the first na
+  int na = t_last + per - kw <= 0 ? 0 : (t_last + per - kw + per - 1) / per;
+  na = na < n ? na : n;
 
   const unsigned qld2 = (unsigned)(p.q_ld * 2), old2 = (unsigned)(Hq * D * 2);
-  unsigned qoff[NJ], ooff[NJ];
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const int r = stage_row<DP, kNW>(w, j), seg = stage_seg<DP>(r), t = r / G, g = r - t * G;
-    const bool in = t < per && 8 * seg < D;
-    const unsigned x = (unsigned)g * 2u * D + 16u * (unsigned)seg;
-    qoff[j] = in ? (unsigned)t * qld2 + x : kDropOffset;
-    ooff[j] = in ? (unsigned)t * old2 + x : kDropOffset;
-  }
-  const unsigned soff = l / G < per ? (unsigned)(l / G) * 8u * Hq + 4u * (unsigned)(l % G) : kDropOffset;
-  auto stage = [&](int t, bf16_t* sq, bf16_t* so, float* ss) {
-    const int left = it.len - t, n = left < per ? left : per;  // rows past the sequence read as
-    const long long a = it.start + t;                          //   zeros: they add nothing
-    const auto qr = buf_rsrc((const bf16_t*)p.q + a * p.q_ld + (long long)hk * G * D,
-                             (unsigned)(n - 1) * qld2 + 2u * D * G);
-    const auto dr = buf_rsrc((const bf16_t*)p.dout + (a * Hq + hk * G) * D, (unsigned)(n - 1) * old2 + 2u * D * G);
+  const unsigned lds0 = lds_address(ring) + 1024u * (unsigned)w;
+  const unsigned lds1 = lds_address(stats) + 256u * (unsigned)(w & 1);
+  // The offsets of a thread's loads are the same each stage, and kept in LDS: registers are full.
+  static_assert(NJ == 4, "four loads a thread");
+  {
+    u32x4 x, y;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const int i = w + kNW * j;
-      const unsigned x = qoff[j], y = ooff[j];
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(qr, (lds_void*)(sq + 512 * i), 16, x, 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(dr, (lds_void*)(so + 512 * i), 16, y, 0, 0, 0);
+      const int r = stage_row<DP, kNW>(w, j), seg = stage_seg<DP>(r), t = r / G, g = r - t * G;
+      const bool in = t < per && 8 * seg < D;
+      const unsigned z = (unsigned)g * 2u * D + 16u * (unsigned)seg;
+      x[j] = in ? (unsigned)t * qld2 + z : kDropOffset;
+      y[j] = in ? (unsigned)t * old2 + z : kDropOffset;
     }
-    if (w < 2) {
-      const auto sr = buf_rsrc(p.stats + 2 * (a * Hq + hk * G) + w * G, (unsigned)(n - 1) * 8u * Hq + 4u * G);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_void*)(ss + kWideRows * w), 4, soff, 0, 0, 0);
-    }
+    offs[0][tid] = x;
+    offs[1][tid] = y;
+    soffs[tid] = l / G < per ? (unsigned)(l / G) * 8u * Hq + 4u * (unsigned)(l % G) : kDropOffset;
+  }
+  // Fetches stage i's rows of q (of do) into its slot; stages past the last have an empty range, and
+  // so have rows past the sequence, which read as zeros and add nothing.
+  auto fetch = [&](int i, u32x4 x, const bf16_t* rows, long long ld, unsigned ld2, unsigned part) {
+    const int t = t_last - i * per, left = it.len - t, m = left < per ? left : per;
+    const unsigned off[NJ] = {x[0], x[1], x[2], x[3]};
+    loads_to_lds16(rsrc_words(rows + (it.start + t) * ld + (long long)hk * G * D,
+                              i < n ? (unsigned)(m - 1) * ld2 + 2u * D * G : 0),
+                   lds0 + 2u * (kSlot * (unsigned)(i & (kRing - 1)) + part), off);
   };
-  auto compute = [&](int t, const bf16_t* sq, const bf16_t* so, const float* ss) {
-    if (t + per <= kw) return;  // every row is before every key of the wavefront
-#ifdef U1
-#pragma unroll 1
-#else
-#pragma unroll
-#endif
-    for (int rb = 0; rb < kWideRows / 32; ++rb) {
-      const AttnLane ln = FRESH(lane);
-      f32x16 s[KB], dp[KB];
-#pragma unroll
-      for (int b = 0; b < KB; ++b) s[b] = dp[b] = zero16();
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const u32x4 a = attn_frag<DP>(sq, ln, 32 * rb, k);
-#pragma unroll
-        for (int b = 0; b < KB; ++b) s[b] = mma32(a, kf[b][k], s[b]);
-      }
-      if constexpr (DK) {
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const u32x4 a = attn_frag<DP>(so, ln, 32 * rb, k);
-#pragma unroll
-          for (int b = 0; b < KB; ++b)
-            dp[b] = mma32(a, VL ? attn_frag<DP>(sV, ln, 32 * (KB * w + b), k) : vf[b][k], dp[b]);
-        }
-      }
-      if (t < kw + 32 * KB - 1) {  // row r is token t + r / G: before the key if r < (key - t) G
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-          const int first = (kw + 32 * b + c - t) * G;
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * rb + 8 * (i / 4) + 4 * h + i % 4 < first) s[b][i] = -INFINITY;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 lse = *(const f32x4*)(ss + 32 * rb + 8 * j + 4 * h);
-        const f32x4 del = *(const f32x4*)(ss + kWideRows + 32 * rb + 8 * j + 4 * h);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float l2 = lse[i];
-#pragma unroll
-          for (int b = 0; b < KB; ++b) {
-            s[b][4 * j + i] = __builtin_amdgcn_exp2f(fmaf(s[b][4 * j + i], cs, -l2));
-            if constexpr (DK) dp[b][4 * j + i] = s[b][4 * j + i] * (dp[b][4 * j + i] + del[i]);
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        u32x4 pb[KB], db[KB];
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-          if constexpr (DV) pb[b] = pack8_of(s[b], k);
-          if constexpr (DK) db[b] = pack8_of(dp[b], k);
-        }
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          if constexpr (DV) {
-            const u32x4 a = attn_frag_tr<DP>(so, ln, 32 * rb + 16 * k, d);
-#pragma unroll
-            for (int b = 0; b < KB; ++b) dv[b][d] = mma32(a, pb[b], dv[b][d]);
-          }
-          if constexpr (DK) {
-            const u32x4 a = attn_frag_tr<DP>(sq, ln, 32 * rb + 16 * k, d);
-#pragma unroll
-            for (int b = 0; b < KB; ++b) dk[b][d] = mma32(a, db[b], dk[b][d]);
-          }
-        }
-      }
-    }
+  auto fetch_q = [&](int i, u32x4 off) { fetch(i, off, (const bf16_t*)p.q, p.q_ld, qld2, 0); };
+  auto fetch_do = [&](int i, u32x4 off) {
+    fetch(i, off, (const bf16_t*)p.dout, (long long)Hq * D, old2, kRows * DP);
   };
-  // from the last stage to the first: a unit's workgroups, which start together and see different
-  // numbers of rows, then read the same rows at the same time, and its XCD's L2 serves most of them
-  if (ta < tb) {
-    int t = ta + (tb - ta - 1) / per * per;
-    stage(t, sQ0, sO0, sS0);
-    for (; t >= ta; t -= 2 * per) {
-      __builtin_amdgcn_s_waitcnt(0x0F70);
-      lds_barrier();
-      if (t - per >= ta) stage(t - per, sQ1, sO1, sS1);
-      compute(t, sQ0, sO0, sS0);
-      if (t - per < ta) break;
-      __builtin_amdgcn_s_waitcnt(0x0F70);
-      lds_barrier();
-      if (t - 2 * per >= ta) stage(t - 2 * per, sQ0, sO0, sS0);
-      compute(t - per, sQ1, sO1, sS1);
+  auto fetch_stats = [&](int i, unsigned off) {  // lse (even wavefronts) or delta (odd ones)
+    const int t = t_last - i * per, left = it.len - t, m = left < per ? left : per;
+    load_to_lds4(rsrc_words(p.stats + 2 * ((it.start + t) * Hq + hk * G) + (w & 1) * G,
+                            i < n ? (unsigned)(m - 1) * 8u * Hq + 4u * G : 0),
+                 lds1 + 512u * (unsigned)(i & (kRing - 1)), off);
+  };
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i) {
+    fetch_q(i, offs[0][tid]);
+    fetch_do(i, offs[1][tid]);
+    fetch_stats(i, soffs[tid]);
+  }
+
+  u32x4 kf[KS], vf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d = 16 * s + 8 * h;
+    kf[s] = vf[s] = u32x4{0, 0, 0, 0};
+    if (key < it.len && d < D) {
+      kf[s] = *(const u32x4*)((const bf16_t*)p.k + (it.start + key) * p.k_ld + hk * D + d);
+      vf[s] = *(const u32x4*)((const bf16_t*)p.v + (it.start + key) * p.v_ld + hk * D + d);
     }
   }
+  f32x16 dk[DB], dv[DB];
 #pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    const int key = kw + 32 * b + c;
-    if (key >= it.len) continue;
-    const long long at = ((it.start + key) * Hkv + hk) * D;
-    if (p.splits > 1) {
-      const long long ps = (long long)blockIdx.y * p.tokens * Hkv * D + at;
-      if constexpr (DK) store_part<DB>(p.part_k + ps, dk[b], p.scale, D, h);
-      if constexpr (DV) store_part<DB>(p.part_v + ps, dv[b], 1.f, D, h);
-    } else {
-      if constexpr (DK) store_rows<DB>((bf16_t*)p.dk + at, dk[b], p.scale, D, h);
-      if constexpr (DV) store_rows<DB>((bf16_t*)p.dv + at, dv[b], 1.f, D, h);
+  for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
+  const float cs = p.scale * kLog2e;
+
+  wait_loads<0>();  // k and v too: no wait for them remains for the loop
+  lds_barrier();
+  u32x4 f[PF];
+#pragma unroll
+  for (int i = 0; i < PF; ++i) f[i] = attn_frag<DP>(ring, lane, 0, i);
+  int i0 = 0;
+  for (; i0 < na; ++i0) {
+    wait_loads<kLoads>();  // all but stage i0 + 2: the next is there
+    lds_barrier();         // everyone's; and the last one's slot is free
+    const bf16_t* sq = ring + (i0 & (kRing - 1)) * kSlot;
+    const bf16_t* so = sq + kRows * DP;
+    const bf16_t* sn = ring + ((i0 + 1) & (kRing - 1)) * kSlot;
+    const float* ss = stats + 128 * (i0 & (kRing - 1));
+    const AttnLane ln = fresh(lane);
+    auto tr = [&](const bf16_t* x, int i) { return attn_frag_tr<DP>(x, ln, 16 * (i / DB), i % DB); };
+    auto stat = [&](int i) { return *(const f32x4*)(ss + 8 * i + 4 * h); };
+    f32x16 s = zero16(), dp = zero16();
+    f32x4 st;  // lse, then delta, of four rows
+    u32x4 pw[2], ds[2], off;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      s = mma32(f[i % PF], kf[i], s);
+      f[i % PF] = i + PF < KS ? attn_frag<DP>(sq, ln, 0, i + PF) : attn_frag<DP>(so, ln, 0, i + PF - KS);
+      if (i == KS - PF) st = stat(0);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    const int t = t_last - i0 * per;
+    if (t < kw + 31) {  // row r is token t + r / G: before the key if r < (key - t) G
+      int first = lane_id() & 31;
+      asm volatile("" : "+v"(first));
+      first = (kw + first - t) * G;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i / 4) + 4 * h + i % 4 < first) s[i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      dp = mma32(f[i % PF], vf[i], dp);
+      f[i % PF] = i + PF < KS ? attn_frag<DP>(so, ln, 0, i + PF) : tr(so, i + PF - KS);
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], cs, -st[i % 4]));
+      if (i % 4 == 3) st = stat(i < 15 ? i / 4 + 1 : 8);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) pw[k] = pack8_of(s, k);
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      dv[i % DB] = mma32(f[i % PF], pw[i / DB], dv[i % DB]);
+      f[i % PF] = i + PF < KS ? tr(so, i + PF) : tr(sq, i + PF - KS);
+      s[i] *= dp[i] + st[i % 4];
+      if (i % 4 == 3 && i < 15) st = stat(8 + i / 4 + 1);
+      if (i == KS - PF) off = offs[0][tid];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) ds[k] = pack8_of(s, k);
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      dk[i % DB] = mma32(f[i % PF], ds[i / DB], dk[i % DB]);
+      f[i % PF] = i + PF < KS ? tr(sq, i + PF) : attn_frag<DP>(sn, ln, 0, i + PF - KS);
+      if (i == 1) {
+        fetch_q(i0 + kRing - 1, off);
+        off = offs[1][tid];
+      }
+      if (i == 6) {
+        fetch_do(i0 + kRing - 1, off);
+        off[0] = soffs[tid];
+      }
+      if (i == 10) fetch_stats(i0 + kRing - 1, off[0]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  for (; i0 < n; ++i0) {  // rows before every key of the wavefront: its part of the loads
+    wait_loads<kLoads>();
+    lds_barrier();
+    fetch_q(i0 + kRing - 1, offs[0][tid]);
+    fetch_do(i0 + kRing - 1, offs[1][tid]);
+    fetch_stats(i0 + kRing - 1, soffs[tid]);
+  }
+  wait_loads<0>();
+  if (key >= it.len) return;
+  const long long at = ((it.start + key) * Hkv + hk) * D;
+  if (p.splits > 1 && it.share == 0 && h == 0) p.shares[at / D] = it.shares;
+  if (it.shares > 1) {
+    const long long ps = (long long)it.share * p.tokens * Hkv * D + at;
+    store_part<DB>(p.part_k + ps, dk, p.scale, D, h);
+    store_part<DB>(p.part_v + ps, dv, 1.f, D, h);
+  } else {
+    store_rows<DB>((bf16_t*)p.dk + at, dk, p.scale, D, h);
+    store_rows<DB>((bf16_t*)p.dv + at, dv, 1.f, D, h);
   }
 }
 
-// The shares' sums, 8 elements a thread.  Bound by its bytes: 4 a share and 2 out.
-__global__ __launch_bounds__(256) void attn_dkv_sum_kernel(const float* pk, const float* pv, bf16_t* dk,
-                                                           bf16_t* dv, int splits, long long n) {
+// The shares' sums, 8 elements a thread, of tiles with more than one.  Bound by its bytes: 4 a share
+// and 2 out.
+__global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnParams p, long long n) {
   const long long i = 8 * ((long long)blockIdx.x * 256 + threadIdx.x);
   if (i >= n) return;
-  const float* src = blockIdx.y ? pv : pk;
+  const int shares = p.shares[i / p.D];
+  if (shares < 2) return;
+  const float* src = blockIdx.y ? p.part_v : p.part_k;
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < splits; ++s)
+  for (int s = 0; s < shares; ++s)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const f32x4 y = *(const f32x4*)(src + s * n + i + 4 * j);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[4 * j + e] += y[e];
     }
-  *(u32x4*)((blockIdx.y ? dv : dk) + i) =
+  *(u32x4*)((bf16_t*)(blockIdx.y ? p.dv : p.dk) + i) =
       u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
 }
 
@@ -236,26 +230,27 @@ __global__ __launch_bounds__(256) void attn_dkv_sum_kernel(const float* pk, cons
 int attn_dkv_tile_tokens() { return kDkvKeys; }
 
 int attn_dkv_splits(long long units, long long T, long long N, int G) {
-  // a workgroup for each compute unit, and no share below eight stages of rows on average
+  if (N > 64) return 1;  // the shares are found by lanes that hold a sequence each
+  // two shares for each compute unit if all tiles were as long as the longest (about one, then:
+  // a sequence's tiles see half its rows on average), and none below sixteen stages of rows
   const long long tiles = units * ((T + kDkvKeys - 1) / kDkvKeys + (N > 0 ? N - 1 : 0));
-  const long long most = T / (N > 0 ? N : 1) * G / (8 * kWideRows);
-  long long s = 256 / (tiles > 0 ? tiles : 1);
+  const long long most = T / (N > 0 ? N : 1) * G / (16 * kRows);
+  long long s = 512 / (tiles > 0 ? tiles : 1);
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 8 ? 8 : s));
 }
 
 hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream) {
-  const long long ranks = attn_ranks(p, kDkvKeys), units = (long long)(p.cu ? 1 : p.N) * p.Hkv;
-  const dim3 grid((unsigned)attn_grid(units, ranks), (unsigned)p.splits);
+  const long long ranks = attn_ranks(p, kDkvKeys) * p.splits, units = (long long)(p.cu ? 1 : p.N) * p.Hkv;
+  const unsigned grid = (unsigned)attn_grid(units, ranks);
   if (p.D <= 128)
     launch_attn_dkv_narrow(p, grid, (int)ranks, stream);
   else
-    attn_dkv_wide_kernel<256, 1, true, true><<<grid, kNT, 0, stream>>>(p, (int)ranks);
+    attn_dkv_wide_kernel<256><<<grid, kNT, 0, stream>>>(p, (int)ranks);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   const long long n = p.tokens * p.Hkv * p.D;
-  attn_dkv_sum_kernel<<<dim3((unsigned)((n + 2047) / 2048), 2), 256, 0, stream>>>(
-      p.part_k, p.part_v, (bf16_t*)p.dk, (bf16_t*)p.dv, p.splits, n);
+  attn_dkv_sum_kernel<<<dim3((unsigned)((n + 2047) / 2048), 2), 256, 0, stream>>>(p, n);
   return hipGetLastError();
 }
 

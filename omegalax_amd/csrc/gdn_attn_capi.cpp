@@ -180,7 +180,7 @@ struct AttnBwdWs {
   size_t stats;
   PlanWs rows, keys;
   int splits;
-  size_t part_k, part_v, total;
+  size_t shares, part_k, part_v, total;
 };
 AttnBwdWs attn_bwd_ws(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N) {
   AttnBwdWs w{};
@@ -188,9 +188,10 @@ AttnBwdWs attn_bwd_ws(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, 
   w.rows = plan_ws(align_up((size_t)(B * T * Hq) * 8), T, N, omx::attn_tile_tokens((int)(Hq / Hkv)));
   w.keys = plan_ws(w.rows.total, T, N, per);
   w.splits = omx::attn_dkv_splits(B * Hkv, T, N, (int)(Hq / Hkv));
-  w.part_k = w.part_v = w.total = w.keys.total;
+  w.shares = w.part_k = w.part_v = w.total = w.keys.total;
   if (w.splits > 1) {
     const size_t one = align_up((size_t)w.splits * B * T * Hkv * D * 4);
+    w.part_k = w.shares + align_up((size_t)(B * T * Hkv) * 4);
     w.part_v = w.part_k + one;
     w.total = w.part_v + one;
   }
@@ -232,6 +233,7 @@ int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, 
   p.q_ld = q_ld; p.k_ld = k_ld; p.v_ld = v_ld; p.cu = cu_seqlens;
   p.dq = dq; p.dk = dk; p.dv = dv;
   p.stats = (float*)((char*)workspace + ws.stats);
+  p.shares = (int32_t*)((char*)workspace + ws.shares);
   p.part_k = (float*)((char*)workspace + ws.part_k);
   p.part_v = (float*)((char*)workspace + ws.part_v);
   p.splits = ws.splits;

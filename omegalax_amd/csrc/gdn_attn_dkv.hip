@@ -46,21 +46,12 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
   attn_place((int)blockIdx.x, (p.cu ? 1 : p.N) * Hkv, ranks, unit, rank);
   if (rank >= ranks) return;
   const int hk = unit % Hkv;
-  AttnTile it;
-  if (!attn_tile(p, unit / Hkv, rank, kDkvKeys, it)) return;
-  // the first tiles' keys are seen by most rows: those first
-  const int k0 = (it.tiles - 1 - it.tile) * kDkvKeys, kw = k0 + 32 * w, key = kw + c;
-  // this share's rows: tokens [ta, tb) in whole stages
-  int ta = k0, tb = it.len;
-  if (p.splits > 1) {
-    const int n = (it.len - k0 + per - 1) / per, each = (n + p.splits - 1) / p.splits;
-    const int first = (int)blockIdx.y * each;
-    ta = first < n ? k0 + first * per : it.len;
-    tb = first + each < n ? ta + each * per : it.len;
-  }
+  DkvShare it;
+  if (!dkv_share(p, unit / Hkv, rank, per, it)) return;
+  const int kw = it.k0 + 32 * w, key = kw + c;
   // stages from the last to the first: a unit's workgroups, which start together and see different
   // numbers of rows, then read the same rows at the same time, and its XCD's L2 serves most of them
-  const int n = (tb - ta + per - 1) / per, t_last = ta + (n - 1) * per;
+  const int n = (it.tb - it.ta + per - 1) / per, t_last = it.ta + (n - 1) * per;
   // of these the wavefront's keys are seen by the first na
   int na = t_last + per - kw <= 0 ? 0 : (t_last + per - kw + per - 1) / per;
   na = na < n ? na : n;
@@ -254,8 +245,9 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
   wait_loads<0>();
   if (key >= it.len) return;
   const long long at = ((it.start + key) * Hkv + hk) * D;
-  if (p.splits > 1) {
-    const long long ps = (long long)blockIdx.y * p.tokens * Hkv * D + at;
+  if (p.splits > 1 && it.share == 0 && h == 0) p.shares[at / D] = it.shares;
+  if (it.shares > 1) {
+    const long long ps = (long long)it.share * p.tokens * Hkv * D + at;
     store_part<DB>(p.part_k + ps, dk, p.scale, D, h);
     store_part<DB>(p.part_v + ps, dv, 1.f, D, h);
   } else {
@@ -266,7 +258,7 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
 
 }  // namespace
 
-void launch_attn_dkv_narrow(const AttnParams& p, dim3 grid, int ranks, hipStream_t stream) {
+void launch_attn_dkv_narrow(const AttnParams& p, unsigned grid, int ranks, hipStream_t stream) {
   if (p.D <= 64)
     attn_dkv_kernel<64><<<grid, kNT, 0, stream>>>(p, ranks);
   else

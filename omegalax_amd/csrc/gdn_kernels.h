@@ -291,7 +291,8 @@ struct AttnParams {
   const void* dout;
   float* stats;                // [tokens, Hkv, 2, G]: lse / ln 2, and minus the sum of dout * o
   void *dq, *dk, *dv;
-  float *part_k, *part_v;      // dk and dv in shares of the rows, when there are `splits` of them
+  float *part_k, *part_v;      // dk and dv in shares of the rows, `splits` of them at most
+  int32_t* shares;             // and of each key's tile how many, when that is more than one
 };
 constexpr int kAttnMaxG = 32, kAttnMaxD = 256;
 // tokens per tile of the forward, tiles of a row at most, and int32 words of the plan
@@ -306,7 +307,7 @@ hipError_t launch_attn_join(const AttnParams& p, hipStream_t stream);
 int attn_dkv_tile_tokens();
 int attn_dkv_splits(long long units, long long T, long long N, int G);
 hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream);
-void launch_attn_dkv_narrow(const AttnParams& p, dim3 grid, int ranks, hipStream_t stream);  // D <= 128
+void launch_attn_dkv_narrow(const AttnParams& p, unsigned grid, int ranks, hipStream_t stream);  // D <= 128
 hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream);
 // the cache's entry points: head dims, append, decode step (`splits` workgroups a key head share
 // the keys, by the tokens a table has room for; its partial sums are of splits + N segments)
