@@ -51,7 +51,7 @@ def check_prefill(q, k, v, spans, *, cu=None, do=None, scale=None, only=None):
 
 @pytest.mark.parametrize("B,T,Hq,Hkv,D", [
     (1, 1, 1, 1, 64), (2, 2, 4, 1, 128), (1, 31, 8, 2, 256), (3, 64, 2, 2, 64), (1, 65, 16, 4, 128),
-    (2, 127, 6, 2, 128), (1, 129, 10, 2, 64), (1, 200, 7, 1, 256), (2, 333, 32, 1, 128),
+    (1, 2000, 3, 1, 72), (2, 127, 6, 2, 128), (1, 129, 10, 2, 64), (1, 200, 7, 1, 256), (2, 333, 32, 1, 128),
     (1, 517, 4, 4, 256), (5, 258, 3, 1, 64), (1, 1030, 16, 8, 128),
 ])
 def test_batches_and_their_gradients(B, T, Hq, Hkv, D):
@@ -168,7 +168,8 @@ def test_a_sequence_keeps_its_infinities_to_itself():
 
 
 @pytest.mark.parametrize("Hq,Hkv,D,T,at", [(4, 2, 128, 300, 170), (2, 2, 64, 130, 64), (8, 1, 256, 90, 33),
-                                           (3, 1, 80, 200, 199), (6, 2, 128, 70, 1)])
+                                           (3, 1, 80, 200, 199), (6, 2, 128, 70, 1),
+                                           (4, 2, 128, 700, 300), (8, 1, 200, 600, 513)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_rows_before_a_token_do_not_see_its_infinities(Hq, Hkv, D, T, at, bad):
     """Keys and values that are not finite, from one token on (a padded row's, say): the rows before
