@@ -331,11 +331,12 @@ int omx_gdn_ab_proj(const void* x, const void* w_a, const void* w_b, void* a, vo
  *   o            [B, T, Hq, D] bf16
  *   lse          [B, T, Hq] f32 or NULL: log sum_j exp(scale q . k), for omx_gdn_attn_bwd
  *   o_rest       [B, T, Hq, D] bf16 or NULL: what the rounding of o left, for omx_gdn_attn_bwd
- *   scale        positive
+ *   scale        positive, at most 2^20; products q . k are to lie above -1e30
  * D is a multiple of 8, at most 256 (compiled for 64, 128 and 256; others run zero-filled at the
  * next).  Strides are multiples of 8 and at most 2^22, q, k, v and o 16-byte aligned.  Scores,
- * softmax and sums are fp32; the weights are rounded to bf16 for their product with v.  A row's
- * values are those of its own sequence alone, whatever lies beside it.
+ * softmax and sums are fp32; the weights are rounded to bf16 for their product with v.  A row
+ * depends on its own sequence alone, whatever lies beside it, and on no key after it: values that
+ * are not finite there do not reach it.
  */
 int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld,
                      int64_t v_ld, const int32_t* cu_seqlens, int64_t N, void* o, float* lse,
@@ -354,6 +355,8 @@ size_t omx_gdn_attn_fwd_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64
  *   d_o          [B, T, Hq, D] bf16
  *   dq           [B, T, Hq, D], dk, dv [B, T, Hkv, D] bf16, dense; dk and dv are summed over each
  *                key head's query heads.  No sum depends on the order of execution.
+ * A value of a sequence's q, k, v or d_o that is not finite may reach all its gradients (the forward
+ * keeps rows from what lies behind them, the backward does not), those of others never.
  */
 int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld,
                      int64_t v_ld, const int32_t* cu_seqlens, int64_t N, const void* o,
@@ -377,7 +380,7 @@ size_t omx_gdn_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t
  *                A negative length marks a sequence that takes no part: nothing is written for
  *                it, and its outputs are zeros.
  * Tokens past table_width * page_size have no place: they are not written, and not attended.  A
- * page that is written to belongs to one sequence; others may be shared.
+ * page that is written to stands once in all of block_table; others may be shared.
  *
  * omx_gdn_kv_write appends the keys and values of new tokens: token i of sequence n goes to
  * position lengths[n] + i.  k, v, their strides and cu_seqlens as for omx_gdn_attn_fwd.

@@ -18,6 +18,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .deltanet import _cu_seqlens, _ptr, _stream, _workspace
@@ -123,7 +124,7 @@ def attention_prefill_bwd(q, k, v, o, lse, do, *, o_rest=None, cu_seqlens=None, 
     ``o`` and ``lse`` are what the forward returned with ``output_lse=True``.  ``o_rest``, what
     the rounding of o left (bf16, as o), makes dq and dk about 6% more exact; autograd keeps it.
     The gradients are dense bf16 tensors of the inputs' shapes; those of a key head are summed
-    over its query heads.
+    over its query heads.  A value of a sequence that is not finite may reach all of its gradients.
     """
     dev, q, k, v, q_ld, k_ld, v_ld, cu, N = _qkv(q, k, v, cu_seqlens)
     B, T, Hq, D = q.shape
@@ -160,6 +161,7 @@ class _AttentionPrefill(torch.autograd.Function):
         return o, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do, _dlse):
         if do is None:
             return None, None, None, None, None
@@ -176,8 +178,8 @@ def attention_prefill(q, k, v, *, cu_seqlens=None, scale=None, output_lse=False)
     key head; views into one projection are read in place).  ``cu_seqlens`` (int32 [N+1], B == 1)
     packs N sequences, as in ``gdn_prefill``.  ``scale`` defaults to D ** -0.5.  Returns o
     [B,T,Hq,D] bf16, or (o, lse) with the fp32 logarithms [B,T,Hq] of the softmax sums.  When
-    gradients are enabled and an input requires them, the call is recorded for autograd (not
-    through lse).
+    gradients are enabled and an input requires them, the call is recorded for autograd (once, and
+    not through lse).  A row sees no key after it, not even one that is not finite.
     """
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
         o, lse = _AttentionPrefill.apply(q, k, v, cu_seqlens, scale)
@@ -218,7 +220,7 @@ def kv_pages_write(k, v, k_pages, v_pages, block_table, lengths, *, cu_seqlens=N
 
     k, v [B,T,Hkv,D] bf16, N = B sequences of T tokens or N packed by ``cu_seqlens`` (B == 1).
     Token i of sequence n goes to position ``lengths[n] + i``; a position without a page is
-    left out.
+    left out.  A page that is written to must stand once in all of ``block_table``.
     """
     _no_grad_only("kv_pages_write", k, v, k_pages, v_pages)
     dev = _device(k, v)

@@ -23,7 +23,6 @@ namespace omx {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void;
-typedef __attribute__((address_space(3))) bf16_t lds_bf16;
 typedef __attribute__((address_space(1))) void glob_void;
 
 // C += A(32x16) B(16x32)

@@ -20,7 +20,6 @@ constexpr float kLow = -1e30f;
 
 constexpr int kNW = 4, kNT = 64 * kNW;
 
-
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
@@ -114,7 +113,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   typedef const __attribute__((address_space(4))) int32_t const_i32;
   const_i32* table = PAGED ? (const_i32*)(p.table + (long long)it.seq * p.table_w) : nullptr;
   int slot = 0, off = 0;
-  struct Pages { int id[4], off[4]; unsigned have; };
+  const int row_bytes = Hkv * D * 2;
+  struct Pages { long long at[4]; unsigned have, fetch; };  // byte offsets in a pool; none past the split
   auto look = [&](int kt) {
     Pages x;
     x.have = 0;
@@ -123,12 +123,13 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       const bool in = kt * kBN + 16 * g < keys && slot < p.table_w;
       int id = in ? table[slot] : -1;
       id = id >= p.n_pages ? -1 : id;
-      x.id[g] = __builtin_amdgcn_readfirstlane(id);
-      x.off[g] = off;
-      x.have |= x.id[g] >= 0 ? 1u << g : 0u;
+      id = __builtin_amdgcn_readfirstlane(id);
+      x.at[g] = ((long long)(id < 0 ? 0 : id) * p.page + off) * row_bytes + 2 * hk * D;
+      x.have |= id >= 0 ? 1u << g : 0u;
       off += 16;
       if (off >= p.page) { off = 0; ++slot; }
     }
+    x.fetch = kt < kt1 ? x.have : 0u;
     return x;
   };
   // Fetches a share of a tile of keys (or values) into LDS: NL instructions from the j0-th on.  They
@@ -143,10 +144,9 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
 #pragma unroll
       for (int j = j0; j < j0 + NL; ++j) {
         const int g0 = kStep * j / 16;  // the group of the instruction's rows
-        int id = x.id[g0], of = x.off[g0];
-        if (DP == 64 && w >= 2) { id = x.id[g0 + 1]; of = x.off[g0 + 1]; }
-        const long long at = ((long long)(id < 0 ? 0 : id) * p.page + of) * Hkv * D + hk * D;
-        load_to_lds16(rsrc_words((const bf16_t*)pool + at, id < 0 || kt >= kt1 ? 0 : 16u * ld2),
+        const bool next = DP == 64 && w >= 2;
+        const long long at = next ? x.at[g0 + 1] : x.at[g0];
+        load_to_lds16(rsrc_words((const char*)pool + at, (x.fetch >> (next ? g0 + 1 : g0)) & 1 ? 16u * ld2 : 0),
                       lds + 1024u * kNW * j, lane_off[j % NO]);
       }
     } else {

@@ -5,7 +5,6 @@
 #include <hip/hip_runtime.h>
 
 #include <climits>
-#include <cmath>
 
 #include "gdn_capi.h"
 #include "gdn_kernels.h"
@@ -56,7 +55,7 @@ int check_ld(const char* fn, const char* name, int64_t ld, int64_t least) {
 }
 
 int check_scale(const char* fn, float scale) {
-  REQUIRE(std::isfinite(scale) && scale > 0.f, "%s: scale must be positive and finite", fn);
+  REQUIRE(scale > 0.f && scale <= 1048576.f, "%s: scale must be positive and at most 2^20", fn);
   return OMX_GDN_OK;
 }
 
