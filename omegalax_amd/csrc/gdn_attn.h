@@ -192,6 +192,22 @@ __device__ __forceinline__ void wait_loads() {
   __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
+// A lane's fragments (elements 8h .. of each 16) of a row of D elements, D a multiple of 8.  No load
+// is behind a branch, where each would be waited for before the next; what lies past D is cleared
+// once all are issued.
+template <int KS>
+__device__ __forceinline__ void load_row(u32x4 (&x)[KS], const void* row, int D, int h) {
+#pragma unroll
+  for (int s = 0; s < KS; ++s) x[s] = *(const u32x4*)((const bf16_t*)row + (16 * s + 8 * h < D ? 16 * s + 8 * h : 0));
+}
+template <int KS>
+__device__ __forceinline__ void clear_past(u32x4 (&x)[KS], int D, int h) {
+  if (D == 16 * KS) return;
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    if (16 * s + 8 * h >= D) x[s] = u32x4{0, 0, 0, 0};
+}
+
 // One staging instruction writes 1 KiB of LDS, 64 / (DP / 8) rows.  Of a tile's instructions a
 // wavefront takes w, w + NW, ...: row of lane l in its j-th, and the segment it fetches.
 template <int DP, int NW>

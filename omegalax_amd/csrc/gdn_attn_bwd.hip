@@ -98,14 +98,12 @@ void attn_dkv_wide_kernel(AttnParams p, int ranks) {
   }
 
   u32x4 kf[KS], vf[KS];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int d = 16 * s + 8 * h;
-    kf[s] = vf[s] = u32x4{0, 0, 0, 0};
-    if (key < it.len && d < D) {
-      kf[s] = *(const u32x4*)((const bf16_t*)p.k + (it.start + key) * p.k_ld + hk * D + d);
-      vf[s] = *(const u32x4*)((const bf16_t*)p.v + (it.start + key) * p.v_ld + hk * D + d);
-    }
+  {
+    const long long tok = it.start + (key < it.len ? key : it.len - 1);
+    load_row(kf, (const bf16_t*)p.k + tok * p.k_ld + hk * D, D, h);
+    load_row(vf, (const bf16_t*)p.v + tok * p.v_ld + hk * D, D, h);
+    clear_past(kf, D, h);
+    clear_past(vf, D, h);
   }
   f32x16 dk[DB], dv[DB];
 #pragma unroll

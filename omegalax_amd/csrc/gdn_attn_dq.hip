@@ -71,20 +71,27 @@ void attn_dq_kernel(AttnParams p, int ranks) {
   }
 
   u32x4 q[KS], dout[KS];
-  float delta = 0.f;
+  float delta = 0.f, lse2;
+  {
+    u32x4 o[KS], rest[KS];
+    const long long rl = live ? tok : it.start + t0, al = rl * Hq + hk * G + (live ? rg : 0);
+    lse2 = p.lse[al] * kLog2e;
+    load_row(dout, (const bf16_t*)p.dout + al * D, D, h);
+    load_row(o, (const bf16_t*)p.o + al * D, D, h);
+    load_row(rest, (const bf16_t*)(p.o_rest ? p.o_rest : p.o) + al * D, D, h);
+    load_row(q, (const bf16_t*)p.q + rl * p.q_ld + (long long)(hk * G + (live ? rg : 0)) * D, D, h);
+    clear_past(dout, D, h);
+    clear_past(o, D, h);
+    clear_past(rest, D, h);
+    clear_past(q, D, h);
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int d = 16 * s + 8 * h;
-    q[s] = dout[s] = u32x4{0, 0, 0, 0};
-    if (live && d < D) {
-      q[s] = *(const u32x4*)((const bf16_t*)p.q + tok * p.q_ld + (long long)(hk * G + rg) * D + d);
-      dout[s] = *(const u32x4*)((const bf16_t*)p.dout + at * D + d);
-      delta = dot8(dout[s], *(const u32x4*)((const bf16_t*)p.o + at * D + d), delta);
-      if (p.o_rest) delta = dot8(dout[s], *(const u32x4*)((const bf16_t*)p.o_rest + at * D + d), delta);
-    }
+    for (int s = 0; s < KS; ++s) delta = dot8(dout[s], o[s], delta);
+    if (p.o_rest)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) delta = dot8(dout[s], rest[s], delta);
   }
   delta = sum_halves(delta);
-  const float lse2 = live ? p.lse[at] * kLog2e : INFINITY;  // idle rows: weights of 0
+  lse2 = live ? lse2 : INFINITY;  // idle rows: weights of 0
   if (live && h == 0) {
     float* st = p.stats + 2 * (tok * Hq + hk * G) + rg;
     st[0] = lse2;
