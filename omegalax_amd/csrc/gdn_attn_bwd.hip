@@ -20,6 +20,9 @@ constexpr int kRows = 32, kRing = 4;  // a stage's rows, stages in LDS
 // stages of 32 rows go past them through a ring in LDS.  A stage is four phases, one product after
 // the other with the loads and arithmetic that run beside it:
 //   S = Q K^T | dP = dO V^T, P = exp(S - lse) | dV^T += dO^T P, dS = P (dP - delta) | dK^T += Q^T dS
+// 3,001 tokens in 5 sequences of 16/2 heads of 256: 74 us (125 with stages of 64 rows twice buffered,
+// the compiler's order and whole tiles in four shares each).  A stage takes 1.5 times its MFMAs; the
+// rest is what comes before the first stage and the partial sums behind the last, about 14 us.
 template <int DP>
 __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(1)))
 void attn_dkv_wide_kernel(AttnParams p, int ranks) {

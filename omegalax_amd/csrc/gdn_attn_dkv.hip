@@ -17,7 +17,8 @@ constexpr int kNW = 4, kNT = 64 * kNW;
 //   1: S and dP of the next stage | P and dS of this one | reads of its transposed fragments
 //   2: dV and dK of this stage    | reads of the next but one's fragments, and the next's lse, delta
 // The order is pinned group by group; left to itself the compiler put all products of a phase
-// behind all loads, two reads ahead (B=4 T=4,096 of 32/8 heads of 128: 1,690 us).  Stages lie in
+// behind all loads, two reads ahead (B=4 T=4,096 of 32/8 heads of 128: 1,690 us, now 1,150; the
+// MFMAs are busy for 56% of it, the clock falls to 1.9 GHz under them).  Stages lie in
 // a ring of six LDS buffers, filled from memory directly.
 constexpr int kRows = 32;        // rows of a stage
 constexpr int kRing = 6;
