@@ -31,7 +31,7 @@ SHAPES = [
     (dict(cu=16), _lib.EINVAL, "batch 1"), (dict(cu=16, B=1, N=0), _lib.EINVAL, "sequence count"),
     (dict(q_ld=504), _lib.EINVAL, "q_ld"), (dict(k_ld=260), _lib.EINVAL, "k_ld"), (dict(v_ld=1 << 23), _lib.EINVAL, "v_ld"),
     (dict(scale=0.0), _lib.EINVAL, "scale"), (dict(scale=float("nan")), _lib.EINVAL, "scale"),
-    (dict(scale=-1.0), _lib.EINVAL, "scale"), (dict(q=None), _lib.EINVAL, "NULL"), (dict(o=None), _lib.EINVAL, "NULL"),
+    (dict(scale=-1.0), _lib.EINVAL, "scale"), (dict(scale=2e6), _lib.EINVAL, "scale"), (dict(q=None), _lib.EINVAL, "NULL"), (dict(o=None), _lib.EINVAL, "NULL"),
     (dict(v=24), _lib.EINVAL, "aligned"),
 ]
 

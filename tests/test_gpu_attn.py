@@ -61,6 +61,31 @@ def test_batches_and_their_gradients(B, T, Hq, Hkv, D):
     check_prefill(q, k, v, spans_of(B, T, None), do=do)
 
 
+@pytest.mark.parametrize("B,T,Hq,Hkv,D", [(1, 900, 7, 1, 128), (1, 700, 32, 1, 256), (1, 1500, 5, 1, 64),
+                                          (3, 600, 3, 1, 256), (1, 1300, 2, 2, 200)])
+def test_few_tiles_of_keys_share_their_rows(B, T, Hq, Hkv, D):
+    say(f"shares of rows B={B} T={T} Hq={Hq} Hkv={Hkv} D={D}")
+    q, k, v, do = (draw(2 * T + i, B, T, h, D) for i, h in enumerate((Hq, Hkv, Hkv, Hq)))
+    check_prefill(q, k, v, spans_of(B, T, None), do=do)
+
+
+def test_packed_rows_past_32_bit_offsets():
+    """2.5 billion elements of q: short sequences at the end, by themselves bit for bit."""
+    N, L, Hq, Hkv, D = 6000, 101, 32, 8, 128
+    T = N * L
+    say(f"{T} tokens of {Hq} heads of {D}")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, do = (torch.randn((1, T, h, D), generator=g, device="cuda", dtype=BF) for h in (Hq, Hkv, Hkv, Hq))
+    cu = torch.arange(0, T + 1, L, dtype=torch.int32, device="cuda")
+    run = lambda q, k, v, do, cu: [*(r := om.attention_prefill(q, k, v, cu_seqlens=cu, output_lse=True)),
+                                   *om.attention_prefill_bwd(q, k, v, *r, do, cu_seqlens=cu)]
+    got = run(q, k, v, do, cu)
+    for n in (0, 3000, N - 1):
+        part = [t[:, n * L:(n + 1) * L] for t in (q, k, v, do)]
+        for a, b in zip(got, run(*part, None)):
+            assert torch.equal(a[:, n * L:(n + 1) * L], b)
+
+
 @pytest.mark.parametrize("D", [8, 24, 80, 96, 136, 200, 248])
 def test_head_dims_between_the_compiled_ones(D):
     say(f"attention D={D}")
@@ -257,10 +282,43 @@ def test_repeated_calls_are_equal_and_other_streams_too():
         assert torch.equal(a, b)
 
 
-def test_captured_forward_and_backward():
-    T = 260
-    x = [draw(i, 1, T, h, 64) for i, h in enumerate((4, 2, 2))]
-    do = draw(5, 1, T, 4, 64)
+def test_streams_at_once():
+    """Two streams' forward and backward calls of their own, at the same time."""
+    sets = [[draw(10 * i + j, 1, 1200, h, D) for j, h in enumerate((8, 2, 2, 8))] for i, D in enumerate((128, 256))]
+    run = lambda q, k, v, do: [*(r := om.attention_prefill(q, k, v, output_lse=True)),
+                               *om.attention_prefill_bwd(q, k, v, *r, do)]
+    want = [run(*s) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(*sets[i]))
+    torch.cuda.synchronize()
+    for w, rs in zip(want, got):
+        for r in rs:
+            assert all(torch.equal(a, b) for a, b in zip(w, r))
+
+
+def test_cotangents_of_any_layout_and_one_derivative():
+    q, k, v = (draw(i, 2, 90, h, 64).requires_grad_(True) for i, h in enumerate((4, 2, 2)))
+    one = torch.ones(2, 90, 4, 64, dtype=BF, device="cuda")
+    want = torch.autograd.grad(om.attention_prefill(q, k, v), (q, k, v), one)
+    got = torch.autograd.grad(om.attention_prefill(q, k, v).sum(), (q, k, v))  # an expanded cotangent
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    got = torch.autograd.grad(om.attention_prefill(q, k, v).transpose(1, 2), (q, k, v),
+                              one.transpose(1, 2).contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    dq, = torch.autograd.grad(om.attention_prefill(q, k, v).float().pow(2).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.float().sum(), k)
+
+
+@pytest.mark.parametrize("T,D", [(260, 64), (900, 128), (700, 256)])
+def test_captured_forward_and_backward(T, D):
+    x = [draw(i, 1, T, h, D) for i, h in enumerate((4, 2, 2))]
+    do = draw(5, 1, T, 4, D)
     cu = torch.tensor([0, 100, 100, T], dtype=torch.int32, device="cuda")
 
     def both():

@@ -278,10 +278,50 @@ def test_shared_pages():
         check(f"sequence {n}", o[n:n + 1], val["o"], tol["o"])
 
 
-def test_captured_decode_steps():
+@pytest.mark.parametrize("N,room", [(3, 40), (70, 5)])
+def test_captured_turns(N, room):
+    """An append and its attention captured once, replayed with other lengths, offsets and pages."""
+    Hq, Hkv, D, page, T = 8, 2, 128, 16, 60 if N == 3 else 150
+    held = [37 * n % 900 for n in range(N)]
+    c, e = (Cache(held, [page + room] * N, page, Hkv, D) for _ in range(2))
+    q, k, v = draw(1, 1, T, Hq, D), draw(2, 1, T, Hkv, D), draw(3, 1, T, Hkv, D)
+    cu = torch.tensor([n * T // N for n in range(N + 1)], dtype=torch.int32, device="cuda")
+
+    def turn(c):
+        om.kv_pages_write(k, v, *c.args(), cu_seqlens=cu)
+        return om.attention_prefill_paged(q, *c.args(), cu_seqlens=cu)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    pools = c.k_pages.clone(), c.v_pages.clone()
+    with torch.cuda.stream(side):
+        turn(c)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = turn(c)
+    c.k_pages.copy_(pools[0])
+    c.v_pages.copy_(pools[1])
+    for r in range(3):
+        for i, t in enumerate((q, k, v)):
+            t.copy_(draw(50 + 3 * r + i, *t.shape))
+        lens = torch.tensor([max(0, h - 5 * r) if n % 7 != 3 else -1 for n, h in enumerate(held)], dtype=torch.int32)
+        order = torch.randperm(N, generator=torch.Generator().manual_seed(r))  # whole tables change hands
+        for x in (c, e):
+            x.lengths.copy_(lens[order] if r else lens)
+            x.block_table.copy_(x.table[order] if r else x.table)
+        want = turn(e)
+        g.replay()
+        torch.cuda.synchronize()
+        assert equal(o, want) and bool(o.isfinite().all())
+        same_pools(c, (e.k_pages, e.v_pages))
+
+
+@pytest.mark.parametrize("width", [0, 200])
+def test_captured_decode_steps(width):
     """One captured step, replayed as the lengths grow, with eager steps of another cache between."""
     Hq, Hkv, D, page = 8, 2, 128, 16
-    c, e = (Cache([500, 30, 700], [8] * 3, page, Hkv, D) for _ in range(2))
+    c, e = (Cache([500, 30, 700], [8] * 3, page, Hkv, D, width=width) for _ in range(2))
     q, k, v = draw(1, 3, Hq, D), draw(2, 3, Hkv, D), draw(3, 3, Hkv, D)
     c0 = c.k_pages.clone(), c.v_pages.clone()
     side = torch.cuda.Stream()
