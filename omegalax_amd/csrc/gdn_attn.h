@@ -155,14 +155,6 @@ __device__ __forceinline__ void load_to_lds16(u32x4 rsrc, unsigned lds, unsigned
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory");
 }
-// (from a uniform base address and a lane's offset, without a range)
-__device__ __forceinline__ void load_to_lds16(const void* base, unsigned lds, unsigned off) {
-  const unsigned long long a = (unsigned long long)base;
-  const unsigned long long u = (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)a) |
-                               (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32)) << 32;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
-               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(u) : "memory");
-}
 // several of them, each 4 KiB further in LDS: a workgroup of four wavefronts takes turns
 __device__ __forceinline__ void loads_to_lds16(u32x4 rsrc, unsigned lds, const unsigned (&off)[4]) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
@@ -364,10 +356,8 @@ constexpr int kDkvKeys = 128;
 // Work of a workgroup of the kernels that sum dk and dv: rows of tokens [ta, tb), whole stages of
 // `per` and at least one, for the 128 keys from k0 on.  When there are few tiles, workgroups share a
 // tile's rows.  Those grow with the tile's place j, counted from its sequence's end: it has
-// ceil((j + 1) / m) shares, with m such that the longest tile has `splits`, so that shares are alike.
-// Measured with both passes of the backward, 16 query heads on 2 key heads of 256: 1,000 tokens 450
-// us with whole tiles, 134 with shares, 4,000 tokens 1,732 and 654; 32 on 8 of 128: 1,000 tokens 139
-// and 99, 4,000 tokens 617 and 572.
+// ceil((j + 1) / m) shares, so that shares are alike, with m = p.share_tiles unless the longest tile
+// would have more than `splits` then.
 struct DkvShare {
   int len, k0, ta, tb, share, shares;
   long long start;
@@ -386,7 +376,8 @@ __device__ __forceinline__ bool dkv_share(const AttnParams& p, int row, int rank
     int first = 0, n = lane_id() == 0 ? p.T : 0;  // lane i: sequence i
     if (p.cu) packed_span(p.cu, p.N, p.T, first, n);
     const int nt = (n + kDkvKeys - 1) / kDkvKeys;
-    const int m = (__builtin_amdgcn_readlane(wave_scan_max(nt), 63) + p.splits - 1) / p.splits;
+    const int least = (__builtin_amdgcn_readlane(wave_scan_max(nt), 63) + p.splits - 1) / p.splits;
+    const int m = p.share_tiles > least ? p.share_tiles : least;
     int mine = 0;  // nt tiles' shares, m tiles a time
     for (int q = 0; q < p.splits; ++q) {
       const int left = nt - q * m;

@@ -178,7 +178,7 @@ namespace {
 struct AttnBwdWs {
   size_t stats;
   PlanWs rows, keys;
-  int splits;
+  omx::DkvPlan share;
   size_t shares, part_k, part_v, total;
 };
 AttnBwdWs attn_bwd_ws(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N) {
@@ -186,10 +186,10 @@ AttnBwdWs attn_bwd_ws(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, 
   const int per = omx::attn_dkv_tile_tokens();
   w.rows = plan_ws(align_up((size_t)(B * T * Hq) * 8), T, N, omx::attn_tile_tokens((int)(Hq / Hkv)));
   w.keys = plan_ws(w.rows.total, T, N, per);
-  w.splits = omx::attn_dkv_splits(B * Hkv, T, N, (int)(Hq / Hkv));
+  w.share = omx::attn_dkv_plan(B * Hkv, T, N, (int)(Hq / Hkv), B * T * Hkv * D * 8);
   w.shares = w.part_k = w.part_v = w.total = w.keys.total;
-  if (w.splits > 1) {
-    const size_t one = align_up((size_t)w.splits * B * T * Hkv * D * 4);
+  if (w.share.splits > 1) {
+    const size_t one = align_up((size_t)w.share.splits * B * T * Hkv * D * 4);
     w.part_k = w.shares + align_up((size_t)(B * T * Hkv) * 4);
     w.part_v = w.part_k + one;
     w.total = w.part_v + one;
@@ -235,7 +235,8 @@ int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, 
   p.shares = (int32_t*)((char*)workspace + ws.shares);
   p.part_k = (float*)((char*)workspace + ws.part_k);
   p.part_v = (float*)((char*)workspace + ws.part_v);
-  p.splits = ws.splits;
+  p.splits = ws.share.splits;
+  p.share_tiles = ws.share.tiles;
   const hipStream_t st = (hipStream_t)stream;
   hipError_t e = use_plan(p, ws.rows, workspace, per, st);
   if (e == hipSuccess) e = omx::launch_attn_dq(p, st);

@@ -293,6 +293,7 @@ struct AttnParams {
   void *dq, *dk, *dv;
   float *part_k, *part_v;      // dk and dv in shares of the rows, `splits` of them at most
   int32_t* shares;             // and of each key's tile how many, when that is more than one
+  int share_tiles;             // rows in a share, in tiles of 128 tokens
 };
 constexpr int kAttnMaxG = 32, kAttnMaxD = 256;
 // tokens per tile of the forward, tiles of a row at most, and int32 words of the plan
@@ -305,7 +306,10 @@ hipError_t launch_attn_join(const AttnParams& p, hipStream_t stream);
 
 // the backward: dq and delta, then dk and dv (keys per tile of the second: its plan's tokens)
 int attn_dkv_tile_tokens();
-int attn_dkv_splits(long long units, long long T, long long N, int G);
+struct DkvPlan {
+  int splits, tiles;  // shares of a tile at most, tiles' rows in a share
+};
+DkvPlan attn_dkv_plan(long long units, long long T, long long N, int G, long long row_bytes);
 hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream);
 void launch_attn_dkv_narrow(const AttnParams& p, unsigned grid, int ranks, hipStream_t stream);  // D <= 128
 hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream);
