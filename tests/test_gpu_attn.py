@@ -95,7 +95,7 @@ def test_head_dims_between_the_compiled_ones(D):
 
 PACKS = [
     [1, 1, 1], [5, 0, 0, 130, 1, 64], [0, 0, 300, 0], [63, 64, 65, 127, 128, 129, 2],
-    [700, 3, 90], [796, 842, 265], [17] * 64, [9, 0, 40] * 30, [1] * 200, [2000, 1] + [33] * 70,
+    [700, 3, 90], [796, 842, 265], [0, 1500, 0, 33], [1800, 20, 50, 7, 300], [17] * 64, [9, 0, 40] * 30, [1] * 200, [2000, 1] + [33] * 70,
 ]
 
 
