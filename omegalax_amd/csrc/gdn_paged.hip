@@ -275,13 +275,17 @@ void attn_decode_kernel(AttnParams p) {
           s[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], cs, -mc));
           ls[n] += s[g][i];
         }
+        // the weights as two bf16 terms (2^-17 together): a step is bound by its bytes, and one term's
+        // rounding was half of its error (2.5e-3 against 64 bits, 1.6e-3 the output's own)
         const u32x2 pb = u32x2{pack_bf16(s[g][0], s[g][1]), pack_bf16(s[g][2], s[g][3])};
+        const u32x2 pr = u32x2{pack_bf16(lo_part(s[g][0]), lo_part(s[g][1])), pack_bf16(lo_part(s[g][2]), lo_part(s[g][3]))};
         const int vr = 16 * g + 4 * g4 + (r >> 2);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           const int col = 16 * d + 4 * (r & 3);
           const u32x2 a = ds_read_tr(sv + vr * DP + (((col >> 3) ^ attn_swz<DP>(vr)) << 3) + (col & 7));
           o[n][d] = mma_pv(a, pb, o[n][d]);
+          o[n][d] = mma_pv(a, pr, o[n][d]);
         }
       }
     }
