@@ -97,10 +97,11 @@ hipError_t use_plan(omx::AttnParams& p, const PlanWs& w, void* workspace, int pe
   return omx::launch_attn_plan(p, per, stream);
 }
 
-// Splits of the keys of a paged prefill: few rows leave compute units idle.
-int paged_splits(int64_t N, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t capacity) {
-  const int64_t per = omx::attn_tile_tokens((int)(Hq / Hkv));
-  const int64_t tiles = ((tokens + per - 1) / per + N - 1) * Hkv;
+// Splits of the keys of a paged prefill: few rows leave compute units idle.  Each row of a batch has
+// its own tiles; packed sequences add at most one tile each to those of all their tokens.
+int paged_splits(const Shape& x, int64_t capacity) {
+  const int64_t per = omx::attn_tile_tokens((int)(x.Hq / x.Hkv)), each = (x.T + per - 1) / per;
+  const int64_t tiles = (x.packed ? each + x.N - 1 : x.N * each) * x.Hkv;
   int64_t s = tiles > 0 ? 512 / tiles : 1;
   const int64_t most = capacity / 128;
   s = s < most ? s : most;
@@ -289,7 +290,7 @@ struct PagedWs {
 PagedWs paged_ws(const Shape& s, int64_t capacity) {
   PagedWs w{};
   w.plan = plan_ws(0, s.T, s.packed ? s.N : 0, omx::attn_tile_tokens((int)(s.Hq / s.Hkv)));
-  w.splits = paged_splits(s.N, s.T, s.Hq, s.Hkv, capacity);
+  w.splits = paged_splits(s, capacity);
   w.split = split_ws(w.plan.total, w.splits, s.B * s.T * s.Hq, s.D);
   w.total = w.split.total;
   return w;

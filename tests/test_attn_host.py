@@ -105,6 +105,27 @@ def test_decode_refuses(over, code, msg):
     assert rc == code and msg in err
 
 
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,page,width", [(8, 512, 32, 8, 128, 64, 128), (16, 512, 16, 2, 256, 64, 128),
+                                                     (16, 256, 16, 2, 256, 16, 1000), (1000, 1, 8, 1, 64, 16, 2000)])
+def test_a_batch_that_fills_the_chip_reads_its_cache_whole(B, T, Hq, Hkv, D, page, width):
+    """Every row has its own tiles: 512 of them leave nothing to share, packed or not, and no
+    partial sums are kept."""
+    size = _lib.lib().omx_gdn_attn_paged_workspace_size
+    assert B * -(-T // (128 // (Hq // Hkv))) * Hkv >= 512
+    assert size(B, T, Hq, Hkv, D, B, 0, page, width) == 0
+
+
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,page,width,shares", [
+    (2, 40, 4, 1, 128, 64, 100, 32), (4, 100, 8, 2, 64, 16, 250, 16), (3, 130, 2, 2, 256, 48, 50, 18), (2, 1, 8, 8, 64, 16, 20, 2)])
+def test_rows_that_leave_the_chip_idle_share_their_keys(B, T, Hq, Hkv, D, page, width, shares):
+    """Shares of 512 workgroups, 32 at most, none of less than 128 keys."""
+    size = _lib.lib().omx_gdn_attn_paged_workspace_size
+    tiles = B * -(-T // (128 // (Hq // Hkv))) * Hkv
+    assert shares == min(512 // tiles, 32, page * width // 128)
+    up = lambda x: -(-x // 256) * 256
+    assert size(B, T, Hq, Hkv, D, B, 0, page, width) == up(shares * B * T * Hq * D * 4) + up(shares * B * T * Hq * 8)
+
+
 def test_empty_calls_are_no_ops():
     assert _run("omx_gdn_attn_fwd", FWD, dict(T=0, q=None, o=None))[0] == _lib.OK
     assert _run("omx_gdn_attn_bwd", BWD, dict(B=0, N=0, q=None))[0] == _lib.OK

@@ -100,6 +100,34 @@ def test_unpacked_rows(B, T):
         check(f"o of row {n}", o[n], val["o"], tol["o"])
 
 
+def shares(B, T, Hq, Hkv, D, c, packed=False):
+    """Of a turn's keys, by the workspace for their partial sums."""
+    size = om._lib.lib().omx_gdn_attn_paged_workspace_size(B, T, Hq, Hkv, D, len(c.held), packed, c.page, c.table.shape[1])
+    return max(1, size // (B * T * Hq * (D + 2) * 4))
+
+
+@pytest.mark.parametrize("held,T,page,Hq,Hkv,D,split", [
+    ([3000, 0, 1111], 20, 64, 4, 1, 128, True), ([2000, 900], 70, 16, 8, 2, 64, True), ([1500, 2222, 5, 640], 33, 48, 8, 1, 256, True),
+    ([700, -1, 2500], 1, 64, 32, 1, 128, True), ([600, 900, 0, 300, 1100, 20, 450, 800], 300, 64, 16, 8, 64, False),
+])
+def test_rows_of_a_batch_over_long_caches(held, T, page, Hq, Hkv, D, split):
+    """Rows that are not packed, few of them with their keys in shares and enough without."""
+    say(f"batch over long caches held={held} T={T} Hq={Hq} Hkv={Hkv} D={D}")
+    B = len(held)
+    c = Cache(held, [T] * B, page, Hkv, D, seed=B)
+    assert (shares(B, T, Hq, Hkv, D, c) > 1) == split
+    q, k, v = draw(1, B, T, Hq, D, scale=1.5), draw(2, B, T, Hkv, D), draw(3, B, T, Hkv, D)
+    om.kv_pages_write(k, v, *c.args())
+    o = om.attention_prefill_paged(q, *c.args())
+    for n in range(B):
+        if held[n] < 0:
+            assert not bool(o[n].any())
+            continue
+        val, tol = one_sequence(q[n].double(), torch.cat([c.keys[n], k[n]]).double(),
+                                torch.cat([c.values[n], v[n]]).double(), held[n])
+        check(f"o of row {n}", o[n], val["o"], tol["o"])
+
+
 @pytest.mark.parametrize("new,held", [(2, 4000), (40, 3000), (130, 5000)])
 @pytest.mark.parametrize("Hq,Hkv,D", [(4, 1, 128), (2, 2, 64), (8, 1, 256)])
 def test_few_rows_over_a_long_cache(new, held, Hq, Hkv, D):
