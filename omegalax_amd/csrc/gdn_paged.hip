@@ -487,12 +487,14 @@ hipError_t launch_kv_write(const AttnParams& p, hipStream_t stream) {
 }
 
 int decode_splits(long long N, long long Hkv, long long D, long long capacity) {
-  // One workgroup a sequence and key head where that is enough for the chip twice over, or where a
-  // sequence is so short that the join costs more than it saves (B=1, 4 key heads of 128, 611 keys:
-  // 12.7 us in one launch, 16.8 in two; at 1,500 keys 18.9 and 16.8).  Otherwise one for each
-  // compute unit: their buffers allow no second (64 ragged sequences of 2 heads of 256: 119.6 us
-  // with two rounds of workgroups, 115.4 with one).
-  if (N * Hkv >= 512 || capacity * D <= (1 << 17)) return 1;
+  // One workgroup a sequence and key head where a sequence is so short that the join costs more than
+  // it saves (B=1, 4 key heads of 128, calls one after the other: 611 keys 14.4 us in one launch, 18.5 in
+  // two, 1,500 keys 21.8 and 18.0), and for more than 1,024 sequences, each row's join summing up all their lengths.
+  // Otherwise one for each compute unit: their buffers allow no second.  Equal ranges against a
+  // workgroup each, 32/8 heads of 128: 64 sequences of 4,000 keys 190 us (187), between 1,000 and 7,000
+  // 207 (230), 63 of 1,000 and one of 30,000 84 (380); 1,024 of 100 199 (196), with one of 30,000 244 (532).
+  // 16/2 heads of 256, sequences of 75 to 525 keys: 512 98 (81), 1,024 182 (156), 4,096 723 (579).
+  if (N > 1024 || capacity * D <= (1 << 17)) return 1;
   if (N * (capacity / 16 + 1) > INT_MAX) return 1;  // stages are counted in 32 bits
   const long long s = 256 / Hkv;
   return (int)(s < 2 ? 1 : s);

@@ -126,6 +126,17 @@ def test_rows_that_leave_the_chip_idle_share_their_keys(B, T, Hq, Hkv, D, page, 
     assert size(B, T, Hq, Hkv, D, B, 0, page, width) == up(shares * B * T * Hq * D * 4) + up(shares * B * T * Hq * 8)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,D,page,width,ranges", [
+    (64, 32, 8, 128, 64, 70, 32), (128, 32, 8, 128, 64, 70, 32), (1024, 8, 1, 64, 16, 200, 256), (512, 16, 2, 256, 64, 10, 128),
+    (1025, 8, 1, 64, 16, 200, 0), (64, 32, 8, 128, 64, 16, 0), (1, 16, 4, 128, 16, 64, 0), (1, 16, 4, 128, 16, 65, 64)])
+def test_decode_batches_share_the_keys_in_equal_ranges(B, Hq, Hkv, D, page, width, ranges):
+    """One workgroup for each compute unit, whatever the number of sequences, up to 1,024 and but for
+    the shortest tables; their partial sums are a sequence's segments."""
+    size = _lib.lib().omx_gdn_attn_decode_workspace_size
+    rows, up = (ranges + B) * Hq if ranges else 0, lambda x: -(-x // 256) * 256
+    assert size(B, Hq, Hkv, D, page, width) == up(rows * D * 4) + up(rows * 8)
+
+
 def test_empty_calls_are_no_ops():
     assert _run("omx_gdn_attn_fwd", FWD, dict(T=0, q=None, o=None))[0] == _lib.OK
     assert _run("omx_gdn_attn_bwd", BWD, dict(B=0, N=0, q=None))[0] == _lib.OK

@@ -172,6 +172,44 @@ def test_decode_steps(held, page, Hq, Hkv, D, width):
         c.lengths += 1
 
 
+def segments(c, Hq):
+    """Room for a decode step's partial sums, in sequences' segments: none in one launch."""
+    N, Hkv, D = len(c.held), c.Hkv, c.D
+    size = om._lib.lib().omx_gdn_attn_decode_workspace_size(N, Hq, Hkv, D, c.page, c.table.shape[1])
+    return size // (Hq * (D + 2) * 4)
+
+
+def step_and_check(c, Hq, seed=50):
+    """One decode step; sequences of negative length take no part."""
+    B, Hkv, D, held = len(c.held), c.Hkv, c.D, c.held
+    q, k, v = draw(seed, B, Hq, D, scale=1.5), draw(seed + 1, B, Hkv, D), draw(seed + 2, B, Hkv, D)
+    want = c.k_pages.clone(), c.v_pages.clone()
+    for n in range(B):
+        if held[n] >= 0:
+            c.put(n, held[n], k[n:n + 1], v[n:n + 1], want)
+    o = om.attention_decode_step(q, k, v, *c.args())
+    same_pools(c, want)
+    for n in range(B):
+        if held[n] < 0:
+            assert not bool(o[n].any())
+            continue
+        val, tol = one_sequence(q[n:n + 1].double(), torch.cat([c.keys[n], k[n:n + 1]]).double(),
+                                torch.cat([c.values[n], v[n:n + 1]]).double(), held[n])
+        check(f"sequence {n}", o[n:n + 1], val["o"], tol["o"])
+
+
+@pytest.mark.parametrize("held,page,Hq,Hkv,D,width", [
+    ([40] * 63 + [2500], 64, 16, 8, 128, 0), ([3000] + [97 * n % 200 for n in range(64)], 16, 8, 8, 64, 0),
+    ([31 * n % 300 for n in range(256)] + [-1], 64, 4, 2, 256, 100), ([7] * 512, 16, 2, 1, 128, 80),
+], ids=lambda x: str(x)[:12])
+def test_decode_steps_of_large_batches(held, page, Hq, Hkv, D, width):
+    """At least 512 sequences' key heads, of lengths that differ: equal ranges of the keys, joined."""
+    say(f"decode, large batch of {len(held)}, Hq={Hq} Hkv={Hkv} D={D}")
+    c = Cache(held, [1] * len(held), page, Hkv, D, seed=9, width=width)
+    assert len(held) * Hkv >= 512 and segments(c, Hq) == 256 // Hkv + len(held)
+    step_and_check(c, Hq)
+
+
 @pytest.mark.parametrize("decode", [False, True])
 def test_pages_that_are_none_and_sequences_that_take_no_part(decode):
     """Tokens of entries outside the pool are left out; negative lengths give zeros; nothing is
