@@ -410,3 +410,34 @@ def test_captured_decode_steps(width):
         assert torch.equal(o, want)
         same_pools(c, (e.k_pages, e.v_pages))
         e.lengths += 1
+
+
+def ragged(N, most, seed):
+    """Lengths up to `most`, some of them zero, some negative."""
+    g = torch.Generator().manual_seed(seed)
+    held = torch.randint(0, most, (N,), generator=g).tolist()
+    return [(-1 if n % 11 == 7 else 0 if n % 13 == 5 else h) for n, h in enumerate(held)]
+
+
+@pytest.mark.parametrize("held,page,Hq,Hkv,D,width", [
+    (ragged(90, 300, 1), 64, 16, 2, 64, 40), (ragged(90, 250, 2), 16, 8, 2, 128, 70), (ragged(90, 200, 3), 48, 12, 1, 256, 12),
+    (ragged(200, 150, 4), 32, 34, 2, 128, 40), ([-1] * 70 + [2000] + [-1, 0, 3], 64, 8, 1, 64, 40),
+], ids=lambda x: str(x)[:12])
+def test_decode_ranges_of_more_than_64_sequences(held, page, Hq, Hkv, D, width):
+    """Ranges found past the first 64 sequences, joined with a wavefront a row."""
+    say(f"decode, ranges of {len(held)} sequences, Hq={Hq} Hkv={Hkv} D={D}")
+    c = Cache(held, [1 if h >= 0 else 0 for h in held], page, Hkv, D, seed=3, width=width)
+    assert len(held) > 64 and len(held) * Hq > 512 and segments(c, Hq) > len(held)
+    step_and_check(c, Hq)
+
+
+@pytest.mark.parametrize("held,page,Hq,Hkv,D", [
+    ([10300], 64, 4, 1, 256), ([5, 9000, 0], 128, 8, 2, 256), ([21000], 256, 2, 1, 128), ([0, 20000] + [3] * 70, 64, 8, 1, 128)])
+def test_decode_rows_of_more_than_64_segments(held, page, Hq, Hkv, D):
+    """A sequence whose keys are so many ranges that its join passes over their sums in turns of 64."""
+    say(f"decode, many segments held={held[:4]} Hq={Hq} Hkv={Hkv} D={D}")
+    c = Cache(held, [1] * len(held), page, Hkv, D, seed=4)
+    stages = [-(-(h + 1) * D // 4096) for h in held]
+    ranges = segments(c, Hq) - len(held)
+    assert ranges == 256 // Hkv and max(stages) // max(8, -(-sum(stages) // ranges)) > 64
+    step_and_check(c, Hq)
