@@ -21,7 +21,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .deltanet import _cu_seqlens, _ptr, _stream, _workspace
+from .deltanet import _cu_seqlens, _no_tangents, _ptr, _stream, _workspace
 
 __all__ = ["attention_prefill", "attention_prefill_bwd", "attention_prefill_paged",
            "attention_decode_step", "kv_pages_write"]
@@ -126,6 +126,7 @@ def attention_prefill_bwd(q, k, v, o, lse, do, *, o_rest=None, cu_seqlens=None, 
     The gradients are dense bf16 tensors of the inputs' shapes; those of a key head are summed
     over its query heads.  A value of a sequence that is not finite may reach all of its gradients.
     """
+    _no_tangents("attention_prefill_bwd", q, k, v, o, lse, do, o_rest)
     dev, q, k, v, q_ld, k_ld, v_ld, cu, N = _qkv(q, k, v, cu_seqlens)
     B, T, Hq, D = q.shape
     Hkv = k.shape[2]
@@ -179,8 +180,10 @@ def attention_prefill(q, k, v, *, cu_seqlens=None, scale=None, output_lse=False)
     packs N sequences, as in ``gdn_prefill``.  ``scale`` defaults to D ** -0.5.  Returns o
     [B,T,Hq,D] bf16, or (o, lse) with the fp32 logarithms [B,T,Hq] of the softmax sums.  When
     gradients are enabled and an input requires them, the call is recorded for autograd (once, and
-    not through lse).  A row sees no key after it, not even one that is not finite.
+    not through lse); forward-mode derivatives are refused.  A row sees no key after it, not even one
+    that is not finite.
     """
+    _no_tangents("attention_prefill", q, k, v)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
         o, lse = _AttentionPrefill.apply(q, k, v, cu_seqlens, scale)
     else:
@@ -213,6 +216,7 @@ def _no_grad_only(name, *ts):
     for t in ts:
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name}: gradients through the cache are not supported")
+    _no_tangents(name, *ts)
 
 
 def kv_pages_write(k, v, k_pages, v_pages, block_table, lengths, *, cu_seqlens=None):

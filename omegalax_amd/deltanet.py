@@ -13,6 +13,7 @@ no fallback: a missing library or a CPU tensor raises.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -68,6 +69,15 @@ def _f32(t):
     if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
         return t
     return t.to(torch.float32).contiguous()
+
+
+def _no_tangents(name, *ts):
+    """The kernels would drop a dual tensor's tangent: such a call is refused."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no forward-mode level is entered
+        return
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name}: forward-mode derivatives are not supported")
 
 
 def _cu_seqlens(cu, B, T, dev):

@@ -154,3 +154,30 @@ def test_python_checks_before_the_library():
     with pytest.raises(ValueError, match="GPU"):
         om.attention_decode_step(q[0], q[0], q[0], q, q, torch.zeros(4, 1, dtype=torch.int32),
                                  torch.zeros(4, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("dual", range(5))
+def test_forward_mode_derivatives_are_refused(dual):
+    """A dual tensor's tangent would be lost: no entry point takes one, with or without no_grad."""
+    torch = pytest.importorskip("torch")
+    from torch.autograd import forward_ad
+    import omegalax_amd as om
+    q = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16)
+    lse, table, lengths = torch.zeros(1, 4, 2), torch.zeros(4, 1, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    calls = [(lambda *x: om.attention_prefill(*x), [q] * 3), (lambda *x: om.attention_prefill_bwd(*x[:4], lse, x[4]), [q] * 5),
+             (lambda *x: om.kv_pages_write(*x, table, lengths), [q] * 4),
+             (lambda *x: om.attention_prefill_paged(*x, table, lengths), [q] * 3),
+             (lambda *x: om.attention_decode_step(*x, table, lengths), [q[0]] * 3 + [q] * 2)]
+    for call, args in calls:
+        if dual >= len(args):
+            continue
+        with forward_ad.dual_level():
+            x = [forward_ad.make_dual(t, torch.ones_like(t)) if i == dual else t for i, t in enumerate(args)]
+            with pytest.raises(ValueError, match="forward-mode"):
+                call(*x)
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                call(*x)
+            with pytest.raises(ValueError, match="GPU"):  # a level alone changes nothing
+                call(*args)
+    with pytest.raises(ValueError, match="forward-mode"):
+        torch.func.jvp(lambda t: om.attention_prefill(t, q, q), (q,), (q,))
