@@ -161,6 +161,8 @@ def chunk_gated_delta_rule_bwd(q_BTHA, k_BTHA, v_BTHU, g_BTH, beta_BTH, do_BTHU,
     and summed over each key head's value heads), dg/dbeta [B,T,H] fp32,
     d_initial_state [N,H,A,U] fp32.
     """
+    _no_tangents("chunk_gated_delta_rule_bwd", q_BTHA, k_BTHA, v_BTHU, g_BTH, beta_BTH, do_BTHU,
+                 initial_state, d_final_state)
     q, k, v, g, beta, initial_state, cu_seqlens, dev, dims = _prep_inputs(
         q_BTHA, k_BTHA, v_BTHU, g_BTH, beta_BTH, initial_state, cu_seqlens)
     B, T, Hk, A, H, U, N = dims
@@ -230,6 +232,7 @@ def chunk_gated_delta_rule(q_BTHA, k_BTHA, v_BTHU, g_BTH, beta_BTH, chunk_size=6
     enabled and an input requires them, the call is recorded for autograd and its
     backward runs omx_gdn_chunk_bwd.
     """
+    _no_tangents("chunk_gated_delta_rule", q_BTHA, k_BTHA, v_BTHU, g_BTH, beta_BTH, initial_state)
     needs_grad = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad
         for t in (q_BTHA, k_BTHA, v_BTHU, g_BTH, beta_BTH, initial_state))
@@ -248,6 +251,7 @@ def recurrent_gated_delta_rule_step(q, k, v, g, beta, state, *, scale=None):
     q/k [B,Hk,A], v [B,H,U] (bf16 or fp32), g/beta [B,H].  Returns o [B,H,U] fp32.
     Semantics of transformers' torch_recurrent_gated_delta_rule (qk L2-norm in kernel).
     """
+    _no_tangents("recurrent_gated_delta_rule_step", q, k, v, g, beta, state)
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     g, beta = _f32(g), _f32(beta)
     dev = _dev(q, k, v, g, beta, state)
@@ -324,6 +328,8 @@ def gdn_prefill_bwd(mixed_qkv, z, a, b, conv_w, A_log, dt_bias, norm_w, d_out, *
     d_dt_bias, d_norm_w, d_initial_state) in fp32.  Conv windows start from zeros (no conv
     history input).
     """
+    _no_tangents("gdn_prefill_bwd", mixed_qkv, z, a, b, conv_w, A_log, dt_bias, norm_w, d_out,
+                 initial_state, d_final_state)
     Hk, dk, Hv, dv = num_k_heads, head_k_dim, num_v_heads, head_v_dim
     x = mixed_qkv.contiguous()
     z = z.contiguous()
@@ -413,6 +419,8 @@ def gdn_prefill(mixed_qkv, z, a, b, conv_w, A_log, dt_bias, norm_w, *, num_k_hea
     enabled and an input requires them (and no conv history is passed), the call is recorded
     for autograd; its backward runs omx_gdn_prefill_bwd.
     """
+    _no_tangents("gdn_prefill", mixed_qkv, z, a, b, conv_w, A_log, dt_bias, norm_w, initial_state,
+                 conv_state)
     cfg = dict(num_k_heads=num_k_heads, head_k_dim=head_k_dim, num_v_heads=num_v_heads,
                head_v_dim=head_v_dim, eps=eps, chunk_size=chunk_size)
     needs_grad = torch.is_grad_enabled() and any(
@@ -471,6 +479,7 @@ def qkv_conv_projection(x, w_qkv, conv_w=None, *, seq_len=None):
     prototype of the projection-side fusion (omx_gdn_qkv_conv_proj), measured against
     the library GEMM by ``bench.py --workload qkv_conv``; the layer itself uses F.linear.
     """
+    _no_tangents("qkv_conv_projection", x, w_qkv, conv_w)
     lead, D = x.shape[:-1], x.shape[-1]
     x2 = x.reshape(-1, D).contiguous()
     w_qkv = w_qkv.contiguous()
@@ -525,6 +534,7 @@ def gdn_ab_projections(x, w_a, w_b):
     bf16, as the two bf16 linear maps give them (fp32 accumulation, rounded once).  When
     gradients are enabled and an input requires them, the call is recorded for autograd.
     """
+    _no_tangents("gdn_ab_projections", x, w_a, w_b)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_a, w_b)):
         return _ABProj.apply(x, w_a, w_b)
     return _ab_proj_fwd(x, w_a, w_b)
@@ -537,6 +547,7 @@ def gdn_decode_step(mixed_qkv, z, a, b, conv_w, A_log, dt_bias, norm_w, conv_sta
     mixed_qkv [B,conv_dim] bf16, z [B,Hv,dv] bf16, a/b [B,Hv] bf16,
     conv_state [B,conv_dim,K-1] bf16, state [B,Hv,dk,dv] fp32.  Returns out [B,Hv*dv] bf16.
     """
+    _no_tangents("gdn_decode_step", mixed_qkv, z, a, b, conv_w, A_log, dt_bias, norm_w, conv_state, state)
     Hk, dk, Hv, dv = num_k_heads, head_k_dim, num_v_heads, head_v_dim
     x = mixed_qkv.contiguous()
     z, a, b = z.contiguous(), a.contiguous(), b.contiguous()
