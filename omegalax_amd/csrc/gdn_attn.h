@@ -141,7 +141,11 @@ __device__ __forceinline__ u32x4 attn_frag_tr(const bf16_t* base, AttnLane ln, i
 // outstanding loads: with the builtin it put a wait for all of them before reads of buffers that
 // they do not touch.  Whoever reads the bytes waits for them with wait_loads.
 // (The resource's words are uniform; readfirstlane also puts one there that the compiler keeps in
-// a vector register, and five wait states then lie between that write and the load.)
+// a vector register, and five wait states then lie between that write and the load.  m0, which
+// holds the LDS address, is named as overwritten: the compiler sets it before each use of its own,
+// and must not count on an earlier value.  It warns that it would not save a reserved register's.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ u32x4 rsrc_words(const void* p, unsigned bytes) {
   const unsigned long long a = (unsigned long long)p;
   return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((unsigned)a),
@@ -153,7 +157,7 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 }
 __device__ __forceinline__ void load_to_lds16(u32x4 rsrc, unsigned lds, unsigned off) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory");
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory", "m0");
 }
 // several of them, each 4 KiB further in LDS: a workgroup of four wavefronts takes turns
 __device__ __forceinline__ void loads_to_lds16(u32x4 rsrc, unsigned lds, const unsigned (&off)[4]) {
@@ -162,20 +166,21 @@ __device__ __forceinline__ void loads_to_lds16(u32x4 rsrc, unsigned lds, const u
                "s_add_u32 m0, m0, 4096\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %5, 0 offen lds\n\t"
                "s_add_u32 m0, m0, 4096\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %5, 0 offen lds"
                :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]),
-                  "s"(rsrc) : "memory", "scc");
+                  "s"(rsrc) : "memory", "m0", "scc");
 }
 __device__ __forceinline__ void loads_to_lds16(u32x4 rsrc, unsigned lds, const unsigned (&off)[2]) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
                "s_add_u32 m0, m0, 4096\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
-               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off[0]), "v"(off[1]), "s"(rsrc) : "memory", "scc");
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off[0]), "v"(off[1]), "s"(rsrc) : "memory", "m0", "scc");
 }
 __device__ __forceinline__ void loads_to_lds16(u32x4 rsrc, unsigned lds, const unsigned (&off)[1]) {
   load_to_lds16(rsrc, lds, off[0]);
 }
 __device__ __forceinline__ void load_to_lds4(u32x4 rsrc, unsigned lds, unsigned off) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
-               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory");
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // waits until at most N of the wavefront's vector memory operations are outstanding
 template <int N>
