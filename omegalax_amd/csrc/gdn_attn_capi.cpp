@@ -128,10 +128,14 @@ omx::AttnParams params(const Shape& s, float scale) {
   return p;
 }
 
-// workgroups of a kernel over tiles of `per` tokens, in the worst case of every packing
-int check_grid(const char* fn, const Shape& s, int64_t per, int64_t waves) {
+// A launch has less than 2^32 threads, 256 a workgroup.
+constexpr int64_t kMaxGroups = (1 << 24) - 1;
+
+// workgroups of a kernel over tiles of `per` tokens, in the worst case of every packing (of up to three
+// key heads, the grid is filled up to a multiple of 8)
+int check_grid(const char* fn, const Shape& s, int64_t per) {
   const int64_t ranks = (s.T + per - 1) / per + (s.packed ? s.N : 0);
-  REQUIRE(((s.packed ? 1 : s.N) * ranks + 8) * s.Hkv * waves <= INT_MAX / 2, "%s: grid too large", fn);
+  REQUIRE((s.packed ? 1 : s.N) * ranks * s.Hkv + 8 <= kMaxGroups, "%s: grid too large", fn);
   return OMX_GDN_OK;
 }
 
@@ -156,7 +160,7 @@ int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, 
   if (!rc) rc = check_ld(fn, "v_ld", v_ld, Hkv * D);
   if (!rc) rc = check_scale(fn, scale);
   const int per = rc ? 1 : omx::attn_tile_tokens((int)(Hq / Hkv));
-  if (!rc) rc = check_grid(fn, s, per, 1);
+  if (!rc) rc = check_grid(fn, s, per);
   if (rc) return rc;
   const PlanWs ws = plan_ws(0, T, s.packed ? N : 0, per);
   REQUIRE(workspace_bytes >= ws.total, "%s: workspace of %zu bytes is smaller than the %zu needed", fn,
@@ -216,7 +220,7 @@ int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, 
   if (!rc) rc = check_ld(fn, "v_ld", v_ld, Hkv * D);
   if (!rc) rc = check_scale(fn, scale);
   const int per = rc ? 1 : omx::attn_tile_tokens((int)(Hq / Hkv));
-  if (!rc) rc = check_grid(fn, s, per, 1);
+  if (!rc) rc = check_grid(fn, s, per);
   if (rc) return rc;
   const AttnBwdWs ws = attn_bwd_ws(B, T, Hq, Hkv, D, s.packed ? N : 0);
   REQUIRE(workspace_bytes >= ws.total, "%s: workspace of %zu bytes is smaller than the %zu needed", fn,
@@ -261,6 +265,7 @@ int omx_gdn_kv_write(const void* k, const void* v, int64_t k_ld, int64_t v_ld, c
   if (!rc) rc = check_ld(fn, "k_ld", k_ld, Hkv * D);
   if (!rc) rc = check_ld(fn, "v_ld", v_ld, Hkv * D);
   if (rc) return rc;
+  REQUIRE(B * T <= kMaxGroups * omx::kv_write_tokens(), "%s: grid too large", fn);
   const int per = omx::attn_dkv_tile_tokens();
   const PlanWs ws = plan_ws(0, T, s.packed ? N : 0, per);
   REQUIRE(workspace_bytes >= ws.total, "%s: workspace of %zu bytes is smaller than the %zu needed", fn,
@@ -316,7 +321,7 @@ int omx_gdn_attn_paged(const void* q, int64_t q_ld, const int32_t* cu_seqlens, i
   if (!rc) rc = check_ld(fn, "q_ld", q_ld, Hq * D);
   if (!rc) rc = check_scale(fn, scale);
   const int per = rc ? 1 : omx::attn_tile_tokens((int)(Hq / Hkv));
-  if (!rc) rc = check_grid(fn, s, per, 1);
+  if (!rc) rc = check_grid(fn, s, per);
   if (rc) return rc;
   if (B * T == 0) return ok();
   rc = check_cache(fn, k_pages, v_pages, n_pages, page_size, block_table, table_width, lengths, D, Hkv);
@@ -328,7 +333,6 @@ int omx_gdn_attn_paged(const void* q, int64_t q_ld, const int32_t* cu_seqlens, i
   REQUIRE(q && o, "%s: a required pointer is NULL", fn);
   REQUIRE(aligned(q, 16) && aligned(o, 16), "%s: q and o must be 16-byte aligned", fn);
   REQUIRE(ws.total == 0 || (workspace && aligned(workspace, 16)), "%s: workspace must be non-NULL and 16-byte aligned", fn);
-  REQUIRE(B * T * Hq <= (int64_t)INT_MAX * 4, "%s: grid too large", fn);
   omx::AttnParams p = params(s, scale);
   p.q = q; p.q_ld = q_ld; p.o = o; p.cu = cu_seqlens;
   p.k_pages = const_cast<void*>(k_pages); p.v_pages = const_cast<void*>(v_pages);
@@ -368,7 +372,7 @@ int omx_gdn_attn_decode_step(const void* q, const void* k, const void* v, int64_
   if (!rc) rc = check_ld(fn, "v_ld", v_ld, Hkv * D);
   if (!rc) rc = check_scale(fn, scale);
   if (rc) return rc;
-  REQUIRE(B <= 65535 * 16 && B * Hq <= INT_MAX / 4, "%s: batch %lld out of range", fn, (long long)B);
+  REQUIRE(B <= 65535 * 16 && B * Hkv <= kMaxGroups && B * Hq <= INT_MAX / 4, "%s: batch %lld out of range", fn, (long long)B);
   if (B == 0) return ok();
   rc = check_cache(fn, k_pages, v_pages, n_pages, page_size, block_table, table_width, lengths, D, Hkv);
   if (rc) return rc;

@@ -316,6 +316,7 @@ hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream);
 // the cache's entry points: head dims, append, decode step (`splits` workgroups a key head share
 // the keys, by the tokens a table has room for; its partial sums are of splits + N segments)
 bool paged_dims_supported(int D);
+int kv_write_tokens();  // tokens a workgroup of the append copies
 hipError_t launch_kv_write(const AttnParams& p, hipStream_t stream);
 int decode_splits(long long N, long long Hkv, long long D, long long capacity);
 hipError_t launch_attn_decode(const AttnParams& p, hipStream_t stream);

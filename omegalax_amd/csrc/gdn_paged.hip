@@ -480,8 +480,10 @@ void decode_dp(const AttnParams& p, hipStream_t stream) {
 
 bool paged_dims_supported(int D) { return D == 64 || D == 128 || D == 256; }
 
+int kv_write_tokens() { return 4 * kWriteTokens; }
+
 hipError_t launch_kv_write(const AttnParams& p, hipStream_t stream) {
-  const long long per = 4 * kWriteTokens;
+  const long long per = kv_write_tokens();
   kv_write_kernel<<<(unsigned)((p.tokens + per - 1) / per), 256, 0, stream>>>(p);
   return hipGetLastError();
 }

@@ -51,6 +51,19 @@ def test_backward_refuses(over, code, msg):
     assert rc == code and msg in err
 
 
+@pytest.mark.parametrize("fn,args,over", [
+    ("omx_gdn_attn_fwd", "FWD", dict(B=1 << 24, N=1 << 24, T=1)), ("omx_gdn_attn_fwd", "FWD", dict(B=1, N=1, T=1 << 29)),
+    ("omx_gdn_attn_fwd", "FWD", dict(B=1 << 22, N=1 << 22, T=300, Hq=2)), ("omx_gdn_attn_bwd", "BWD", dict(B=1 << 24, N=1 << 24, T=1)),
+    ("omx_gdn_attn_paged", "PAGED", dict(B=1 << 24, N=1 << 24, T=1)), ("omx_gdn_kv_write", "WRITE", dict(B=1 << 28, N=1 << 28, T=1)),
+    ("omx_gdn_attn_decode_step", "DECODE", dict(B=1 << 19, Hq=32, Hkv=32, q_ld=4096, k_ld=4096, v_ld=4096)),
+])
+def test_launches_of_too_many_threads_are_refused(fn, args, over):
+    """A launch holds less than 2^32 threads, 256 of them a workgroup: one more is an error of the
+    arguments, before anything is launched."""
+    rc, err = _run(fn, globals()[args], dict(over, ws=256, ws_bytes=1 << 50))
+    assert rc == _lib.EINVAL and ("grid too large" in err or "out of range" in err)
+
+
 def test_many_packed_sequences_need_their_plan():
     L = _lib.lib()
     assert L.omx_gdn_attn_fwd_workspace_size(5000, 4, 2, 64) == 0
