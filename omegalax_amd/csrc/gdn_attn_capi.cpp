@@ -134,7 +134,8 @@ constexpr int64_t kMaxGroups = (1 << 24) - 1;
 // workgroups of a kernel over tiles of `per` tokens, in the worst case of every packing (of up to three
 // key heads, the grid is filled up to a multiple of 8)
 int check_grid(const char* fn, const Shape& s, int64_t per) {
-  const int64_t ranks = (s.T + per - 1) / per + (s.packed ? s.N : 0);
+  int64_t ranks = (s.T + per - 1) / per + (s.packed ? s.N : 0);
+  ranks = ranks < s.T ? ranks : s.T;  // each tile has a token
   REQUIRE((s.packed ? 1 : s.N) * ranks * s.Hkv + 8 <= kMaxGroups, "%s: grid too large", fn);
   return OMX_GDN_OK;
 }
