@@ -497,7 +497,8 @@ int decode_splits(long long N, long long Hkv, long long D, long long capacity) {
   // 207 (230), 63 of 1,000 and one of 30,000 84 (380); 1,024 of 100 199 (196), with one of 30,000 244 (532).
   // 16/2 heads of 256, sequences of 75 to 525 keys: 512 98 (81), 1,024 182 (156), 4,096 723 (579).
   if (N > 1024 || capacity * D <= (1 << 17)) return 1;
-  if (N * (capacity / 16 + 1) > INT_MAX) return 1;  // stages are counted in 32 bits
+  // stages are counted in 32 bits, and a range's end lies up to a range past the last
+  if (N * (capacity / 16 + 1) > INT_MAX / 2) return 1;
   const long long s = 256 / Hkv;
   return (int)(s < 2 ? 1 : s);
 }

@@ -149,6 +149,7 @@ def test_rows_that_leave_the_chip_idle_share_their_keys(B, T, Hq, Hkv, D, page, 
 
 @pytest.mark.parametrize("B,Hq,Hkv,D,page,width,ranges", [
     (64, 32, 8, 128, 64, 70, 32), (128, 32, 8, 128, 64, 70, 32), (1024, 8, 1, 64, 16, 200, 256), (512, 16, 2, 256, 64, 10, 128),
+    (7, 8, 1, 256, 65536, 32767, 256), (11, 8, 1, 256, 65536, 32767, 0),  # 2^30 stages of 16 keys: they are counted in 32 bits
     (1025, 8, 1, 64, 16, 200, 0), (64, 32, 8, 128, 64, 16, 0), (1, 16, 4, 128, 16, 64, 0), (1, 16, 4, 128, 16, 65, 64)])
 def test_decode_batches_share_the_keys_in_equal_ranges(B, Hq, Hkv, D, page, width, ranges):
     """One workgroup for each compute unit, whatever the number of sequences, up to 1,024 and but for
