@@ -413,6 +413,5 @@ __device__ __forceinline__ bool dkv_share(const AttnParams& p, int row, int rank
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 }  // namespace omx

@@ -445,45 +445,34 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnParams p) {
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6, part = w % W;
   const long long rows = p.tokens * p.Hkv * p.G, row = (long long)blockIdx.x * (4 / W) + w / W;
   const bool live = row < rows;
-  float a[4], M = kLow * kLog2e, den = 0.f;  // splits <= 256
-  float acc[E];
+  float acc[E], den = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   if (live) {
-    float ls[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int s = 64 * r + l;
-      const bool in = s < p.splits;
-      a[r] = in ? p.part_ml[2 * (s * rows + row)] : kLow * kLog2e;
-      ls[r] = in ? p.part_ml[2 * (s * rows + row) + 1] : 0.f;
-      M = fmaxf(M, a[r]);
+    static_assert(kAttnMaxSplits <= 64, "a share a lane");
+    float a = kLow * kLog2e, ls = 0.f;
+    if (l < p.splits) {
+      a = p.part_ml[2 * (l * rows + row)];
+      ls = p.part_ml[2 * (l * rows + row) + 1];
     }
+    float M = a;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    a = ls == 0.f ? 0.f : __builtin_amdgcn_exp2f(a - M);
+    den = wave_sum(a * ls);
+    for (int s = part; s < p.splits; s += 8 * W) {  // eight reads in flight
+      fE x[8];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      a[r] = ls[r] == 0.f ? 0.f : __builtin_amdgcn_exp2f(a[r] - M);
-      den += a[r] * ls[r];
-    }
-    den = wave_sum(den);
+      for (int u = 0; u < 8; ++u) {
+        const int su = s + W * u < p.splits ? s + W * u : p.splits - 1;
+        x[u] = *(const fE*)(p.part_o + (su * rows + row) * DP + E * l);
+      }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int s1 = p.splits - 64 * r < 64 ? p.splits - 64 * r : 64;
-      for (int s = part; s < s1; s += 8 * W) {  // eight reads in flight
-        fE x[8];
+      for (int u = 0; u < 8; ++u) {
+        const float as = __shfl(a, s + W * u, 64);
+        const float f = s + W * u < p.splits ? as : 0.f;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int su = s + W * u < s1 ? s + W * u : s1 - 1;
-          x[u] = *(const fE*)(p.part_o + ((64 * r + su) * rows + row) * DP + E * l);
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float as = __shfl(a[r], s + W * u, 64);
-          const float f = s + W * u < s1 ? as : 0.f;
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] += f * x[u][e];
-        }
+        for (int e = 0; e < E; ++e) acc[e] += f * x[u][e];
       }
     }
   }
@@ -565,6 +554,24 @@ __global__ __launch_bounds__(kPlanNT) void attn_plan_kernel(const int32_t* cu, c
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
 
+template <int DP>
+void join(const AttnParams& p, hipStream_t stream) {
+  const long long rows = p.tokens * p.Hkv * p.G;
+  if (p.splits > 8)
+    attn_join_kernel<DP, 4><<<(unsigned)rows, 256, 0, stream>>>(p);
+  else
+    attn_join_kernel<DP, 1><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(p);
+}
+
+hipError_t launch_attn_join(const AttnParams& p, hipStream_t stream) {
+  switch (padded_dim(p.D)) {
+    case 64: join<64>(p, stream); break;
+    case 128: join<128>(p, stream); break;
+    default: join<256>(p, stream); break;
+  }
+  return hipGetLastError();
+}
+
 }  // namespace
 
 int attn_tile_tokens(int G) { return kBM / G; }
@@ -608,24 +615,6 @@ hipError_t launch_attn_fwd(const AttnParams& p, hipStream_t stream) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !paged || p.splits == 1) return e;
   return launch_attn_join(p, stream);
-}
-
-template <int DP>
-static void join(const AttnParams& p, hipStream_t stream) {
-  const long long rows = p.tokens * p.Hkv * p.G;
-  if (p.splits > 8)
-    attn_join_kernel<DP, 4><<<(unsigned)rows, 256, 0, stream>>>(p);
-  else
-    attn_join_kernel<DP, 1><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(p);
-}
-
-hipError_t launch_attn_join(const AttnParams& p, hipStream_t stream) {
-  switch (padded_dim(p.D)) {
-    case 64: join<64>(p, stream); break;
-    case 128: join<128>(p, stream); break;
-    default: join<256>(p, stream); break;
-  }
-  return hipGetLastError();
 }
 
 }  // namespace omx

@@ -284,7 +284,7 @@ struct AttnParams {
   const int32_t* table;        // [N, table_w]
   const int32_t* held;         // [N]
   int table_w, page, n_pages;
-  // work split over the keys: partial sums, joined by launch_attn_join
+  // work split over the keys: partial sums, which a second kernel joins
   int splits;
   float *part_o, *part_ml;
   // backward
@@ -296,13 +296,13 @@ struct AttnParams {
   int share_tiles;             // rows in a share, in tiles of 128 tokens
 };
 constexpr int kAttnMaxG = 32, kAttnMaxD = 256;
+constexpr int kAttnMaxSplits = 32;  // shares of the keys of new tokens over a cache
 // tokens per tile of the forward, tiles of a row at most, and int32 words of the plan
 int attn_tile_tokens(int G);
 long long attn_ranks(const AttnParams& p, int per);
 size_t attn_plan_words(long long T, long long N, int per);
 hipError_t launch_attn_plan(const AttnParams& p, int per, hipStream_t stream);
 hipError_t launch_attn_fwd(const AttnParams& p, hipStream_t stream);
-hipError_t launch_attn_join(const AttnParams& p, hipStream_t stream);
 
 // the backward: dq and delta, then dk and dv (keys per tile of the second: its plan's tokens)
 int attn_dkv_tile_tokens();
