@@ -231,13 +231,14 @@ __global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnParams p, long lo
 int attn_dkv_tile_tokens() { return kDkvKeys; }
 
 // How tiles of keys are shared.  The time is estimated, in stages, for sequences of equal length and
-// each number m of tiles' rows (4 g stages each) in a share: 256 workgroups, one a compute unit,
-// make a round; shares that fill one or two end with the longest, more of them even out up to half
-// a share, and whole tiles, which go longest first, altogether; around a workgroup's stages pass
-// 16 more, and its partial sums take a twentieth.  Of 1 to 16 shares that takes the best within 2%
-// in 15 of 19 layouts and lengths of one sequence (heads of 64, 128 and 256, 700 to 16,000 tokens),
-// within 8% in all; they are 1.0 to 4.2 times as fast as whole tiles: 4,000 tokens of 16/2 heads of
-// 256, both passes, 1,694 us whole, 499 in 7 shares, 617 in 8.  Partial sums take 512 MiB at most.
+// each number m of tiles' rows (4 g stages each) in a share: workgroups, one a compute unit, make
+// a round; shares that fill one or two end with the longest, more of them even out up to half a share,
+// and whole tiles, which go longest first, altogether; around a workgroup's stages pass
+// 16 more, and its partial sums take a twentieth.  Of 1 to 16 shares that takes the best within 1%
+// in 20 of 21 layouts and lengths (heads of 64, 128 and 256, one sequence of 700 to 16,000 tokens and
+// five of 3,001), within 5% in all; they are 1.0 to 4.2 times as fast as whole tiles: 4,000 tokens of
+// 16/2 heads of 256, both passes, 1,704 us whole, 496 in 7 shares, 620 in 8.  Partial sums take 512 MiB
+// at most.
 DkvPlan attn_dkv_plan(long long units, long long T, long long N, int G, long long row_bytes) {
   DkvPlan plan{1, 0};
   if (N > 64 || T == 0 || units == 0) return plan;  // shares are found by lanes that hold a sequence each
@@ -246,7 +247,7 @@ DkvPlan attn_dkv_plan(long long units, long long T, long long N, int G, long lon
   long long room = (512ll << 20) / row_bytes;
   room = room < 16 ? room : 16;
   units *= seqs;
-  const double tile = 4. * G, even = (double)(units * nt) * nt * tile / 512;
+  const double tile = 4. * G, even = (double)(units * nt) * nt * tile / (2 * kComputeUnits);
   double best = 0;
   for (long long s = 1; s <= room && s <= nt; ++s) {
     const long long m = (nt + s - 1) / s;
@@ -256,7 +257,7 @@ DkvPlan attn_dkv_plan(long long units, long long T, long long N, int G, long lon
       shares += n;
       parts += q > 0 ? n : 0;
     }
-    const long long rounds = (units * shares + 255) / 256;
+    const long long rounds = (units * shares + kComputeUnits - 1) / kComputeUnits;
     const double each = m * tile;
     const double ends = s == 1 ? even : (rounds <= 2 ? rounds * each : even + each / 2);
     const double cost = (ends > each ? ends : each) + 16. * rounds + units * parts / 20.;

@@ -104,7 +104,7 @@ hipError_t use_plan(omx::AttnParams& p, const PlanWs& w, void* workspace, int pe
 int paged_splits(const Shape& x, int64_t capacity) {
   const int64_t per = omx::attn_tile_tokens((int)(x.Hq / x.Hkv)), each = (x.T + per - 1) / per;
   const int64_t tiles = (x.packed ? each + x.N - 1 : x.N * each) * x.Hkv;
-  int64_t s = tiles > 0 ? 512 / tiles : 1;
+  int64_t s = tiles > 0 ? 2 * omx::kComputeUnits / tiles : 1;
   const int64_t most = capacity / 128;
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > omx::kAttnMaxSplits ? omx::kAttnMaxSplits : s));

@@ -296,6 +296,9 @@ struct AttnParams {
   int share_tiles;             // rows in a share, in tiles of 128 tokens
 };
 constexpr int kAttnMaxG = 32, kAttnMaxD = 256;
+// Compute units that the rules for sharing work count with, an MI355X's: workspace sizes are functions of
+// the arguments alone, asked for on whichever device is current.
+constexpr int kComputeUnits = 256;
 constexpr int kAttnMaxSplits = 32;  // shares of the keys of new tokens over a cache
 // tokens per tile of the forward, tiles of a row at most, and int32 words of the plan
 int attn_tile_tokens(int G);

@@ -499,7 +499,7 @@ int decode_splits(long long N, long long Hkv, long long D, long long capacity) {
   if (N > 1024 || capacity * D <= (1 << 17)) return 1;
   // stages are counted in 32 bits, and a range's end lies up to a range past the last
   if (N * (capacity / 16 + 1) > INT_MAX / 2) return 1;
-  const long long s = 256 / Hkv;
+  const long long s = kComputeUnits / Hkv;
   return (int)(s < 2 ? 1 : s);
 }
 
