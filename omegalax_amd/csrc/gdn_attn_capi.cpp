@@ -74,6 +74,15 @@ int check_cache(const char* fn, const void* kp, const void* vp, int64_t n_pages,
   return OMX_GDN_OK;
 }
 
+// What a workspace size is told for: shapes and tables that an entry point may take.  Others have none.
+bool sized(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N) {
+  return B >= 0 && B <= kMaxTokens && T >= 0 && T <= kMaxTokens && B * T <= kMaxTokens && N >= 0 && N <= kMaxTokens &&
+         Hkv >= 1 && Hq >= 1 && Hq <= 4096 && Hq % Hkv == 0 && Hq / Hkv <= omx::kAttnMaxG && D >= 1 && D <= omx::kAttnMaxD;
+}
+bool sized_table(int64_t page, int64_t table_w) {
+  return page >= 1 && page <= 65536 && table_w >= 0 && table_w <= kMaxTokens && page * table_w <= kMaxTokens;
+}
+
 size_t align_up(size_t x) { return (x + 255) / 256 * 256; }
 
 // The plan of more than 64 packed sequences for tiles of `per` tokens: tile list, offsets.
@@ -147,7 +156,7 @@ int check_grid(const char* fn, const Shape& s, int64_t per) {
 extern "C" {
 
 size_t omx_gdn_attn_fwd_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64_t N) {
-  if (T < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq / Hkv > omx::kAttnMaxG || N < 0) return 0;
+  if (!sized(1, T, Hq, Hkv, 1, N)) return 0;
   return plan_ws(0, T, N, omx::attn_tile_tokens((int)(Hq / Hkv))).total;
 }
 
@@ -207,7 +216,7 @@ AttnBwdWs attn_bwd_ws(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, 
 }  // namespace
 
 size_t omx_gdn_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N) {
-  if (B < 0 || T < 0 || D < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq / Hkv > omx::kAttnMaxG || N < 0) return 0;
+  if (!sized(B, T, Hq, Hkv, D, N)) return 0;
   return attn_bwd_ws(B, T, Hq, Hkv, D, N).total;
 }
 
@@ -254,7 +263,7 @@ int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, 
 }
 
 size_t omx_gdn_kv_write_workspace_size(int64_t T, int64_t N) {
-  if (T < 0 || N < 0) return 0;
+  if (!sized(1, T, 1, 1, 1, N)) return 0;
   return plan_ws(0, T, N, omx::attn_dkv_tile_tokens()).total;
 }
 
@@ -308,9 +317,7 @@ PagedWs paged_ws(const Shape& s, int64_t capacity) {
 size_t omx_gdn_attn_paged_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N,
                                          int packed, int64_t page_size, int64_t table_width) {
   const Shape s{N, B, T, Hq, Hkv, D, packed != 0};
-  if (B < 0 || T < 0 || N < 0 || D < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq / Hkv > omx::kAttnMaxG || page_size < 1 ||
-      table_width < 0)
-    return 0;
+  if (!sized(B, T, Hq, Hkv, D, N) || !sized_table(page_size, table_width)) return 0;
   return paged_ws(s, page_size * table_width).total;
 }
 
@@ -358,7 +365,7 @@ SplitWs decode_ws(int splits, int64_t B, int64_t Hq, int64_t D) {
 
 size_t omx_gdn_attn_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t page_size,
                                           int64_t table_width) {
-  if (B < 1 || Hq < 1 || Hkv < 1 || D < 1 || page_size < 1 || table_width < 0) return 0;
+  if (B < 1 || !sized(B, 1, Hq, Hkv, D, B) || !sized_table(page_size, table_width)) return 0;
   return decode_ws(omx::decode_splits(B, Hkv, D, page_size * table_width), B, Hq, D).total;
 }
 

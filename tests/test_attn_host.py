@@ -159,6 +159,33 @@ def test_decode_batches_share_the_keys_in_equal_ranges(B, Hq, Hkv, D, page, widt
     assert size(B, Hq, Hkv, D, page, width) == up(rows * D * 4) + up(rows * 8)
 
 
+BIG = [-1, 0, 1 << 31, 1 << 40, (1 << 63) - 1, -(1 << 63)]
+
+
+@pytest.mark.parametrize("fn,good", [
+    ("fwd", [5000, 4, 2, 65]), ("bwd", [2, 5000, 4, 2, 128, 0]), ("paged", [1, 40, 4, 2, 128, 1, 0, 64, 100]),
+    ("decode", [3, 4, 2, 128, 64, 100])])
+def test_workspace_sizes_of_impossible_shapes(fn, good):
+    """Any numbers get an answer: those that no entry point takes have no size."""
+    size = getattr(_lib.lib(), f"omx_gdn_attn_{fn}_workspace_size")
+    assert size(*good) > 0
+    for i in range(len(good)):
+        for j in range(len(good)):
+            for x in BIG[2:]:
+                for y in BIG:
+                    if fn == "paged" and 6 in (i, j):  # a flag, not a number
+                        continue
+                    args = list(good)
+                    args[j], args[i] = y, x
+                    assert size(*args) == 0
+
+
+def test_workspace_size_of_an_impossible_append():
+    size = _lib.lib().omx_gdn_kv_write_workspace_size
+    assert size(5000, 65) > 0
+    assert not any(size(x, y) for x in BIG[2:] for y in (65, *BIG)) and not any(size(5000, x) for x in BIG[2:])
+
+
 def test_empty_calls_are_no_ops():
     assert _run("omx_gdn_attn_fwd", FWD, dict(T=0, q=None, o=None))[0] == _lib.OK
     assert _run("omx_gdn_attn_bwd", BWD, dict(B=0, N=0, q=None))[0] == _lib.OK
