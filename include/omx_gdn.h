@@ -333,7 +333,8 @@ int omx_gdn_ab_proj(const void* x, const void* w_a, const void* w_b, void* a, vo
  *   o_rest       [B, T, Hq, D] bf16 or NULL: what the rounding of o left, for omx_gdn_attn_bwd
  *   scale        positive, at most 2^20; products q . k are to lie above -1e30
  * D is a multiple of 8, at most 256 (compiled for 64, 128 and 256; others run zero-filled at the
- * next).  Strides are multiples of 8 and at most 2^22, q, k, v and o 16-byte aligned.  Scores,
+ * next).  Strides are multiples of 8 and at most 2^22, q, k, v and o 16-byte aligned.  A call has
+ * less than 2^24 tiles of 128 (token, query head) rows, over all key heads.  Scores,
  * softmax and sums are fp32; the weights are rounded to bf16 for their product with v.  A row
  * depends on its own sequence alone, whatever lies beside it, and on no key after it: values that
  * are not finite there do not reach it.
@@ -383,7 +384,8 @@ size_t omx_gdn_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t
  * page that is written to stands once in all of block_table; others may be shared.
  *
  * omx_gdn_kv_write appends the keys and values of new tokens: token i of sequence n goes to
- * position lengths[n] + i.  k, v, their strides and cu_seqlens as for omx_gdn_attn_fwd.
+ * position lengths[n] + i.  k, v, their strides and cu_seqlens as for omx_gdn_attn_fwd; less than
+ * 2^28 tokens.
  */
 int omx_gdn_kv_write(const void* k, const void* v, int64_t k_ld, int64_t v_ld,
                      const int32_t* cu_seqlens, int64_t N, void* k_pages, void* v_pages,

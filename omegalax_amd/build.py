@@ -39,8 +39,10 @@ def hipcc() -> str:
 
 
 # MFMA-heavy sources: keep MFMA accumulators in VGPRs, so the VALU work on them
-# (scaling, packing to bf16) needs no AGPR<->VGPR copies
-MFMA_VGPR_SOURCES = {"gdn_attn.hip", "gdn_attn_dkv.hip", "gdn_attn_dq.hip", "gdn_chunk.hip", "gdn_prep.hip", "gdn_qkv.hip"}
+# (scaling, packing to bf16) needs no AGPR<->VGPR copies.  Not gdn_attn_bwd.hip, whose wide kernel
+# fills both halves of the register file: with the flag 133 of its registers spill, without it 3.
+MFMA_VGPR_SOURCES = {"gdn_attn.hip", "gdn_attn_dkv.hip", "gdn_attn_dq.hip", "gdn_chunk.hip",
+                     "gdn_prep.hip", "gdn_qkv.hip"}
 MFMA_VGPR_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 
 

@@ -275,8 +275,8 @@ void attn_decode_kernel(AttnParams p) {
           s[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], cs, -mc));
           ls[n] += s[g][i];
         }
-        // the weights as two bf16 terms (2^-17 together): a step is bound by its bytes, and one term's
-        // rounding was half of its error (2.5e-3 against 64 bits, 1.6e-3 the output's own)
+        // the weights as two bf16 terms (off by at most 2^-16 together): a step is bound by its bytes, and
+        // one term's rounding was half of its error (2.5e-3 against 64 bits, 1.7e-3 the output's own)
         const u32x2 pb = u32x2{pack_bf16(s[g][0], s[g][1]), pack_bf16(s[g][2], s[g][3])};
         const u32x2 pr = u32x2{pack_bf16(lo_part(s[g][0]), lo_part(s[g][1])), pack_bf16(lo_part(s[g][2]), lo_part(s[g][3]))};
         const int vr = 16 * g + 4 * g4 + (r >> 2);
@@ -491,11 +491,12 @@ hipError_t launch_kv_write(const AttnParams& p, hipStream_t stream) {
 int decode_splits(long long N, long long Hkv, long long D, long long capacity) {
   // One workgroup a sequence and key head where a sequence is so short that the join costs more than
   // it saves (B=1, 4 key heads of 128, calls one after the other: 611 keys 14.4 us in one launch, 18.5 in
-  // two, 1,500 keys 21.8 and 18.0), and for more than 1,024 sequences, each row's join summing up all their lengths.
-  // Otherwise one for each compute unit: their buffers allow no second.  Equal ranges against a
-  // workgroup each, 32/8 heads of 128: 64 sequences of 4,000 keys 190 us (187), between 1,000 and 7,000
-  // 207 (230), 63 of 1,000 and one of 30,000 84 (380); 1,024 of 100 199 (196), with one of 30,000 244 (532).
-  // 16/2 heads of 256, sequences of 75 to 525 keys: 512 98 (81), 1,024 182 (156), 4,096 723 (579).
+  // two, 1,500 keys 21.8 and 18.0), and for more than 1,024 sequences, where each row's join sums up all
+  // their lengths.  Otherwise one for each compute unit: their buffers allow no second.  Equal ranges
+  // against a workgroup each, 32/8 heads of 128: 64 sequences of 4,000 keys 190 us (187), between 1,000
+  // and 7,000 207 (230), 63 of 1,000 and one of 30,000 84 (380); 1,024 of 100 199 (196), with one of
+  // 30,000 244 (532).  16/2 heads of 256, sequences of 75 to 525 keys: 512 98 (81), 1,024 182 (156),
+  // 4,096 723 (579).
   if (N > 1024 || capacity * D <= (1 << 17)) return 1;
   // stages are counted in 32 bits, and a range's end lies up to a range past the last
   if (N * (capacity / 16 + 1) > INT_MAX / 2) return 1;
