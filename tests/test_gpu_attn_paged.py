@@ -441,3 +441,70 @@ def test_decode_rows_of_more_than_64_segments(held, page, Hq, Hkv, D):
     ranges = segments(c, Hq) - len(held)
     assert ranges == 256 // Hkv and max(stages) // max(8, -(-sum(stages) // ranges)) > 64
     step_and_check(c, Hq)
+
+
+def test_captured_steps_of_a_large_batch():
+    """A step of 70 sequences in equal ranges, captured once: replays with other lengths (none, long,
+    past the table, taking no part), eager steps and other allocations between them."""
+    N, Hq, Hkv, D, page, width = 70, 16, 8, 64, 16, 160
+    c, e = (Cache([300] * N, [1] * N, page, Hkv, D, width=width) for _ in range(2))
+    assert segments(c, Hq) == 256 // Hkv + N
+    for x in (c, e):  # tables without holes, over pages that hold numbers
+        g = torch.Generator().manual_seed(3)
+        x.k_pages = torch.randn((N * width, page, Hkv, D), generator=g).to(BF).cuda()
+        x.v_pages = torch.randn((N * width, page, Hkv, D), generator=g).to(BF).cuda()
+        x.block_table = torch.randperm(N * width, generator=g).to(torch.int32).view(N, width).cuda()
+    q, k, v = draw(1, N, Hq, D), draw(2, N, Hkv, D), draw(3, N, Hkv, D)
+    first = c.k_pages.clone(), c.v_pages.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        om.attention_decode_step(q, k, v, *c.args())
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = om.attention_decode_step(q, k, v, *c.args())
+    c.k_pages.copy_(first[0])
+    c.v_pages.copy_(first[1])
+    for r in range(4):
+        lens = torch.randint(0, (40, 2600, 300, 3000)[r], (N,), generator=torch.Generator().manual_seed(r))
+        lens[r::9] = -1
+        for x in (c, e):
+            x.lengths.copy_(lens.to(torch.int32))
+        for i, t in enumerate((q, k, v)):
+            t.copy_(draw(80 + 3 * r + i, *t.shape))
+        want = om.attention_decode_step(q, k, v, *e.args())
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want) and bool(o.isfinite().all())
+        same_pools(c, (e.k_pages, e.v_pages))
+
+
+def test_streams_at_once_over_caches():
+    """Turns and decode steps of two caches on two streams at the same time, each as by itself."""
+    shapes = [([900, 40, 2000], 30, 64, 8, 2, 128), ([700] * 40 + [3] * 30, 2, 64, 16, 8, 64)]
+    sets = []
+    for i, (held, T, page, Hq, Hkv, D) in enumerate(shapes):
+        c = Cache(held, [T + 1] * len(held), page, Hkv, D, seed=i, width=40)
+        B = len(held)
+        sets.append((c, draw(1, B, T, Hq, D), draw(2, B, T, Hkv, D), draw(3, B, T, Hkv, D), draw(4, B, Hq, D),
+                     draw(5, B, Hkv, D), draw(6, B, Hkv, D), c.lengths + T))
+
+    def run(c, q, k, v, q1, k1, v1, longer):
+        om.kv_pages_write(k, v, *c.args())
+        o = om.attention_prefill_paged(q, *c.args())
+        return o, om.attention_decode_step(q1, k1, v1, *c.args()[:3], longer)
+
+    want = [run(*s) for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(*sets[i]))
+    torch.cuda.synchronize()
+    for w, rs in zip(want, got):
+        assert all(bool(t.isfinite().all()) for t in w)
+        for r in rs:
+            assert all(torch.equal(a, b) for a, b in zip(w, r))
