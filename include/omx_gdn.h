@@ -370,6 +370,28 @@ size_t omx_gdn_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t
                                        int64_t N);
 
 /*
+ * The same attention, forward and backward, with a window: query i sees its last `window` keys,
+ * i - window + 1 .. i of its sequence (window >= 1), and of those before them the first `sinks`
+ * (sinks >= 0), which stay visible.  Other arguments and the forward's workspace size as above; key
+ * tiles that no row sees are neither read nor multiplied.  A row depends on the keys that it sees alone.
+ */
+int omx_gdn_attn_window_fwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld,
+                            int64_t v_ld, const int32_t* cu_seqlens, int64_t N, void* o, float* lse,
+                            void* o_rest, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                            float scale, int64_t window, int64_t sinks, void* workspace,
+                            size_t workspace_bytes, void* stream);
+int omx_gdn_attn_window_bwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld,
+                            int64_t v_ld, const int32_t* cu_seqlens, int64_t N, const void* o,
+                            const float* lse, const void* o_rest, const void* d_o, void* dq, void* dk,
+                            void* dv, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                            float scale, int64_t window, int64_t sinks, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace omx_gdn_attn_window_bwd needs (16-byte aligned; N = 0 without cu_seqlens). */
+size_t omx_gdn_attn_window_bwd_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                              int64_t N, int64_t window, int64_t sinks);
+
+/*
  * The paged key-value cache, which the next three entry points share.
  *   k_pages, v_pages  [n_pages, page_size, Hkv, D] bf16, 16-byte aligned; D 64, 128 or 256,
  *                page_size a multiple of 16 up to 65536.  Slots that no token was written to may

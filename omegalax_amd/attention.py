@@ -16,6 +16,7 @@ one ``attention_decode_step``.
 from __future__ import annotations
 
 import functools
+import operator
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -28,6 +29,7 @@ __all__ = ["attention_prefill", "attention_prefill_bwd", "attention_prefill_page
 
 
 _BF16 = torch.bfloat16
+_MOST = (1 << 31) - 1
 
 
 @functools.lru_cache(maxsize=4096)
@@ -89,6 +91,18 @@ def _dense(name, t, shape):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _sight(window, sinks):
+    """(window, sinks) as whole numbers, or None for all keys.  The kernels count in 32 bits."""
+    if window is None:
+        if sinks:
+            raise ValueError("sinks are the keys that stay visible behind a window: give one")
+        return None
+    window, sinks = operator.index(window), operator.index(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window must be at least 1 and sinks not negative (got {window}, {sinks})")
+    return min(window, _MOST), min(sinks, _MOST)
+
+
 def _scale(scale, D):
     return float(D ** -0.5) if scale is None else float(scale)
 
@@ -104,7 +118,7 @@ def _qkv(q, k, v, cu_seqlens, dims=4):
     return dev, q, k, v, q_ld, k_ld, v_ld, cu_seqlens, N
 
 
-def _prefill_fwd(q, k, v, cu_seqlens, scale, with_lse, with_rest):
+def _prefill_fwd(q, k, v, cu_seqlens, scale, sight, with_lse, with_rest):
     dev, q, k, v, q_ld, k_ld, v_ld, cu, N = _qkv(q, k, v, cu_seqlens)
     B, T, Hq, D = q.shape
     Hkv = k.shape[2]
@@ -113,20 +127,22 @@ def _prefill_fwd(q, k, v, cu_seqlens, scale, with_lse, with_rest):
     rest = torch.empty_like(o) if with_rest else None
     ws_bytes = _workspace_bytes("omx_gdn_attn_fwd_workspace_size", T, Hq, Hkv, 0 if cu is None else N)
     ws = _workspace(ws_bytes, dev)
-    _call(dev, "omx_gdn_attn_fwd", _ptr(q), _ptr(k), _ptr(v), q_ld, k_ld, v_ld, _ptr(cu), N, _ptr(o),
-          _ptr(lse), _ptr(rest), B, T, Hq, Hkv, D, _scale(scale, D), _ptr(ws), ws_bytes)
+    _call(dev, "omx_gdn_attn_window_fwd" if sight else "omx_gdn_attn_fwd", _ptr(q), _ptr(k), _ptr(v), q_ld, k_ld,
+          v_ld, _ptr(cu), N, _ptr(o), _ptr(lse), _ptr(rest), B, T, Hq, Hkv, D, _scale(scale, D), *(sight or ()),
+          _ptr(ws), ws_bytes)
     return o, lse, rest
 
 
-def attention_prefill_bwd(q, k, v, o, lse, do, *, o_rest=None, cu_seqlens=None, scale=None):
+def attention_prefill_bwd(q, k, v, o, lse, do, *, o_rest=None, cu_seqlens=None, scale=None, window=None, sinks=0):
     """Gradients (dq, dk, dv) of ``attention_prefill`` for the cotangent ``do`` of its output.
 
-    ``o`` and ``lse`` are what the forward returned with ``output_lse=True``.  ``o_rest``, what
+    ``window`` and ``sinks`` are the forward's.  ``o`` and ``lse`` are what the forward returned with ``output_lse=True``.  ``o_rest``, what
     the rounding of o left (bf16, as o), makes dq and dk about 6% more exact; autograd keeps it.
     The gradients are dense bf16 tensors of the inputs' shapes; those of a key head are summed
     over its query heads.  A value of a sequence that is not finite may reach all of its gradients.
     """
     _no_tangents("attention_prefill_bwd", q, k, v, o, lse, do, o_rest)
+    sight = _sight(window, sinks)
     dev, q, k, v, q_ld, k_ld, v_ld, cu, N = _qkv(q, k, v, cu_seqlens)
     B, T, Hq, D = q.shape
     Hkv = k.shape[2]
@@ -140,11 +156,12 @@ def attention_prefill_bwd(q, k, v, o, lse, do, *, o_rest=None, cu_seqlens=None, 
     dq = torch.empty((B, T, Hq, D), dtype=torch.bfloat16, device=dev)
     dk = torch.empty((B, T, Hkv, D), dtype=torch.bfloat16, device=dev)
     dv = torch.empty_like(dk)
-    ws_bytes = _workspace_bytes("omx_gdn_attn_bwd_workspace_size", B, T, Hq, Hkv, D, 0 if cu is None else N)
+    name = "omx_gdn_attn_window_bwd" if sight else "omx_gdn_attn_bwd"
+    ws_bytes = _workspace_bytes(name + "_workspace_size", B, T, Hq, Hkv, D, 0 if cu is None else N, *(sight or ()))
     ws = _workspace(ws_bytes, dev)
-    _call(dev, "omx_gdn_attn_bwd", _ptr(q), _ptr(k), _ptr(v), q_ld, k_ld, v_ld, _ptr(cu), N, _ptr(o),
-          _ptr(lse), _ptr(o_rest), _ptr(do), _ptr(dq), _ptr(dk), _ptr(dv), B, T, Hq, Hkv, D, _scale(scale, D),
-          _ptr(ws), ws_bytes)
+    _call(dev, name, _ptr(q), _ptr(k), _ptr(v), q_ld, k_ld, v_ld, _ptr(cu), N, _ptr(o), _ptr(lse), _ptr(o_rest),
+          _ptr(do), _ptr(dq), _ptr(dk), _ptr(dv), B, T, Hq, Hkv, D, _scale(scale, D), *(sight or ()), _ptr(ws),
+          ws_bytes)
     return dq, dk, dv
 
 
@@ -153,10 +170,11 @@ class _AttentionPrefill(torch.autograd.Function):
     from the saved output and logarithms (no score is kept)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, cu_seqlens, scale):
-        o, lse, rest = _prefill_fwd(q, k, v, cu_seqlens, scale, True, True)
+    def forward(ctx, q, k, v, cu_seqlens, scale, sight):
+        o, lse, rest = _prefill_fwd(q, k, v, cu_seqlens, scale, sight, True, True)
         ctx.save_for_backward(q, k, v, o, lse, rest, cu_seqlens)
         ctx.scale = scale
+        ctx.window, ctx.sinks = sight or (None, 0)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return o, lse
@@ -165,29 +183,31 @@ class _AttentionPrefill(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, do, _dlse):
         if do is None:
-            return None, None, None, None, None
+            return None, None, None, None, None, None
         q, k, v, o, lse, rest, cu_seqlens = ctx.saved_tensors
         dq, dk, dv = attention_prefill_bwd(q, k, v, o, lse, do, o_rest=rest, cu_seqlens=cu_seqlens,
-                                           scale=ctx.scale)
-        return dq, dk, dv, None, None
+                                           scale=ctx.scale, window=ctx.window, sinks=ctx.sinks)
+        return dq, dk, dv, None, None, None
 
 
-def attention_prefill(q, k, v, *, cu_seqlens=None, scale=None, output_lse=False):
+def attention_prefill(q, k, v, *, cu_seqlens=None, scale=None, output_lse=False, window=None, sinks=0):
     """Causal softmax attention of whole prompts.
 
     q [B,T,Hq,D], k and v [B,T,Hkv,D] bf16 (D a multiple of 8 up to 256; up to 32 query heads per
     key head; views into one projection are read in place).  ``cu_seqlens`` (int32 [N+1], B == 1)
-    packs N sequences, as in ``gdn_prefill``.  ``scale`` defaults to D ** -0.5.  Returns o
+    packs N sequences, as in ``gdn_prefill``.  With a ``window`` a query sees that many last keys, its
+    own among them, and the first ``sinks`` of its sequence, which stay visible.  ``scale`` defaults to D ** -0.5.  Returns o
     [B,T,Hq,D] bf16, or (o, lse) with the fp32 logarithms [B,T,Hq] of the softmax sums.  When
     gradients are enabled and an input requires them, the call is recorded for autograd (once, and
-    not through lse); forward-mode derivatives are refused.  A row sees no key after it, not even one
-    that is not finite.
+    not through lse); forward-mode derivatives are refused.  A row sees no key after it, nor one behind
+    its window, not even one that is not finite.
     """
     _no_tangents("attention_prefill", q, k, v)
+    sight = _sight(window, sinks)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
-        o, lse = _AttentionPrefill.apply(q, k, v, cu_seqlens, scale)
+        o, lse = _AttentionPrefill.apply(q, k, v, cu_seqlens, scale, sight)
     else:
-        o, lse, _ = _prefill_fwd(q, k, v, cu_seqlens, scale, output_lse, False)
+        o, lse, _ = _prefill_fwd(q, k, v, cu_seqlens, scale, sight, output_lse, False)
     return (o, lse) if output_lse else o
 
 

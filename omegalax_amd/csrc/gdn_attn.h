@@ -412,6 +412,99 @@ __device__ __forceinline__ bool dkv_share(const AttnParams& p, int row, int rank
   return true;
 }
 
+// The same with a window.  A tile of keys is seen by the rows up to window - 1 behind its last key; one
+// that holds sinks (its first ceil(sinks / 128) of them) by all rows behind it.  Those have up to
+// p.sink_splits shares and come first, the others up to p.splits, of p.share_tiles tiles' rows or so.
+__device__ __forceinline__ int window_shares(int tiles, int per, int most) {
+  const int n = (tiles + per - 1) / per;
+  return n < 1 ? 1 : (n < most ? n : most);
+}
+__device__ __forceinline__ int window_tiles(int window) { return (window - 1) / kDkvKeys + 2; }
+
+struct WindowShare : DkvShare {
+  int seq;
+  bool sink;
+};
+__device__ __forceinline__ bool dkv_window_share(const AttnParams& p, int row, int rank, int per, WindowShare& it) {
+  const int sinks = (int)((p.sinks + kDkvKeys - 1ll) / kDkvKeys), reach = window_tiles(p.window);
+  int len, tile, share = 0, shares = 1;
+  long long start;
+  if (p.splits == 1 && p.sink_splits == 1) {
+    AttnTile t;
+    if (!attn_tile(p, row, rank, kDkvKeys, t)) return false;
+    len = t.len, tile = t.tiles - 1 - t.tile, start = t.start, it.seq = t.seq;
+  } else {
+    int first = 0, n = lane_id() == 0 ? p.T : 0;  // lane i: sequence i
+    if (p.cu) packed_span(p.cu, p.N, p.T, first, n);
+    const int nt = (n + kDkvKeys - 1) / kDkvKeys, ns = nt < sinks ? nt : sinks;
+    const int a = window_shares(nt, p.share_tiles, p.sink_splits);
+    const int b = window_shares(nt < reach ? nt : reach, p.share_tiles, p.splits);
+    const int end = wave_scan(ns * a + (nt - ns) * b);
+    const unsigned long long past = __ballot(end > rank);
+    if (!past) return false;
+    const int s = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+    const int nsinks = __builtin_amdgcn_readlane(ns, s), na = __builtin_amdgcn_readlane(a, s);
+    const int nb = __builtin_amdgcn_readlane(b, s);
+    int x = rank - (s > 0 ? __builtin_amdgcn_readlane(end, s - 1) : 0);
+    if (x < nsinks * na) {
+      tile = x / na, share = x % na, shares = na;
+    } else {
+      x -= nsinks * na;
+      tile = nsinks + x / nb, share = x % nb, shares = nb;
+    }
+    start = (p.cu ? 0 : (long long)row * p.T) + __builtin_amdgcn_readlane(first, s);
+    len = __builtin_amdgcn_readlane(n, s);
+    it.seq = p.cu ? s : row;
+  }
+  const int k0 = tile * kDkvKeys;
+  it.sink = tile < sinks;
+  int ta = k0, tb = len;
+  if (!it.sink && len - k0 > kDkvKeys - 1 + p.window) tb = k0 + kDkvKeys - 1 + p.window;
+  if (shares > 1) {  // whole stages
+    const long long n = (tb - k0 + per - 1) / per;
+    ta = k0 + (int)(n * share / shares) * per;
+    if (share + 1 < shares) tb = k0 + (int)(n * (share + 1) / shares) * per;
+  }
+  it.len = len, it.k0 = k0, it.ta = ta, it.tb = tb, it.share = share, it.shares = shares, it.start = start;
+  return true;
+}
+
+// Where a workgroup's partial sums of a key go: element `at` of the tokens' keys, `slot` of the sinks'.
+__device__ __forceinline__ long long dkv_part(const AttnParams& p, const DkvShare& it, long long at, float*& k, float*& v) {
+  k = p.part_k, v = p.part_v;
+  return (long long)it.share * p.tokens * p.Hkv * p.D + at;
+}
+__device__ __forceinline__ long long dkv_part(const AttnParams& p, const WindowShare& it, long long at, float*& k, float*& v) {
+  if (!it.sink) return dkv_part(p, (const DkvShare&)it, at, k, v);
+  k = p.sink_k, v = p.sink_v;
+  const long long keys = (p.sinks + kDkvKeys - 1ll) / kDkvKeys * kDkvKeys, row = (long long)p.Hkv * p.D;
+  return (((long long)it.share * p.N + it.seq) * keys) * row + (at - it.start * row);
+}
+
+// Which of the 64 keys from k0 on a row at `pos` sees, a bit a key.  (Compared key by key, the bounds took 32
+// registers more, and with those of a cache thousands were spilled.)
+__device__ __forceinline__ unsigned long long keys_below(int n) {
+  return n <= 0 ? 0ull : (n < 64 ? (1ull << n) - 1 : ~0ull);
+}
+__device__ __forceinline__ unsigned long long window_bits(const AttnParams& p, int pos, int k0) {
+  const int upto = pos + 1 - k0;
+  return keys_below(upto) & (~keys_below(upto - p.window) | keys_below(p.sinks - k0));
+}
+
+// Rows r of a stage that starts at token t which do not see key `key`: those before it, r < first, and with
+// a window r >= past.
+struct RowMask {
+  int first, past;
+};
+__device__ __forceinline__ RowMask row_mask(const AttnParams& p, int key, int t) {
+  const int back = key > t ? key - t : 0, on = p.window - (t - key);
+  return {back * p.G, key < p.sinks ? 1 << 30 : (on < 0 ? 0 : (on < 64 ? on * p.G : 1 << 30))};
+}
+// whether some row of a stage of `per` tokens is past the window of some of 32 keys
+__device__ __forceinline__ bool past_window(const AttnParams& p, int kw, int t, int per) {
+  return t + (per - 1) - kw >= p.window && kw + 32 > p.sinks;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 }  // namespace omx

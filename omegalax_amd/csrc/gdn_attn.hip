@@ -31,7 +31,8 @@ constexpr int kNW = 4, kNT = 64 * kNW;
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
-template <int DP, bool PAGED>
+// WIN: a row sees its last p.window keys and the first p.sinks.
+template <int DP, bool PAGED, bool WIN>
 __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
 void attn_fwd_kernel(AttnParams p, int ranks) {
   constexpr int KS = DP / 16, DB = DP / 32;      // steps of a score, blocks of an output row
@@ -93,6 +94,16 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   // the tile's keys: 0 .. last, in tiles of kBN, of which this split takes [kt0, kt1)
   const int keys = held + t0 + nt;
   int kt0 = 0, kt1 = (keys + kBN - 1) / kBN;
+  // With a window these tiles are counted without the `skip` ones between the sinks' and the first
+  // row's window, which no row sees: tile kt begins at key key0(kt).
+  int sink_tiles = 0, skip = 0;
+  if constexpr (WIN) {
+    const int lo = held + t0 - p.window + 1;
+    sink_tiles = (p.sinks + kBN - 1) / kBN;
+    skip = lo / kBN > sink_tiles ? lo / kBN - sink_tiles : 0;
+    kt1 -= skip;
+  }
+  auto key0 = [&](int kt) { return (WIN && kt >= sink_tiles ? kt + skip : kt) * kBN; };
   if (PAGED && p.splits > 1) {
     const int each = (kt1 + p.splits - 1) / p.splits;
     kt0 = split * each < kt1 ? split * each : kt1;
@@ -126,9 +137,13 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   auto look = [&](int kt) {
     Pages x;
     x.have = 0;
+    if (WIN && kt == sink_tiles && skip > 0) {  // on from the sinks to the window
+      slot = key0(kt) / p.page;
+      off = key0(kt) - slot * p.page;
+    }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const bool in = kt * kBN + 16 * g < keys && slot < p.table_w;
+      const bool in = key0(kt) + 16 * g < keys && slot < p.table_w;
       int id = in ? table[slot] : -1;
       id = id >= p.n_pages ? -1 : id;
       id = __builtin_amdgcn_readfirstlane(id);
@@ -158,12 +173,12 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
                       lds + 1024u * kNW * j, lane_off[j % NO]);
       }
     } else {
-      int left = it.len - kt * kBN;  // rows past the sequence read as zeros
+      int left = it.len - key0(kt);  // rows past the sequence read as zeros
       left = left < kBN ? left : kBN;
       unsigned at[NL];
 #pragma unroll
       for (int j = 0; j < NL; ++j) at[j] = lane_off[(j0 + j) % NO] + (unsigned)((j0 + j) / NO * NO * kStep) * ld2;
-      loads_to_lds16(rsrc_words((const bf16_t*)rows + (it.start + (long long)kt * kBN) * ld + hk * D,
+      loads_to_lds16(rsrc_words((const bf16_t*)rows + (it.start + key0(kt)) * ld + hk * D,
                                 kt < kt1 ? (unsigned)(left - 1) * ld2 + 2u * D : 0),
                      lds + 1024u * kNW * j0, at);
     }
@@ -192,9 +207,23 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   };
   auto mask = [&](int kt, f32x16 (&s)[2], unsigned have) {
     mx = -INFINITY;
+    if constexpr (WIN) {
+      unsigned long long see = window_bits(p, pos, key0(kt));
+      if constexpr (PAGED)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (!((have >> g) & 1)) see &= ~(0xffffull << 16 * g);
+      see >>= 4 * h;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        if (!((see >> (32 * (e / 16) + 8 * (e % 16 / 4) + e % 4)) & 1)) s[e / 16][e % 16] = -INFINITY;
+        mx = fmaxf(mx, s[e / 16][e % 16]);
+      }
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
-      const int key = kt * kBN + 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * h + e % 4;
+      const int key = key0(kt) + 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * h + e % 4;
       if (key > pos || (PAGED && !((have >> (e / 8)) & 1))) s[e / 16][e % 16] = -INFINITY;
       mx = fmaxf(mx, s[e / 16][e % 16]);
     }
@@ -260,7 +289,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   auto clear = [&](int kt, bf16_t* sv, unsigned have) {
     for (int i = tid; i < kBN * DP / 8; i += kNT) {
       const int r = i / (DP / 8);
-      if (kt * kBN + r >= keys || !((have >> (r / 16)) & 1)) *(u32x4*)(sv + 8 * i) = u32x4{0, 0, 0, 0};
+      if (key0(kt) + r >= keys || !((have >> (r / 16)) & 1)) *(u32x4*)(sv + 8 * i) = u32x4{0, 0, 0, 0};
     }
   };
   unsigned have = 15;
@@ -269,7 +298,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     wait_loads<0>();  // this wavefront's part of the tiles
     lds_barrier();    // everyone's; and the other buffers are free
     if constexpr (PAGED) {
-      if (have != 15 || (kt + 1) * kBN > keys) {  // uniform in the workgroup
+      if (have != 15 || key0(kt) + kBN > keys) {  // uniform in the workgroup
         clear(kt, sV + (kt & 1) * kTile, have);
         lds_barrier();
       }
@@ -286,8 +315,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     Pages p0;
     p0.have = pn.have = pk.have = 15;
     if constexpr (PAGED) {
-      slot = kt0 * kBN / p.page;
-      off = kt0 * kBN - slot * p.page;
+      slot = key0(kt0) / p.page;
+      off = key0(kt0) - slot * p.page;
       p0 = look(kt0);
       pn = look(kt0 + 1);
       pk = look(kt0 + 2);
@@ -302,13 +331,14 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     wait_loads<0>();
     lds_barrier();
     // the wavefront's own last tile: rows of it see no keys of later ones
-    const int last_kt = w_hi / kBN < kt1 - 1 ? w_hi / kBN : kt1 - 1;
+    const int w_kt = w_hi / kBN - skip, last_kt = w_kt < kt1 - 1 ? w_kt : kt1 - 1;
     int kt = kt0;
     if (kt <= last_kt) {
       f32x16 s0[2], s1[2];
       auto turn = [&](auto more, f32x16 (&s)[2], f32x16 (&sn)[2]) {
         enter(kt);
-        if (kt * kBN + kBN - 1 > w_lo || have != 15) mask(kt, s, have);
+        const int k0 = key0(kt);
+        if (k0 + kBN - 1 > w_lo || have != 15 || (WIN && k0 <= w_hi - p.window && k0 + kBN > p.sinks)) mask(kt, s, have);
         phase1(more, s, sn, sK + ((kt + 1) & 1) * kTile, sV + (kt & 1) * kTile, kt);
         phase2(more, sn, sV + (kt & 1) * kTile, kt);
         leave(kt);
@@ -358,10 +388,10 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       float acc[DP / 64];
 #pragma unroll
       for (int e = 0; e < DP / 64; ++e) acc[e] = 0.f;
-      const int last = kt1 * kBN - 1 < pos1 ? kt1 * kBN - 1 : pos1;
-      for (int k0 = kt0 * kBN; k0 <= last; k0 += 64) {  // a key a lane
-        const int key = k0 + l;
-        bool see = key <= last;
+      static_assert(kBN == 64, "a key a lane");
+      for (int kt = kt0; kt < kt1 && key0(kt) <= pos1; ++kt) {
+        const int key = key0(kt) + l;
+        bool see = key <= pos1 && (!WIN || key > pos1 - p.window || key < p.sinks);
         long long at = (it.start + key) * p.k_ld + hk * D, av = (it.start + key) * p.v_ld + hk * D;
         if constexpr (PAGED) {
           const int sl = key / p.page;
@@ -599,13 +629,18 @@ hipError_t launch_attn_fwd(const AttnParams& p, hipStream_t stream) {
   const long long ranks = attn_ranks(p, per), units = (long long)(p.cu ? 1 : p.N) * p.Hkv;
   const bool paged = p.k_pages != nullptr;
   const dim3 grid((unsigned)attn_grid(units, ranks), paged ? (unsigned)p.splits : 1u);
+  const bool win = p.window > 0;
   switch (padded_dim(p.D)) {
-#define OMX_FWD(DP)                                                                   \
-  case DP:                                                                            \
-    if (paged)                                                                        \
-      attn_fwd_kernel<DP, true><<<grid, kNT, 0, stream>>>(p, (int)ranks);             \
-    else                                                                              \
-      attn_fwd_kernel<DP, false><<<grid, kNT, 0, stream>>>(p, (int)ranks);            \
+#define OMX_FWD(DP)                                                            \
+  case DP:                                                                     \
+    if (paged && win)                                                          \
+      attn_fwd_kernel<DP, true, true><<<grid, kNT, 0, stream>>>(p, (int)ranks); \
+    else if (paged)                                                            \
+      attn_fwd_kernel<DP, true, false><<<grid, kNT, 0, stream>>>(p, (int)ranks); \
+    else if (win)                                                              \
+      attn_fwd_kernel<DP, false, true><<<grid, kNT, 0, stream>>>(p, (int)ranks); \
+    else                                                                       \
+      attn_fwd_kernel<DP, false, false><<<grid, kNT, 0, stream>>>(p, (int)ranks); \
     break;
     OMX_FWD(64)
     OMX_FWD(128)

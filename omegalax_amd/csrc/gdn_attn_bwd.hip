@@ -7,6 +7,8 @@
 // Two kernels, each of which owns what it sums, so no sum depends on the order of atomics: one
 // passes over the keys for a tile of rows (dq, and delta for the other), one over the rows for a
 // tile of keys (dk, dv).  The scores and do . v are formed in both, 7 products in place of 5.
+#include <type_traits>
+
 #include "gdn_attn.h"
 
 namespace omx {
@@ -23,7 +25,8 @@ constexpr int kRows = 32, kRing = 4;  // a stage's rows, stages in LDS
 // 3,001 tokens in 5 sequences of 16/2 heads of 256: 74 us (125 with stages of 64 rows twice buffered,
 // the compiler's order and whole tiles in four shares each).  A stage takes 1.5 times its MFMAs; the
 // rest is what comes before the first stage and the partial sums behind the last, about 14 us.
-template <int DP>
+// WIN: a row sees its last p.window keys and the first p.sinks.
+template <int DP, bool WIN>
 __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(1)))
 void attn_dkv_wide_kernel(AttnParams p, int ranks) {
   constexpr int KS = DP / 16, DB = DP / 32, PF = 4;
@@ -44,8 +47,12 @@ void attn_dkv_wide_kernel(AttnParams p, int ranks) {
   attn_place((int)blockIdx.x, (p.cu ? 1 : p.N) * Hkv, ranks, unit, rank);
   if (rank >= ranks) return;
   const int hk = unit % Hkv;
-  DkvShare it;
-  if (!dkv_share(p, unit / Hkv, rank, per, it)) return;
+  std::conditional_t<WIN, WindowShare, DkvShare> it;
+  if constexpr (WIN) {
+    if (!dkv_window_share(p, unit / Hkv, rank, per, it)) return;
+  } else {
+    if (!dkv_share(p, unit / Hkv, rank, per, it)) return;
+  }
   const int kw = it.k0 + 32 * w, key = kw + c;  // the wavefront's first key, the lane's
 
   // stages from the last to the first: a unit's workgroups, which start together and see different
@@ -140,7 +147,17 @@ void attn_dkv_wide_kernel(AttnParams p, int ranks) {
       __builtin_amdgcn_sched_barrier(0);
     }
     const int t = t_last - i0 * per;
-    if (t < kw + 31) {  // row r is token t + r / G: before the key if r < (key - t) G
+    if (WIN && (t < kw + 31 || past_window(p, kw, t, per))) {
+      int c1 = lane_id() & 31;
+      asm volatile("" : "+v"(c1));
+      const RowMask m = row_mask(p, kw + c1, t);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = 8 * (i / 4) + 4 * h + i % 4;
+        if (r < m.first || r >= m.past) s[i] = -INFINITY;
+      }
+    }
+    if (!WIN && t < kw + 31) {  // row r is token t + r / G: before the key if r < (key - t) G
       int first = lane_id() & 31;
       asm volatile("" : "+v"(first));
       first = (kw + first - t) * G;
@@ -195,11 +212,16 @@ void attn_dkv_wide_kernel(AttnParams p, int ranks) {
   wait_loads<0>();
   if (key >= it.len) return;
   const long long at = ((it.start + key) * Hkv + hk) * D;
-  if (p.splits > 1 && it.share == 0 && h == 0) p.shares[at / D] = it.shares;
+  if constexpr (WIN) {
+    if (p.splits > 1 && it.share == 0 && h == 0) p.shares[at / D] = it.sink ? 1 : it.shares;
+  } else {
+    if (p.splits > 1 && it.share == 0 && h == 0) p.shares[at / D] = it.shares;
+  }
   if (it.shares > 1) {
-    const long long ps = (long long)it.share * p.tokens * Hkv * D + at;
-    store_part<DB>(p.part_k + ps, dk, p.scale, D, h);
-    store_part<DB>(p.part_v + ps, dv, 1.f, D, h);
+    float *pk, *pv;
+    const long long ps = dkv_part(p, it, at, pk, pv);
+    store_part<DB>(pk + ps, dk, p.scale, D, h);
+    store_part<DB>(pv + ps, dv, 1.f, D, h);
   } else {
     store_rows<DB>((bf16_t*)p.dk + at, dk, p.scale, D, h);
     store_rows<DB>((bf16_t*)p.dv + at, dv, 1.f, D, h);
@@ -226,6 +248,35 @@ __global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnParams p, long lo
       u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
 }
 
+// The same of the tiles that hold sinks, whose shares lie by sequence.
+__global__ __launch_bounds__(256) void attn_sink_sum_kernel(AttnParams p, long long n) {
+  const long long i = 8 * ((long long)blockIdx.x * 256 + threadIdx.x);
+  const long long row = (long long)p.Hkv * p.D, keys = attn_sink_keys(p.sinks);
+  const int seq = (int)((i < n ? i : 0) / (row * keys));
+  int first = 0, len = p.T;
+  if (p.cu) {
+    packed_span(p.cu, p.N, p.T, first, len);
+    first = __shfl(first, seq, 64);
+    len = __shfl(len, seq, 64);
+  }
+  const long long in = (i < n ? i : 0) - seq * row * keys;  // of the sequence
+  if (i >= n || in / row >= len) return;
+  const int shares = window_shares((len + kDkvKeys - 1) / kDkvKeys, p.share_tiles, p.sink_splits);
+  if (shares < 2) return;
+  const float* src = blockIdx.y ? p.sink_v : p.sink_k;
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < shares; ++s)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x4 y = *(const f32x4*)(src + s * n + i + 4 * j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * j + e] += y[e];
+    }
+  const long long at = ((p.cu ? 0 : (long long)seq * p.T) + first) * row + in;
+  *(u32x4*)((bf16_t*)(blockIdx.y ? p.dv : p.dk) + at) =
+      u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+}
+
 }  // namespace
 
 int attn_dkv_tile_tokens() { return kDkvKeys; }
@@ -240,7 +291,7 @@ int attn_dkv_tile_tokens() { return kDkvKeys; }
 // 16/2 heads of 256, both passes, 1,704 us whole, 496 in 7 shares, 620 in 8.  Partial sums take 512 MiB
 // at most.
 DkvPlan attn_dkv_plan(long long units, long long T, long long N, int G, long long row_bytes) {
-  DkvPlan plan{1, 0};
+  DkvPlan plan{1, 0, 1};
   if (N > 64 || T == 0 || units == 0) return plan;  // shares are found by lanes that hold a sequence each
   const long long seqs = N > 0 ? N : 1, nt = (T / seqs + kDkvKeys - 1) / kDkvKeys;
   const long long longest = (T + kDkvKeys - 1) / kDkvKeys;  // of sequences of any lengths
@@ -271,18 +322,75 @@ DkvPlan attn_dkv_plan(long long units, long long T, long long N, int G, long lon
   return plan;
 }
 
+// With a window most tiles are seen by as many rows, and those with sinks by all behind them: their
+// shares are as long as the others'.  Partial sums take 768 MiB at most.
+DkvPlan attn_dkv_window_plan(long long B, long long T, long long N, int Hkv, int G, int D, int window, int sinks) {
+  DkvPlan plan{1, 1, 1};
+  const long long seqs = N > 0 ? N : B;
+  if (N > 64 || T == 0 || seqs == 0) return plan;
+  const long long longest = (T + kDkvKeys - 1) / kDkvKeys, avg = N > 0 ? (T / N + kDkvKeys - 1) / kDkvKeys : longest;
+  const long long nt = avg < 1 ? 1 : avg, sink = (sinks + 127ll) / 128, ns = nt < sink ? nt : sink;
+  long long reach = (window - 1) / kDkvKeys + 2;
+  const long long most = longest < reach ? longest : reach;  // tiles' rows that see a tile without sinks
+  reach = nt < reach ? nt : reach;
+  const long long row = (long long)Hkv * D * 8, room = (512ll << 20) / (B * T * row);
+  const long long sink_room = sink > 0 ? (256ll << 20) / (seqs * attn_sink_keys(sinks) * row) : 1;
+  const long long units = (long long)Hkv * seqs;
+  const double tile = 4. * G;
+  double best = 0;
+  for (long long s = 1; s <= 16 && s <= most && (s == 1 || s <= room); ++s) {
+    const long long m = (most + s - 1) / s;
+    long long a = (longest + m - 1) / m, b = (reach + m - 1) / m;
+    a = a < sink_room ? a : sink_room;
+    a = ns > 0 ? (a < 255 ? (a < 1 ? 1 : a) : 255) : 1;
+    const long long groups = units * (ns * a + (nt - ns) * b);
+    const double each = tile * ((double)(most + s - 1) / s), far = ns > 0 ? tile * nt / (nt < a ? nt : a) : 0.;
+    const double work = units * tile * (ns * nt + (nt - ns) * reach) / kComputeUnits;
+    const long long rounds = (groups + kComputeUnits - 1) / kComputeUnits;
+    double ends = rounds <= 2 ? rounds * each : work + each / 2;
+    ends = ends > far ? ends : far;
+    const double cost = ends + 16. * rounds + units * ((a > 1 ? ns * a : 0) + (b > 1 ? (nt - ns) * b : 0)) / 20.;
+    if (s == 1 || cost < best) {
+      best = cost;
+      plan = DkvPlan{(int)((most + m - 1) / m), (int)m, (int)a};
+    }
+  }
+  return plan;
+}
+
+namespace {
+long long dkv_units(const AttnParams& p) { return (long long)(p.cu ? 1 : p.N) * p.Hkv; }
+long long dkv_ranks(const AttnParams& p) {
+  long long ranks = attn_ranks(p, kDkvKeys) * p.splits;
+  if (p.window > 0 && p.sink_splits > 1) ranks += attn_sink_keys(p.sinks) / kDkvKeys * p.sink_splits * (p.cu ? p.N : 1);
+  return ranks;
+}
+}  // namespace
+
+long long attn_dkv_groups(const AttnParams& p) { return attn_grid(dkv_units(p), dkv_ranks(p)); }
+
 hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream) {
-  const long long ranks = attn_ranks(p, kDkvKeys) * p.splits, units = (long long)(p.cu ? 1 : p.N) * p.Hkv;
-  const unsigned grid = (unsigned)attn_grid(units, ranks);
+  const long long ranks = dkv_ranks(p);
+  const unsigned grid = (unsigned)attn_dkv_groups(p);
   if (p.D <= 128)
     launch_attn_dkv_narrow(p, grid, (int)ranks, stream);
+  else if (p.window > 0)
+    attn_dkv_wide_kernel<256, true><<<grid, kNT, 0, stream>>>(p, (int)ranks);
   else
-    attn_dkv_wide_kernel<256><<<grid, kNT, 0, stream>>>(p, (int)ranks);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.splits == 1) return e;
-  const long long n = p.tokens * p.Hkv * p.D;
-  attn_dkv_sum_kernel<<<dim3((unsigned)((n + 2047) / 2048), 2), 256, 0, stream>>>(p, n);
-  return hipGetLastError();
+    attn_dkv_wide_kernel<256, false><<<grid, kNT, 0, stream>>>(p, (int)ranks);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (p.splits > 1) {
+    const long long n = p.tokens * p.Hkv * p.D;
+    attn_dkv_sum_kernel<<<dim3((unsigned)((n + 2047) / 2048), 2), 256, 0, stream>>>(p, n);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && p.window > 0 && p.sink_splits > 1) {
+    const long long n = (long long)p.N * attn_sink_keys(p.sinks) * p.Hkv * p.D;
+    attn_sink_sum_kernel<<<dim3((unsigned)((n + 2047) / 2048), 2), 256, 0, stream>>>(p, n);
+    e = hipGetLastError();
+  }
+  return e;
 }
 
 }  // namespace omx

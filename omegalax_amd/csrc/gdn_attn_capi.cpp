@@ -151,6 +151,24 @@ int check_grid(const char* fn, const Shape& s, int64_t per) {
   return OMX_GDN_OK;
 }
 
+// What a row sees: its last `window` keys, all of them for 0, and the first `sinks`.
+struct Sight {
+  int64_t window, sinks;
+};
+constexpr Sight kAllKeys{0, 0};
+
+int check_sight(const char* fn, const Sight& x) {
+  REQUIRE(x.window >= 1, "%s: window %lld must be at least 1", fn, (long long)x.window);
+  REQUIRE(x.sinks >= 0, "%s: sinks %lld must not be negative", fn, (long long)x.sinks);
+  return OMX_GDN_OK;
+}
+// that of sequences of at most `keys`: kernels for a window only where it leaves out a key
+void look_at(omx::AttnParams& p, const Sight& x, int64_t keys) {
+  if (x.window == 0 || x.window >= keys || x.sinks >= keys - x.window) return;
+  p.window = (int)x.window;
+  p.sinks = (int)x.sinks;
+}
+
 }  // namespace
 
 extern "C" {
@@ -160,11 +178,11 @@ size_t omx_gdn_attn_fwd_workspace_size(int64_t T, int64_t Hq, int64_t Hkv, int64
   return plan_ws(0, T, N, omx::attn_tile_tokens((int)(Hq / Hkv))).total;
 }
 
-int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
-                     const int32_t* cu_seqlens, int64_t N, void* o, float* lse, void* o_rest, int64_t B, int64_t T,
-                     int64_t Hq, int64_t Hkv, int64_t D, float scale, void* workspace, size_t workspace_bytes,
-                     void* stream) {
-  const char* fn = "omx_gdn_attn_fwd";
+namespace {
+int attn_fwd(const char* fn, const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+             const int32_t* cu_seqlens, int64_t N, void* o, float* lse, void* o_rest, int64_t B, int64_t T, int64_t Hq,
+             int64_t Hkv, int64_t D, float scale, const Sight& sight, void* workspace, size_t workspace_bytes,
+             void* stream) {
   const Shape s{N, B, T, Hq, Hkv, D, cu_seqlens != nullptr};
   int rc = check_shape(fn, s);
   if (!rc) rc = check_ld(fn, "q_ld", q_ld, Hq * D);
@@ -185,9 +203,30 @@ int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, 
   omx::AttnParams p = params(s, scale);
   p.q = q; p.k = k; p.v = v; p.o = o; p.o_rest = o_rest; p.lse = lse;
   p.q_ld = q_ld; p.k_ld = k_ld; p.v_ld = v_ld; p.cu = cu_seqlens;
+  look_at(p, sight, T);
   hipError_t e = use_plan(p, ws, workspace, per, (hipStream_t)stream);
   if (e == hipSuccess) e = omx::launch_attn_fwd(p, (hipStream_t)stream);
   return launch_status(e, fn);
+}
+}  // namespace
+
+int omx_gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+                     const int32_t* cu_seqlens, int64_t N, void* o, float* lse, void* o_rest, int64_t B, int64_t T,
+                     int64_t Hq, int64_t Hkv, int64_t D, float scale, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  return attn_fwd("omx_gdn_attn_fwd", q, k, v, q_ld, k_ld, v_ld, cu_seqlens, N, o, lse, o_rest, B, T, Hq, Hkv, D, scale,
+                  kAllKeys, workspace, workspace_bytes, stream);
+}
+
+int omx_gdn_attn_window_fwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+                            const int32_t* cu_seqlens, int64_t N, void* o, float* lse, void* o_rest, int64_t B,
+                            int64_t T, int64_t Hq, int64_t Hkv, int64_t D, float scale, int64_t window, int64_t sinks,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  const Sight sight{window, sinks};
+  const int rc = check_sight("omx_gdn_attn_window_fwd", sight);
+  if (rc) return rc;
+  return attn_fwd("omx_gdn_attn_window_fwd", q, k, v, q_ld, k_ld, v_ld, cu_seqlens, N, o, lse, o_rest, B, T, Hq, Hkv, D,
+                  scale, sight, workspace, workspace_bytes, stream);
 }
 
 namespace {
@@ -196,14 +235,18 @@ struct AttnBwdWs {
   size_t stats;
   PlanWs rows, keys;
   omx::DkvPlan share;
-  size_t shares, part_k, part_v, total;
+  size_t shares, part_k, part_v, sink_k, sink_v, total;
+  omx::AttnParams sight;  // its window and sinks
 };
-AttnBwdWs attn_bwd_ws(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N) {
+AttnBwdWs attn_bwd_ws(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N, const Sight& sight) {
   AttnBwdWs w{};
   const int per = omx::attn_dkv_tile_tokens();
   w.rows = plan_ws(align_up((size_t)(B * T * Hq) * 8), T, N, omx::attn_tile_tokens((int)(Hq / Hkv)));
   w.keys = plan_ws(w.rows.total, T, N, per);
-  w.share = omx::attn_dkv_plan(B * Hkv, T, N, (int)(Hq / Hkv), B * T * Hkv * D * 8);
+  look_at(w.sight, sight, T);
+  const int window = w.sight.window, sinks = w.sight.sinks;
+  w.share = window > 0 ? omx::attn_dkv_window_plan(B, T, N, (int)Hkv, (int)(Hq / Hkv), (int)D, window, sinks)
+                       : omx::attn_dkv_plan(B * Hkv, T, N, (int)(Hq / Hkv), B * T * Hkv * D * 8);
   w.shares = w.part_k = w.part_v = w.total = w.keys.total;
   if (w.share.splits > 1) {
     const size_t one = align_up((size_t)w.share.splits * B * T * Hkv * D * 4);
@@ -211,20 +254,19 @@ AttnBwdWs attn_bwd_ws(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, 
     w.part_v = w.part_k + one;
     w.total = w.part_v + one;
   }
+  w.sink_k = w.sink_v = w.total;
+  if (w.share.sink_splits > 1) {
+    const size_t one = align_up((size_t)w.share.sink_splits * (N > 0 ? N : B) * omx::attn_sink_keys(sinks) * Hkv * D * 4);
+    w.sink_v = w.sink_k + one;
+    w.total = w.sink_v + one;
+  }
   return w;
 }
-}  // namespace
 
-size_t omx_gdn_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N) {
-  if (!sized(B, T, Hq, Hkv, D, N)) return 0;
-  return attn_bwd_ws(B, T, Hq, Hkv, D, N).total;
-}
-
-int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
-                     const int32_t* cu_seqlens, int64_t N, const void* o, const float* lse, const void* o_rest, const void* d_o,
-                     void* dq, void* dk, void* dv, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
-                     float scale, void* workspace, size_t workspace_bytes, void* stream) {
-  const char* fn = "omx_gdn_attn_bwd";
+int attn_bwd(const char* fn, const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+             const int32_t* cu_seqlens, int64_t N, const void* o, const float* lse, const void* o_rest, const void* d_o,
+             void* dq, void* dk, void* dv, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, float scale,
+             const Sight& sight, void* workspace, size_t workspace_bytes, void* stream) {
   const Shape s{N, B, T, Hq, Hkv, D, cu_seqlens != nullptr};
   int rc = check_shape(fn, s);
   if (!rc) rc = check_ld(fn, "q_ld", q_ld, Hq * D);
@@ -234,7 +276,7 @@ int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, 
   const int per = rc ? 1 : omx::attn_tile_tokens((int)(Hq / Hkv));
   if (!rc) rc = check_grid(fn, s, per);
   if (rc) return rc;
-  const AttnBwdWs ws = attn_bwd_ws(B, T, Hq, Hkv, D, s.packed ? N : 0);
+  const AttnBwdWs ws = attn_bwd_ws(B, T, Hq, Hkv, D, s.packed ? N : 0, sight);
   REQUIRE(workspace_bytes >= ws.total, "%s: workspace of %zu bytes is smaller than the %zu needed", fn,
           workspace_bytes, ws.total);
   if (B * T == 0) return ok();
@@ -254,12 +296,51 @@ int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, 
   p.part_v = (float*)((char*)workspace + ws.part_v);
   p.splits = ws.share.splits;
   p.share_tiles = ws.share.tiles;
+  p.window = ws.sight.window;
+  p.sinks = ws.sight.sinks;
+  p.sink_splits = ws.share.sink_splits;
+  p.sink_k = (float*)((char*)workspace + ws.sink_k);
+  p.sink_v = (float*)((char*)workspace + ws.sink_v);
+  if (p.window > 0)
+    REQUIRE(omx::attn_dkv_groups(p) <= kMaxGroups, "%s: grid too large", fn);
   const hipStream_t st = (hipStream_t)stream;
   hipError_t e = use_plan(p, ws.rows, workspace, per, st);
   if (e == hipSuccess) e = omx::launch_attn_dq(p, st);
   if (e == hipSuccess) e = use_plan(p, ws.keys, workspace, omx::attn_dkv_tile_tokens(), st);
   if (e == hipSuccess) e = omx::launch_attn_dkv(p, st);
   return launch_status(e, fn);
+}
+}  // namespace
+
+size_t omx_gdn_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N) {
+  if (!sized(B, T, Hq, Hkv, D, N)) return 0;
+  return attn_bwd_ws(B, T, Hq, Hkv, D, N, kAllKeys).total;
+}
+
+size_t omx_gdn_attn_window_bwd_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N,
+                                              int64_t window, int64_t sinks) {
+  if (!sized(B, T, Hq, Hkv, D, N) || window < 1 || sinks < 0) return 0;
+  return attn_bwd_ws(B, T, Hq, Hkv, D, N, Sight{window, sinks}).total;
+}
+
+int omx_gdn_attn_bwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+                     const int32_t* cu_seqlens, int64_t N, const void* o, const float* lse, const void* o_rest, const void* d_o,
+                     void* dq, void* dk, void* dv, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                     float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  return attn_bwd("omx_gdn_attn_bwd", q, k, v, q_ld, k_ld, v_ld, cu_seqlens, N, o, lse, o_rest, d_o, dq, dk, dv, B, T, Hq,
+                  Hkv, D, scale, kAllKeys, workspace, workspace_bytes, stream);
+}
+
+int omx_gdn_attn_window_bwd(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+                            const int32_t* cu_seqlens, int64_t N, const void* o, const float* lse, const void* o_rest,
+                            const void* d_o, void* dq, void* dk, void* dv, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                            int64_t D, float scale, int64_t window, int64_t sinks, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  const Sight sight{window, sinks};
+  const int rc = check_sight("omx_gdn_attn_window_bwd", sight);
+  if (rc) return rc;
+  return attn_bwd("omx_gdn_attn_window_bwd", q, k, v, q_ld, k_ld, v_ld, cu_seqlens, N, o, lse, o_rest, d_o, dq, dk, dv, B,
+                  T, Hq, Hkv, D, scale, sight, workspace, workspace_bytes, stream);
 }
 
 size_t omx_gdn_kv_write_workspace_size(int64_t T, int64_t N) {

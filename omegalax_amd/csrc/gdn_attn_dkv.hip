@@ -1,4 +1,6 @@
 // Gradients of causal softmax attention: dk and dv, for heads of up to 128 (see gdn_attn_bwd.hip).
+#include <type_traits>
+
 #include "gdn_attn.h"
 
 namespace omx {
@@ -28,7 +30,8 @@ struct Slot {
   static constexpr int i = I;
 };
 
-template <int DP>
+// WIN: a row sees its last p.window keys and the first p.sinks.
+template <int DP, bool WIN>
 __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void attn_dkv_kernel(AttnParams p, int ranks) {
   constexpr int KS = DP / 16, DB = DP / 32, NG = 2 * KS, EG = 16 / NG;
@@ -47,8 +50,12 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
   attn_place((int)blockIdx.x, (p.cu ? 1 : p.N) * Hkv, ranks, unit, rank);
   if (rank >= ranks) return;
   const int hk = unit % Hkv;
-  DkvShare it;
-  if (!dkv_share(p, unit / Hkv, rank, per, it)) return;
+  std::conditional_t<WIN, WindowShare, DkvShare> it;
+  if constexpr (WIN) {
+    if (!dkv_window_share(p, unit / Hkv, rank, per, it)) return;
+  } else {
+    if (!dkv_share(p, unit / Hkv, rank, per, it)) return;
+  }
   const int kw = it.k0 + 32 * w, key = kw + c;
   // stages from the last to the first: a unit's workgroups, which start together and see different
   // numbers of rows, then read the same rows at the same time, and its XCD's L2 serves most of them
@@ -183,6 +190,15 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
   };
   // row r of a stage is token t + r / G: before the key if r < (key - t) G
   auto mask = [&](f32x16& s, int t) {
+    if constexpr (WIN) {
+      const RowMask m = row_mask(p, key, t);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = 8 * (i / 4) + 4 * h + i % 4;
+        if (r < m.first || r >= m.past) s[i] = -INFINITY;
+      }
+      return;
+    }
     const int first = (key - t) * G;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -196,7 +212,7 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
     constexpr int I = decltype(slot)::i;
     if (i < na) {
       const int t = t_last - i * per;
-      if (t < kw + 31) mask(s, t);
+      if (t < kw + 31 || (WIN && past_window(p, kw, t, per))) mask(s, t);
       phase1(s, dp, sn, dpn, ring + I * kSlot);
     }
     wait_loads<(kRing - 4) * kLoads>();
@@ -246,11 +262,16 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
   wait_loads<0>();
   if (key >= it.len) return;
   const long long at = ((it.start + key) * Hkv + hk) * D;
-  if (p.splits > 1 && it.share == 0 && h == 0) p.shares[at / D] = it.shares;
+  if constexpr (WIN) {
+    if (p.splits > 1 && it.share == 0 && h == 0) p.shares[at / D] = it.sink ? 1 : it.shares;
+  } else {
+    if (p.splits > 1 && it.share == 0 && h == 0) p.shares[at / D] = it.shares;
+  }
   if (it.shares > 1) {
-    const long long ps = (long long)it.share * p.tokens * Hkv * D + at;
-    store_part<DB>(p.part_k + ps, dk, p.scale, D, h);
-    store_part<DB>(p.part_v + ps, dv, 1.f, D, h);
+    float *pk, *pv;
+    const long long ps = dkv_part(p, it, at, pk, pv);
+    store_part<DB>(pk + ps, dk, p.scale, D, h);
+    store_part<DB>(pv + ps, dv, 1.f, D, h);
   } else {
     store_rows<DB>((bf16_t*)p.dk + at, dk, p.scale, D, h);
     store_rows<DB>((bf16_t*)p.dv + at, dv, 1.f, D, h);
@@ -260,10 +281,14 @@ void attn_dkv_kernel(AttnParams p, int ranks) {
 }  // namespace
 
 void launch_attn_dkv_narrow(const AttnParams& p, unsigned grid, int ranks, hipStream_t stream) {
-  if (p.D <= 64)
-    attn_dkv_kernel<64><<<grid, kNT, 0, stream>>>(p, ranks);
+  if (p.D <= 64 && p.window > 0)
+    attn_dkv_kernel<64, true><<<grid, kNT, 0, stream>>>(p, ranks);
+  else if (p.D <= 64)
+    attn_dkv_kernel<64, false><<<grid, kNT, 0, stream>>>(p, ranks);
+  else if (p.window > 0)
+    attn_dkv_kernel<128, true><<<grid, kNT, 0, stream>>>(p, ranks);
   else
-    attn_dkv_kernel<128><<<grid, kNT, 0, stream>>>(p, ranks);
+    attn_dkv_kernel<128, false><<<grid, kNT, 0, stream>>>(p, ranks);
 }
 
 }  // namespace omx

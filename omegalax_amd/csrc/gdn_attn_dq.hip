@@ -19,7 +19,8 @@ struct No { static constexpr bool value = false; };
 // Bound by the MFMAs, three products a block: B=4 T=4,096 of 32/8 heads of 128 760 to 820 us (the
 // compiler's own order, tiles of 64 keys: 805 to 860); with few tiles by the longest and the loads
 // before it: 3,001 tokens in 5 sequences of 16/2 heads of 256 56 us (73).
-template <int DP>
+// WIN: as for the forward.
+template <int DP, bool WIN>
 __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
 void attn_dq_kernel(AttnParams p, int ranks) {
   constexpr int KS = DP / 16, DB = DP / 32, EG = 16 / KS, PF = 4;
@@ -46,7 +47,15 @@ void attn_dq_kernel(AttnParams p, int ranks) {
   const int pos = t0 + rt, w_lo = t0 + (32 * w) / G, w_hi = t0 + (32 * w + 31) / G;
 
   // fetches block kb's keys (and values) into its slot; blocks past the last have an empty range
-  const int nb = (t0 + nt + kBN - 1) / kBN;
+  // (with a window counted without the `skip` ones that no row sees: block kb begins at key0(kb))
+  int nb = (t0 + nt + kBN - 1) / kBN, sink_blocks = 0, skip = 0;
+  if constexpr (WIN) {
+    const int lo = t0 - p.window + 1;
+    sink_blocks = (p.sinks + kBN - 1) / kBN;
+    skip = lo / kBN > sink_blocks ? lo / kBN - sink_blocks : 0;
+    nb -= skip;
+  }
+  auto key0 = [&](int kb) { return (WIN && kb >= sink_blocks ? kb + skip : kb) * kBN; };
   constexpr int kStep = 64 / (DP / 8) * kNW, NO = kStep % 16 ? 2 : 1;
   static_assert(NO * kStep % 16 == 0 && NO <= NJ, "rows whose swizzle repeats");
   const unsigned kld2 = (unsigned)(p.k_ld * 2), vld2 = (unsigned)(p.v_ld * 2);
@@ -59,9 +68,9 @@ void attn_dq_kernel(AttnParams p, int ranks) {
   }
   const unsigned lds0 = lds_address(ring) + 1024u * (unsigned)w;
   auto fetch = [&](int kb, const void* rows, long long ld, unsigned ld2, const unsigned (&off)[NJ], unsigned part) {
-    int left = it.len - kb * kBN;  // rows past the sequence read as zeros
+    int left = it.len - key0(kb);  // rows past the sequence read as zeros
     left = left < kBN ? left : kBN;
-    loads_to_lds16(rsrc_words((const bf16_t*)rows + (it.start + (long long)kb * kBN) * ld + hk * D,
+    loads_to_lds16(rsrc_words((const bf16_t*)rows + (it.start + key0(kb)) * ld + hk * D,
                               kb < nb ? (unsigned)(left - 1) * ld2 + 2u * D : 0),
                    lds0 + 2u * (kSlot * (unsigned)(kb & (kRing - 1)) + part), off);
   };
@@ -109,6 +118,13 @@ void attn_dq_kernel(AttnParams p, int ranks) {
   auto slot = [&](int kb) { return ring + (kb & (kRing - 1)) * kSlot; };
   auto tr = [&](const bf16_t* sk, AttnLane ln, int t) { return attn_frag_tr<DP>(sk, ln, 16 * (t / DB), t % DB); };
   auto mask = [&](int kb, f32x16& s) {
+    if constexpr (WIN) {
+      const unsigned see = (unsigned)window_bits(p, pos, key0(kb)) >> 4 * h;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (!((see >> (8 * (i / 4) + i % 4)) & 1)) s[i] = -INFINITY;
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       if (kb * kBN + 8 * (i / 4) + 4 * h + i % 4 > pos) s[i] = -INFINITY;
@@ -119,7 +135,8 @@ void attn_dq_kernel(AttnParams p, int ranks) {
     wait_loads<kLoads>();  // all but block kb + 2: block kb + 1 is there
     lds_barrier();         // everyone's; and block kb - 1's slot is free
     const bf16_t *st = slot(kb), *st1 = slot(kb + 1);
-    if (kb * kBN + kBN - 1 > w_lo) mask(kb, s);
+    const int k0 = key0(kb);
+    if (k0 + kBN - 1 > w_lo || (WIN && k0 <= w_hi - p.window && k0 + kBN > p.sinks)) mask(kb, s);
     const AttnLane ln = fresh(lane);
     f32x16 dp = zero16();
 #pragma unroll
@@ -167,7 +184,7 @@ void attn_dq_kernel(AttnParams p, int ranks) {
 #pragma unroll
   for (int t = 0; t < PF; ++t) f[t] = attn_frag<DP>(slot(0) + kVal, lane, 0, t);
   // the wavefront's own last block: rows of it see no keys of later ones
-  const int last = w_hi / kBN < nb - 1 ? w_hi / kBN : nb - 1;
+  const int w_kb = w_hi / kBN - skip, last = w_kb < nb - 1 ? w_kb : nb - 1;
   int kb = 0;
   while (kb + 1 < last) {
     turn(Yes(), kb++, s0, s1);
@@ -193,9 +210,20 @@ void attn_dq_kernel(AttnParams p, int ranks) {
 hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream) {
   const long long ranks = attn_ranks(p, kBM / p.G), units = (long long)(p.cu ? 1 : p.N) * p.Hkv;
   const unsigned grid = (unsigned)attn_grid(units, ranks);
-  if (p.D <= 64) attn_dq_kernel<64><<<grid, kNT, 0, stream>>>(p, (int)ranks);
-  else if (p.D <= 128) attn_dq_kernel<128><<<grid, kNT, 0, stream>>>(p, (int)ranks);
-  else attn_dq_kernel<256><<<grid, kNT, 0, stream>>>(p, (int)ranks);
+  const int r = (int)ranks;
+  switch (p.D <= 64 ? 64 : (p.D <= 128 ? 128 : 256)) {
+#define OMX_DQ(DP)                                                   \
+  case DP:                                                           \
+    if (p.window > 0)                                                \
+      attn_dq_kernel<DP, true><<<grid, kNT, 0, stream>>>(p, r);      \
+    else                                                             \
+      attn_dq_kernel<DP, false><<<grid, kNT, 0, stream>>>(p, r);     \
+    break;
+    OMX_DQ(64)
+    OMX_DQ(128)
+    OMX_DQ(256)
+#undef OMX_DQ
+  }
   return hipGetLastError();
 }
 

@@ -294,6 +294,10 @@ struct AttnParams {
   float *part_k, *part_v;      // dk and dv in shares of the rows, `splits` of them at most
   int32_t* shares;             // and of each key's tile how many, when that is more than one
   int share_tiles;             // rows in a share, in tiles of 128 tokens
+  // a row sees its last `window` keys (0: all of them) and the first `sinks`
+  int window, sinks;
+  int sink_splits;             // shares of a tile of keys that are sinks at most, and where they lie:
+  float *sink_k, *sink_v;      //   [sink_splits, sequences, attn_sink_keys(sinks), Hkv, D]
 };
 constexpr int kAttnMaxG = 32, kAttnMaxD = 256;
 // Compute units that the rules for sharing work count with, an MI355X's: workspace sizes are functions of
@@ -311,10 +315,16 @@ hipError_t launch_attn_fwd(const AttnParams& p, hipStream_t stream);
 int attn_dkv_tile_tokens();
 struct DkvPlan {
   int splits, tiles;  // shares of a tile at most, tiles' rows in a share
+  int sink_splits;    // with a window, shares of a tile of sinks at most
 };
 DkvPlan attn_dkv_plan(long long units, long long T, long long N, int G, long long row_bytes);
+// the same with a window, of B sequences or N packed ones
+DkvPlan attn_dkv_window_plan(long long B, long long T, long long N, int Hkv, int G, int D, int window, int sinks);
+// keys of the tiles that hold sinks
+constexpr long long attn_sink_keys(long long sinks) { return (sinks + 127) / 128 * 128; }
 hipError_t launch_attn_dq(const AttnParams& p, hipStream_t stream);
 void launch_attn_dkv_narrow(const AttnParams& p, unsigned grid, int ranks, hipStream_t stream);  // D <= 128
+long long attn_dkv_groups(const AttnParams& p);  // its workgroups
 hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream);
 // the cache's entry points: head dims, append, decode step (`splits` workgroups a key head share
 // the keys, by the tokens a table has room for; its partial sums are of splits + N segments)
