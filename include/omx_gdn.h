@@ -455,6 +455,55 @@ int omx_gdn_attn_decode_step(const void* q, const void* k, const void* v, int64_
 size_t omx_gdn_attn_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                                           int64_t page_size, int64_t table_width);
 
+/*
+ * A paged cache in 8 bits.  k_pages and v_pages are e4m3 numbers (OCP: largest 448, NaN but no infinity),
+ * laid out as those of bf16, and
+ *   k_exps, v_exps  int8 [n_pages, page_size / 16, Hkv]: the exponent e of each block of 16 tokens of a
+ *                head, whose numbers c stand for c 2^e.
+ * An append takes for e the largest that one of the block's tokens asks for, ceil(log2(max |x| / 448))
+ * within [-100, 120], and rounds each value to the nearest c.  A block that holds older tokens keeps its
+ * exponent or raises it; then their numbers are divided by the power of two between and rounded again.
+ * Values that are not finite become NaN and do not count for e; sizes above 1.875 2^127 are clamped to it.
+ * What no token was written to may hold anything.  Other arguments as for omx_gdn_kv_write, and its
+ * workspace size; less than 2^24 workgroups of 64 tokens and a key head.
+ */
+int omx_gdn_kv_write8(const void* k, const void* v, int64_t k_ld, int64_t v_ld,
+                      const int32_t* cu_seqlens, int64_t N, void* k_pages, void* v_pages,
+                      int8_t* k_exps, int8_t* v_exps, int64_t n_pages, int64_t page_size,
+                      const int32_t* block_table, int64_t table_width, const int32_t* lengths,
+                      int64_t B, int64_t T, int64_t Hkv, int64_t D, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/*
+ * omx_gdn_attn_paged and omx_gdn_attn_decode_step with a window, over a cache of bf16 (k_exps and v_exps
+ * NULL) or of 8 bits.  The query at position i sees positions i - window + 1 .. i and those below `sinks`;
+ * window 0 (and sinks 0): all up to i.  A length past table_width * page_size counts as that.  Positions
+ * that no query sees are not read, and need no page.  The decode step of a cache in 8 bits attends the new
+ * token as the cache holds it.
+ */
+int omx_gdn_attn_paged_window(const void* q, int64_t q_ld, const int32_t* cu_seqlens, int64_t N,
+                              const void* k_pages, const void* v_pages, const int8_t* k_exps,
+                              const int8_t* v_exps, int64_t n_pages, int64_t page_size,
+                              const int32_t* block_table, int64_t table_width,
+                              const int32_t* lengths, void* o, int64_t B, int64_t T, int64_t Hq,
+                              int64_t Hkv, int64_t D, float scale, int64_t window, int64_t sinks,
+                              void* workspace, size_t workspace_bytes, void* stream);
+int omx_gdn_attn_decode_window(const void* q, const void* k, const void* v, int64_t q_ld,
+                               int64_t k_ld, int64_t v_ld, void* k_pages, void* v_pages,
+                               int8_t* k_exps, int8_t* v_exps, int64_t n_pages, int64_t page_size,
+                               const int32_t* block_table, int64_t table_width,
+                               const int32_t* lengths, void* out, int64_t B, int64_t Hq,
+                               int64_t Hkv, int64_t D, float scale, int64_t window, int64_t sinks,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace these two need (16-byte aligned), as for the calls without a window. */
+size_t omx_gdn_attn_paged_window_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                                                int64_t D, int64_t N, int packed, int64_t page_size,
+                                                int64_t table_width, int64_t window, int64_t sinks);
+size_t omx_gdn_attn_decode_window_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                                 int64_t page_size, int64_t table_width,
+                                                 int64_t window, int64_t sinks);
+
 #ifdef __cplusplus
 }
 #endif

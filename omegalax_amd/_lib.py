@@ -69,6 +69,14 @@ SIGNATURES = {
     "omx_gdn_attn_decode_step": (_i, [_p] * 3 + [_i64] * 3 + [_p, _p, _i64, _i64, _p, _i64, _p, _p]
                                  + [_i64] * 4 + [_f, _p, _sz, _p]),
     "omx_gdn_attn_decode_workspace_size": (_sz, [_i64] * 6),
+    "omx_gdn_kv_write8": (_i, [_p, _p, _i64, _i64, _p, _i64] + [_p] * 4 + [_i64, _i64, _p, _i64, _p]
+                          + [_i64] * 4 + [_p, _sz, _p]),
+    "omx_gdn_attn_paged_window": (_i, [_p, _i64, _p, _i64] + [_p] * 4 + [_i64, _i64, _p, _i64, _p, _p]
+                                  + [_i64] * 5 + [_f, _i64, _i64, _p, _sz, _p]),
+    "omx_gdn_attn_paged_window_workspace_size": (_sz, [_i64] * 6 + [_i] + [_i64] * 4),
+    "omx_gdn_attn_decode_window": (_i, [_p] * 3 + [_i64] * 3 + [_p] * 4 + [_i64, _i64, _p, _i64, _p, _p]
+                                   + [_i64] * 4 + [_f, _i64, _i64, _p, _sz, _p]),
+    "omx_gdn_attn_decode_window_workspace_size": (_sz, [_i64] * 8),
     "omx_gdn_qkv_conv_proj": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _p]),
 }
 

@@ -12,6 +12,11 @@ sequence in order, and ``lengths`` [N] int32, the tokens each sequence held befo
 caller advances ``lengths``; a negative one marks a sequence that takes no part.  Serving a turn is
 ``kv_pages_write`` and then ``attention_prefill_paged`` with the same lengths; each further token is
 one ``attention_decode_step``.
+
+A cache in 8 bits has pages of float8_e4m3fn, and ``k_exps``, ``v_exps`` int8 [pages, page_size / 16,
+Hkv]: the exponent e of each block of 16 tokens of a head, whose numbers c stand for c 2^e.  A ``window``
+lets a query see that many last positions, its own among them, and the first ``sinks``; what none will see
+again needs no page.
 """
 from __future__ import annotations
 
@@ -211,8 +216,18 @@ def attention_prefill(q, k, v, *, cu_seqlens=None, scale=None, output_lse=False,
     return (o, lse) if output_lse else o
 
 
-def _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D):
+def _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D, k_exps=None, v_exps=None):
     """Checks of the cache's tensors, which are used where they lie."""
+    dtype = _BF16
+    if k_exps is not None or v_exps is not None:
+        if k_exps is None or v_exps is None:
+            raise ValueError("k_exps and v_exps go together")
+        dtype = torch.float8_e4m3fn
+        blocks = (k_pages.shape[0], k_pages.shape[1] // 16, Hkv) if k_pages.dim() == 4 else None
+        for name, t in (("k_exps", k_exps), ("v_exps", v_exps)):
+            if t.dtype is not torch.int8 or tuple(t.shape) != blocks or not t.is_contiguous() or t.device != dev:
+                raise ValueError(f"{name} must be int8 {blocks}, contiguous and on {dev} (got {t.dtype}, "
+                                 f"{tuple(t.shape)} on {t.device})")
     for t in (k_pages, v_pages, block_table, lengths):
         if t.device != dev:
             _device(t)
@@ -222,14 +237,22 @@ def _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D):
         raise ValueError(f"k_pages and v_pages must both be [pages, page_size, {Hkv}, {D}] "
                          f"(got {tuple(shape)}, {tuple(v_pages.shape)})")
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.dtype is not _BF16 or not t.is_contiguous():
-            raise ValueError(f"{name} must be bf16 and contiguous (got {t.dtype})")
+        if t.dtype is not dtype or not t.is_contiguous():
+            raise ValueError(f"{name} must be {'bf16' if dtype is _BF16 else 'float8_e4m3fn'} and contiguous "
+                             f"(got {t.dtype}{', without exponents' if t.dtype is torch.float8_e4m3fn else ''})")
     if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != N:
         raise ValueError(f"block_table must be int32 [{N}, width] (got {block_table.dtype}, "
                          f"{tuple(block_table.shape)})")
     if lengths.dtype is not torch.int32 or lengths.dim() != 1 or lengths.shape[0] != N:
         raise ValueError(f"lengths must be int32 [{N}] (got {lengths.dtype}, {tuple(lengths.shape)})")
     return block_table.contiguous(), lengths.contiguous(), shape[0], shape[1]
+
+
+def _variant(k_exps, v_exps, sight):
+    """(the entry points' suffix, its exponents' pointers, its window and sinks) of a call over a cache."""
+    if k_exps is None and sight is None:
+        return "", (), ()
+    return "_window", (_ptr(k_exps), _ptr(v_exps)), sight or (0, 0)
 
 
 def _no_grad_only(name, *ts):
@@ -239,12 +262,14 @@ def _no_grad_only(name, *ts):
     _no_tangents(name, *ts)
 
 
-def kv_pages_write(k, v, k_pages, v_pages, block_table, lengths, *, cu_seqlens=None):
+def kv_pages_write(k, v, k_pages, v_pages, block_table, lengths, *, cu_seqlens=None, k_exps=None, v_exps=None):
     """Appends new tokens' keys and values to a paged cache, in place.
 
     k, v [B,T,Hkv,D] bf16, N = B sequences of T tokens or N packed by ``cu_seqlens`` (B == 1).
     Token i of sequence n goes to position ``lengths[n] + i``; a position without a page is
-    left out.  A page that is written to must stand once in all of ``block_table``.
+    left out.  A page that is written to must stand once in all of ``block_table``.  With ``k_exps``
+    and ``v_exps`` the cache is one in 8 bits, and a block's older tokens are rounded again when a new
+    one is larger than its exponent allows for.
     """
     _no_grad_only("kv_pages_write", k, v, k_pages, v_pages)
     dev = _device(k, v)
@@ -253,21 +278,24 @@ def kv_pages_write(k, v, k_pages, v_pages, block_table, lengths, *, cu_seqlens=N
         raise ValueError(f"shape mismatch: k{tuple(k.shape)} v{tuple(v.shape)}")
     B, T, Hkv, D = k.shape
     cu, N = (None, B) if cu_seqlens is None else _cu_seqlens(cu_seqlens, B, T, dev)
-    table, lengths, pages, page = _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D)
+    table, lengths, pages, page = _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D, k_exps, v_exps)
     ws_bytes = _workspace_bytes("omx_gdn_kv_write_workspace_size", T, 0 if cu is None else N)
     ws = _workspace(ws_bytes, dev)
-    _call(dev, "omx_gdn_kv_write", _ptr(k), _ptr(v), k_ld, v_ld, _ptr(cu), N, _ptr(k_pages), _ptr(v_pages),
-          pages, page, _ptr(table), table.shape[1], _ptr(lengths), B, T, Hkv, D, _ptr(ws), ws_bytes)
+    name, exps = ("omx_gdn_kv_write", ()) if k_exps is None else ("omx_gdn_kv_write8", (_ptr(k_exps), _ptr(v_exps)))
+    _call(dev, name, _ptr(k), _ptr(v), k_ld, v_ld, _ptr(cu), N, _ptr(k_pages), _ptr(v_pages), *exps, pages, page,
+          _ptr(table), table.shape[1], _ptr(lengths), B, T, Hkv, D, _ptr(ws), ws_bytes)
 
 
-def attention_prefill_paged(q, k_pages, v_pages, block_table, lengths, *, cu_seqlens=None, scale=None):
+def attention_prefill_paged(q, k_pages, v_pages, block_table, lengths, *, cu_seqlens=None, scale=None, k_exps=None,
+                            v_exps=None, window=None, sinks=0):
     """Attention of new tokens over a paged cache that already holds their keys and values.
 
     q [B,T,Hq,D] bf16, N = B sequences of T new tokens or N packed by ``cu_seqlens`` (B == 1).
-    Query i of sequence n attends positions 0 .. ``lengths[n] + i``.  Returns o [B,T,Hq,D] bf16,
-    zeros for a query that no key is left for.
+    Query i of sequence n attends positions 0 .. ``lengths[n] + i``, with a ``window`` that many last
+    ones and the first ``sinks``.  Returns o [B,T,Hq,D] bf16, zeros for a query that no key is left for.
     """
     _no_grad_only("attention_prefill_paged", q, k_pages, v_pages)
+    sight = _sight(window, sinks)
     dev = _device(q)
     q, q_ld = _tokens("q", q, 4)
     B, T, Hq, D = q.shape
@@ -275,32 +303,38 @@ def attention_prefill_paged(q, k_pages, v_pages, block_table, lengths, *, cu_seq
     if cu_seqlens is not None:
         cu_seqlens, N = _cu_seqlens(cu_seqlens, B, T, dev)
     Hkv = k_pages.shape[2] if k_pages.dim() == 4 else 0
-    table, lengths, pages, page = _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D)
+    table, lengths, pages, page = _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D, k_exps, v_exps)
     o = torch.empty((B, T, Hq, D), dtype=torch.bfloat16, device=dev)
-    ws_bytes = _workspace_bytes("omx_gdn_attn_paged_workspace_size", B, T, Hq, Hkv, D, N, int(cu_seqlens is not None),
-                                                            page, table.shape[1])
+    more, exps, sight = _variant(k_exps, v_exps, sight)
+    ws_bytes = _workspace_bytes(f"omx_gdn_attn_paged{more}_workspace_size", B, T, Hq, Hkv, D, N,
+                                int(cu_seqlens is not None), page, table.shape[1], *sight)
     ws = _workspace(ws_bytes, dev)
-    _call(dev, "omx_gdn_attn_paged", _ptr(q), q_ld, _ptr(cu_seqlens), N, _ptr(k_pages), _ptr(v_pages), pages,
-          page, _ptr(table), table.shape[1], _ptr(lengths), _ptr(o), B, T, Hq, Hkv, D, _scale(scale, D),
+    _call(dev, "omx_gdn_attn_paged" + more, _ptr(q), q_ld, _ptr(cu_seqlens), N, _ptr(k_pages), _ptr(v_pages), *exps,
+          pages, page, _ptr(table), table.shape[1], _ptr(lengths), _ptr(o), B, T, Hq, Hkv, D, _scale(scale, D), *sight,
           _ptr(ws), ws_bytes)
     return o
 
 
-def attention_decode_step(q, k, v, k_pages, v_pages, block_table, lengths, *, scale=None):
+def attention_decode_step(q, k, v, k_pages, v_pages, block_table, lengths, *, scale=None, k_exps=None, v_exps=None,
+                          window=None, sinks=0):
     """One new token per sequence: writes its key and value to the cache in place and attends.
 
     q [B,Hq,D], k and v [B,Hkv,D] bf16.  The token goes to position ``lengths[b]`` and attends
-    positions 0 .. ``lengths[b]``.  Returns out [B,Hq,D] bf16.
+    positions 0 .. ``lengths[b]``, with a ``window`` that many last ones and the first ``sinks``.  Of a
+    cache in 8 bits it attends itself as the cache holds it.  Returns out [B,Hq,D] bf16.
     """
     _no_grad_only("attention_decode_step", q, k, v, k_pages, v_pages)
+    sight = _sight(window, sinks)
     dev, q, k, v, q_ld, k_ld, v_ld, _, B = _qkv(q, k, v, None, dims=3)
     Hq, D = q.shape[1:]
     Hkv = k.shape[1]
-    table, lengths, pages, page = _cache(dev, k_pages, v_pages, block_table, lengths, B, Hkv, D)
+    table, lengths, pages, page = _cache(dev, k_pages, v_pages, block_table, lengths, B, Hkv, D, k_exps, v_exps)
     out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=dev)
-    ws_bytes = _workspace_bytes("omx_gdn_attn_decode_workspace_size", B, Hq, Hkv, D, page, table.shape[1])
+    more, exps, sight = _variant(k_exps, v_exps, sight)
+    ws_bytes = _workspace_bytes(f"omx_gdn_attn_decode{more}_workspace_size", B, Hq, Hkv, D, page, table.shape[1],
+                                *sight)
     ws = _workspace(ws_bytes, dev)
-    _call(dev, "omx_gdn_attn_decode_step", _ptr(q), _ptr(k), _ptr(v), q_ld, k_ld, v_ld, _ptr(k_pages),
-          _ptr(v_pages), pages, page, _ptr(table), table.shape[1], _ptr(lengths), _ptr(out), B, Hq, Hkv, D,
-          _scale(scale, D), _ptr(ws), ws_bytes)
+    _call(dev, "omx_gdn_attn_decode" + (more or "_step"), _ptr(q), _ptr(k), _ptr(v), q_ld, k_ld, v_ld, _ptr(k_pages),
+          _ptr(v_pages), *exps, pages, page, _ptr(table), table.shape[1], _ptr(lengths), _ptr(out), B, Hq, Hkv, D,
+          _scale(scale, D), *sight, _ptr(ws), ws_bytes)
     return out

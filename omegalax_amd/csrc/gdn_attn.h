@@ -83,6 +83,19 @@ __device__ __forceinline__ void store_part(float* row, const f32x16 (&x)[DB], fl
     }
 }
 
+// A cache in 8 bits: e4m3 numbers, with a power of two for each 16 tokens of a head, kept as its
+// exponent.  Number times power is a bf16 value as it stands (the conversion applies both; verified on
+// MI355X for every code), so whoever reads it goes on as with a cache of bf16.
+__device__ __forceinline__ float exp_scale(int e) { return __uint_as_float((unsigned)((e < -127 ? -127 : e) + 127) << 23); }
+__device__ __forceinline__ u32x2 widen4(uint32_t c, float scale) {
+  return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, true))};
+}
+__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi, float scale) {
+  const u32x2 a = widen4(lo, scale), b = widen4(hi, scale);
+  return u32x4{a[0], a[1], b[0], b[1]};
+}
+
 // s + the products of two rows' 8 bf16 elements
 __device__ __forceinline__ float dot8(u32x4 a, u32x4 b, float s) {
 #pragma unroll

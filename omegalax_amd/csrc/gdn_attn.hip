@@ -32,9 +32,11 @@ struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
 // WIN: a row sees its last p.window keys and the first p.sinks.
-template <int DP, bool PAGED, bool WIN>
+// CACHE: the keys and values are those of prompts (0), of pages in bf16 (1) or in 8 bits (2).
+template <int DP, int CACHE, bool WIN>
 __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
 void attn_fwd_kernel(AttnParams p, int ranks) {
+  constexpr bool PAGED = CACHE != 0, EIGHT = CACHE == 2;
   constexpr int KS = DP / 16, DB = DP / 32;      // steps of a score, blocks of an output row
   constexpr int NG = 2 * KS, EG = 32 / NG;       // products of a tile's scores (and of its values)
   constexpr int PF = 4;                          // fragments read ahead of their products
@@ -96,9 +98,9 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   int kt0 = 0, kt1 = (keys + kBN - 1) / kBN;
   // With a window these tiles are counted without the `skip` ones between the sinks' and the first
   // row's window, which no row sees: tile kt begins at key key0(kt).
-  int sink_tiles = 0, skip = 0;
+  int sink_tiles = 0, skip = 0, lo = 0;
   if constexpr (WIN) {
-    const int lo = held + t0 - p.window + 1;
+    lo = held + t0 - p.window + 1;
     sink_tiles = (p.sinks + kBN - 1) / kBN;
     skip = lo / kBN > sink_tiles ? lo / kBN - sink_tiles : 0;
     kt1 -= skip;
@@ -132,8 +134,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   typedef const __attribute__((address_space(4))) int32_t const_i32;
   const_i32* table = PAGED ? (const_i32*)(p.table + (long long)it.seq * p.table_w) : nullptr;
   int slot = 0, off = 0;
-  const int row_bytes = Hkv * D * 2;
-  struct Pages { long long at[4]; unsigned have, fetch; };  // byte offsets in a pool; none past the split
+  const int row_bytes = EIGHT ? Hkv * D : Hkv * D * 2;
+  struct Pages { long long at[4], exp[4]; unsigned have, fetch; };  // byte offsets in a pool; none past the split
   auto look = [&](int kt) {
     Pages x;
     x.have = 0;
@@ -147,7 +149,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       int id = in ? table[slot] : -1;
       id = id >= p.n_pages ? -1 : id;
       id = __builtin_amdgcn_readfirstlane(id);
-      x.at[g] = ((long long)(id < 0 ? 0 : id) * p.page + off) * row_bytes + 2 * hk * D;
+      x.at[g] = ((long long)(id < 0 ? 0 : id) * p.page + off) * row_bytes + (EIGHT ? 1 : 2) * hk * D;
+      if constexpr (EIGHT) x.exp[g] = ((long long)(id < 0 ? 0 : id) * (p.page / 16) + off / 16) * Hkv + hk;
       x.have |= id >= 0 ? 1u << g : 0u;
       off += 16;
       if (off >= p.page) { off = 0; ++slot; }
@@ -183,6 +186,37 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
                      lds + 1024u * kNW * j0, at);
     }
   };
+  // Of a cache in 8 bits a thread loads NR segments of 16 numbers and their exponents into registers, a
+  // tile ahead, and puts them into LDS as bf16 once the tile's products are issued.
+  constexpr int NR = DP / 64, kRows8 = 4096 / DP;  // rows of the workgroup's j-th load: kRows8 j ..
+  struct Raw { u32x4 x[NR]; int e[NR]; };
+  const int row8 = tid / (DP / 16), seg8 = tid % (DP / 16);
+  auto load8 = [&](const Pages& x, const void* pool, const int8_t* exps) {
+    Raw r;
+    const int wrow = __builtin_amdgcn_readfirstlane(row8);
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+      const int g = (kRows8 * j + wrow) / 16;
+      const bool there = (x.fetch >> g) & 1;
+      r.x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+          buf_rsrc((const char*)pool + x.at[g], there ? 15u * row_bytes + DP : 0u),
+          ((kRows8 * j + row8) & 15) * row_bytes + 16 * seg8, 0, 0));
+      r.e[j] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(buf_rsrc(exps + x.exp[g], there ? 1u : 0u), 0, 0, 0);
+    }
+    return r;
+  };
+  auto store8 = [&](const Raw& r, bf16_t* dst) {
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+      const int row = kRows8 * j + row8;
+      const float scale = exp_scale(r.e[j]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *(u32x4*)(dst + row * DP + (((2 * seg8 + i) ^ attn_swz<DP>(row)) << 3)) =
+            widen8(r.x[j][2 * i], r.x[j][2 * i + 1], scale);
+    }
+  };
+  Raw rk, rv;  // of the tiles that phase 2 and phase 1 would fetch
   auto fetch_k = [&](int kt, const Pages& x, int j) { fetch(kt, x, p.k_pages, p.k, p.k_ld, kld2, koff, sK, NL * j); };
   auto fetch_v = [&](int kt, const Pages& x, int j) { fetch(kt, x, p.v_pages, p.v, p.v_ld, vld2, voff, sV, NL * j); };
 
@@ -263,7 +297,12 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
         sum[e & 3] += s[b][i];
         if (e & 1) pb[e / 8][e / 2 % 4] = pack_bf16(s[b][i - 1], s[b][i]);
       }
-      if (t % (NG / NF) == 0) fetch_v(kt + 1, pn, t / (NG / NF));
+      if constexpr (EIGHT) {
+        if (t == 0) rv = load8(pn, p.v_pages, p.v_exps);
+        if (t == NG / 2) rk = load8(pk, p.k_pages, p.k_exps);
+      } else if (t % (NG / NF) == 0) {
+        fetch_v(kt + 1, pn, t / (NG / NF));
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     lsum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -279,17 +318,18 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
 #pragma unroll
         for (int e = EG * t; e < EG * (t + 1); ++e) mx = fmaxf(mx, sn[e / 16][e % 16]);
       }
-      if (t % (NG / 2 / NF) == 0 && t < NG / 2) fetch_k(kt + 2, pk, t / (NG / 2 / NF));
+      if (!EIGHT && t % (NG / 2 / NF) == 0 && t < NG / 2) fetch_k(kt + 2, pk, t / (NG / 2 / NF));
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  // rows of a staged tile that hold no key are cleared: a weight of zero does not clear them
-  // of a NaN
+  // rows of a staged tile that hold no key, or none that a row sees, are cleared: a weight of zero does
+  // not clear them of a NaN
   auto clear = [&](int kt, bf16_t* sv, unsigned have) {
     for (int i = tid; i < kBN * DP / 8; i += kNT) {
       const int r = i / (DP / 8);
-      if (key0(kt) + r >= keys || !((have >> (r / 16)) & 1)) *(u32x4*)(sv + 8 * i) = u32x4{0, 0, 0, 0};
+      const int key = key0(kt) + r;
+      if (key >= keys || !((have >> (r / 16)) & 1) || (WIN && key < lo && key >= p.sinks)) *(u32x4*)(sv + 8 * i) = u32x4{0, 0, 0, 0};
     }
   };
   unsigned have = 15;
@@ -298,13 +338,18 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     wait_loads<0>();  // this wavefront's part of the tiles
     lds_barrier();    // everyone's; and the other buffers are free
     if constexpr (PAGED) {
-      if (have != 15 || key0(kt) + kBN > keys) {  // uniform in the workgroup
+      const int k0 = key0(kt);
+      if (have != 15 || k0 + kBN > keys || (WIN && k0 < lo && k0 + kBN > p.sinks)) {  // uniform in the workgroup
         clear(kt, sV + (kt & 1) * kTile, have);
         lds_barrier();
       }
     }
   };
   auto leave = [&](int kt) {
+    if constexpr (EIGHT) {
+      store8(rv, sV + ((kt + 1) & 1) * kTile);
+      store8(rk, sK + (kt & 1) * kTile);
+    }
     if constexpr (PAGED) {
       have = pn.have;
       pn = pk;
@@ -322,11 +367,20 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       pk = look(kt0 + 2);
       have = p0.have;
     }
+    if constexpr (EIGHT) {
+      const Raw first = load8(p0, p.k_pages, p.k_exps);
+      rv = load8(p0, p.v_pages, p.v_exps);
+      rk = load8(pn, p.k_pages, p.k_exps);
+      store8(first, sK + (kt0 & 1) * kTile);
+      store8(rv, sV + (kt0 & 1) * kTile);
+      store8(rk, sK + ((kt0 + 1) & 1) * kTile);
+    } else {
 #pragma unroll
-    for (int j = 0; j < NF; ++j) {
-      fetch_k(kt0, p0, j);
-      fetch_v(kt0, p0, j);
-      fetch_k(kt0 + 1, pn, j);
+      for (int j = 0; j < NF; ++j) {
+        fetch_k(kt0, p0, j);
+        fetch_v(kt0, p0, j);
+        fetch_k(kt0 + 1, pn, j);
+      }
     }
     wait_loads<0>();
     lds_barrier();
@@ -358,10 +412,15 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     }
     for (; kt < kt1; ++kt) {  // other wavefronts' tiles: its part of the loads
       enter(kt);
+      if constexpr (EIGHT) {
+        rv = load8(pn, p.v_pages, p.v_exps);
+        rk = load8(pk, p.k_pages, p.k_exps);
+      } else {
 #pragma unroll
-      for (int j = 0; j < NF; ++j) {
-        fetch_v(kt + 1, pn, j);
-        fetch_k(kt + 2, pk, j);
+        for (int j = 0; j < NF; ++j) {
+          fetch_v(kt + 1, pn, j);
+          fetch_k(kt + 2, pk, j);
+        }
       }
       leave(kt);
     }
@@ -399,20 +458,39 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
           see = id >= 0 && id < p.n_pages;
           at = av = ((long long)id * p.page + (key - sl * p.page)) * Hkv * D + hk * D;
         }
-        float s1 = 0.f;
-        if (see)
+        float s1 = 0.f, vs = 0.f;
+        if constexpr (EIGHT) {
+          if (see) {
+            const long long block = at / D / (16 * Hkv) * Hkv + hk;
+            const float ks = exp_scale(p.k_exps[block]);
+            vs = exp_scale(p.v_exps[block]);
+            for (int d = 0; d < D; d += 8) {
+              const u32x2 x = *(const u32x2*)((const char*)p.k_pages + at + d);
+              s1 = dot8(*(const u32x4*)(q1 + d), widen8(x[0], x[1], ks), s1);
+            }
+          }
+        } else if (see) {
           for (int d = 0; d < D; d += 8)
             s1 = dot8(*(const u32x4*)(q1 + d), *(const u32x4*)((const bf16_t*)(PAGED ? p.k_pages : p.k) + at + d), s1);
+        }
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s1, cs, -m1));
         unsigned long long seen = __ballot(see);
         while (seen) {
           const int j = __ffsll(seen) - 1;
           seen &= seen - 1;
           const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p1), j));
-          const bf16_t* vj = (const bf16_t*)(PAGED ? p.v_pages : p.v) + __shfl(av, j, 64);
+          const long long aj = __shfl(av, j, 64);
+          const float vsj = EIGHT ? __shfl(vs, j, 64) : 0.f;
 #pragma unroll
-          for (int e = 0; e < DP / 64; ++e)
-            if (64 * e + l < D) acc[e] = fmaf(pj, bf2f(vj[64 * e + l]), acc[e]);
+          for (int e = 0; e < DP / 64; ++e) {
+            if (64 * e + l >= D) continue;
+            float x;
+            if constexpr (EIGHT)
+              x = bf2f((bf16_t)(widen4(((const uint8_t*)p.v_pages)[aj + 64 * e + l], vsj)[0] & 0xffffu));
+            else
+              x = bf2f(((const bf16_t*)(PAGED ? p.v_pages : p.v))[aj + 64 * e + l]);
+            acc[e] = fmaf(pj, x, acc[e]);
+          }
         }
       }
 #pragma unroll
@@ -631,21 +709,26 @@ hipError_t launch_attn_fwd(const AttnParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)attn_grid(units, ranks), paged ? (unsigned)p.splits : 1u);
   const bool win = p.window > 0;
   switch (padded_dim(p.D)) {
-#define OMX_FWD(DP)                                                            \
-  case DP:                                                                     \
-    if (paged && win)                                                          \
-      attn_fwd_kernel<DP, true, true><<<grid, kNT, 0, stream>>>(p, (int)ranks); \
-    else if (paged)                                                            \
-      attn_fwd_kernel<DP, true, false><<<grid, kNT, 0, stream>>>(p, (int)ranks); \
-    else if (win)                                                              \
-      attn_fwd_kernel<DP, false, true><<<grid, kNT, 0, stream>>>(p, (int)ranks); \
-    else                                                                       \
-      attn_fwd_kernel<DP, false, false><<<grid, kNT, 0, stream>>>(p, (int)ranks); \
+#define OMX_FWD1(DP, CACHE)                                                      \
+  if (win)                                                                       \
+    attn_fwd_kernel<DP, CACHE, true><<<grid, kNT, 0, stream>>>(p, (int)ranks);   \
+  else                                                                           \
+    attn_fwd_kernel<DP, CACHE, false><<<grid, kNT, 0, stream>>>(p, (int)ranks);
+#define OMX_FWD(DP)                                                              \
+  case DP:                                                                       \
+    if (paged && p.k_exps) {                                                     \
+      OMX_FWD1(DP, 2)                                                            \
+    } else if (paged) {                                                          \
+      OMX_FWD1(DP, 1)                                                            \
+    } else {                                                                     \
+      OMX_FWD1(DP, 0)                                                            \
+    }                                                                            \
     break;
     OMX_FWD(64)
     OMX_FWD(128)
     OMX_FWD(256)
 #undef OMX_FWD
+#undef OMX_FWD1
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !paged || p.splits == 1) return e;

@@ -110,7 +110,7 @@ hipError_t use_plan(omx::AttnParams& p, const PlanWs& w, void* workspace, int pe
 // its own tiles; packed sequences add at most one tile each to those of all their tokens.  Two
 // workgroups a compute unit, shares of 128 keys at least, 32 at most: with up to 64, 16 new tokens on
 // 100,000 of 8/2 heads of 128 take 67 us (85), on 6,000 19 (17); 8/1 heads of 256 on 20,000 56 (43).
-int paged_splits(const Shape& x, int64_t capacity) {
+int paged_splits(const Shape& x, int64_t capacity) {  // capacity: keys that a tile sees at most
   const int64_t per = omx::attn_tile_tokens((int)(x.Hq / x.Hkv)), each = (x.T + per - 1) / per;
   const int64_t tiles = (x.packed ? each + x.N - 1 : x.N * each) * x.Hkv;
   int64_t s = tiles > 0 ? 2 * omx::kComputeUnits / tiles : 1;
@@ -167,6 +167,23 @@ void look_at(omx::AttnParams& p, const Sight& x, int64_t keys) {
   if (x.window == 0 || x.window >= keys || x.sinks >= keys - x.window) return;
   p.window = (int)x.window;
   p.sinks = (int)x.sinks;
+}
+// keys of at most `keys` that `rows` queries in a row see together, in whole tiles of 64
+int64_t seen_keys(const Sight& x, int64_t keys, int64_t rows) {
+  if (x.window == 0 || x.window >= keys || x.sinks >= keys - x.window) return keys;
+  const int64_t n = x.window + x.sinks + rows + 128;
+  return n < keys ? n : keys;
+}
+// the exponents of a cache in 8 bits: both or neither
+int check_exps(const char* fn, const int8_t* k_exps, const int8_t* v_exps) {
+  REQUIRE(!k_exps == !v_exps, "%s: k_exps and v_exps go together", fn);
+  return OMX_GDN_OK;
+}
+int check_any_sight(const char* fn, const Sight& x) {
+  REQUIRE(x.window >= 0, "%s: window %lld must not be negative (0: all keys)", fn, (long long)x.window);
+  REQUIRE(x.sinks >= 0 && (x.window > 0 || x.sinks == 0), "%s: sinks %lld must not be negative, and need a window", fn,
+          (long long)x.sinks);
+  return OMX_GDN_OK;
 }
 
 }  // namespace
@@ -348,17 +365,21 @@ size_t omx_gdn_kv_write_workspace_size(int64_t T, int64_t N) {
   return plan_ws(0, T, N, omx::attn_dkv_tile_tokens()).total;
 }
 
-int omx_gdn_kv_write(const void* k, const void* v, int64_t k_ld, int64_t v_ld, const int32_t* cu_seqlens, int64_t N,
-                     void* k_pages, void* v_pages, int64_t n_pages, int64_t page_size, const int32_t* block_table,
-                     int64_t table_width, const int32_t* lengths, int64_t B, int64_t T, int64_t Hkv, int64_t D,
-                     void* workspace, size_t workspace_bytes, void* stream) {
-  const char* fn = "omx_gdn_kv_write";
+namespace {
+// (k_exps null: a cache of bf16)
+int kv_write(const char* fn, const void* k, const void* v, int64_t k_ld, int64_t v_ld, const int32_t* cu_seqlens,
+             int64_t N, void* k_pages, void* v_pages, int8_t* k_exps, int8_t* v_exps, int64_t n_pages,
+             int64_t page_size, const int32_t* block_table, int64_t table_width, const int32_t* lengths, int64_t B,
+             int64_t T, int64_t Hkv, int64_t D, void* workspace, size_t workspace_bytes, void* stream) {
   const Shape s{N, B, T, Hkv, Hkv, D, cu_seqlens != nullptr};
   int rc = check_shape(fn, s);
   if (!rc) rc = check_ld(fn, "k_ld", k_ld, Hkv * D);
   if (!rc) rc = check_ld(fn, "v_ld", v_ld, Hkv * D);
   if (rc) return rc;
-  REQUIRE(B * T <= kMaxGroups * omx::kv_write_tokens(), "%s: grid too large", fn);
+  if (k_exps)
+    REQUIRE((B * T / omx::kv_write8_tokens() + 1) * Hkv <= kMaxGroups, "%s: grid too large", fn);
+  else
+    REQUIRE(B * T <= kMaxGroups * omx::kv_write_tokens(), "%s: grid too large", fn);
   const int per = omx::attn_dkv_tile_tokens();
   const PlanWs ws = plan_ws(0, T, s.packed ? N : 0, per);
   REQUIRE(workspace_bytes >= ws.total, "%s: workspace of %zu bytes is smaller than the %zu needed", fn,
@@ -371,12 +392,32 @@ int omx_gdn_kv_write(const void* k, const void* v, int64_t k_ld, int64_t v_ld, c
   REQUIRE(ws.total == 0 || (workspace && aligned(workspace, 16)), "%s: workspace must be non-NULL and 16-byte aligned", fn);
   omx::AttnParams p = params(s, 1.f);
   p.k = k; p.v = v; p.k_ld = k_ld; p.v_ld = v_ld; p.cu = cu_seqlens;
-  p.k_pages = k_pages; p.v_pages = v_pages; p.table = block_table; p.held = lengths;
+  p.k_pages = k_pages; p.v_pages = v_pages; p.k_exps = k_exps; p.v_exps = v_exps; p.table = block_table; p.held = lengths;
   p.table_w = (int)table_width; p.page = (int)page_size; p.n_pages = (int)n_pages;
   hipError_t e = use_plan(p, ws, workspace, per, (hipStream_t)stream);
-  if (e == hipSuccess) e = omx::launch_kv_write(p, (hipStream_t)stream);
+  if (e == hipSuccess) e = k_exps ? omx::launch_kv_write8(p, (hipStream_t)stream) : omx::launch_kv_write(p, (hipStream_t)stream);
   return launch_status(e, fn);
 }
+}  // namespace
+
+int omx_gdn_kv_write(const void* k, const void* v, int64_t k_ld, int64_t v_ld, const int32_t* cu_seqlens, int64_t N,
+                     void* k_pages, void* v_pages, int64_t n_pages, int64_t page_size, const int32_t* block_table,
+                     int64_t table_width, const int32_t* lengths, int64_t B, int64_t T, int64_t Hkv, int64_t D,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  return kv_write("omx_gdn_kv_write", k, v, k_ld, v_ld, cu_seqlens, N, k_pages, v_pages, nullptr, nullptr, n_pages,
+                  page_size, block_table, table_width, lengths, B, T, Hkv, D, workspace, workspace_bytes, stream);
+}
+
+int omx_gdn_kv_write8(const void* k, const void* v, int64_t k_ld, int64_t v_ld, const int32_t* cu_seqlens, int64_t N,
+                      void* k_pages, void* v_pages, int8_t* k_exps, int8_t* v_exps, int64_t n_pages,
+                      int64_t page_size, const int32_t* block_table, int64_t table_width, const int32_t* lengths,
+                      int64_t B, int64_t T, int64_t Hkv, int64_t D, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+  REQUIRE(k_exps && v_exps, "%s: a required pointer is NULL", "omx_gdn_kv_write8");
+  return kv_write("omx_gdn_kv_write8", k, v, k_ld, v_ld, cu_seqlens, N, k_pages, v_pages, k_exps, v_exps, n_pages,
+                  page_size, block_table, table_width, lengths, B, T, Hkv, D, workspace, workspace_bytes, stream);
+}
+
 
 namespace {
 struct PagedWs {
@@ -385,10 +426,10 @@ struct PagedWs {
   int splits;
   size_t total;
 };
-PagedWs paged_ws(const Shape& s, int64_t capacity) {
+PagedWs paged_ws(const Shape& s, int64_t capacity, const Sight& sight) {
   PagedWs w{};
   w.plan = plan_ws(0, s.T, s.packed ? s.N : 0, omx::attn_tile_tokens((int)(s.Hq / s.Hkv)));
-  w.splits = paged_splits(s, capacity);
+  w.splits = paged_splits(s, seen_keys(sight, capacity, omx::attn_tile_tokens((int)(s.Hq / s.Hkv))));
   w.split = split_ws(w.plan.total, w.splits, s.B * s.T * s.Hq, s.D);
   w.total = w.split.total;
   return w;
@@ -399,14 +440,15 @@ size_t omx_gdn_attn_paged_workspace_size(int64_t B, int64_t T, int64_t Hq, int64
                                          int packed, int64_t page_size, int64_t table_width) {
   const Shape s{N, B, T, Hq, Hkv, D, packed != 0};
   if (!sized(B, T, Hq, Hkv, D, N) || !sized_table(page_size, table_width)) return 0;
-  return paged_ws(s, page_size * table_width).total;
+  return paged_ws(s, page_size * table_width, kAllKeys).total;
 }
 
-int omx_gdn_attn_paged(const void* q, int64_t q_ld, const int32_t* cu_seqlens, int64_t N, const void* k_pages,
-                       const void* v_pages, int64_t n_pages, int64_t page_size, const int32_t* block_table,
-                       int64_t table_width, const int32_t* lengths, void* o, int64_t B, int64_t T, int64_t Hq,
-                       int64_t Hkv, int64_t D, float scale, void* workspace, size_t workspace_bytes, void* stream) {
-  const char* fn = "omx_gdn_attn_paged";
+namespace {
+int attn_paged(const char* fn, const void* q, int64_t q_ld, const int32_t* cu_seqlens, int64_t N, const void* k_pages,
+               const void* v_pages, const int8_t* k_exps, const int8_t* v_exps, int64_t n_pages, int64_t page_size,
+               const int32_t* block_table, int64_t table_width, const int32_t* lengths, void* o, int64_t B, int64_t T,
+               int64_t Hq, int64_t Hkv, int64_t D, float scale, const Sight& sight, void* workspace,
+               size_t workspace_bytes, void* stream) {
   const Shape s{N, B, T, Hq, Hkv, D, cu_seqlens != nullptr};
   int rc = check_shape(fn, s);
   if (!rc) rc = check_ld(fn, "q_ld", q_ld, Hq * D);
@@ -418,7 +460,7 @@ int omx_gdn_attn_paged(const void* q, int64_t q_ld, const int32_t* cu_seqlens, i
   rc = check_cache(fn, k_pages, v_pages, n_pages, page_size, block_table, table_width, lengths, D, Hkv);
   if (rc) return rc;
   REQUIRE(table_width * page_size + T <= kMaxTokens, "%s: too many tokens", fn);
-  const PagedWs ws = paged_ws(s, page_size * table_width);
+  const PagedWs ws = paged_ws(s, page_size * table_width, sight);
   REQUIRE(workspace_bytes >= ws.total, "%s: workspace of %zu bytes is smaller than the %zu needed", fn,
           workspace_bytes, ws.total);
   REQUIRE(q && o, "%s: a required pointer is NULL", fn);
@@ -427,6 +469,8 @@ int omx_gdn_attn_paged(const void* q, int64_t q_ld, const int32_t* cu_seqlens, i
   omx::AttnParams p = params(s, scale);
   p.q = q; p.q_ld = q_ld; p.o = o; p.cu = cu_seqlens;
   p.k_pages = const_cast<void*>(k_pages); p.v_pages = const_cast<void*>(v_pages);
+  p.k_exps = const_cast<int8_t*>(k_exps); p.v_exps = const_cast<int8_t*>(v_exps);
+  look_at(p, sight, table_width * page_size + T);
   p.table = block_table; p.held = lengths;
   p.table_w = (int)table_width; p.page = (int)page_size; p.n_pages = (int)n_pages;
   p.splits = ws.splits;
@@ -436,8 +480,44 @@ int omx_gdn_attn_paged(const void* q, int64_t q_ld, const int32_t* cu_seqlens, i
   if (e == hipSuccess) e = omx::launch_attn_fwd(p, (hipStream_t)stream);
   return launch_status(e, fn);
 }
+}  // namespace
+
+int omx_gdn_attn_paged(const void* q, int64_t q_ld, const int32_t* cu_seqlens, int64_t N, const void* k_pages,
+                       const void* v_pages, int64_t n_pages, int64_t page_size, const int32_t* block_table,
+                       int64_t table_width, const int32_t* lengths, void* o, int64_t B, int64_t T, int64_t Hq,
+                       int64_t Hkv, int64_t D, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+  return attn_paged("omx_gdn_attn_paged", q, q_ld, cu_seqlens, N, k_pages, v_pages, nullptr, nullptr, n_pages, page_size,
+                    block_table, table_width, lengths, o, B, T, Hq, Hkv, D, scale, kAllKeys, workspace, workspace_bytes,
+                    stream);
+}
+
+size_t omx_gdn_attn_paged_window_workspace_size(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t N,
+                                                int packed, int64_t page_size, int64_t table_width, int64_t window,
+                                                int64_t sinks) {
+  const Shape s{N, B, T, Hq, Hkv, D, packed != 0};
+  if (!sized(B, T, Hq, Hkv, D, N) || !sized_table(page_size, table_width) || window < 0 || sinks < 0) return 0;
+  return paged_ws(s, page_size * table_width, Sight{window, sinks}).total;
+}
+
+int omx_gdn_attn_paged_window(const void* q, int64_t q_ld, const int32_t* cu_seqlens, int64_t N, const void* k_pages,
+                              const void* v_pages, const int8_t* k_exps, const int8_t* v_exps, int64_t n_pages,
+                              int64_t page_size, const int32_t* block_table, int64_t table_width,
+                              const int32_t* lengths, void* o, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                              float scale, int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  const char* fn = "omx_gdn_attn_paged_window";
+  const Sight sight{window, sinks};
+  int rc = check_any_sight(fn, sight);
+  if (!rc) rc = check_exps(fn, k_exps, v_exps);
+  if (rc) return rc;
+  return attn_paged(fn, q, q_ld, cu_seqlens, N, k_pages, v_pages, k_exps, v_exps, n_pages, page_size, block_table,
+                    table_width, lengths, o, B, T, Hq, Hkv, D, scale, sight, workspace, workspace_bytes, stream);
+}
 
 namespace {
+int decode_splits(const Sight& sight, int64_t B, int64_t Hkv, int64_t D, int64_t capacity) {
+  return omx::decode_splits(B, Hkv, D, seen_keys(sight, capacity, 1));
+}
 SplitWs decode_ws(int splits, int64_t B, int64_t Hq, int64_t D) {
   // (one count of splits + B segments, of one row a head each)
   return splits > 1 ? split_ws(0, splits + (int)B, Hq, D) : split_ws(0, 1, 0, D);
@@ -447,15 +527,15 @@ SplitWs decode_ws(int splits, int64_t B, int64_t Hq, int64_t D) {
 size_t omx_gdn_attn_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t page_size,
                                           int64_t table_width) {
   if (B < 1 || !sized(B, 1, Hq, Hkv, D, B) || !sized_table(page_size, table_width)) return 0;
-  return decode_ws(omx::decode_splits(B, Hkv, D, page_size * table_width), B, Hq, D).total;
+  return decode_ws(decode_splits(kAllKeys, B, Hkv, D, page_size * table_width), B, Hq, D).total;
 }
 
-int omx_gdn_attn_decode_step(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
-                             void* k_pages, void* v_pages, int64_t n_pages, int64_t page_size,
-                             const int32_t* block_table, int64_t table_width, const int32_t* lengths, void* out,
-                             int64_t B, int64_t Hq, int64_t Hkv, int64_t D, float scale, void* workspace,
-                             size_t workspace_bytes, void* stream) {
-  const char* fn = "omx_gdn_attn_decode_step";
+namespace {
+int attn_decode(const char* fn, const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+                void* k_pages, void* v_pages, int8_t* k_exps, int8_t* v_exps, int64_t n_pages, int64_t page_size,
+                const int32_t* block_table, int64_t table_width, const int32_t* lengths, void* out, int64_t B,
+                int64_t Hq, int64_t Hkv, int64_t D, float scale, const Sight& sight, void* workspace,
+                size_t workspace_bytes, void* stream) {
   const Shape s{B, B, 1, Hq, Hkv, D, false};
   int rc = check_shape(fn, s);
   if (!rc) rc = check_ld(fn, "q_ld", q_ld, Hq * D);
@@ -467,7 +547,7 @@ int omx_gdn_attn_decode_step(const void* q, const void* k, const void* v, int64_
   if (B == 0) return ok();
   rc = check_cache(fn, k_pages, v_pages, n_pages, page_size, block_table, table_width, lengths, D, Hkv);
   if (rc) return rc;
-  const int splits = omx::decode_splits(B, Hkv, D, page_size * table_width);
+  const int splits = decode_splits(sight, B, Hkv, D, page_size * table_width);
   const SplitWs ws = decode_ws(splits, B, Hq, D);
   REQUIRE(workspace_bytes >= ws.total, "%s: workspace of %zu bytes is smaller than the %zu needed", fn,
           workspace_bytes, ws.total);
@@ -477,12 +557,47 @@ int omx_gdn_attn_decode_step(const void* q, const void* k, const void* v, int64_
   omx::AttnParams p = params(s, scale);
   p.q = q; p.k = k; p.v = v; p.o = out;
   p.q_ld = q_ld; p.k_ld = k_ld; p.v_ld = v_ld;
+  p.k_exps = k_exps; p.v_exps = v_exps;
+  look_at(p, sight, table_width * page_size + 1);
   p.k_pages = k_pages; p.v_pages = v_pages; p.table = block_table; p.held = lengths;
   p.table_w = (int)table_width; p.page = (int)page_size; p.n_pages = (int)n_pages;
   p.splits = splits;
   p.part_o = (float*)((char*)workspace + ws.o);
   p.part_ml = (float*)((char*)workspace + ws.ml);
-  return launch_status(omx::launch_attn_decode(p, (hipStream_t)stream), fn);
+  return launch_status(k_exps ? omx::launch_attn_decode8(p, (hipStream_t)stream) : omx::launch_attn_decode(p, (hipStream_t)stream), fn);
 }
+}  // namespace
+
+int omx_gdn_attn_decode_step(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+                             void* k_pages, void* v_pages, int64_t n_pages, int64_t page_size,
+                             const int32_t* block_table, int64_t table_width, const int32_t* lengths, void* out,
+                             int64_t B, int64_t Hq, int64_t Hkv, int64_t D, float scale, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  return attn_decode("omx_gdn_attn_decode_step", q, k, v, q_ld, k_ld, v_ld, k_pages, v_pages, nullptr, nullptr, n_pages,
+                     page_size, block_table, table_width, lengths, out, B, Hq, Hkv, D, scale, kAllKeys, workspace,
+                     workspace_bytes, stream);
+}
+
+size_t omx_gdn_attn_decode_window_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t page_size,
+                                                 int64_t table_width, int64_t window, int64_t sinks) {
+  if (B < 1 || !sized(B, 1, Hq, Hkv, D, B) || !sized_table(page_size, table_width) || window < 0 || sinks < 0) return 0;
+  return decode_ws(decode_splits(Sight{window, sinks}, B, Hkv, D, page_size * table_width), B, Hq, D).total;
+}
+
+int omx_gdn_attn_decode_window(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+                               void* k_pages, void* v_pages, int8_t* k_exps, int8_t* v_exps, int64_t n_pages,
+                               int64_t page_size, const int32_t* block_table, int64_t table_width,
+                               const int32_t* lengths, void* out, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                               float scale, int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  const char* fn = "omx_gdn_attn_decode_window";
+  const Sight sight{window, sinks};
+  int rc = check_any_sight(fn, sight);
+  if (!rc) rc = check_exps(fn, k_exps, v_exps);
+  if (rc) return rc;
+  return attn_decode(fn, q, k, v, q_ld, k_ld, v_ld, k_pages, v_pages, k_exps, v_exps, n_pages, page_size, block_table,
+                     table_width, lengths, out, B, Hq, Hkv, D, scale, sight, workspace, workspace_bytes, stream);
+}
+
 
 }  // extern "C"

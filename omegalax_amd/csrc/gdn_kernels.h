@@ -284,6 +284,7 @@ struct AttnParams {
   const int32_t* table;        // [N, table_w]
   const int32_t* held;         // [N]
   int table_w, page, n_pages;
+  int8_t *k_exps, *v_exps;     // of pages of e4m3 numbers: [n_pages, page / 16, Hkv]; null: bf16
   // work split over the keys: partial sums, which a second kernel joins
   int splits;
   float *part_o, *part_ml;
@@ -333,5 +334,9 @@ int kv_write_tokens();  // tokens a workgroup of the append copies
 hipError_t launch_kv_write(const AttnParams& p, hipStream_t stream);
 int decode_splits(long long N, long long Hkv, long long D, long long capacity);
 hipError_t launch_attn_decode(const AttnParams& p, hipStream_t stream);
+// the same of a cache in 8 bits
+int kv_write8_tokens();
+hipError_t launch_kv_write8(const AttnParams& p, hipStream_t stream);
+hipError_t launch_attn_decode8(const AttnParams& p, hipStream_t stream);
 
 }  // namespace omx

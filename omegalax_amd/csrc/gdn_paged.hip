@@ -1,15 +1,8 @@
 // The paged key-value cache: the append of new tokens and the decode step of one token a sequence.
-#include <climits>
-
-#include "gdn_attn.h"
+#include "gdn_paged.h"
 
 namespace omx {
 namespace {
-
-typedef const __attribute__((address_space(4))) int32_t const_i32;
-
-// C += A(16x16) B(16x16), contraction of 16 keys
-__device__ __forceinline__ f32x4 mma_pv(u32x2 a, u32x2 b, f32x4 c) { return mma16k16(a, b, c); }
 
 // ------------------------------------------------------------------------------------ append
 // Token i of sequence n goes to position held[n] + i: page table[n, position / page], row
@@ -80,23 +73,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(AttnParams p) {
 // may differ as they like, and all workgroups still end together.  A range's part of one sequence
 // is a segment; workgroup w's of sequence b is kept at w + b (a staircase: each next segment has
 // the next w or the next b), and the join adds up a sequence's.  A sequence in one segment needs none.
-constexpr int kDecNW = 4;
-template <int DP> constexpr int kStageKeys = 4096 / DP;  // 64, 32, 16 keys: 8 KiB of each of K, V
-
-// stages of a sequence, one at least: it writes the output
-__device__ __forceinline__ int stages_of(int held, int cap, int sk) {
-  const int keys = held < 0 ? 0 : (held < cap ? held + 1 : cap);
-  const int n = (keys + sk - 1) / sk;
-  return n < 1 ? 1 : n;
-}
-
-// stages of each range: equal shares, but no less than two stages a wavefront
-__device__ __forceinline__ int range_stages(int all, int splits) {
-  const int per = (all + splits - 1) / splits;
-  return per > 2 * kDecNW ? per : 2 * kDecNW;
-}
-
-template <int DP, int NQ>
+template <int DP, int NQ, bool WIN>
 __global__ __launch_bounds__(64 * kDecNW) __attribute__((amdgpu_waves_per_eu(1)))
 void attn_decode_kernel(AttnParams p) {
   constexpr int SK = kStageKeys<DP>, NG = SK / 16;  // keys of a stage, its groups of 16
@@ -115,37 +92,14 @@ void attn_decode_kernel(AttnParams p) {
 
   // the range: stages [x, x1) of all sequences', from stage st0 of sequence b on
   int b = wg, st0 = 0, x = 0, x1 = INT_MAX;
-  if (p.splits > 1) {
-    // lane n holds the stages of sequence n, n + 64, ..: the first 64 are read once
-    const int v0 = l < p.N ? stages_of(p.held[l], cap, SK) : 0;
-    int v = v0;
-    for (int n = l + 64; n < p.N; n += 64) v += stages_of(p.held[n], cap, SK);
-    const int all = wave_total(v), per = range_stages(all, p.splits);
-    if ((long long)wg * per >= all) return;
-    x = wg * per;
-    x1 = x + per < all ? x + per : all;
-    v = v0;
-    for (int n0 = 0, base = 0;;) {  // x < all: some 64 sequences hold it
-      const int upto = base + wave_scan(v);
-      const unsigned long long past = __ballot(upto > x);
-      if (past) {
-        const int s = __ffsll(past) - 1;
-        b = n0 + s;
-        st0 = x - __builtin_amdgcn_readlane(upto - v, s);
-        break;
-      }
-      base = __builtin_amdgcn_readlane(upto, 63);
-      n0 += 64;
-      v = n0 + l < p.N ? stages_of(p.held[n0 + l], cap, SK) : 0;
-    }
-  }
+  if (p.splits > 1 && !decode_range<WIN>(p, wg, cap, SK, b, st0, x, x1)) return;
 
   for (;;) {  // a segment a turn
   const_i32* table = (const_i32*)(p.table + (long long)b * p.table_w);
   const int held = ((const_i32*)p.held)[b];
   // keys: those held and the new one, at position `held`; past the table there is no room for it
-  const int keys = held < 0 ? 0 : (held < cap ? held + 1 : cap);
-  const int nst = stages_of(held, cap, SK);
+  const Seen seen = seen_of<WIN>(p, held, cap, SK);
+  const int keys = seen.keys, nst = seen.stages;
   const int st1 = nst - st0 < x1 - x ? nst : st0 + (x1 - x);
   const bool alone = st0 == 0 && st1 == nst;
 
@@ -177,7 +131,7 @@ void attn_decode_kernel(AttnParams p) {
     Ids x;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const int key = st * SK + 16 * g;
+      const int key = (WIN ? seen.at(st) : st) * SK + 16 * g;
       const int slot = key / p.page;
       int id = key < keys ? table[slot] : -1;  // key < keys <= cap: the slot is in the table
       x.id[g] = id >= 0 && id < p.n_pages ? id : -1;
@@ -208,15 +162,17 @@ void attn_decode_kernel(AttnParams p) {
   };
 
   auto compute = [&](int st, bf16_t* sk, bf16_t* sv, unsigned have) {
-    const int key0 = st * SK;
+    const int key0 = (WIN ? seen.at(st) : st) * SK;
     constexpr unsigned kAll = (1u << NG) - 1;
-    const bool whole = have == kAll && key0 + SK < keys;  // every row a held key
+    const bool whole = have == kAll && key0 + SK < keys &&  // every row a held key, and seen
+                       !(WIN && key0 < seen.lo && key0 + SK > p.sinks);
     if (!whole) {
-      // rows without a key are cleared (a weight of zero does not clear a NaN), and the new
+      // rows without a key, or not seen, are cleared (a weight of zero does not clear a NaN), and the new
       // token's row comes from the arguments: its page has no copy of it yet
       for (int i = l; i < SK * DP / 8; i += 64) {
         const int row = i / (DP / 8);
-        if (key0 + row >= keys || !((have >> (row / 16)) & 1)) *(u32x4*)(sv + 8 * i) = u32x4{0, 0, 0, 0};
+        const int key = key0 + row;
+        if (key >= keys || !((have >> (row / 16)) & 1) || (WIN && key < seen.lo && key >= p.sinks)) *(u32x4*)(sv + 8 * i) = u32x4{0, 0, 0, 0};
       }
       const int row = held - key0;
       if (row >= 0 && row < SK && held < cap && ((have >> (row / 16)) & 1)) {
@@ -251,7 +207,8 @@ void attn_decode_kernel(AttnParams p) {
       for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (!whole && (key0 + 16 * g + 4 * g4 + i >= keys || !((have >> g) & 1))) s[g][i] = -INFINITY;
+          const int key = key0 + 16 * g + 4 * g4 + i;
+          if (!whole && (key >= keys || !((have >> g) & 1) || (WIN && key < seen.lo && key >= p.sinks))) s[g][i] = -INFINITY;
           mx = fmaxf(mx, s[g][i]);
         }
       if (__any((mx - m[n]) * cs > 8.f)) {
@@ -388,92 +345,19 @@ void attn_decode_kernel(AttnParams p) {
   }
 }
 
-// Joins a row's segments, with W of a workgroup's four wavefronts on one row.
-template <int DP, int W>
-__global__ __launch_bounds__(256) void decode_join_kernel(AttnParams p) {
-  constexpr int E = DP / 64, SK = kStageKeys<DP>;
-  typedef float fE __attribute__((ext_vector_type(E)));
-  __shared__ float sAcc[4][DP];
-  const int l = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % W;
-  const int Hq = p.Hkv * p.G;
-  const int rows = p.N * Hq, row = (int)blockIdx.x * (4 / W) + w / W;
-  const bool live = row < rows;
-  const int b = live ? row / Hq : 0, head = live ? row % Hq : 0;
-  const int cap = p.table_w * p.page, nst = stages_of(p.held[b], cap, SK);
-  int v = 0, y = 0;
-  for (int n = l; n < p.N; n += 64) {
-    const int x = stages_of(p.held[n], cap, SK);
-    v += x;
-    if (n < b) y += x;
-  }
-  const int before = wave_total(y), per = range_stages(wave_total(v), p.splits);
-  const int w0 = before / per, segs = live ? (before + nst - 1) / per - w0 + 1 : 1;
-  if (segs == 1 && W == 1) return;  // written already (with W > 1 a whole workgroup agrees on it below)
-  float M = -3e38f, den = 0.f, acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  if (segs > 1) {
-    for (int s = l; s < segs; s += 64) M = fmaxf(M, p.part_ml[2 * ((long long)(w0 + s + b) * Hq + head)]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    for (int s0 = 0; s0 < segs; s0 += 64) {  // weights a lane, then the sums, eight reads in flight
-      const int n = segs - s0 < 64 ? segs - s0 : 64;
-      float a = 0.f;
-      if (l < n) {
-        const long long at = (long long)(w0 + s0 + l + b) * Hq + head;
-        const float ls = p.part_ml[2 * at + 1];
-        a = ls == 0.f ? 0.f : __builtin_amdgcn_exp2f(p.part_ml[2 * at] - M);
-        den += a * ls;
-      }
-      for (int s = part; s < n; s += 8 * W) {
-        fE v[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int su = s + W * u < n ? s + W * u : n - 1;
-          v[u] = *(const fE*)(p.part_o + ((long long)(w0 + s0 + su + b) * Hq + head) * DP + E * l);
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float as = __shfl(a, (s + W * u) & 63, 64);
-          const float f = s + W * u < n ? as : 0.f;
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] += f * v[u][e];
-        }
-      }
-    }
-    den = wave_sum(den);
-  }
-  if constexpr (W > 1) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) sAcc[w][E * l + e] = acc[e];
-    __syncthreads();
-    if (part != 0 || segs == 1) return;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-#pragma unroll
-      for (int u = 1; u < W; ++u) acc[e] += sAcc[w + u][E * l + e];
-  }
-  const float inv = den > 0.f ? 1.f / den : (den == 0.f ? 0.f : den);
-  bf16_t* op = (bf16_t*)p.o + (long long)row * DP + E * l;
-#pragma unroll
-  for (int e = 0; e < E; ++e) op[e] = f2bf(acc[e] * inv);
-}
-
-template <int DP>
+template <int DP, bool WIN>
 void decode_dp(const AttnParams& p, hipStream_t stream) {
   const unsigned grid = (unsigned)((p.splits > 1 ? p.splits : p.N) * p.Hkv);
   if (p.G <= 16)
-    attn_decode_kernel<DP, 1><<<grid, 64 * kDecNW, 0, stream>>>(p);
+    attn_decode_kernel<DP, 1, WIN><<<grid, 64 * kDecNW, 0, stream>>>(p);
   else
-    attn_decode_kernel<DP, 2><<<grid, 64 * kDecNW, 0, stream>>>(p);
-  if (p.splits == 1) return;
-  // a row has at most as many segments as its key head has workgroups; four wavefronts share a row
-  // where there are few rows
-  const unsigned rows = (unsigned)(p.N * p.Hkv * p.G);
-  if (rows <= 512)
-    decode_join_kernel<DP, 4><<<rows, 256, 0, stream>>>(p);
-  else
-    decode_join_kernel<DP, 1><<<(rows + 3) / 4, 256, 0, stream>>>(p);
+    attn_decode_kernel<DP, 2, WIN><<<grid, 64 * kDecNW, 0, stream>>>(p);
+  if (p.splits > 1) launch_decode_join<DP, WIN>(p, stream);
+}
+template <int DP>
+void decode_dp(const AttnParams& p, hipStream_t stream) {
+  if (p.window > 0) decode_dp<DP, true>(p, stream);
+  else decode_dp<DP, false>(p, stream);
 }
 
 }  // namespace
