@@ -504,6 +504,44 @@ size_t omx_gdn_attn_decode_window_workspace_size(int64_t B, int64_t Hq, int64_t 
                                                  int64_t page_size, int64_t table_width,
                                                  int64_t window, int64_t sinks);
 
+/*
+ * Pages of a cache, dealt and returned on the GPU.  Free pages lie on a stack: free_pages int32 [n_pages],
+ * of which the first free_count[0] (int32 [1], read as within [0, n_pages]) are free.  block_table, page_size
+ * and lengths as for the cache; N at most 2^20.
+ *
+ * omx_gdn_pages_assign gives new_tokens[n] more tokens of each sequence (int32 [N]; none for a length or a
+ * number below zero) their places: entries of block_table for positions lengths[n] .. lengths[n] +
+ * new_tokens[n] - 1 that name no page take one from the stack's top, in order of sequence and position;
+ * entries that name one keep it.  lengths are not advanced.
+ *   T            tokens that there is room for below; those past it, packed, get no place
+ *   cu_seqlens   int32 [N + 1]: the packed new tokens' offsets, at most T
+ *   positions    int32 [T]: each packed token's position in its sequence; -1 from cu_seqlens[N] on
+ *   slots        int64 [T]: page * page_size + row of each; -1 where there is no page, and from there on
+ *   missing      int32 [1]: pages that the stack was short of; the last entries stay without one then
+ */
+int omx_gdn_pages_assign(int32_t* block_table, int64_t N, int64_t table_width,
+                         const int32_t* lengths, const int32_t* new_tokens, int32_t* free_pages,
+                         int32_t* free_count, int64_t n_pages, int64_t page_size, int64_t T,
+                         int32_t* cu_seqlens, int32_t* positions, int64_t* slots, int32_t* missing,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace omx_gdn_pages_assign needs (16-byte aligned): none up to 4,096 sequences. */
+size_t omx_gdn_pages_assign_workspace_size(int64_t N);
+
+/*
+ * Returns the pages that lie wholly past the lengths[n] tokens that a sequence keeps (0: all of its pages;
+ * negative: it keeps them all), and with a window (0: none) those whose positions the token at lengths[n] no
+ * longer sees, but for the first `sinks`.  Their entries become -1.  A page that stands in two rows is to go
+ * back from one of them only.  What omx_gdn_pages_assign dealt last goes back to the same places.
+ */
+int omx_gdn_pages_release(int32_t* block_table, int64_t N, int64_t table_width,
+                          const int32_t* lengths, int32_t* free_pages, int32_t* free_count,
+                          int64_t n_pages, int64_t page_size, int64_t window, int64_t sinks,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of device workspace omx_gdn_pages_release needs (16-byte aligned): counts of large tables. */
+size_t omx_gdn_pages_release_workspace_size(int64_t N, int64_t table_width);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,7 +6,7 @@ reference's interface (omegalax/models/qwen3_5/deltanet.py).
 """
 from .attention import (  # noqa: F401
     attention_decode_step, attention_prefill, attention_prefill_bwd, attention_prefill_paged,
-    kv_pages_write,
+    kv_pages_assign, kv_pages_release, kv_pages_write,
 )
 from .deltanet import (  # noqa: F401
     GDNError, chunk_gated_delta_rule, chunk_gated_delta_rule_bwd, gdn_ab_projections,

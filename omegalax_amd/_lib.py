@@ -77,6 +77,10 @@ SIGNATURES = {
     "omx_gdn_attn_decode_window": (_i, [_p] * 3 + [_i64] * 3 + [_p] * 4 + [_i64, _i64, _p, _i64, _p, _p]
                                    + [_i64] * 4 + [_f, _i64, _i64, _p, _sz, _p]),
     "omx_gdn_attn_decode_window_workspace_size": (_sz, [_i64] * 8),
+    "omx_gdn_pages_assign": (_i, [_p, _i64, _i64] + [_p] * 4 + [_i64] * 3 + [_p] * 5 + [_sz, _p]),
+    "omx_gdn_pages_assign_workspace_size": (_sz, [_i64]),
+    "omx_gdn_pages_release": (_i, [_p, _i64, _i64] + [_p] * 3 + [_i64] * 4 + [_p, _sz, _p]),
+    "omx_gdn_pages_release_workspace_size": (_sz, [_i64] * 2),
     "omx_gdn_qkv_conv_proj": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _p]),
 }
 

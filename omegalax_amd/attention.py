@@ -30,7 +30,7 @@ from . import _lib
 from .deltanet import _cu_seqlens, _no_tangents, _ptr, _stream, _workspace
 
 __all__ = ["attention_prefill", "attention_prefill_bwd", "attention_prefill_paged",
-           "attention_decode_step", "kv_pages_write"]
+           "attention_decode_step", "kv_pages_assign", "kv_pages_release", "kv_pages_write"]
 
 
 _BF16 = torch.bfloat16
@@ -338,3 +338,64 @@ def attention_decode_step(q, k, v, k_pages, v_pages, block_table, lengths, *, sc
           _ptr(v_pages), *exps, pages, page, _ptr(table), table.shape[1], _ptr(lengths), _ptr(out), B, Hq, Hkv, D,
           _scale(scale, D), *sight, _ptr(ws), ws_bytes)
     return out
+
+
+def _pages(block_table, lengths, free_pages, free_count):
+    """Checks of what deals pages; the table and the stack are changed where they lie."""
+    dev = _device(block_table, lengths, free_pages, free_count)
+    N = lengths.shape[0] if lengths.dim() == 1 else -1
+    for name, t, ok, want in (
+            ("block_table", block_table, block_table.dim() == 2 and block_table.shape[0] == N, f"[{N}, width]"),
+            ("lengths", lengths, N >= 0, "[N]"), ("free_pages", free_pages, free_pages.dim() == 1, "[pages]"),
+            ("free_count", free_count, tuple(free_count.shape) == (1,), "[1]")):
+        if t.dtype is not torch.int32 or not ok:
+            raise ValueError(f"{name} must be int32 {want} (got {t.dtype}, {tuple(t.shape)})")
+        if t is not lengths and not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    return dev, N, lengths.contiguous()
+
+
+def kv_pages_assign(block_table, lengths, new_tokens, free_pages, free_count, *, page_size, tokens):
+    """Gives new tokens their pages, on the GPU and in place; what the appends and attention of a step take.
+
+    ``new_tokens`` int32 [N]: how many more tokens each sequence gets behind its ``lengths[n]``.  Entries
+    of ``block_table`` that they need and that name no page take one from the stack of free pages,
+    ``free_pages`` int32 [pages] with the first ``free_count`` (int32 [1]) of them free, in order; others
+    keep theirs.  ``tokens``: the most that there is room for, all sequences together.  Returns
+    (cu_seqlens int32 [N + 1], positions int32 [tokens], slots int64 [tokens], missing int32 [1]): the packed
+    tokens' offsets, their positions in their sequences, page * page_size + row of each (-1 past the last,
+    and where there is no page), and how many pages the stack was short of.
+    """
+    dev, N, lengths = _pages(block_table, lengths, free_pages, free_count)
+    _device(block_table, new_tokens)
+    if new_tokens.dtype is not torch.int32 or tuple(new_tokens.shape) != (N,):
+        raise ValueError(f"new_tokens must be int32 [{N}] (got {new_tokens.dtype}, {tuple(new_tokens.shape)})")
+    new_tokens = new_tokens.contiguous()
+    T = operator.index(tokens)
+    if T < 0:
+        raise ValueError(f"tokens must not be negative (got {T})")
+    cu = torch.empty(N + 1, dtype=torch.int32, device=dev)
+    positions = torch.empty(T, dtype=torch.int32, device=dev)
+    slots = torch.empty(T, dtype=torch.int64, device=dev)
+    missing = torch.empty(1, dtype=torch.int32, device=dev)
+    ws_bytes = _workspace_bytes("omx_gdn_pages_assign_workspace_size", N)
+    ws = _workspace(ws_bytes, dev)
+    _call(dev, "omx_gdn_pages_assign", _ptr(block_table), N, block_table.shape[1], _ptr(lengths), _ptr(new_tokens),
+          _ptr(free_pages), _ptr(free_count), free_pages.shape[0], operator.index(page_size), T, _ptr(cu),
+          _ptr(positions), _ptr(slots), _ptr(missing), _ptr(ws), ws_bytes)
+    return cu, positions, slots, missing
+
+
+def kv_pages_release(block_table, lengths, free_pages, free_count, *, page_size, window=None, sinks=0):
+    """Returns pages to the stack that ``kv_pages_assign`` takes them from, on the GPU and in place.
+
+    Those wholly past the ``lengths[n]`` tokens that a sequence keeps (0: it has ended, all of them; negative:
+    none), and with a ``window`` those whose positions its next token no longer sees, but for the first
+    ``sinks``.  Their entries become -1.  A page that two rows share is to go back from one of them only.
+    """
+    dev, N, lengths = _pages(block_table, lengths, free_pages, free_count)
+    window, sinks = _sight(window, sinks) or (0, 0)
+    ws_bytes = _workspace_bytes("omx_gdn_pages_release_workspace_size", N, block_table.shape[1])
+    ws = _workspace(ws_bytes, dev)
+    _call(dev, "omx_gdn_pages_release", _ptr(block_table), N, block_table.shape[1], _ptr(lengths), _ptr(free_pages),
+          _ptr(free_count), free_pages.shape[0], operator.index(page_size), window, sinks, _ptr(ws), ws_bytes)

@@ -600,4 +600,72 @@ int omx_gdn_attn_decode_window(const void* q, const void* k, const void* v, int6
 }
 
 
+namespace {
+int check_pages(const char* fn, const int32_t* table, int64_t N, int64_t table_w, const int32_t* lengths,
+                const int32_t* free_pages, const int32_t* free_count, int64_t n_pages, int64_t page) {
+  REQUIRE(N >= 0 && N <= (1 << 20), "%s: sequence count %lld out of range", fn, (long long)N);
+  REQUIRE(page >= 16 && page % 16 == 0 && page <= 65536, "%s: page size %lld must be a multiple of 16 in [16, 65536]",
+          fn, (long long)page);
+  REQUIRE(n_pages >= 0 && n_pages <= INT_MAX, "%s: page count %lld out of range", fn, (long long)n_pages);
+  REQUIRE(table_w >= 0 && table_w <= kMaxTokens && table_w * page <= kMaxTokens,
+          "%s: block table of %lld pages of %lld tokens out of range", fn, (long long)table_w, (long long)page);
+  REQUIRE((lengths || N == 0) && (table || N * table_w == 0) && (free_pages || n_pages == 0) && free_count,
+          "%s: a required pointer is NULL", fn);
+  return OMX_GDN_OK;
+}
+omx::PagesParams pages(int32_t* table, int64_t N, int64_t table_w, const int32_t* lengths, int32_t* free_pages,
+                       int32_t* free_count, int64_t n_pages, int64_t page, void* workspace) {
+  omx::PagesParams p{};
+  p.table = table; p.N = (int)N; p.table_w = (int)table_w; p.lengths = lengths; p.free = free_pages; p.count = free_count;
+  p.n_pages = (int)n_pages; p.page = (int)page; p.first = (int32_t*)workspace;
+  return p;
+}
+}  // namespace
+
+size_t omx_gdn_pages_assign_workspace_size(int64_t N) {
+  return N < 0 || N > (1 << 20) ? 0 : align_up(omx::pages_assign_words(N) * 4);
+}
+
+int omx_gdn_pages_assign(int32_t* block_table, int64_t N, int64_t table_width, const int32_t* lengths,
+                         const int32_t* new_tokens, int32_t* free_pages, int32_t* free_count, int64_t n_pages,
+                         int64_t page_size, int64_t T, int32_t* cu_seqlens, int32_t* positions, int64_t* slots,
+                         int32_t* missing, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "omx_gdn_pages_assign";
+  const int rc = check_pages(fn, block_table, N, table_width, lengths, free_pages, free_count, n_pages, page_size);
+  if (rc) return rc;
+  REQUIRE(T >= 0 && T <= kMaxTokens, "%s: too many tokens (%lld)", fn, (long long)T);
+  // entries of new tokens are counted in 32 bits: those of T tokens, and two more for each sequence
+  REQUIRE(T / page_size + 2 * N <= INT_MAX, "%s: too many tokens (%lld)", fn, (long long)T);
+  const size_t need = omx_gdn_pages_assign_workspace_size(N);
+  REQUIRE(workspace_bytes >= need, "%s: workspace of %zu bytes is smaller than the %zu needed", fn, workspace_bytes, need);
+  REQUIRE(need == 0 || (workspace && aligned(workspace, 16)), "%s: workspace must be non-NULL and 16-byte aligned", fn);
+  REQUIRE((new_tokens || N == 0) && cu_seqlens && missing && ((positions && slots) || T == 0), "%s: a required pointer is NULL", fn);
+  omx::PagesParams p = pages(block_table, N, table_width, lengths, free_pages, free_count, n_pages, page_size, workspace);
+  p.new_tokens = new_tokens; p.T = T; p.cu = cu_seqlens; p.positions = positions; p.slots = (long long*)slots; p.missing = missing;
+  return launch_status(omx::launch_pages_assign(p, (hipStream_t)stream), fn);
+}
+
+size_t omx_gdn_pages_release_workspace_size(int64_t N, int64_t table_width) {
+  if (N < 0 || N > (1 << 20) || table_width < 0 || table_width > kMaxTokens) return 0;
+  return align_up(omx::pages_release_words(N * table_width) * 4);
+}
+
+int omx_gdn_pages_release(int32_t* block_table, int64_t N, int64_t table_width, const int32_t* lengths,
+                          int32_t* free_pages, int32_t* free_count, int64_t n_pages, int64_t page_size, int64_t window,
+                          int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "omx_gdn_pages_release";
+  int rc = check_pages(fn, block_table, N, table_width, lengths, free_pages, free_count, n_pages, page_size);
+  if (!rc) rc = check_any_sight(fn, Sight{window, sinks});
+  if (rc) return rc;
+  REQUIRE(N * table_width <= kMaxGroups * 4096, "%s: grid too large", fn);
+  const size_t need = omx_gdn_pages_release_workspace_size(N, table_width);
+  REQUIRE(workspace_bytes >= need, "%s: workspace of %zu bytes is smaller than the %zu needed", fn, workspace_bytes, need);
+  REQUIRE(need == 0 || (workspace && aligned(workspace, 16)), "%s: workspace must be non-NULL and 16-byte aligned", fn);
+  if (N * table_width == 0) return ok();
+  omx::PagesParams p = pages(block_table, N, table_width, lengths, free_pages, free_count, n_pages, page_size, workspace);
+  p.window = window < kMaxTokens ? (int)window : 0;  // no position is behind a window of all
+  p.sinks = sinks;
+  return launch_status(omx::launch_pages_release(p, (hipStream_t)stream), fn);
+}
+
 }  // extern "C"

@@ -339,4 +339,25 @@ int kv_write8_tokens();
 hipError_t launch_kv_write8(const AttnParams& p, hipStream_t stream);
 hipError_t launch_attn_decode8(const AttnParams& p, hipStream_t stream);
 
+// Pages dealt to new tokens from a stack, and returned to it (gdn_pages.hip).
+struct PagesParams {
+  int32_t* table;              // [N, table_w]
+  const int32_t* lengths;      // [N]: tokens held, or kept
+  const int32_t* new_tokens;   // [N]
+  int32_t* free;               // [n_pages], of which [0, count) are free
+  int32_t* count;
+  int N, table_w, page, n_pages;
+  long long T;                 // tokens that positions and slots have room for
+  int32_t *cu, *positions;     // [N + 1], [T]
+  long long* slots;            // [T]
+  int32_t* missing;            // pages that the stack did not have
+  int32_t* first;              // workspace
+  int window;                  // return: what the next token sees, 0 all
+  long long sinks;
+};
+size_t pages_assign_words(long long N);         // int32 words of workspace
+size_t pages_release_words(long long entries);
+hipError_t launch_pages_assign(const PagesParams& p, hipStream_t stream);
+hipError_t launch_pages_release(const PagesParams& p, hipStream_t stream);
+
 }  // namespace omx

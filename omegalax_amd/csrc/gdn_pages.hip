@@ -1,0 +1,282 @@
+// Pages of a paged cache, dealt and returned on the GPU: no length leaves it.
+//
+// Free pages lie on a stack: free[0 .. count).  Of the entries that new tokens need and that name no page
+// yet, in order of sequence and slot, the k-th takes free[count - 1 - k]; of those that are returned, n in
+// all, the k-th goes to free[count + n - 1 - k], so that what is dealt and returned leaves the stack as it was.
+// Every place is a prefix sum, so the order of execution changes nothing.  Bound by latency: a few
+// dependent reads, and for many tokens the 12 bytes written for each.
+#include <climits>
+
+#include "gdn_attn.h"
+
+namespace omx {
+namespace {
+
+constexpr int kNT = 1024;
+
+// Inclusive sum over the workgroup, and its total; `s` holds a word a wavefront.
+template <int NT, class I>
+__device__ __forceinline__ I block_scan(I v, I* s, I& total) {
+  const int l = lane_id(), w = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const I x = __shfl_up(v, o, 64);
+    if (l >= o) v += x;
+  }
+  __syncthreads();
+  if (l == 63) s[w] = v;
+  __syncthreads();
+  I before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) {
+    if (i < w) before += s[i];
+    total += s[i];
+  }
+  return before + v;
+}
+
+__device__ __forceinline__ bool a_page(int id, int n_pages) { return id >= 0 && id < n_pages; }
+__device__ __forceinline__ int on_stack(const PagesParams& p) {
+  const int c = *p.count;
+  return c < 0 ? 0 : (c < p.n_pages ? c : p.n_pages);
+}
+
+// the last n in [0, N) with start[n] <= x, for start[0] <= x; S: of any memory
+template <class S>
+__device__ __forceinline__ int last_upto(const S* start, int N, int x) {
+  int lo = 0, hi = N;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// positions and slots of packed tokens t
+template <class S>
+__device__ __forceinline__ void map_token(const PagesParams& p, const S* cu, int used, int t) {
+  int pos = -1;
+  long long slot = -1;
+  if (t < used) {
+    const int n = last_upto(cu, p.N, t);
+    const long long at = (long long)p.lengths[n] + (t - cu[n]), i = at / p.page;
+    pos = at < INT_MAX ? (int)at : INT_MAX;
+    const int id = i < p.table_w ? p.table[(long long)n * p.table_w + i] : -1;
+    if (a_page(id, p.n_pages)) slot = (long long)id * p.page + (at - i * p.page);
+  }
+  p.positions[t] = pos;
+  p.slots[t] = slot;
+}
+
+// One workgroup: the sequences' offsets, then their entries, flat, and (MAP) their tokens.
+// `first`: [N + 1] entries before each sequence's, in LDS (kLdsSeqs of them at most) or memory.
+constexpr int kLdsSeqs = 4096;
+
+template <bool LDS>
+__global__ __launch_bounds__(kNT) void pages_assign_kernel(PagesParams p, int map) {
+  __shared__ int sFirst[LDS ? kLdsSeqs + 1 : 1], sCu[LDS ? kLdsSeqs + 1 : 1];
+  __shared__ long long sWave[kNT / 64];
+  const int tid = threadIdx.x;
+  const int count = on_stack(p);
+  int* first = LDS ? sFirst : p.first;
+  int* cu = LDS ? sCu : p.cu;
+  // tokens and entries of the sequences before, in one sum: no more than 2^31 tokens and 2^31 entries
+  long long tokens = 0, entries = 0;
+  for (int n0 = 0; n0 < p.N; n0 += kNT) {
+    const int n = n0 + tid;
+    const int held = n < p.N ? p.lengths[n] : -1, more = n < p.N ? p.new_tokens[n] : 0;
+    long long m = held >= 0 && more > 0 ? (more < p.T ? more : p.T) : 0, total;
+    const long long end = tokens + block_scan<kNT>(m, sWave, total);
+    // tokens past T have no place
+    const long long a = end - m < p.T ? end - m : p.T, b = end < p.T ? end : p.T;
+    m = b - a;
+    tokens += total;
+    long long slots = 0;
+    if (m > 0) {
+      const long long i0 = held / p.page, i1 = (held + m - 1) / p.page + 1;
+      slots = (i1 < p.table_w ? i1 : p.table_w) - i0;
+      slots = slots > 0 ? slots : 0;
+    }
+    const long long upto = entries + block_scan<kNT>(slots, sWave, total);
+    entries += total;
+    if (n < p.N) {
+      first[n] = (int)(upto - slots);
+      cu[n] = (int)a;
+      if (LDS) p.cu[n] = (int)a;
+    }
+  }
+  const int used = (int)(tokens < p.T ? tokens : p.T), all = (int)entries;
+  if (tid == 0) {
+    first[p.N] = all;
+    cu[p.N] = p.cu[p.N] = used;
+  }
+  __syncthreads();
+  // the entries, four a thread
+  int needed = 0;
+  for (int f0 = 0; f0 < all; f0 += 4 * kNT) {
+    int* at[4];
+    int need[4], mine = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int f = f0 + 4 * tid + i;
+      need[i] = 0;
+      at[i] = nullptr;
+      if (f < all) {
+        const int n = last_upto(first, p.N, f);
+        at[i] = p.table + (long long)n * p.table_w + p.lengths[n] / p.page + (f - first[n]);
+        need[i] = !a_page(*at[i], p.n_pages);
+      }
+      mine += need[i];
+    }
+    long long total;
+    int k = needed + (int)block_scan<kNT>((long long)mine, sWave, total) - mine;
+    needed += (int)total;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!need[i]) continue;
+      if (k < count) *at[i] = p.free[count - 1 - k];
+      ++k;
+    }
+  }
+  if (tid == 0) {
+    *p.count = needed < count ? count - needed : 0;
+    *p.missing = needed < count ? 0 : needed - count;
+  }
+  if (!map) return;
+  __syncthreads();
+  for (int t = tid; t < p.T; t += kNT) map_token(p, cu, used, t);
+}
+
+__global__ __launch_bounds__(256) void pages_map_kernel(PagesParams p) {
+  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (t < p.T) map_token(p, p.cu, p.cu[p.N], (int)t);
+}
+
+// Whether entry i of row n goes back: past the tokens that are kept, or with a window behind what the
+// next token sees, but for the sinks'.
+__device__ __forceinline__ bool goes_back(const PagesParams& p, int id, int n, int i) {
+  const long long keep = p.lengths[n], from = (long long)i * p.page;
+  if (keep < 0 || !a_page(id, p.n_pages)) return false;
+  return from >= keep || (p.window > 0 && from >= p.sinks && from + p.page <= keep + 1 - p.window);
+}
+
+// Entries of the tables, flat, kPer a workgroup of kBackNT threads, four neighbours a thread and turn.
+constexpr int kBackNT = 256, kPer = 4096;
+
+__device__ __forceinline__ int back_of(const PagesParams& p, long long f, int (&id)[4]) {
+  int mask = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long e = f + i;
+    id[i] = -1;
+    if (e >= (long long)p.N * p.table_w) continue;
+    const int n = (int)(e / p.table_w);
+    id[i] = p.table[e];
+    if (goes_back(p, id[i], n, (int)(e - (long long)n * p.table_w))) mask |= 1 << i;
+  }
+  return mask;
+}
+__device__ __forceinline__ void give_back(const PagesParams& p, long long f, const int (&id)[4], int mask, long long top) {
+  // the first of them goes to free[top], the next below it
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (!((mask >> i) & 1)) continue;
+    if (top < p.n_pages) p.free[top] = id[i];
+    p.table[f + i] = -1;
+    --top;
+  }
+}
+
+// few entries: one workgroup, which counts them and then passes over them again
+__global__ __launch_bounds__(kNT) void pages_release_one_kernel(PagesParams p) {
+  __shared__ int sWave[kNT / 64];
+  const long long all = (long long)p.N * p.table_w;
+  int id[4], mine = 0, total;
+  for (long long f = 4 * threadIdx.x; f < all; f += 4 * kNT) mine += __popc(back_of(p, f, id));
+  const int count = on_stack(p);
+  block_scan<kNT>(mine, sWave, total);
+  const int n = total;
+  int done = 0;
+  for (long long f0 = 0; f0 < all; f0 += 4 * kNT) {
+    const long long f = f0 + 4 * threadIdx.x;
+    const int mask = back_of(p, f, id), k = __popc(mask);
+    const int before = done + block_scan<kNT>(k, sWave, total) - k;
+    done += total;
+    give_back(p, f, id, mask, (long long)count + n - 1 - before);
+  }
+  if (threadIdx.x == 0) *p.count = count + n < p.n_pages ? count + n : p.n_pages;
+}
+
+// many: a count for each kPer entries, and the stack's count as it was
+__global__ __launch_bounds__(kBackNT) void pages_count_kernel(PagesParams p) {
+  __shared__ int sWave[kBackNT / 64];
+  int id[4], mine = 0, total;
+#pragma unroll
+  for (int j = 0; j < kPer / (4 * kBackNT); ++j)
+    mine += __popc(back_of(p, (long long)blockIdx.x * kPer + 4 * (j * kBackNT + (int)threadIdx.x), id));
+  block_scan<kBackNT>(mine, sWave, total);
+  if (threadIdx.x != 0) return;
+  p.first[1 + blockIdx.x] = total;
+  if (blockIdx.x == 0) p.first[0] = on_stack(p);
+}
+
+__global__ __launch_bounds__(kBackNT) void pages_release_kernel(PagesParams p) {
+  __shared__ int sWave[kBackNT / 64];
+  __shared__ long long sSum[kBackNT / 64];
+  long long before = 0, n = 0, total;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += kBackNT) {
+    const int x = p.first[1 + i];
+    n += x;
+    if (i < (int)blockIdx.x) before += x;
+  }
+  block_scan<kBackNT>(before, sSum, total);
+  before = total;
+  block_scan<kBackNT>(n, sSum, total);
+  n = total;
+  const int count = p.first[0];
+  for (int j = 0; j < kPer / (4 * kBackNT); ++j) {
+    const long long f = (long long)blockIdx.x * kPer + 4 * (j * kBackNT + (int)threadIdx.x);
+    int id[4], here;
+    const int mask = back_of(p, f, id), k = __popc(mask);
+    const int upto = block_scan<kBackNT>(k, sWave, here);
+    give_back(p, f, id, mask, count + n - 1 - (before + upto - k));
+    before += here;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.count = (int)(count + n < p.n_pages ? count + n : p.n_pages);
+}
+
+constexpr long long kOneRelease = 1 << 15;  // entries that one workgroup passes over
+constexpr long long kOneMap = 4096;         // tokens that the assigning workgroup maps
+
+}  // namespace
+
+size_t pages_assign_words(long long N) { return N > kLdsSeqs ? (size_t)N + 1 : 0; }
+
+hipError_t launch_pages_assign(const PagesParams& p, hipStream_t stream) {
+  const int map = p.T <= kOneMap;
+  if (p.N <= kLdsSeqs)
+    pages_assign_kernel<true><<<1, kNT, 0, stream>>>(p, map);
+  else
+    pages_assign_kernel<false><<<1, kNT, 0, stream>>>(p, map);
+  if (!map) pages_map_kernel<<<(unsigned)((p.T + 255) / 256), 256, 0, stream>>>(p);
+  return hipGetLastError();
+}
+
+size_t pages_release_words(long long entries) {
+  return entries > kOneRelease ? (size_t)((entries + kPer - 1) / kPer + 1) : 0;
+}
+
+hipError_t launch_pages_release(const PagesParams& p, hipStream_t stream) {
+  const long long entries = (long long)p.N * p.table_w;
+  if (entries <= kOneRelease) {
+    pages_release_one_kernel<<<1, kNT, 0, stream>>>(p);
+  } else {
+    const unsigned grid = (unsigned)((entries + kPer - 1) / kPer);
+    pages_count_kernel<<<grid, kBackNT, 0, stream>>>(p);
+    pages_release_kernel<<<grid, kBackNT, 0, stream>>>(p);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace omx
