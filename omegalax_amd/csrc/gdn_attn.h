@@ -165,6 +165,14 @@ __device__ __forceinline__ u32x4 rsrc_words(const void* p, unsigned bytes) {
                (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffffu),
                (unsigned)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
 }
+// the same for the builtin loads: of a resource that the compiler does not know to be uniform they become
+// a loop over its values
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_rsrc(const void* p, unsigned bytes) {
+  const unsigned long long a = (unsigned long long)p;
+  const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((unsigned)a);
+  const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+  return buf_rsrc((const void*)((unsigned long long)hi << 32 | lo), (unsigned)__builtin_amdgcn_readfirstlane(bytes));
+}
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return (unsigned)(unsigned long long)(const __attribute__((address_space(3))) char*)p;
 }
@@ -426,20 +434,29 @@ __device__ __forceinline__ bool dkv_share(const AttnParams& p, int row, int rank
 }
 
 // The same with a window.  A tile of keys is seen by the rows up to window - 1 behind its last key; one
-// that holds sinks (its first ceil(sinks / 128) of them) by all rows behind it.  Those have up to
-// p.sink_splits shares and come first, the others up to p.splits, of p.share_tiles tiles' rows or so.
+// that holds sinks (its first ceil(sinks / 128) of them) by all rows behind it.  Those come first, with up
+// to p.sink_splits shares each, the others as without a window, with up to p.splits, all of p.share_tiles
+// tiles' rows or so.
 __device__ __forceinline__ int window_shares(int tiles, int per, int most) {
   const int n = (tiles + per - 1) / per;
   return n < 1 ? 1 : (n < most ? n : most);
 }
-__device__ __forceinline__ int window_tiles(int window) { return (window - 1) / kDkvKeys + 2; }
+// shares of the last n tiles of a sequence: of the x-th from its end min(x / m, splits - 1) + 1
+__device__ __forceinline__ int tail_shares(int n, int m, int splits) {
+  int sum = 0;
+  for (int q = 0; q < splits; ++q) {
+    const int left = n - q * m;
+    sum += (q + 1) * (left < 0 ? 0 : (left < m || q + 1 == splits ? left : m));
+  }
+  return sum;
+}
 
 struct WindowShare : DkvShare {
   int seq;
   bool sink;
 };
 __device__ __forceinline__ bool dkv_window_share(const AttnParams& p, int row, int rank, int per, WindowShare& it) {
-  const int sinks = (int)((p.sinks + kDkvKeys - 1ll) / kDkvKeys), reach = window_tiles(p.window);
+  const int sinks = (int)((p.sinks + kDkvKeys - 1ll) / kDkvKeys);
   int len, tile, share = 0, shares = 1;
   long long start;
   if (p.splits == 1 && p.sink_splits == 1) {
@@ -451,19 +468,21 @@ __device__ __forceinline__ bool dkv_window_share(const AttnParams& p, int row, i
     if (p.cu) packed_span(p.cu, p.N, p.T, first, n);
     const int nt = (n + kDkvKeys - 1) / kDkvKeys, ns = nt < sinks ? nt : sinks;
     const int a = window_shares(nt, p.share_tiles, p.sink_splits);
-    const int b = window_shares(nt < reach ? nt : reach, p.share_tiles, p.splits);
-    const int end = wave_scan(ns * a + (nt - ns) * b);
+    const int end = wave_scan(ns * a + tail_shares(nt - ns, p.share_tiles, p.splits));
     const unsigned long long past = __ballot(end > rank);
     if (!past) return false;
     const int s = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
     const int nsinks = __builtin_amdgcn_readlane(ns, s), na = __builtin_amdgcn_readlane(a, s);
-    const int nb = __builtin_amdgcn_readlane(b, s);
     int x = rank - (s > 0 ? __builtin_amdgcn_readlane(end, s - 1) : 0);
     if (x < nsinks * na) {
       tile = x / na, share = x % na, shares = na;
     } else {
-      x -= nsinks * na;
-      tile = nsinks + x / nb, share = x % nb, shares = nb;
+      x = __builtin_amdgcn_readlane(end, s) - 1 - rank;  // from the sequence's last tile on
+      int q = 0;
+      while (q + 1 < p.splits && x >= (q + 1) * p.share_tiles) x -= ++q * p.share_tiles;
+      shares = q + 1;
+      tile = __builtin_amdgcn_readlane(nt, s) - 1 - (q * p.share_tiles + x / shares);
+      share = x % shares;
     }
     start = (p.cu ? 0 : (long long)row * p.T) + __builtin_amdgcn_readlane(first, s);
     len = __builtin_amdgcn_readlane(n, s);

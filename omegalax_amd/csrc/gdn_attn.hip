@@ -191,17 +191,23 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   constexpr int NR = DP / 64, kRows8 = 4096 / DP;  // rows of the workgroup's j-th load: kRows8 j ..
   struct Raw { u32x4 x[NR]; int e[NR]; };
   const int row8 = tid / (DP / 16), seg8 = tid % (DP / 16);
+  // (the wavefront's group of the j-th, by selects: an index into the pages would put them into memory)
+  auto mine8 = [&](const long long (&x)[4], int j) {
+    const long long a = x[0], b = x[1], c = x[2], d = x[3];
+    if constexpr (DP == 256) return j == 0 ? a : (j == 1 ? b : (j == 2 ? c : d));
+    const long long even = w & 2 ? b : a, odd = w & 2 ? d : c;
+    if constexpr (DP == 128) return j == 0 ? even : odd;
+    return w == 0 ? a : (w == 1 ? b : (w == 2 ? c : d));
+  };
   auto load8 = [&](const Pages& x, const void* pool, const int8_t* exps) {
     Raw r;
-    const int wrow = __builtin_amdgcn_readfirstlane(row8);
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
-      const int g = (kRows8 * j + wrow) / 16;
-      const bool there = (x.fetch >> g) & 1;
+      const bool there = (x.fetch >> (DP == 256 ? j : (DP == 128 ? 2 * j + w / 2 : w))) & 1;
       r.x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-          buf_rsrc((const char*)pool + x.at[g], there ? 15u * row_bytes + DP : 0u),
+          uniform_rsrc((const char*)pool + mine8(x.at, j), there ? 15u * row_bytes + DP : 0u),
           ((kRows8 * j + row8) & 15) * row_bytes + 16 * seg8, 0, 0));
-      r.e[j] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(buf_rsrc(exps + x.exp[g], there ? 1u : 0u), 0, 0, 0);
+      r.e[j] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(exps + mine8(x.exp, j), there ? 1u : 0u), 0, 0, 0);
     }
     return r;
   };

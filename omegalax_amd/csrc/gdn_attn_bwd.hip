@@ -322,37 +322,47 @@ DkvPlan attn_dkv_plan(long long units, long long T, long long N, int G, long lon
   return plan;
 }
 
-// With a window most tiles are seen by as many rows, and those with sinks by all behind them: their
-// shares are as long as the others'.  Partial sums take 768 MiB at most.
+// The same with a window, where a tile is seen by the rows of `reach` tiles at most, and one with sinks by
+// all behind it.  Partial sums take 768 MiB at most.
 DkvPlan attn_dkv_window_plan(long long B, long long T, long long N, int Hkv, int G, int D, int window, int sinks) {
   DkvPlan plan{1, 1, 1};
   const long long seqs = N > 0 ? N : B;
   if (N > 64 || T == 0 || seqs == 0) return plan;
-  const long long longest = (T + kDkvKeys - 1) / kDkvKeys, avg = N > 0 ? (T / N + kDkvKeys - 1) / kDkvKeys : longest;
-  const long long nt = avg < 1 ? 1 : avg, sink = (sinks + 127ll) / 128, ns = nt < sink ? nt : sink;
-  long long reach = (window - 1) / kDkvKeys + 2;
-  const long long most = longest < reach ? longest : reach;  // tiles' rows that see a tile without sinks
-  reach = nt < reach ? nt : reach;
-  const long long row = (long long)Hkv * D * 8, room = (512ll << 20) / (B * T * row);
-  const long long sink_room = sink > 0 ? (256ll << 20) / (seqs * attn_sink_keys(sinks) * row) : 1;
+  const long long longest = (T + kDkvKeys - 1) / kDkvKeys;
+  long long nt = ((N > 0 ? T / N : T) + kDkvKeys - 1) / kDkvKeys;  // of sequences of equal length
+  nt = nt < 1 ? 1 : nt;
+  const long long sink = attn_sink_keys(sinks) / kDkvKeys, ns = nt < sink ? nt : sink;
+  const long long reach = (window - 1) / kDkvKeys + 2, most = longest < reach ? longest : reach;
+  const long long row = (long long)Hkv * D * 8;
+  long long room = (512ll << 20) / (B * T * row), sink_room = sink > 0 ? (256ll << 20) / (seqs * attn_sink_keys(sinks) * row) : 1;
+  room = room < 1 ? 1 : (room < 16 ? room : 16);
+  sink_room = sink_room < 1 ? 1 : (sink_room < 255 ? sink_room : 255);
   const long long units = (long long)Hkv * seqs;
   const double tile = 4. * G;
   double best = 0;
-  for (long long s = 1; s <= 16 && s <= most && (s == 1 || s <= room); ++s) {
-    const long long m = (most + s - 1) / s;
-    long long a = (longest + m - 1) / m, b = (reach + m - 1) / m;
+  for (long long s = 1; s <= room && s <= most; ++s) {
+    const long long m = (most + s - 1) / s, b = (most + m - 1) / m;
+    long long a = (longest + m - 1) / m;
     a = a < sink_room ? a : sink_room;
-    a = ns > 0 ? (a < 255 ? (a < 1 ? 1 : a) : 255) : 1;
-    const long long groups = units * (ns * a + (nt - ns) * b);
-    const double each = tile * ((double)(most + s - 1) / s), far = ns > 0 ? tile * nt / (nt < a ? nt : a) : 0.;
-    const double work = units * tile * (ns * nt + (nt - ns) * reach) / kComputeUnits;
-    const long long rounds = (groups + kComputeUnits - 1) / kComputeUnits;
-    double ends = rounds <= 2 ? rounds * each : work + each / 2;
-    ends = ends > far ? ends : far;
-    const double cost = ends + 16. * rounds + units * ((a > 1 ? ns * a : 0) + (b > 1 ? (nt - ns) * b : 0)) / 20.;
+    // the shares of a sequence, those with partial sums, and the rows of all, in tiles
+    const long long as = (nt + m - 1) / m < a ? (nt + m - 1) / m : a, tail = nt - ns, full = tail < reach ? tail : reach;
+    long long shares = ns * as, parts = as > 1 ? shares : 0;
+    const long long rows = full * (full + 1) / 2 + (tail - full) * reach + ns * (2 * nt - ns + 1) / 2;
+    for (long long q = 0; q < b; ++q) {
+      const long long left = tail - q * m, n = (q + 1) * (left < 0 ? 0 : (left < m || q + 1 == b ? left : m));
+      shares += n;
+      parts += q > 0 ? n : 0;
+    }
+    const long long rounds = (units * shares + kComputeUnits - 1) / kComputeUnits;
+    double each = tile * (nt < reach ? nt : reach) / (double)(nt < reach ? (nt + m - 1) / m : b);
+    const double far = ns > 0 ? tile * nt / as : 0.;
+    each = each > far ? each : far;
+    const double even = units * tile * rows / kComputeUnits;
+    const double ends = rounds <= 2 ? rounds * each : even + each / 2;
+    const double cost = (ends > each ? ends : each) + 16. * rounds + units * parts / 20.;
     if (s == 1 || cost < best) {
       best = cost;
-      plan = DkvPlan{(int)((most + m - 1) / m), (int)m, (int)a};
+      plan = DkvPlan{(int)b, (int)m, (int)(ns > 0 ? a : 1)};
     }
   }
   return plan;

@@ -247,16 +247,16 @@ void attn_decode8_kernel(AttnParams p) {
       id = there ? id : 0;
       const long long at = (((long long)id * p.page + off) * Hkv + hk) * DP;
       const long long block = ((long long)id * (p.page / 16) + off / 16) * Hkv + hk;
-      const auto kr = buf_rsrc((const char*)p.k_pages + at, there ? 15u * ld + DP : 0u);
-      const auto vr = buf_rsrc((const char*)p.v_pages + at, there ? 15u * ld + DP : 0u);
+      const auto kr = uniform_rsrc((const char*)p.k_pages + at, there ? 15u * ld + DP : 0u);
+      const auto vr = uniform_rsrc((const char*)p.v_pages + at, there ? 15u * ld + DP : 0u);
 #pragma unroll
       for (int j = g * (NR / NG); j < (g + 1) * (NR / NG); ++j) {
         const unsigned off = (unsigned)((RJ * j + lrow) & 15) * ld + 16u * (unsigned)seg;
         y.k[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, off, 0, 0));
         y.v[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0));
       }
-      y.ke[g] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(buf_rsrc(p.k_exps + block, there ? 1u : 0u), 0, 0, 0);
-      y.ve[g] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(buf_rsrc(p.v_exps + block, there ? 1u : 0u), 0, 0, 0);
+      y.ke[g] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(p.k_exps + block, there ? 1u : 0u), 0, 0, 0);
+      y.ve[g] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(p.v_exps + block, there ? 1u : 0u), 0, 0, 0);
     }
     return y;
   };
