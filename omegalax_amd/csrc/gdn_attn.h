@@ -86,7 +86,7 @@ __device__ __forceinline__ void store_part(float* row, const f32x16 (&x)[DB], fl
 // A cache in 8 bits: e4m3 numbers, with a power of two for each 16 tokens of a head, kept as its
 // exponent.  Number times power is a bf16 value as it stands (the conversion applies both; verified on
 // MI355X for every code), so whoever reads it goes on as with a cache of bf16.
-__device__ __forceinline__ float exp_scale(int e) { return __uint_as_float((unsigned)((e < -127 ? -127 : e) + 127) << 23); }
+__device__ __forceinline__ float exp_scale(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
 __device__ __forceinline__ u32x2 widen4(uint32_t c, float scale) {
   return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, false)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, true))};
@@ -172,6 +172,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_rsrc(const void* p, un
   const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((unsigned)a);
   const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
   return buf_rsrc((const void*)((unsigned long long)hi << 32 | lo), (unsigned)__builtin_amdgcn_readfirstlane(bytes));
+}
+// zero, as a lane's offset that the compiler takes for one of its own: a value that it knows to be the same for
+// all lanes goes to a scalar register, and is waited for, as soon as it is loaded
+__device__ __forceinline__ unsigned lane_zero() {
+  unsigned z = 0;
+  asm("" : "+v"(z));
+  return z;
 }
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return (unsigned)(unsigned long long)(const __attribute__((address_space(3))) char*)p;

@@ -186,18 +186,21 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
                      lds + 1024u * kNW * j0, at);
     }
   };
-  // Of a cache in 8 bits a thread loads NR segments of 16 numbers and their exponents into registers, a
-  // tile ahead, and puts them into LDS as bf16 once the tile's products are issued.
+  // Of a cache in 8 bits a thread loads NR segments of 16 numbers and their exponents into registers, two
+  // tiles ahead of the values' products and three of the keys', and a tile later puts them into LDS as
+  // bf16, a half segment beside every other product of the values.
   constexpr int NR = DP / 64, kRows8 = 4096 / DP;  // rows of the workgroup's j-th load: kRows8 j ..
   struct Raw { u32x4 x[NR]; int e[NR]; };
   const int row8 = tid / (DP / 16), seg8 = tid % (DP / 16);
   // (the wavefront's group of the j-th, by selects: an index into the pages would put them into memory)
+  const unsigned zero8 = lane_zero();
   auto mine8 = [&](const long long (&x)[4], int j) {
     const long long a = x[0], b = x[1], c = x[2], d = x[3];
     if constexpr (DP == 256) return j == 0 ? a : (j == 1 ? b : (j == 2 ? c : d));
     const long long even = w & 2 ? b : a, odd = w & 2 ? d : c;
     if constexpr (DP == 128) return j == 0 ? even : odd;
-    return w == 0 ? a : (w == 1 ? b : (w == 2 ? c : d));
+    const long long low = w & 1 ? b : a, high = w & 1 ? d : c;
+    return w & 2 ? high : low;
   };
   auto load8 = [&](const Pages& x, const void* pool, const int8_t* exps) {
     Raw r;
@@ -207,22 +210,20 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       r.x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
           uniform_rsrc((const char*)pool + mine8(x.at, j), there ? 15u * row_bytes + DP : 0u),
           ((kRows8 * j + row8) & 15) * row_bytes + 16 * seg8, 0, 0));
-      r.e[j] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(exps + mine8(x.exp, j), there ? 1u : 0u), 0, 0, 0);
+      r.e[j] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(exps + mine8(x.exp, j), there ? 1u : 0u), zero8, 0, 0);
     }
     return r;
   };
-  auto store8 = [&](const Raw& r, bf16_t* dst) {
-#pragma unroll
-    for (int j = 0; j < NR; ++j) {
-      const int row = kRows8 * j + row8;
-      const float scale = exp_scale(r.e[j]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        *(u32x4*)(dst + row * DP + (((2 * seg8 + i) ^ attn_swz<DP>(row)) << 3)) =
-            widen8(r.x[j][2 * i], r.x[j][2 * i + 1], scale);
-    }
+  auto store8 = [&](const Raw& r, bf16_t* dst, int n) {  // the n-th of 2 NR halves
+    const int row = kRows8 * (n / 2) + row8;
+    *(u32x4*)(dst + row * DP + (((2 * seg8 + n % 2) ^ attn_swz<DP>(row)) << 3)) =
+        widen8(r.x[n / 2][2 * (n % 2)], r.x[n / 2][2 * (n % 2) + 1], exp_scale(r.e[n / 2]));
   };
-  Raw rk, rv;  // of the tiles that phase 2 and phase 1 would fetch
+  auto store8_all = [&](const Raw& r, bf16_t* dst) {
+#pragma unroll
+    for (int n = 0; n < 2 * NR; ++n) store8(r, dst, n);
+  };
+  Raw rv, rk;  // values of the next tile, keys of the one after
   auto fetch_k = [&](int kt, const Pages& x, int j) { fetch(kt, x, p.k_pages, p.k, p.k_ld, kld2, koff, sK, NL * j); };
   auto fetch_v = [&](int kt, const Pages& x, int j) { fetch(kt, x, p.v_pages, p.v, p.v_ld, vld2, voff, sV, NL * j); };
 
@@ -232,6 +233,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   //   1: scores of the next tile  | weights and their sum of this one | reads of k, then of v
   //   2: weighted values of this  | maximum of the next one's scores  | reads of v
   Pages pn, pk;  // of the tile whose values come next, and of the one after, whose keys do
+  Pages pl;      // of the third, in 8 bits
   u32x4 f[PF], pb[4];
   float mx = 0.f;
   auto kfrag = [&](const bf16_t* sk, AttnLane ln, int t) { return attn_frag<DP>(sk, ln, 32 * (t & 1), t / 2); };
@@ -303,12 +305,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
         sum[e & 3] += s[b][i];
         if (e & 1) pb[e / 8][e / 2 % 4] = pack_bf16(s[b][i - 1], s[b][i]);
       }
-      if constexpr (EIGHT) {
-        if (t == 0) rv = load8(pn, p.v_pages, p.v_exps);
-        if (t == NG / 2) rk = load8(pk, p.k_pages, p.k_exps);
-      } else if (t % (NG / NF) == 0) {
-        fetch_v(kt + 1, pn, t / (NG / NF));
-      }
+      if (!EIGHT && t % (NG / NF) == 0) fetch_v(kt + 1, pn, t / (NG / NF));
       __builtin_amdgcn_sched_barrier(0);
     }
     lsum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -324,7 +321,15 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
 #pragma unroll
         for (int e = EG * t; e < EG * (t + 1); ++e) mx = fmaxf(mx, sn[e / 16][e % 16]);
       }
-      if (!EIGHT && t % (NG / 2 / NF) == 0 && t < NG / 2) fetch_k(kt + 2, pk, t / (NG / 2 / NF));
+      if constexpr (EIGHT) {
+        static_assert(8 * NR <= NG, "halves of values, then of keys, beside every other product");
+        if (t % 2 == 0 && t / 2 < 2 * NR) store8(rv, sV + ((kt + 1) & 1) * kTile, t / 2);
+        if (t % 2 == 0 && t / 2 >= 2 * NR && t / 2 < 4 * NR) store8(rk, sK + (kt & 1) * kTile, t / 2 - 2 * NR);
+        if (t == 4 * NR) rv = load8(pk, p.v_pages, p.v_exps);
+        if (t == 8 * NR - 1) rk = load8(pl, p.k_pages, p.k_exps);
+      } else if (t % (NG / 2 / NF) == 0 && t < NG / 2) {
+        fetch_k(kt + 2, pk, t / (NG / 2 / NF));
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -341,7 +346,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   unsigned have = 15;
   // tile kt's values and the next one's keys are there
   auto enter = [&](int kt) {
-    wait_loads<0>();  // this wavefront's part of the tiles
+    if constexpr (!EIGHT) wait_loads<0>();  // this wavefront's part of the tiles
     lds_barrier();    // everyone's; and the other buffers are free
     if constexpr (PAGED) {
       const int k0 = key0(kt);
@@ -352,14 +357,15 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     }
   };
   auto leave = [&](int kt) {
-    if constexpr (EIGHT) {
-      store8(rv, sV + ((kt + 1) & 1) * kTile);
-      store8(rk, sK + (kt & 1) * kTile);
-    }
     if constexpr (PAGED) {
       have = pn.have;
       pn = pk;
-      pk = look(kt + 3);
+      if constexpr (EIGHT) {
+        pk = pl;
+        pl = look(kt + 4);
+      } else {
+        pk = look(kt + 3);
+      }
     }
   };
   if (kt0 < kt1) {
@@ -374,12 +380,14 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       have = p0.have;
     }
     if constexpr (EIGHT) {
-      const Raw first = load8(p0, p.k_pages, p.k_exps);
-      rv = load8(p0, p.v_pages, p.v_exps);
-      rk = load8(pn, p.k_pages, p.k_exps);
-      store8(first, sK + (kt0 & 1) * kTile);
-      store8(rv, sV + (kt0 & 1) * kTile);
-      store8(rk, sK + ((kt0 + 1) & 1) * kTile);
+      pl = look(kt0 + 3);
+      const Raw k0 = load8(p0, p.k_pages, p.k_exps), v0 = load8(p0, p.v_pages, p.v_exps);
+      const Raw k1 = load8(pn, p.k_pages, p.k_exps);
+      rv = load8(pn, p.v_pages, p.v_exps);
+      rk = load8(pk, p.k_pages, p.k_exps);
+      store8_all(k0, sK + (kt0 & 1) * kTile);
+      store8_all(v0, sV + (kt0 & 1) * kTile);
+      store8_all(k1, sK + ((kt0 + 1) & 1) * kTile);
     } else {
 #pragma unroll
       for (int j = 0; j < NF; ++j) {
@@ -387,8 +395,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
         fetch_v(kt0, p0, j);
         fetch_k(kt0 + 1, pn, j);
       }
+      wait_loads<0>();
     }
-    wait_loads<0>();
     lds_barrier();
     // the wavefront's own last tile: rows of it see no keys of later ones
     const int w_kt = w_hi / kBN - skip, last_kt = w_kt < kt1 - 1 ? w_kt : kt1 - 1;
@@ -419,8 +427,10 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     for (; kt < kt1; ++kt) {  // other wavefronts' tiles: its part of the loads
       enter(kt);
       if constexpr (EIGHT) {
-        rv = load8(pn, p.v_pages, p.v_exps);
-        rk = load8(pk, p.k_pages, p.k_exps);
+        store8_all(rv, sV + ((kt + 1) & 1) * kTile);
+        store8_all(rk, sK + (kt & 1) * kTile);
+        rv = load8(pk, p.v_pages, p.v_exps);
+        rk = load8(pl, p.k_pages, p.k_exps);
       } else {
 #pragma unroll
         for (int j = 0; j < NF; ++j) {

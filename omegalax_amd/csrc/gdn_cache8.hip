@@ -195,6 +195,7 @@ void attn_decode8_kernel(AttnParams p) {
   const int cap = p.table_w * p.page;
   const int lrow = l / LR, seg = l % LR;
   bf16_t *sk = sK[w], *sv = sV[w];
+  const unsigned zero = lane_zero();
 
   int b = wg, st0 = 0, x = 0, x1 = INT_MAX;
   if (p.splits > 1 && !decode_range<WIN>(p, wg, cap, SK, b, st0, x, x1)) return;
@@ -255,8 +256,8 @@ void attn_decode8_kernel(AttnParams p) {
         y.k[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, off, 0, 0));
         y.v[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0));
       }
-      y.ke[g] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(p.k_exps + block, there ? 1u : 0u), 0, 0, 0);
-      y.ve[g] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(p.v_exps + block, there ? 1u : 0u), 0, 0, 0);
+      y.ke[g] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(p.k_exps + block, there ? 1u : 0u), zero, 0, 0);
+      y.ve[g] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(p.v_exps + block, there ? 1u : 0u), zero, 0, 0);
     }
     return y;
   };
