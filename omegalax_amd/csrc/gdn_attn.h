@@ -204,6 +204,28 @@ __device__ __forceinline__ void loads_to_lds16(u32x4 rsrc, unsigned lds, const u
 __device__ __forceinline__ void loads_to_lds16(u32x4 rsrc, unsigned lds, const unsigned (&off)[1]) {
   load_to_lds16(rsrc, lds, off[0]);
 }
+// N of them, each 1 KiB further in LDS: one wavefront
+__device__ __forceinline__ void loads_to_lds16_on(u32x4 rsrc, unsigned lds, const unsigned (&off)[4]) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
+               "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %5, 0 offen lds\n\t"
+               "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %5, 0 offen lds\n\t"
+               "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %5, 0 offen lds"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]),
+                  "s"(rsrc) : "memory", "m0", "scc");
+}
+__device__ __forceinline__ void loads_to_lds16_on(u32x4 rsrc, unsigned lds, const unsigned (&off)[2]) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+               "s_add_u32 m0, m0, 1024\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off[0]), "v"(off[1]), "s"(rsrc) : "memory", "m0", "scc");
+}
+__device__ __forceinline__ void loads_to_lds16_on(u32x4 rsrc, unsigned lds, const unsigned (&off)[1]) {
+  load_to_lds16(rsrc, lds, off[0]);
+}
+// a byte a lane, into the low byte of 4 at `lds` + 4 lane
+__device__ __forceinline__ void load_to_lds1(u32x4 rsrc, unsigned lds, unsigned off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_ubyte %1, %2, 0 offen lds"
+               :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory", "m0");
+}
 __device__ __forceinline__ void load_to_lds4(u32x4 rsrc, unsigned lds, unsigned off) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc) : "memory", "m0");

@@ -174,6 +174,14 @@ int64_t seen_keys(const Sight& x, int64_t keys, int64_t rows) {
   const int64_t n = x.window + x.sinks + rows + 128;
   return n < keys ? n : keys;
 }
+// a key's page by a product, for keys of 31 bits: with 2^(l-1) < page <= 2^l the multiplier, rounded up, is off by
+// less than 2^l in 2^(31+l), too little to carry a quotient's fraction over
+void divide_by_page(omx::AttnParams& p, int64_t page) {
+  int l = 0;
+  while (((int64_t)1 << l) < page) ++l;
+  p.page_mul = (unsigned)((((uint64_t)1 << (31 + l)) + page - 1) / page);
+  p.page_shift = (unsigned)(l - 1);
+}
 // the exponents of a cache in 8 bits: both or neither
 int check_exps(const char* fn, const int8_t* k_exps, const int8_t* v_exps) {
   REQUIRE(!k_exps == !v_exps, "%s: k_exps and v_exps go together", fn);
@@ -559,6 +567,7 @@ int attn_decode(const char* fn, const void* q, const void* k, const void* v, int
   p.q_ld = q_ld; p.k_ld = k_ld; p.v_ld = v_ld;
   p.k_exps = k_exps; p.v_exps = v_exps;
   look_at(p, sight, table_width * page_size + 1);
+  divide_by_page(p, page_size);
   p.k_pages = k_pages; p.v_pages = v_pages; p.table = block_table; p.held = lengths;
   p.table_w = (int)table_width; p.page = (int)page_size; p.n_pages = (int)n_pages;
   p.splits = splits;

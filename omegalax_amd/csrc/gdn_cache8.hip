@@ -64,6 +64,13 @@ __device__ __forceinline__ float most16(u32x4 a, u32x4 b) {
     }
   return m;
 }
+// Transposed read of 8-bit elements: lanes 2i and 2i + 1 of 16 give the addresses of the two halves of row
+// i's 16 columns, and lane j gets column j of the 8 rows (verified on MI355X).
+__device__ __forceinline__ u32x2 ds_read_tr8(const uint8_t* p) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+      (__attribute__((address_space(3))) i32x2*)(unsigned long long)(const __attribute__((address_space(3))) uint8_t*)p));
+}
 // 2^(a - b) of exponents a <= b
 __device__ __forceinline__ float exp_shift(int a, int b) { return a - b < -126 ? 0.f : exp_scale(a - b); }
 
@@ -177,16 +184,37 @@ __global__ __launch_bounds__(256) void kv_write8_kernel(AttnParams p, int span) 
 }
 
 // ------------------------------------------------------------------------------------ decode
-// As for the cache of bf16 (gdn_paged.hip), whose products these are; a stage goes through registers, two
-// stages ahead, and is put into LDS as bf16.  The wavefront whose stage holds the new token's block writes it.
+// As for the cache of bf16 (gdn_paged.hip): equal ranges of all sequences' stages, a wavefront's stages in
+// turns, read once for all query heads of a key head.  A stage's numbers go from memory to LDS as they
+// are, two stages deep (128 KiB in flight a compute unit), and become bf16 on the way from there into a
+// product, each once: keys by rows of 8, values by transposed reads of 8 keys, the 8 that a lane's weights
+// of two blocks stand for.  The wavefront whose stage holds the new token's block puts the token into it,
+// there and in the cache.
+template <int DP> constexpr int kStage8 = 8192 / DP;  // keys: 8 KiB of K, 8 of V
+
+// Place of 16-byte segment s of row r: s ^ swz8(r).  Reads of 16 rows' 8 bytes at one column, and transposed
+// ones of 8 rows at two neighbouring, rows 4a .. and 16 + 4a .., then fall into different banks.
+template <int DP>
+__device__ __forceinline__ int swz8(int r) {
+  if constexpr (DP == 256) return (r ^ (((r >> 4) & 1) << 2)) & 15;
+  if constexpr (DP == 128) return ((r >> 1) & 7) ^ (((r >> 4) & 1) << 1);
+  return ((r >> 2) & 3) ^ ((r >> 4) & 1);
+}
+
+// wavefronts of a workgroup: two a SIMD where their registers allow it
+template <int NQ> constexpr int kDec8NW = NQ == 1 ? 8 : 4;
+
 template <int DP, int NQ, bool WIN>
-__global__ __launch_bounds__(64 * kDecNW) __attribute__((amdgpu_waves_per_eu(1)))
+__global__ __launch_bounds__(64 * kDec8NW<NQ>) __attribute__((amdgpu_waves_per_eu(kDec8NW<NQ> / 4)))
 void attn_decode8_kernel(AttnParams p) {
-  constexpr int SK = kStageKeys<DP>, NG = SK / 16;  // keys of a stage, its blocks
+  constexpr int SK = kStage8<DP>, NG = SK / 16, NC = SK / 32;  // keys of a stage, its blocks, pairs of them
   constexpr int KS = DP / 32, DB = DP / 16;
-  constexpr int NR = 4, RJ = 1024 / DP, LR = DP / 16;  // loads of K (and of V), their rows, a row's lanes
-  __shared__ __align__(16) bf16_t sK[kDecNW][SK * DP], sV[kDecNW][SK * DP];
-  __shared__ float sM[kDecNW][16 * NQ], sL[kDecNW][16 * NQ];
+  constexpr int NI = DP / 64, RI = 1024 / DP, LR = DP / 16;     // loads of a block, their rows, a row's lanes
+  constexpr int kV = SK * DP, kE = 2 * kV, kSlot = kE + 512;    // a slot: K, V, their exponents (4 bytes each)
+  constexpr int kLoads = NG * NI + 1;                           // of K, and of V
+  constexpr int NW = kDec8NW<NQ>;
+  __shared__ __align__(16) uint8_t slots[NW][kSlot];
+  __shared__ float sM[NW][16 * NQ], sL[NW][16 * NQ];
 
   const int tid = threadIdx.x, l = tid & 63, g4 = l >> 4, r = l & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -194,8 +222,14 @@ void attn_decode8_kernel(AttnParams p) {
   const int hk = (int)blockIdx.x % Hkv, wg = (int)blockIdx.x / Hkv;
   const int cap = p.table_w * p.page;
   const int lrow = l / LR, seg = l % LR;
-  bf16_t *sk = sK[w], *sv = sV[w];
-  const unsigned zero = lane_zero();
+  const unsigned ld = (unsigned)(Hkv * DP);
+  // a lane's offsets in a block's loads; the swizzle tells even blocks from odd ones
+  unsigned off[2][NI];
+#pragma unroll
+  for (int i = 0; i < 2 * NI; ++i) {
+    const int row = RI * (i % NI) + lrow;
+    off[i / NI][i % NI] = (unsigned)row * ld + 16u * (unsigned)(seg ^ swz8<DP>(16 * (i / NI) + row));
+  }
 
   int b = wg, st0 = 0, x = 0, x1 = INT_MAX;
   if (p.splits > 1 && !decode_range<WIN>(p, wg, cap, SK, b, st0, x, x1)) return;
@@ -228,171 +262,201 @@ void attn_decode8_kernel(AttnParams p) {
   }
   const float cs = p.scale * kLog2e;
 
-  // a stage's codes and exponents, and which of its blocks are there
-  struct Raw {
-    u32x4 k[NR], v[NR];
-    int ke[NG], ve[NG];
-    unsigned have;
-  };
-  auto load = [&](int st) {
-    Raw y;
+  // blocks of a stage: their number in the cache, none from st1 on
+  struct Ids { unsigned at[NG], have; };
+  auto look = [&](int st) __attribute__((always_inline)) {
+    Ids y;
     y.have = 0;
-    const unsigned ld = (unsigned)(Hkv * DP);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const int key = seen.at(st) * SK + 16 * g;
-      const int slot = key / p.page, off = key - slot * p.page;
-      int id = st < st1 && key < keys ? table[slot] : -1;  // key < keys <= cap: the slot is in the table
+      const int key = (WIN ? seen.at(st) : st) * SK + 16 * g;
+      const int slot = (int)(__umulhi((unsigned)key, p.page_mul) >> p.page_shift), off = key - slot * p.page;
+      const int id = st < st1 && key < keys ? table[slot] : -1;  // key < keys <= cap: the slot is in the table
       const bool there = id >= 0 && id < p.n_pages;
       y.have |= there ? 1u << g : 0u;
-      id = there ? id : 0;
-      const long long at = (((long long)id * p.page + off) * Hkv + hk) * DP;
-      const long long block = ((long long)id * (p.page / 16) + off / 16) * Hkv + hk;
-      const auto kr = uniform_rsrc((const char*)p.k_pages + at, there ? 15u * ld + DP : 0u);
-      const auto vr = uniform_rsrc((const char*)p.v_pages + at, there ? 15u * ld + DP : 0u);
-#pragma unroll
-      for (int j = g * (NR / NG); j < (g + 1) * (NR / NG); ++j) {
-        const unsigned off = (unsigned)((RJ * j + lrow) & 15) * ld + 16u * (unsigned)seg;
-        y.k[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, off, 0, 0));
-        y.v[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vr, off, 0, 0));
-      }
-      y.ke[g] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(p.k_exps + block, there ? 1u : 0u), zero, 0, 0);
-      y.ve[g] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(p.v_exps + block, there ? 1u : 0u), zero, 0, 0);
+      y.at[g] = there ? (unsigned)id * (unsigned)(p.page / 16) + (unsigned)(off / 16) : 0u;
     }
     return y;
   };
+  // Fetches a stage's keys (or values); what is not there has an empty range and reads as zeros, so that
+  // every stage counts the same loads.
+  uint8_t* const slot = slots[w];
+  const unsigned lds = lds_address(slot);
+  auto stage = [&](const Ids& y, const void* pages, const int8_t* exps, unsigned to,
+                   unsigned to_exps) __attribute__((always_inline)) {
+    unsigned eo = kDropOffset;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const bool there = (y.have >> g) & 1;
+      const long long at = ((long long)y.at[g] * 16 * Hkv + hk) * DP;
+      loads_to_lds16_on(rsrc_words((const char*)pages + at, there ? 15u * ld + DP : 0u), lds + to + 1024u * NI * g, off[g & 1]);
+      if (there && l == g) eo = y.at[g] * (unsigned)Hkv + (unsigned)hk;
+    }
+    load_to_lds1(rsrc_words(exps, kDropOffset), lds + to_exps, eo);
+  };
+  auto stage_k = [&](const Ids& y) __attribute__((always_inline)) { stage(y, p.k_pages, p.k_exps, 0, kE); };
+  auto stage_v = [&](const Ids& y) __attribute__((always_inline)) { stage(y, p.v_pages, p.v_exps, kV, kE + 256); };
   // the new token's codes into the stage that holds its block, and into the cache
-  auto amend = [&](int key0, u32x4 (&c)[NR], int (&e)[NG], const bf16_t* src, void* pages, int8_t* exps) {
+  auto amend = [&](int key0, uint8_t* codes, uint8_t* ex, const bf16_t* src, void* pages,
+                   int8_t* exps) __attribute__((always_inline)) {
     const u32x4 a = *(const u32x4*)(src + hk * DP + 16 * seg), a2 = *(const u32x4*)(src + hk * DP + 16 * seg + 8);
     float most = most16(a, a2);
 #pragma unroll
     for (int i = 1; i < LR; i <<= 1) most = fmaxf(most, __shfl_xor(most, i, 64));
     const int gb = (held - key0) / 16, r0 = held % 16;
     const int slot = held / p.page, off = held - slot * p.page - r0;
-    const long long at = (((long long)table[slot] * p.page + off) * Hkv + hk) * DP;
-    const long long block = ((long long)table[slot] * (p.page / 16) + off / 16) * Hkv + hk;
-    int before = kLeastExp;
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-      if (g == gb && r0 > 0) before = e[g];
+    const long long block = (long long)table[slot] * (p.page / 16) + off / 16;
+    const int before = r0 > 0 ? (int)(int8_t)ex[4 * gb] : kLeastExp;
     const int ask = asked_exp(most), now = ask > before ? ask : before;
     const float shift = exp_shift(before, now);
     const u32x4 mine = code16(a, a2, exp_scale(-now));
 #pragma unroll
-    for (int j = 0; j < NR; ++j) {
-      const int row = RJ * j + lrow, r1 = row & 15;
-      if (row / 16 != gb || r1 > r0) continue;
-      if (r1 == r0) c[j] = mine;
-      else if (now > before) c[j] = again16(c[j], shift);
-      if (r1 == r0 || now > before) *(u32x4*)((uint8_t*)pages + at + (long long)r1 * Hkv * DP + 16 * seg) = c[j];
+    for (int j = 0; j < NI; ++j) {
+      const int row = RI * j + lrow;
+      if (row > r0 || (row < r0 && now <= before)) continue;
+      u32x4* c = (u32x4*)(codes + (16 * gb + row) * DP + ((seg ^ swz8<DP>(16 * gb + row)) << 4));
+      *c = row == r0 ? mine : again16(*c, shift);
+      *(u32x4*)((uint8_t*)pages + (block * 16 * Hkv + hk) * DP + (long long)row * Hkv * DP + 16 * seg) = *c;
     }
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-      if (g == gb) e[g] = now;
-    if (l == 0) exps[block] = (int8_t)now;
+    if (l == 0) {
+      exps[block * Hkv + hk] = (int8_t)now;
+      ex[4 * gb] = (uint8_t)now;
+    }
   };
-  auto compute = [&](int st, Raw& y) {
-    const int key0 = seen.at(st) * SK;
-    constexpr unsigned kAll = (1u << NG) - 1;
-    const unsigned have = y.have;
-    const bool whole = have == kAll && key0 + SK < keys &&  // every row a held key, and seen
-                       !(WIN && key0 < seen.lo && key0 + SK > p.sinks);
-    if (!whole) {
-      const int row = held - key0;
-      if (row >= 0 && row < SK && held < cap && ((have >> (row / 16)) & 1)) {
-        amend(key0, y.k, y.ke, (const bf16_t*)p.k + b * p.k_ld, p.k_pages, p.k_exps);
-        amend(key0, y.v, y.ve, (const bf16_t*)p.v + b * p.v_ld, p.v_pages, p.v_exps);
+  uint8_t *const sk = slot, *const sv = slot + kV;
+  // lane 2i + j of 16 reads 8 of the 16 columns of row 4 g4 + i (16 more from i = 4 on)
+  const int vrow = 4 * g4 + ((r >> 1) & 3) + 16 * (r >> 3);
+  // A wavefront's stages, st0 + w and then every NW-th.  The next one's keys are fetched once this one's
+  // scores are formed, its values once theirs are added up.
+  {
+    int st = st0 + w;
+    Ids y = look(st), next;
+    // the queries are there before the compiler, which does not count the loads below, waits for them
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[n][s]));
+    stage_k(y);
+    stage_v(y);
+    for (; st < st1; st += NW, y = next) {
+      next = look(st + NW);
+      const unsigned have = y.have;
+      const int key0 = (WIN ? seen.at(st) : st) * SK;
+      constexpr unsigned kAll = (1u << NG) - 1;
+      const bool whole = have == kAll && key0 + SK < keys &&  // every row a held key, and seen
+                         !(WIN && key0 < seen.lo && key0 + SK > p.sinks);
+      const int nrow = held - key0;  // the new token's
+      const bool mine = nrow >= 0 && nrow < SK && held < cap && ((have >> (nrow / 16)) & 1);
+
+      asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kLoads) : "memory");  // the keys: all but the values
+      if (mine) {
+        amend(key0, sk, slot + kE, (const bf16_t*)p.k + b * p.k_ld, p.k_pages, p.k_exps);
+        wave_lds_fence();
       }
-    }
-#pragma unroll
-    for (int j = 0; j < NR; ++j) {
-      const int row = RJ * j + lrow, g = RJ * j / 16;
-      const float ks = exp_scale(y.ke[g]), vs = exp_scale(y.ve[g]);
-      const int key = key0 + row;
-      // rows without a key, or not seen, are cleared: a weight of zero does not clear a NaN
-      const bool no = !whole && (key >= keys || !((have >> g) & 1) || (WIN && key < seen.lo && key >= p.sinks));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int to = row * DP + (((2 * seg + i) ^ attn_swz<DP>(row)) << 3);
-        *(u32x4*)(sk + to) = widen8(y.k[j][2 * i], y.k[j][2 * i + 1], ks);
-        *(u32x4*)(sv + to) = no ? u32x4{0, 0, 0, 0} : widen8(y.v[j][2 * i], y.v[j][2 * i + 1], vs);
-      }
-    }
-    wave_lds_fence();
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      f32x4 s[NG];
+      const int ke = (int)(int8_t)slot[kE + 4 * (l & (NG - 1))];
+      f32x4 s[NQ][NG];
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        s[g] = zero4();
+        const float scale = exp_scale(__builtin_amdgcn_readlane(ke, g));
+        const uint8_t* row = sk + (16 * g + r) * DP;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[n][g] = zero4();
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          const u32x4 a = *(const u32x4*)(sk + (16 * g + r) * DP + (((4 * k + g4) ^ attn_swz<DP>(r)) << 3));
-          s[g] = mma16(a, q[n][k], s[g]);
+          const u32x2 c = *(const u32x2*)(row + (((2 * k + (g4 >> 1)) ^ swz8<DP>(16 * (g & 1) + r)) << 4) + 8 * (g4 & 1));
+          const u32x4 a = widen8(c[0], c[1], scale);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) s[n][g] = mma16(a, q[n][k], s[n][g]);
         }
       }
-      float mx = -INFINITY;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads are done
+      stage_k(next);
+
+      u32x4 pb[NQ][NC], pr[NQ][NC];
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
+      for (int n = 0; n < NQ; ++n) {
+        if (!whole) {
+          // (as selects: of conditions that are evaluated in turn the compiler made branches, and lost one)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = key0 + 16 * g + 4 * g4 + i;
-          if (!whole && (key >= keys || !((have >> g) & 1) || (WIN && key < seen.lo && key >= p.sinks))) s[g][i] = -INFINITY;
-          mx = fmaxf(mx, s[g][i]);
+          for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = key0 + 16 * g + 4 * g4 + i;
+              const bool no = (key >= keys) | !((have >> g) & 1) | (WIN & (key < seen.lo) & (key >= p.sinks));
+              s[n][g][i] = no ? -INFINITY : s[n][g][i];
+            }
         }
-      if (__any((mx - m[n]) * cs > 8.f)) {
-        // the row's maximum over the four lanes that share it
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mn = fmaxf(m[n], mx);
-        const float a = __builtin_amdgcn_exp2f((m[n] - mn) * cs);
-        m[n] = mn;
-        ls[n] *= a;
+        float mx = -INFINITY;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[n][d][i] *= a;
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[n][g][i]);
+        if (__any((mx - m[n]) * cs > 8.f)) {
+          // the row's maximum over the four lanes that share it
+          mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+          const float mn = fmaxf(m[n], mx);
+          const float a = __builtin_amdgcn_exp2f((m[n] - mn) * cs);
+          m[n] = mn;
+          ls[n] *= a;
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][d][i] *= a;
+        }
+        const float mc = m[n] * cs;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[n][g][i] = __builtin_amdgcn_exp2f(fmaf(s[n][g][i], cs, -mc));
+            ls[n] += s[n][g][i];
+          }
+          // the weights as two bf16 terms (off by at most 2^-16 together)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float u = s[n][g][2 * i], v = s[n][g][2 * i + 1];
+            pb[n][g / 2][2 * (g & 1) + i] = pack_bf16(u, v);
+            pr[n][g / 2][2 * (g & 1) + i] = pack_bf16(lo_part(u), lo_part(v));
+          }
+        }
       }
-      const float mc = m[n] * cs;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], cs, -mc));
-          ls[n] += s[g][i];
+
+      asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kLoads) : "memory");  // the values: all but the next keys
+      if (!whole) {
+        if (mine) amend(key0, sv, slot + kE + 256, (const bf16_t*)p.v + b * p.v_ld, p.v_pages, p.v_exps);
+        // rows without a key, or not seen, are cleared: a weight of zero does not clear a NaN
+        for (int i = l; i < SK * LR; i += 64) {
+          const int row = i / LR, key = key0 + row;
+          if (key >= keys || !((have >> (row / 16)) & 1) || (WIN && key < seen.lo && key >= p.sinks))
+            *(u32x4*)(sv + 16 * i) = u32x4{0, 0, 0, 0};
         }
-        // the weights as two bf16 terms (off by at most 2^-16 together)
-        const u32x2 pb = u32x2{pack_bf16(s[g][0], s[g][1]), pack_bf16(s[g][2], s[g][3])};
-        const u32x2 pr = u32x2{pack_bf16(lo_part(s[g][0]), lo_part(s[g][1])), pack_bf16(lo_part(s[g][2]), lo_part(s[g][3]))};
-        const int vr = 16 * g + 4 * g4 + (r >> 2);
+        wave_lds_fence();
+      }
+      const int ve = (int)(int8_t)slot[kE + 256 + 4 * (l & (NG - 1))];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const float s0 = exp_scale(__builtin_amdgcn_readlane(ve, 2 * c)), s1 = exp_scale(__builtin_amdgcn_readlane(ve, 2 * c + 1));
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          const int col = 16 * d + 4 * (r & 3);
-          const u32x2 a = ds_read_tr(sv + vr * DP + (((col >> 3) ^ attn_swz<DP>(vr)) << 3) + (col & 7));
-          o[n][d] = mma_pv(a, pb, o[n][d]);
-          o[n][d] = mma_pv(a, pr, o[n][d]);
+          const u32x2 v = ds_read_tr8(sv + (32 * c + vrow) * DP + ((d ^ swz8<DP>(vrow)) << 4) + 8 * (r & 1));
+          const u32x2 lo = widen4(v[0], s0), hi = widen4(v[1], s1);
+          const u32x4 a = u32x4{lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            o[n][d] = mma16(a, pb[n][c], o[n][d]);
+            o[n][d] = mma16(a, pr[n][c], o[n][d]);
+          }
         }
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads are done
+      stage_v(next);
     }
-    // the buffers are free for the next stage once these reads are done
-    __builtin_amdgcn_s_waitcnt(0xc07f);
-    __builtin_amdgcn_wave_barrier();
-  };
-
-  {
-    int st = st0 + w;  // this wavefront's stages: st0 + w, then every fourth
-    Raw y0 = load(st), y1 = load(st + kDecNW);
-    for (; st < st1; st += 2 * kDecNW) {
-      compute(st, y0);
-      y0 = load(st + 2 * kDecNW);
-      if (st + kDecNW >= st1) break;
-      compute(st + kDecNW, y1);
-      y1 = load(st + 3 * kDecNW);
-    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is on its way into LDS
   }
 
-  // ---------------------------------------------------------------- the four wavefronts' sums
-  // buffers of K and V, 16 KiB a wavefront together, hold 16 rows of DP fp32
+  // ---------------------------------------------------------------- the wavefronts' sums
+  // a wavefront's slot holds 16 rows of DP fp32
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     ls[n] += __shfl_xor(ls[n], 16, 64);
@@ -405,28 +469,23 @@ void attn_decode8_kernel(AttnParams p) {
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    // rows of DP fp32: row r in the first half of the columns in K's buffer, the rest in V's
 #pragma unroll
-    for (int d = 0; d < DB; ++d) {
-      float* dst = (float*)(d < DB / 2 ? sk : sv);
-      *(f32x4*)(dst + r * (DP / 2) + 16 * (d % (DB / 2)) + 4 * g4) = o[n][d];
-    }
+    for (int d = 0; d < DB; ++d) *(f32x4*)((float*)slot + r * DP + 16 * d + 4 * g4) = o[n][d];
     __syncthreads();
     const int rows = G - 16 * n < 16 ? G - 16 * n : 16;
-    for (int i = tid; i < rows * DP / 4; i += 64 * kDecNW) {
+    for (int i = tid; i < rows * DP / 4; i += 64 * NW) {
       const int row = i / (DP / 4), col = 4 * (i % (DP / 4));
       float M = sM[0][16 * n + row];
 #pragma unroll
-      for (int u = 1; u < kDecNW; ++u) M = fmaxf(M, sM[u][16 * n + row]);
+      for (int u = 1; u < NW; ++u) M = fmaxf(M, sM[u][16 * n + row]);
       f32x4 acc = zero4();
       float den = 0.f;
 #pragma unroll
-      for (int u = 0; u < kDecNW; ++u) {
+      for (int u = 0; u < NW; ++u) {
         const float lx = sL[u][16 * n + row];
         const float a = lx == 0.f ? 0.f : __builtin_amdgcn_exp2f(sM[u][16 * n + row] - M);
         den += a * lx;
-        const float* src = (const float*)(col < DP / 2 ? sK[u] : sV[u]);
-        acc += a * *(const f32x4*)(src + row * (DP / 2) + (col % (DP / 2)));
+        acc += a * *(const f32x4*)((const float*)slots[u] + row * DP + col);
       }
       const long long at = (long long)b * Hq + hk * G + 16 * n + row;
       if (!alone) {
@@ -455,10 +514,10 @@ template <int DP, bool WIN>
 void decode8_dp(const AttnParams& p, hipStream_t stream) {
   const unsigned grid = (unsigned)((p.splits > 1 ? p.splits : p.N) * p.Hkv);
   if (p.G <= 16)
-    attn_decode8_kernel<DP, 1, WIN><<<grid, 64 * kDecNW, 0, stream>>>(p);
+    attn_decode8_kernel<DP, 1, WIN><<<grid, 64 * kDec8NW<1>, 0, stream>>>(p);
   else
-    attn_decode8_kernel<DP, 2, WIN><<<grid, 64 * kDecNW, 0, stream>>>(p);
-  if (p.splits > 1) launch_decode_join<DP, WIN>(p, stream);
+    attn_decode8_kernel<DP, 2, WIN><<<grid, 64 * kDec8NW<2>, 0, stream>>>(p);
+  if (p.splits > 1) launch_decode_join<DP, WIN, kStage8<DP>>(p, stream);
 }
 template <int DP>
 void decode8_dp(const AttnParams& p, hipStream_t stream) {

@@ -284,6 +284,7 @@ struct AttnParams {
   const int32_t* table;        // [N, table_w]
   const int32_t* held;         // [N]
   int table_w, page, n_pages;
+  unsigned page_mul, page_shift;  // key / page = key page_mul / 2^(32 + page_shift) for 31-bit keys
   int8_t *k_exps, *v_exps;     // of pages of e4m3 numbers: [n_pages, page / 16, Hkv]; null: bf16
   // work split over the keys: partial sums, which a second kernel joins
   int splits;

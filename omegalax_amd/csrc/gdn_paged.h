@@ -80,9 +80,9 @@ __device__ __forceinline__ bool decode_range(const AttnParams& p, int wg, int ca
 
 namespace {
 // Joins a row's segments, with W of a workgroup's four wavefronts on one row.
-template <int DP, int W, bool WIN>
+template <int DP, int W, bool WIN, int SK>
 __global__ __launch_bounds__(256) void decode_join_kernel(AttnParams p) {
-  constexpr int E = DP / 64, SK = kStageKeys<DP>;
+  constexpr int E = DP / 64;
   typedef float fE __attribute__((ext_vector_type(E)));
   __shared__ float sAcc[4][DP];
   const int l = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % W;
@@ -150,15 +150,15 @@ __global__ __launch_bounds__(256) void decode_join_kernel(AttnParams p) {
   for (int e = 0; e < E; ++e) op[e] = f2bf(acc[e] * inv);
 }
 
-template <int DP, bool WIN>
+template <int DP, bool WIN, int SK>
 void launch_decode_join(const AttnParams& p, hipStream_t stream) {
   // a row has at most as many segments as its key head has workgroups; four wavefronts share a row
   // where there are few rows
   const unsigned rows = (unsigned)(p.N * p.Hkv * p.G);
   if (rows <= 512)
-    decode_join_kernel<DP, 4, WIN><<<rows, 256, 0, stream>>>(p);
+    decode_join_kernel<DP, 4, WIN, SK><<<rows, 256, 0, stream>>>(p);
   else
-    decode_join_kernel<DP, 1, WIN><<<(rows + 3) / 4, 256, 0, stream>>>(p);
+    decode_join_kernel<DP, 1, WIN, SK><<<(rows + 3) / 4, 256, 0, stream>>>(p);
 }
 }  // namespace
 

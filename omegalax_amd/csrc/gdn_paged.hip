@@ -352,7 +352,7 @@ void decode_dp(const AttnParams& p, hipStream_t stream) {
     attn_decode_kernel<DP, 1, WIN><<<grid, 64 * kDecNW, 0, stream>>>(p);
   else
     attn_decode_kernel<DP, 2, WIN><<<grid, 64 * kDecNW, 0, stream>>>(p);
-  if (p.splits > 1) launch_decode_join<DP, WIN>(p, stream);
+  if (p.splits > 1) launch_decode_join<DP, WIN, kStageKeys<DP>>(p, stream);
 }
 template <int DP>
 void decode_dp(const AttnParams& p, hipStream_t stream) {
