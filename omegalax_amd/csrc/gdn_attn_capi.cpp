@@ -656,7 +656,7 @@ int omx_gdn_pages_assign(int32_t* block_table, int64_t N, int64_t table_width, c
 
 size_t omx_gdn_pages_release_workspace_size(int64_t N, int64_t table_width) {
   if (N < 0 || N > (1 << 20) || table_width < 0 || table_width > kMaxTokens) return 0;
-  return align_up(omx::pages_release_words(N * table_width) * 4);
+  return align_up(omx::pages_release_words(N, table_width) * 4);
 }
 
 int omx_gdn_pages_release(int32_t* block_table, int64_t N, int64_t table_width, const int32_t* lengths,
@@ -673,7 +673,7 @@ int omx_gdn_pages_release(int32_t* block_table, int64_t N, int64_t table_width, 
   if (N * table_width == 0) return ok();
   omx::PagesParams p = pages(block_table, N, table_width, lengths, free_pages, free_count, n_pages, page_size, workspace);
   p.window = window < kMaxTokens ? (int)window : 0;  // no position is behind a window of all
-  p.sinks = sinks;
+  p.sinks = (int)(sinks < kMaxTokens ? sinks : kMaxTokens);
   return launch_status(omx::launch_pages_release(p, (hipStream_t)stream), fn);
 }
 

@@ -353,11 +353,10 @@ struct PagesParams {
   long long* slots;            // [T]
   int32_t* missing;            // pages that the stack did not have
   int32_t* first;              // workspace
-  int window;                  // return: what the next token sees, 0 all
-  long long sinks;
+  int window, sinks;           // return: what the next token sees, 0 all
 };
 size_t pages_assign_words(long long N);         // int32 words of workspace
-size_t pages_release_words(long long entries);
+size_t pages_release_words(long long N, long long table_w);
 hipError_t launch_pages_assign(const PagesParams& p, hipStream_t stream);
 hipError_t launch_pages_release(const PagesParams& p, hipStream_t stream);
 

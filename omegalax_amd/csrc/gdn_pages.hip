@@ -69,13 +69,17 @@ __device__ __forceinline__ void map_token(const PagesParams& p, const S* cu, int
   p.slots[t] = slot;
 }
 
-// One workgroup: the sequences' offsets, then their entries, flat, and (MAP) their tokens.
+// Four counts of up to 16 bits each in one word: a turn of the loops below takes 4 kNT neighbouring entries of
+// a table four times over, four a thread each time, and finds all their places by one sum.
+__device__ __forceinline__ int field(unsigned long long x, int j) { return (int)(x >> 16 * j & 0xffff); }
+
+// One workgroup: the sequences' offsets, then their entries, flat, and (map) their tokens.
 // `first`: [N + 1] entries before each sequence's, in LDS (kLdsSeqs of them at most) or memory.
 constexpr int kLdsSeqs = 4096;
 
 template <bool LDS>
 __global__ __launch_bounds__(kNT) void pages_assign_kernel(PagesParams p, int map) {
-  __shared__ int sFirst[LDS ? kLdsSeqs + 1 : 1], sCu[LDS ? kLdsSeqs + 1 : 1];
+  __shared__ int sFirst[LDS ? kLdsSeqs + 1 : 1], sCu[LDS ? kLdsSeqs + 1 : 1], sSlot[LDS ? kLdsSeqs : 1];
   __shared__ long long sWave[kNT / 64];
   const int tid = threadIdx.x;
   const int count = on_stack(p);
@@ -103,7 +107,10 @@ __global__ __launch_bounds__(kNT) void pages_assign_kernel(PagesParams p, int ma
     if (n < p.N) {
       first[n] = (int)(upto - slots);
       cu[n] = (int)a;
-      if (LDS) p.cu[n] = (int)a;
+      if (LDS) {
+        p.cu[n] = (int)a;
+        sSlot[n] = held / p.page;
+      }
     }
   }
   const int used = (int)(tokens < p.T ? tokens : p.T), all = (int)entries;
@@ -112,31 +119,40 @@ __global__ __launch_bounds__(kNT) void pages_assign_kernel(PagesParams p, int ma
     cu[p.N] = p.cu[p.N] = used;
   }
   __syncthreads();
-  // the entries, four a thread
   int needed = 0;
-  for (int f0 = 0; f0 < all; f0 += 4 * kNT) {
-    int* at[4];
-    int need[4], mine = 0;
+  for (int f0 = 0; f0 < all; f0 += 16 * kNT) {
+    int* at[16];
+    int id[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int f = f0 + 4 * tid + i;
-      need[i] = 0;
-      at[i] = nullptr;
-      if (f < all) {
-        const int n = last_upto(first, p.N, f);
-        at[i] = p.table + (long long)n * p.table_w + p.lengths[n] / p.page + (f - first[n]);
-        need[i] = !a_page(*at[i], p.n_pages);
+    for (int j = 0; j < 4; ++j) {  // all reads before the sum
+      const int f = f0 + 4 * (j * kNT + tid);
+      int n = f < all ? last_upto(first, p.N, f) : 0, upto = f < all ? first[n + 1] : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        id[4 * j + i] = 0;
+        at[4 * j + i] = nullptr;
+        if (f + i >= all) continue;
+        while (f + i >= upto) upto = first[++n + 1];  // (entries of a sequence that follows)
+        const int slot = LDS ? sSlot[n] : p.lengths[n] / p.page;
+        at[4 * j + i] = p.table + (long long)n * p.table_w + slot + (f + i - first[n]);
+        id[4 * j + i] = *at[4 * j + i];
       }
-      mine += need[i];
     }
-    long long total;
-    int k = needed + (int)block_scan<kNT>((long long)mine, sWave, total) - mine;
-    needed += (int)total;
+    unsigned long long mine = 0, total;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (!need[i]) continue;
-      if (k < count) *at[i] = p.free[count - 1 - k];
-      ++k;
+    for (int e = 0; e < 16; ++e)
+      if (at[e] && !a_page(id[e], p.n_pages)) mine += 1ull << 16 * (e / 4);
+    const unsigned long long upto = block_scan<kNT>(mine, (unsigned long long*)sWave, total) - mine;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      int k = needed + field(upto, j);
+#pragma unroll
+      for (int e = 4 * j; e < 4 * j + 4; ++e) {
+        if (!at[e] || a_page(id[e], p.n_pages)) continue;
+        if (k < count) *at[e] = p.free[count - 1 - k];
+        ++k;
+      }
+      needed += field(total, j);
     }
   }
   if (tid == 0) {
@@ -153,28 +169,33 @@ __global__ __launch_bounds__(256) void pages_map_kernel(PagesParams p) {
   if (t < p.T) map_token(p, p.cu, p.cu[p.N], (int)t);
 }
 
-// Whether entry i of row n goes back: past the tokens that are kept, or with a window behind what the
-// next token sees, but for the sinks'.
-__device__ __forceinline__ bool goes_back(const PagesParams& p, int id, int n, int i) {
-  const long long keep = p.lengths[n], from = (long long)i * p.page;
-  if (keep < 0 || !a_page(id, p.n_pages)) return false;
-  return from >= keep || (p.window > 0 && from >= p.sinks && from + p.page <= keep + 1 - p.window);
+// Whether entry i of a row that keeps `keep` tokens goes back: past those, or with a window behind what the
+// next token sees, but for the sinks'.  (A table's positions fit 31 bits.)
+__device__ __forceinline__ bool goes_back(const PagesParams& p, int id, int keep, int i) {
+  const int from = i * p.page;
+  const bool past = from >= keep, behind = (p.window > 0) & (from >= p.sinks) & (from + p.page - 1 <= keep - p.window);
+  return a_page(id, p.n_pages) & (keep >= 0) & (past | behind);
 }
 
 // Entries of the tables, flat, kPer a workgroup of kBackNT threads, four neighbours a thread and turn.
 constexpr int kBackNT = 256, kPer = 4096;
 
+// which of four neighbours go back
 __device__ __forceinline__ int back_of(const PagesParams& p, long long f, int (&id)[4]) {
-  int mask = 0;
+  const long long all = (long long)p.N * p.table_w;
+  int n = f < all ? (int)(f / p.table_w) : 0, slot[4], kept[4], mask = 0;
+  slot[0] = (int)(f - (long long)n * p.table_w);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long e = f + i;
-    id[i] = -1;
-    if (e >= (long long)p.N * p.table_w) continue;
-    const int n = (int)(e / p.table_w);
-    id[i] = p.table[e];
-    if (goes_back(p, id[i], n, (int)(e - (long long)n * p.table_w))) mask |= 1 << i;
+  for (int i = 0; i < 4; ++i) {  // reads first
+    id[i] = f + i < all ? p.table[f + i] : -1;
+    kept[i] = f + i < all ? p.lengths[n] : -1;
+    if (i == 3) break;
+    slot[i + 1] = slot[i] + 1;
+    if (slot[i + 1] == p.table_w) slot[i + 1] = 0, ++n;
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (goes_back(p, id[i], kept[i], slot[i])) mask |= 1 << i;
   return mask;
 }
 __device__ __forceinline__ void give_back(const PagesParams& p, long long f, const int (&id)[4], int mask, long long top) {
@@ -188,22 +209,72 @@ __device__ __forceinline__ void give_back(const PagesParams& p, long long f, con
   }
 }
 
-// few entries: one workgroup, which counts them and then passes over them again
+// few entries, kOneRelease at most, of kLdsRows rows: one workgroup, which keeps them all in registers.  Its
+// instructions bound it, so what a row returns lies in LDS as slots: those from sFrom on, and with a window
+// those from its sinks' on before sBehind.
+constexpr int kLdsRows = 8192;
+constexpr int kTurns = 8;  // of four entries a thread
+constexpr long long kOneRelease = 4 * kTurns * kNT;
+
+template <bool WIN>
 __global__ __launch_bounds__(kNT) void pages_release_one_kernel(PagesParams p) {
-  __shared__ int sWave[kNT / 64];
-  const long long all = (long long)p.N * p.table_w;
-  int id[4], mine = 0, total;
-  for (long long f = 4 * threadIdx.x; f < all; f += 4 * kNT) mine += __popc(back_of(p, f, id));
+  typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
+  __shared__ unsigned long long sWave[kNT / 64];
+  __shared__ int sFrom[kLdsRows], sBehind[WIN ? kLdsRows : 1];
+  const int all = p.N * p.table_w, sinks = (p.sinks + p.page - 1) / p.page;
   const int count = on_stack(p);
-  block_scan<kNT>(mine, sWave, total);
-  const int n = total;
+  for (int n = threadIdx.x; n < p.N; n += kNT) {
+    const int keep = p.lengths[n];
+    sFrom[n] = keep < 0 ? INT_MAX : keep / p.page + (keep % p.page != 0);
+    if (WIN) sBehind[n] = keep < p.window ? 0 : (keep - p.window + 1) / p.page;
+  }
+  int id[kTurns][4], mask[kTurns];
+#pragma unroll
+  for (int j = 0; j < kTurns; ++j) {
+    const int f = 4 * (j * kNT + (int)threadIdx.x);
+    if (f + 3 < all) {
+      const i32x4u x = *(const i32x4u*)(p.table + f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) id[j][i] = x[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) id[j][i] = f + i < all ? p.table[f + i] : -1;
+    }
+  }
+  __syncthreads();
+  // the first entry's row and slot, from turn to turn
+  const int down = 4 * kNT / p.table_w, on = 4 * kNT % p.table_w;
+  int n0 = 4 * (int)threadIdx.x / p.table_w, slot0 = 4 * (int)threadIdx.x % p.table_w;
+  unsigned long long mine[2] = {0, 0}, upto[2], total[2];
+#pragma unroll
+  for (int j = 0; j < kTurns; ++j) {
+    mask[j] = 0;
+    if (4 * j * kNT >= all) continue;  // uniform
+    int n = n0, slot = slot0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = n < p.N ? n : p.N - 1;
+      const bool behind = WIN ? (slot >= sinks) & (slot < sBehind[m]) : false;
+      if (a_page(id[j][i], p.n_pages) & ((slot >= sFrom[m]) | behind)) mask[j] |= 1 << i;
+      if (++slot == p.table_w) slot = 0, ++n;
+    }
+    mine[j / 4] += (unsigned long long)__popc(mask[j]) << 16 * (j % 4);
+    n0 += down;
+    slot0 += on;
+    if (slot0 >= p.table_w) slot0 -= p.table_w, ++n0;
+  }
+  int n = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    upto[h] = block_scan<kNT>(mine[h], sWave, total[h]) - mine[h];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) n += field(total[h], j);
+  }
   int done = 0;
-  for (long long f0 = 0; f0 < all; f0 += 4 * kNT) {
-    const long long f = f0 + 4 * threadIdx.x;
-    const int mask = back_of(p, f, id), k = __popc(mask);
-    const int before = done + block_scan<kNT>(k, sWave, total) - k;
-    done += total;
-    give_back(p, f, id, mask, (long long)count + n - 1 - before);
+#pragma unroll
+  for (int j = 0; j < kTurns; ++j) {
+    give_back(p, 4 * (j * kNT + (int)threadIdx.x), id[j], mask[j], (long long)count + n - 1 - done - field(upto[j / 4], j % 4));
+    done += field(total[j / 4], j % 4);
   }
   if (threadIdx.x == 0) *p.count = count + n < p.n_pages ? count + n : p.n_pages;
 }
@@ -246,7 +317,6 @@ __global__ __launch_bounds__(kBackNT) void pages_release_kernel(PagesParams p) {
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.count = (int)(count + n < p.n_pages ? count + n : p.n_pages);
 }
 
-constexpr long long kOneRelease = 1 << 15;  // entries that one workgroup passes over
 constexpr long long kOneMap = 4096;         // tokens that the assigning workgroup maps
 
 }  // namespace
@@ -263,14 +333,17 @@ hipError_t launch_pages_assign(const PagesParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-size_t pages_release_words(long long entries) {
-  return entries > kOneRelease ? (size_t)((entries + kPer - 1) / kPer + 1) : 0;
+size_t pages_release_words(long long N, long long table_w) {
+  return N * table_w > kOneRelease || N > kLdsRows ? (size_t)((N * table_w + kPer - 1) / kPer + 1) : 0;
 }
 
 hipError_t launch_pages_release(const PagesParams& p, hipStream_t stream) {
   const long long entries = (long long)p.N * p.table_w;
-  if (entries <= kOneRelease) {
-    pages_release_one_kernel<<<1, kNT, 0, stream>>>(p);
+  if (pages_release_words(p.N, p.table_w) == 0) {
+    if (p.window > 0)
+      pages_release_one_kernel<true><<<1, kNT, 0, stream>>>(p);
+    else
+      pages_release_one_kernel<false><<<1, kNT, 0, stream>>>(p);
   } else {
     const unsigned grid = (unsigned)((entries + kPer - 1) / kPer);
     pages_count_kernel<<<grid, kBackNT, 0, stream>>>(p);
