@@ -465,7 +465,7 @@ size_t omx_gdn_attn_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, in
  * exponent or raises it; then their numbers are divided by the power of two between and rounded again.
  * Values that are not finite become NaN and do not count for e; sizes above 1.875 2^127 are clamped to it.
  * What no token was written to may hold anything.  Other arguments as for omx_gdn_kv_write, and its
- * workspace size; less than 2^24 workgroups of 64 tokens and a key head.
+ * workspace size; less than 2^23 times 64 tokens of a key head.
  */
 int omx_gdn_kv_write8(const void* k, const void* v, int64_t k_ld, int64_t v_ld,
                       const int32_t* cu_seqlens, int64_t N, void* k_pages, void* v_pages,

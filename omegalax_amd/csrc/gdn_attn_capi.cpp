@@ -385,7 +385,7 @@ int kv_write(const char* fn, const void* k, const void* v, int64_t k_ld, int64_t
   if (!rc) rc = check_ld(fn, "v_ld", v_ld, Hkv * D);
   if (rc) return rc;
   if (k_exps)
-    REQUIRE((B * T / omx::kv_write8_tokens() + 1) * Hkv <= kMaxGroups, "%s: grid too large", fn);
+    REQUIRE((B * T / omx::kv_write8_tokens() + 1) * 2 * Hkv <= kMaxGroups, "%s: grid too large", fn);
   else
     REQUIRE(B * T <= kMaxGroups * omx::kv_write_tokens(), "%s: grid too large", fn);
   const int per = omx::attn_dkv_tile_tokens();

@@ -77,14 +77,19 @@ __device__ __forceinline__ float exp_shift(int a, int b) { return a - b < -126 ?
 // ------------------------------------------------------------------------------------ append
 // Token i of sequence n goes to position held[n] + i, as in the cache of bf16.  A wavefront takes the
 // blocks that begin with one of its kSpan tokens (a block of a sequence's first new token among them),
-// whole and for one head: a lane has 16 columns of every DP / 64-th group of rows.  The largest values
-// are found over the wavefront, and the block's older tokens read only if its exponent grows.
+// whole and for one head's keys or values: a lane has 16 columns of every DP / 64-th group of rows.  The largest values
+// are found over the wavefront; the block's older tokens are written only if its exponent grows.
 constexpr int kSpan = 16;
 
 template <int DP>
 __global__ __launch_bounds__(256) void kv_write8_kernel(AttnParams p, int span) {
   constexpr int NR = DP / 64, LR = DP / 16, RJ = 64 / LR;  // rows: NR loads of RJ, LR lanes each
-  const int l = lane_id(), hk = (int)blockIdx.y, seg = l % LR;
+  const int l = lane_id(), hk = (int)blockIdx.y >> 1, seg = l % LR;
+  const bool value = blockIdx.y & 1;
+  const bf16_t* src = (const bf16_t*)(value ? p.v : p.k) + hk * DP + 16 * seg;
+  const long long src_ld = value ? p.v_ld : p.k_ld;
+  uint8_t* pool = (uint8_t*)(value ? p.v_pages : p.k_pages);
+  int8_t* exps = value ? p.v_exps : p.k_exps;
   const long long t0 = ((long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * span;
   const long long t1 = t0 + span < p.tokens ? t0 + span : p.tokens;
   const bool lanes = p.cu && !p.plan;  // lane n holds sequence n's end
@@ -128,56 +133,54 @@ __global__ __launch_bounds__(256) void kv_write8_kernel(AttnParams p, int span) 
     }
     const int r0 = (int)(pos % 16);
     const int m = stop - t < 16 - r0 ? (int)(stop - t) : 16 - r0;
+    // the rows are on their way before the table is read
+    u32x4 x[NR][2];
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+      const int r = RJ * j + l / LR - r0;
+      x[j][0] = x[j][1] = u32x4{0, 0, 0, 0};
+      if (r >= 0 && r < m) {
+        x[j][0] = *(const u32x4*)(src + (t + r) * src_ld);
+        x[j][1] = *(const u32x4*)(src + (t + r) * src_ld + 8);
+      }
+    }
     const long long slot = pos / p.page;
     const int id = slot < p.table_w ? p.table[(long long)seq * p.table_w + slot] : -1;
     if (id >= 0 && id < p.n_pages) {
       const int row = (int)(pos - slot * p.page) - r0;  // the block's first, of the page
-      const long long at = (((long long)id * p.page + row) * p.Hkv + hk) * DP + 16 * seg;
-      const long long block = ((long long)id * (p.page / 16) + row / 16) * p.Hkv + hk;
-      u32x4 x[2][NR][2];
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-        for (int j = 0; j < NR; ++j) {
-          const int r = RJ * j + l / LR - r0;
-          x[kv][j][0] = x[kv][j][1] = u32x4{0, 0, 0, 0};
-          if (r >= 0 && r < m) {
-            const bf16_t* src = kv ? (const bf16_t*)p.v + (t + r) * p.v_ld : (const bf16_t*)p.k + (t + r) * p.k_ld;
-            x[kv][j][0] = *(const u32x4*)(src + hk * DP + 16 * seg);
-            x[kv][j][1] = *(const u32x4*)(src + hk * DP + 16 * seg + 8);
-          }
-        }
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        int8_t* exps = kv ? p.v_exps : p.k_exps;
-        uint8_t* pool = (uint8_t*)(kv ? p.v_pages : p.k_pages) + at;
-        float most = 0.f;
-#pragma unroll
-        for (int j = 0; j < NR; ++j) most = fmaxf(most, most16(x[kv][j][0], x[kv][j][1]));
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-        int e = asked_exp(most);
-        if (r0 > 0) {
-          const int before = exps[block];
-          if (before < e) {
-            const float shift = exp_shift(before, e);
-#pragma unroll
-            for (int j = 0; j < NR; ++j) {
-              const int r = RJ * j + l / LR;
-              u32x4* c = (u32x4*)(pool + (long long)r * p.Hkv * DP);
-              if (r < r0) *c = again16(*c, shift);
-            }
-          }
-          e = e > before ? e : before;
-        }
-        const float down = exp_scale(-e);
+      uint8_t* to = pool + (((long long)id * p.page + row) * p.Hkv + hk) * DP + 16 * seg;
+      int8_t* at = exps + ((long long)id * (p.page / 16) + row / 16) * p.Hkv + hk;
+      int before = kLeastExp;
+      u32x4 old[NR];  // the block's older tokens, read beside their exponent
+      if (r0 > 0) {
+        before = *at;
 #pragma unroll
         for (int j = 0; j < NR; ++j) {
           const int r = RJ * j + l / LR;
-          if (r >= r0 && r < r0 + m) *(u32x4*)(pool + (long long)r * p.Hkv * DP) = code16(x[kv][j][0], x[kv][j][1], down);
+          old[j] = *(const u32x4*)(to + (long long)(r < r0 ? r : 0) * p.Hkv * DP);
         }
-        if (l == 0) exps[block] = (int8_t)e;
       }
+      float most = 0.f;
+#pragma unroll
+      for (int j = 0; j < NR; ++j) most = fmaxf(most, most16(x[j][0], x[j][1]));
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+      const int ask = asked_exp(most), e = ask > before ? ask : before;
+      if (r0 > 0 && e > before) {
+        const float shift = exp_shift(before, e);
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+          const int r = RJ * j + l / LR;
+          if (r < r0) *(u32x4*)(to + (long long)r * p.Hkv * DP) = again16(old[j], shift);
+        }
+      }
+      const float down = exp_scale(-e);
+#pragma unroll
+      for (int j = 0; j < NR; ++j) {
+        const int r = RJ * j + l / LR;
+        if (r >= r0 && r < r0 + m) *(u32x4*)(to + (long long)r * p.Hkv * DP) = code16(x[j][0], x[j][1], down);
+      }
+      if (l == 0) *at = (int8_t)e;
     }
     t += m;
   }
@@ -530,7 +533,7 @@ void decode8_dp(const AttnParams& p, hipStream_t stream) {
 int kv_write8_tokens() { return 4 * kSpan; }
 
 hipError_t launch_kv_write8(const AttnParams& p, hipStream_t stream) {
-  const dim3 grid((unsigned)((p.tokens + 4 * kSpan - 1) / (4 * kSpan)), (unsigned)p.Hkv);
+  const dim3 grid((unsigned)((p.tokens + 4 * kSpan - 1) / (4 * kSpan)), 2u * (unsigned)p.Hkv);
   if (p.D == 64) kv_write8_kernel<64><<<grid, 256, 0, stream>>>(p, kSpan);
   else if (p.D == 128) kv_write8_kernel<128><<<grid, 256, 0, stream>>>(p, kSpan);
   else kv_write8_kernel<256><<<grid, 256, 0, stream>>>(p, kSpan);
