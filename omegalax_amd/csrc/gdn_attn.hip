@@ -135,7 +135,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   const_i32* table = PAGED ? (const_i32*)(p.table + (long long)it.seq * p.table_w) : nullptr;
   int slot = 0, off = 0;
   const int row_bytes = EIGHT ? Hkv * D : Hkv * D * 2;
-  struct Pages { long long at[4], exp[4]; unsigned have, fetch; };  // byte offsets in a pool; none past the split
+  // (of bf16 the groups' byte offsets in a pool, of 8 bits the numbers of their blocks; none past the split)
+  struct Pages { long long at[EIGHT ? 1 : 4]; unsigned blk[EIGHT ? 4 : 1], have, fetch; };
   auto look = [&](int kt) {
     Pages x;
     x.have = 0;
@@ -149,8 +150,10 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       int id = in ? table[slot] : -1;
       id = id >= p.n_pages ? -1 : id;
       id = __builtin_amdgcn_readfirstlane(id);
-      x.at[g] = ((long long)(id < 0 ? 0 : id) * p.page + off) * row_bytes + (EIGHT ? 1 : 2) * hk * D;
-      if constexpr (EIGHT) x.exp[g] = ((long long)(id < 0 ? 0 : id) * (p.page / 16) + off / 16) * Hkv + hk;
+      if constexpr (EIGHT)
+        x.blk[g] = (unsigned)(id < 0 ? 0 : id) * (unsigned)(p.page / 16) + (unsigned)(off / 16);
+      else
+        x.at[g] = ((long long)(id < 0 ? 0 : id) * p.page + off) * row_bytes + 2 * hk * D;
       x.have |= id >= 0 ? 1u << g : 0u;
       off += 16;
       if (off >= p.page) { off = 0; ++slot; }
@@ -194,12 +197,12 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   const int row8 = tid / (DP / 16), seg8 = tid % (DP / 16);
   // (the wavefront's group of the j-th, by selects: an index into the pages would put them into memory)
   const unsigned zero8 = lane_zero();
-  auto mine8 = [&](const long long (&x)[4], int j) {
-    const long long a = x[0], b = x[1], c = x[2], d = x[3];
+  auto mine8 = [&](const Pages& x, int j) {
+    const unsigned a = x.blk[0], b = x.blk[EIGHT ? 1 : 0], c = x.blk[EIGHT ? 2 : 0], d = x.blk[EIGHT ? 3 : 0];
     if constexpr (DP == 256) return j == 0 ? a : (j == 1 ? b : (j == 2 ? c : d));
-    const long long even = w & 2 ? b : a, odd = w & 2 ? d : c;
+    const unsigned even = w & 2 ? b : a, odd = w & 2 ? d : c;
     if constexpr (DP == 128) return j == 0 ? even : odd;
-    const long long low = w & 1 ? b : a, high = w & 1 ? d : c;
+    const unsigned low = w & 1 ? b : a, high = w & 1 ? d : c;
     return w & 2 ? high : low;
   };
   auto load8 = [&](const Pages& x, const void* pool, const int8_t* exps) {
@@ -207,10 +210,11 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
       const bool there = (x.fetch >> (DP == 256 ? j : (DP == 128 ? 2 * j + w / 2 : w))) & 1;
+      const long long blk = (long long)mine8(x, j) * Hkv;
       r.x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-          uniform_rsrc((const char*)pool + mine8(x.at, j), there ? 15u * row_bytes + DP : 0u),
+          uniform_rsrc((const char*)pool + (blk * 16 + hk) * DP, there ? 15u * row_bytes + DP : 0u),
           ((kRows8 * j + row8) & 15) * row_bytes + 16 * seg8, 0, 0));
-      r.e[j] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(exps + mine8(x.exp, j), there ? 1u : 0u), zero8, 0, 0);
+      r.e[j] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(exps + blk + hk, there ? 1u : 0u), zero8, 0, 0);
     }
     return r;
   };
