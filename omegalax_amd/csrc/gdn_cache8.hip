@@ -213,7 +213,8 @@ void attn_decode8_kernel(AttnParams p) {
   constexpr int SK = kStage8<DP>, NG = SK / 16, NC = SK / 32;  // keys of a stage, its blocks, pairs of them
   constexpr int KS = DP / 32, DB = DP / 16;
   constexpr int NI = DP / 64, RI = 1024 / DP, LR = DP / 16;     // loads of a block, their rows, a row's lanes
-  constexpr int kV = SK * DP, kE = 2 * kV, kSlot = kE + 512;    // a slot: K, V, their exponents (4 bytes each)
+  constexpr int kV = SK * DP, kE = 2 * kV, kNew = kE + 512;     // a slot: K, V, their exponents (4 bytes each)
+  constexpr int kSlot = kNew + 2048;                            // and the new token's k and v
   constexpr int kLoads = NG * NI + 1;                           // of K, and of V
   constexpr int NW = kDec8NW<NQ>;
   __shared__ __align__(16) uint8_t slots[NW][kSlot];
@@ -245,15 +246,6 @@ void attn_decode8_kernel(AttnParams p) {
   const int st1 = nst - st0 < x1 - x ? nst : st0 + (x1 - x);
   const bool alone = st0 == 0 && st1 == nst;
 
-  u32x4 q[NQ][KS];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n)
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      q[n][s] = u32x4{0, 0, 0, 0};
-      if (16 * n + r < G)
-        q[n][s] = *(const u32x4*)((const bf16_t*)p.q + b * p.q_ld + (long long)(hk * G + 16 * n + r) * DP + 32 * s + 8 * g4);
-    }
   f32x4 o[NQ][DB];
   float m[NQ], ls[NQ];
 #pragma unroll
@@ -300,9 +292,9 @@ void attn_decode8_kernel(AttnParams p) {
   auto stage_k = [&](const Ids& y) __attribute__((always_inline)) { stage(y, p.k_pages, p.k_exps, 0, kE); };
   auto stage_v = [&](const Ids& y) __attribute__((always_inline)) { stage(y, p.v_pages, p.v_exps, kV, kE + 256); };
   // the new token's codes into the stage that holds its block, and into the cache
-  auto amend = [&](int key0, uint8_t* codes, uint8_t* ex, const bf16_t* src, void* pages,
+  auto amend = [&](int key0, uint8_t* codes, uint8_t* ex, const uint8_t* src, void* pages,
                    int8_t* exps) __attribute__((always_inline)) {
-    const u32x4 a = *(const u32x4*)(src + hk * DP + 16 * seg), a2 = *(const u32x4*)(src + hk * DP + 16 * seg + 8);
+    const u32x4 a = *(const u32x4*)(src + 32 * seg), a2 = *(const u32x4*)(src + 32 * seg + 16);
     float most = most16(a, a2);
 #pragma unroll
     for (int i = 1; i < LR; i <<= 1) most = fmaxf(most, __shfl_xor(most, i, 64));
@@ -334,13 +326,23 @@ void attn_decode8_kernel(AttnParams p) {
   {
     int st = st0 + w;
     Ids y = look(st), next;
-    // the queries are there before the compiler, which does not count the loads below, waits for them
+    {  // the new token's row, for the wavefront that will put it into its block
+      const unsigned to = l < DP / 8 ? 16u * (unsigned)l : kDropOffset;
+      load_to_lds16(rsrc_words((const bf16_t*)p.k + b * p.k_ld + hk * DP, 2u * DP), lds + kNew, to);
+      load_to_lds16(rsrc_words((const bf16_t*)p.v + b * p.v_ld + hk * DP, 2u * DP), lds + kNew + 1024u, to);
+    }
+    stage_k(y);
+    stage_v(y);
+    // (behind the loads into LDS, which the compiler does not count: it waits for all of them with these)
+    u32x4 q[NQ][KS];
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(q[n][s]));
-    stage_k(y);
-    stage_v(y);
+      for (int s = 0; s < KS; ++s) {
+        q[n][s] = u32x4{0, 0, 0, 0};
+        if (16 * n + r < G)
+          q[n][s] = *(const u32x4*)((const bf16_t*)p.q + b * p.q_ld + (long long)(hk * G + 16 * n + r) * DP + 32 * s + 8 * g4);
+      }
     for (; st < st1; st += NW, y = next) {
       next = look(st + NW);
       const unsigned have = y.have;
@@ -353,7 +355,7 @@ void attn_decode8_kernel(AttnParams p) {
 
       asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kLoads) : "memory");  // the keys: all but the values
       if (mine) {
-        amend(key0, sk, slot + kE, (const bf16_t*)p.k + b * p.k_ld, p.k_pages, p.k_exps);
+        amend(key0, sk, slot + kE, slot + kNew, p.k_pages, p.k_exps);
         wave_lds_fence();
       }
       const int ke = (int)(int8_t)slot[kE + 4 * (l & (NG - 1))];
@@ -427,7 +429,7 @@ void attn_decode8_kernel(AttnParams p) {
 
       asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kLoads) : "memory");  // the values: all but the next keys
       if (!whole) {
-        if (mine) amend(key0, sv, slot + kE + 256, (const bf16_t*)p.v + b * p.v_ld, p.v_pages, p.v_exps);
+        if (mine) amend(key0, sv, slot + kE + 256, slot + kNew + 1024, p.v_pages, p.v_exps);
         // rows without a key, or not seen, are cleared: a weight of zero does not clear a NaN
         for (int i = l; i < SK * LR; i += 64) {
           const int row = i / LR, key = key0 + row;
