@@ -273,8 +273,8 @@ void attn_decode8_kernel(AttnParams p) {
     }
     return y;
   };
-  // Fetches a stage's keys (or values); what is not there has an empty range and reads as zeros, so that
-  // every stage counts the same loads.
+  // Fetches a stage's keys (or values); a block that is not there has an empty range and reads as zeros, so
+  // that every stage counts the same loads.
   uint8_t* const slot = slots[w];
   const unsigned lds = lds_address(slot);
   auto stage = [&](const Ids& y, const void* pages, const int8_t* exps, unsigned to,
@@ -331,8 +331,10 @@ void attn_decode8_kernel(AttnParams p) {
       load_to_lds16(rsrc_words((const bf16_t*)p.k + b * p.k_ld + hk * DP, 2u * DP), lds + kNew, to);
       load_to_lds16(rsrc_words((const bf16_t*)p.v + b * p.v_ld + hk * DP, 2u * DP), lds + kNew + 1024u, to);
     }
-    stage_k(y);
-    stage_v(y);
+    if (st < st1) {
+      stage_k(y);
+      stage_v(y);
+    }
     // (behind the loads into LDS, which the compiler does not count: it waits for all of them with these)
     u32x4 q[NQ][KS];
 #pragma unroll
@@ -344,7 +346,8 @@ void attn_decode8_kernel(AttnParams p) {
           q[n][s] = *(const u32x4*)((const bf16_t*)p.q + b * p.q_ld + (long long)(hk * G + 16 * n + r) * DP + 32 * s + 8 * g4);
       }
     for (; st < st1; st += NW, y = next) {
-      next = look(st + NW);
+      const bool more = st + NW < st1;
+      if (more) next = look(st + NW);
       const unsigned have = y.have;
       const int key0 = (WIN ? seen.at(st) : st) * SK;
       constexpr unsigned kAll = (1u << NG) - 1;
@@ -375,7 +378,7 @@ void attn_decode8_kernel(AttnParams p) {
         }
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads are done
-      stage_k(next);
+      if (more) stage_k(next);
 
       u32x4 pb[NQ][NC], pr[NQ][NC];
 #pragma unroll
@@ -427,7 +430,10 @@ void attn_decode8_kernel(AttnParams p) {
         }
       }
 
-      asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kLoads) : "memory");  // the values: all but the next keys
+      if (more)
+        asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kLoads) : "memory");  // the values: all but the next keys
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (!whole) {
         if (mine) amend(key0, sv, slot + kE + 256, slot + kNew + 1024, p.v_pages, p.v_exps);
         // rows without a key, or not seen, are cleared: a weight of zero does not clear a NaN
@@ -455,7 +461,7 @@ void attn_decode8_kernel(AttnParams p) {
         }
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads are done
-      stage_v(next);
+      if (more) stage_v(next);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is on its way into LDS
   }
@@ -471,12 +477,12 @@ void attn_decode8_kernel(AttnParams p) {
       sL[w][16 * n + r] = ls[n];
     }
   }
-  __syncthreads();
+  lds_barrier();
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) *(f32x4*)((float*)slot + r * DP + 16 * d + 4 * g4) = o[n][d];
-    __syncthreads();
+    lds_barrier();
     const int rows = G - 16 * n < 16 ? G - 16 * n : 16;
     for (int i = tid; i < rows * DP / 4; i += 64 * NW) {
       const int row = i / (DP / 4), col = 4 * (i % (DP / 4));
@@ -506,7 +512,7 @@ void attn_decode8_kernel(AttnParams p) {
             u32x2{pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
       }
     }
-    __syncthreads();
+    lds_barrier();
   }
   x += st1 - st0;
   if (p.splits == 1 || x >= x1) return;
