@@ -214,7 +214,9 @@ void attn_decode8_kernel(AttnParams p) {
   constexpr int KS = DP / 32, DB = DP / 16;
   constexpr int NI = DP / 64, RI = 1024 / DP, LR = DP / 16;     // loads of a block, their rows, a row's lanes
   constexpr int kV = SK * DP, kE = 2 * kV, kNew = kE + 512;     // a slot: K, V, their exponents (4 bytes each)
-  constexpr int kSlot = kNew + 2048;                            // and the new token's k and v
+  constexpr int kSlot = kNew + 2560;                            // and the new token's k, v and old exponents
+  constexpr int kSum = DP + 16;                                 // a row of sums: four rows fill the banks
+  static_assert(16 * kSum * 4 <= kSlot, "a slot holds 16 rows of sums");
   constexpr int kLoads = NG * NI + 1;                           // of K, and of V
   constexpr int NW = kDec8NW<NQ>;
   __shared__ __align__(16) uint8_t slots[NW][kSlot];
@@ -291,31 +293,45 @@ void attn_decode8_kernel(AttnParams p) {
   };
   auto stage_k = [&](const Ids& y) __attribute__((always_inline)) { stage(y, p.k_pages, p.k_exps, 0, kE); };
   auto stage_v = [&](const Ids& y) __attribute__((always_inline)) { stage(y, p.v_pages, p.v_exps, kV, kE + 256); };
-  // the new token's codes into the stage that holds its block, and into the cache
-  auto amend = [&](int key0, uint8_t* codes, uint8_t* ex, const uint8_t* src, void* pages,
-                   int8_t* exps) __attribute__((always_inline)) {
-    const u32x4 a = *(const u32x4*)(src + 32 * seg), a2 = *(const u32x4*)(src + 32 * seg + 16);
+  // The new token as its block will hold it: a lane's 16 codes, the block's exponent, and by what its older
+  // codes are multiplied if that grew.  Formed while the first stage is on its way.
+  struct New {
+    u32x4 codes;
+    int now;
+    float shift;
+    bool grew;
+  };
+  const int r0 = held & 15;
+  auto quantise = [&](const uint8_t* row, int before) __attribute__((always_inline)) {
+    const u32x4 a = *(const u32x4*)(row + 32 * seg), a2 = *(const u32x4*)(row + 32 * seg + 16);
     float most = most16(a, a2);
 #pragma unroll
     for (int i = 1; i < LR; i <<= 1) most = fmaxf(most, __shfl_xor(most, i, 64));
-    const int gb = (held - key0) / 16, r0 = held % 16;
-    const int slot = held / p.page, off = held - slot * p.page - r0;
-    const long long block = (long long)table[slot] * (p.page / 16) + off / 16;
-    const int before = r0 > 0 ? (int)(int8_t)ex[4 * gb] : kLeastExp;
-    const int ask = asked_exp(most), now = ask > before ? ask : before;
-    const float shift = exp_shift(before, now);
-    const u32x4 mine = code16(a, a2, exp_scale(-now));
+    const int ask = asked_exp(most);
+    New y;
+    before = r0 > 0 ? before : kLeastExp;
+    y.now = ask > before ? ask : before;
+    y.grew = ask > before;
+    y.shift = exp_shift(before, y.now);
+    y.codes = code16(a, a2, exp_scale(-y.now));
+    return y;
+  };
+  // puts it into the stage that holds its block, number `at`, and into the cache
+  auto amend = [&](const New& y, int gb, unsigned at, uint8_t* codes, uint8_t* ex, void* pages,
+                   int8_t* exps) __attribute__((always_inline)) {
+    uint8_t* to = (uint8_t*)pages + ((long long)at * 16 * Hkv + hk) * DP + 16 * seg;
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int row = RI * j + lrow;
-      if (row > r0 || (row < r0 && now <= before)) continue;
+      if (row > r0 || (row < r0 && !y.grew)) continue;
       u32x4* c = (u32x4*)(codes + (16 * gb + row) * DP + ((seg ^ swz8<DP>(16 * gb + row)) << 4));
-      *c = row == r0 ? mine : again16(*c, shift);
-      *(u32x4*)((uint8_t*)pages + (block * 16 * Hkv + hk) * DP + (long long)row * Hkv * DP + 16 * seg) = *c;
+      const u32x4 x = row == r0 ? y.codes : again16(*c, y.shift);
+      *c = x;
+      *(u32x4*)(to + (long long)row * Hkv * DP) = x;
     }
     if (l == 0) {
-      exps[block * Hkv + hk] = (int8_t)now;
-      ex[4 * gb] = (uint8_t)now;
+      exps[(long long)at * Hkv + hk] = (int8_t)y.now;
+      ex[4 * gb] = (uint8_t)y.now;
     }
   };
   uint8_t *const sk = slot, *const sv = slot + kV;
@@ -326,14 +342,29 @@ void attn_decode8_kernel(AttnParams p) {
   {
     int st = st0 + w;
     Ids y = look(st), next;
-    {  // the new token's row, for the wavefront that will put it into its block
+    // whose stage holds the new token's block, of number `into`
+    const int st_new = (held < 0 || held >= cap ? 0 : held / SK) - seen.skip;  // (the window's part, or without a skip)
+    const int new_slot = held < 0 || held >= cap ? -1 : (int)(__umulhi((unsigned)held, p.page_mul) >> p.page_shift);
+    const int new_id = new_slot >= 0 && st_new >= st && st_new < st1 && (st_new - st) % NW == 0 ? table[new_slot] : -1;
+    const bool ours = new_id >= 0 && new_id < p.n_pages;
+    const unsigned into = (unsigned)new_id * (unsigned)(p.page / 16) + (unsigned)((held - new_slot * p.page) / 16);
+    New nk{}, nv{};
+    if (ours) {
       const unsigned to = l < DP / 8 ? 16u * (unsigned)l : kDropOffset;
+      const unsigned eo = l == 0 ? into * (unsigned)Hkv + (unsigned)hk : kDropOffset;
       load_to_lds16(rsrc_words((const bf16_t*)p.k + b * p.k_ld + hk * DP, 2u * DP), lds + kNew, to);
       load_to_lds16(rsrc_words((const bf16_t*)p.v + b * p.v_ld + hk * DP, 2u * DP), lds + kNew + 1024u, to);
+      load_to_lds1(rsrc_words(p.k_exps, kDropOffset), lds + kNew + 2048u, eo);
+      load_to_lds1(rsrc_words(p.v_exps, kDropOffset), lds + kNew + 2304u, eo);
     }
     if (st < st1) {
       stage_k(y);
       stage_v(y);
+    }
+    if (ours) {
+      asm volatile("s_waitcnt vmcnt(%0)" :: "n"(2 * kLoads) : "memory");  // all but the stage
+      nk = quantise(slot + kNew, (int)(int8_t)slot[kNew + 2048]);
+      nv = quantise(slot + kNew + 1024, (int)(int8_t)slot[kNew + 2304]);
     }
     // (behind the loads into LDS, which the compiler does not count: it waits for all of them with these)
     u32x4 q[NQ][KS];
@@ -353,12 +384,12 @@ void attn_decode8_kernel(AttnParams p) {
       constexpr unsigned kAll = (1u << NG) - 1;
       const bool whole = have == kAll && key0 + SK < keys &&  // every row a held key, and seen
                          !(WIN && key0 < seen.lo && key0 + SK > p.sinks);
-      const int nrow = held - key0;  // the new token's
-      const bool mine = nrow >= 0 && nrow < SK && held < cap && ((have >> (nrow / 16)) & 1);
+      const bool mine = ours && st == st_new;
+      const int gb = (held - key0) / 16;  // the new token's block
 
       asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kLoads) : "memory");  // the keys: all but the values
       if (mine) {
-        amend(key0, sk, slot + kE, slot + kNew, p.k_pages, p.k_exps);
+        amend(nk, gb, into, sk, slot + kE, p.k_pages, p.k_exps);
         wave_lds_fence();
       }
       const int ke = (int)(int8_t)slot[kE + 4 * (l & (NG - 1))];
@@ -435,7 +466,7 @@ void attn_decode8_kernel(AttnParams p) {
       else
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (!whole) {
-        if (mine) amend(key0, sv, slot + kE + 256, slot + kNew + 1024, p.v_pages, p.v_exps);
+        if (mine) amend(nv, gb, into, sv, slot + kE + 256, p.v_pages, p.v_exps);
         // rows without a key, or not seen, are cleared: a weight of zero does not clear a NaN
         for (int i = l; i < SK * LR; i += 64) {
           const int row = i / LR, key = key0 + row;
@@ -467,7 +498,7 @@ void attn_decode8_kernel(AttnParams p) {
   }
 
   // ---------------------------------------------------------------- the wavefronts' sums
-  // a wavefront's slot holds 16 rows of DP fp32
+  // a wavefront's slot holds 16 rows of kSum fp32
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     ls[n] += __shfl_xor(ls[n], 16, 64);
@@ -481,7 +512,8 @@ void attn_decode8_kernel(AttnParams p) {
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-    for (int d = 0; d < DB; ++d) *(f32x4*)((float*)slot + r * DP + 16 * d + 4 * g4) = o[n][d];
+    for (int d = 0; d < DB; ++d)
+      if (16 * n + r < G) *(f32x4*)((float*)slot + r * kSum + 16 * d + 4 * g4) = o[n][d];
     lds_barrier();
     const int rows = G - 16 * n < 16 ? G - 16 * n : 16;
     for (int i = tid; i < rows * DP / 4; i += 64 * NW) {
@@ -496,7 +528,7 @@ void attn_decode8_kernel(AttnParams p) {
         const float lx = sL[u][16 * n + row];
         const float a = lx == 0.f ? 0.f : __builtin_amdgcn_exp2f(sM[u][16 * n + row] - M);
         den += a * lx;
-        acc += a * *(const f32x4*)((const float*)slots[u] + row * DP + col);
+        acc += a * *(const f32x4*)((const float*)slots[u] + row * kSum + col);
       }
       const long long at = (long long)b * Hq + hk * G + 16 * n + row;
       if (!alone) {
