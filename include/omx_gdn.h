@@ -478,7 +478,7 @@ int omx_gdn_kv_write8(const void* k, const void* v, int64_t k_ld, int64_t v_ld,
  * omx_gdn_attn_paged and omx_gdn_attn_decode_step with a window, over a cache of bf16 (k_exps and v_exps
  * NULL) or of 8 bits.  The query at position i sees positions i - window + 1 .. i and those below `sinks`;
  * window 0 (and sinks 0): all up to i.  A length past table_width * page_size counts as that.  Positions
- * that no query sees are not read, and need no page.  The decode step of a cache in 8 bits attends the new
+ * that no query sees need no page, and what they hold has no influence.  The decode step of a cache in 8 bits attends the new
  * token as the cache holds it.
  */
 int omx_gdn_attn_paged_window(const void* q, int64_t q_ld, const int32_t* cu_seqlens, int64_t N,

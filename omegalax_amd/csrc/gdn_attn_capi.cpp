@@ -523,8 +523,8 @@ int omx_gdn_attn_paged_window(const void* q, int64_t q_ld, const int32_t* cu_seq
 }
 
 namespace {
-int decode_splits(const Sight& sight, int64_t B, int64_t Hkv, int64_t D, int64_t capacity) {
-  return omx::decode_splits(B, Hkv, D, seen_keys(sight, capacity, 1));
+int decode_splits(const Sight& sight, int64_t B, int64_t Hkv, int64_t D, int64_t capacity, bool eight) {
+  return omx::decode_splits(B, Hkv, D, capacity, seen_keys(sight, capacity, 1), eight);
 }
 SplitWs decode_ws(int splits, int64_t B, int64_t Hq, int64_t D) {
   // (one count of splits + B segments, of one row a head each)
@@ -535,7 +535,7 @@ SplitWs decode_ws(int splits, int64_t B, int64_t Hq, int64_t D) {
 size_t omx_gdn_attn_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t page_size,
                                           int64_t table_width) {
   if (B < 1 || !sized(B, 1, Hq, Hkv, D, B) || !sized_table(page_size, table_width)) return 0;
-  return decode_ws(decode_splits(kAllKeys, B, Hkv, D, page_size * table_width), B, Hq, D).total;
+  return decode_ws(decode_splits(kAllKeys, B, Hkv, D, page_size * table_width, false), B, Hq, D).total;
 }
 
 namespace {
@@ -555,7 +555,7 @@ int attn_decode(const char* fn, const void* q, const void* k, const void* v, int
   if (B == 0) return ok();
   rc = check_cache(fn, k_pages, v_pages, n_pages, page_size, block_table, table_width, lengths, D, Hkv);
   if (rc) return rc;
-  const int splits = decode_splits(sight, B, Hkv, D, page_size * table_width);
+  const int splits = decode_splits(sight, B, Hkv, D, page_size * table_width, k_exps != nullptr);
   const SplitWs ws = decode_ws(splits, B, Hq, D);
   REQUIRE(workspace_bytes >= ws.total, "%s: workspace of %zu bytes is smaller than the %zu needed", fn,
           workspace_bytes, ws.total);
@@ -590,7 +590,8 @@ int omx_gdn_attn_decode_step(const void* q, const void* k, const void* v, int64_
 size_t omx_gdn_attn_decode_window_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t page_size,
                                                  int64_t table_width, int64_t window, int64_t sinks) {
   if (B < 1 || !sized(B, 1, Hq, Hkv, D, B) || !sized_table(page_size, table_width) || window < 0 || sinks < 0) return 0;
-  return decode_ws(decode_splits(Sight{window, sinks}, B, Hkv, D, page_size * table_width), B, Hq, D).total;
+  // (for either cache: one in 8 bits is shared later, never sooner)
+  return decode_ws(decode_splits(Sight{window, sinks}, B, Hkv, D, page_size * table_width, false), B, Hq, D).total;
 }
 
 int omx_gdn_attn_decode_window(const void* q, const void* k, const void* v, int64_t q_ld, int64_t k_ld, int64_t v_ld,

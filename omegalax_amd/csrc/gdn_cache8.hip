@@ -343,11 +343,12 @@ void attn_decode8_kernel(AttnParams p) {
     int st = st0 + w;
     Ids y = look(st), next;
     // whose stage holds the new token's block, of number `into`
-    const int st_new = (held < 0 || held >= cap ? 0 : held / SK) - seen.skip;  // (the window's part, or without a skip)
-    const int new_slot = held < 0 || held >= cap ? -1 : (int)(__umulhi((unsigned)held, p.page_mul) >> p.page_shift);
-    const int new_id = new_slot >= 0 && st_new >= st && st_new < st1 && (st_new - st) % NW == 0 ? table[new_slot] : -1;
+    const bool room = held >= 0 && held < cap;
+    const int at_new = room ? held : 0, st_new = at_new / SK - seen.skip;  // (in the window's part, or nothing is skipped)
+    const int new_slot = (int)(__umulhi((unsigned)at_new, p.page_mul) >> p.page_shift);
+    const int new_id = room && st_new >= st && st_new < st1 && (st_new - st) % NW == 0 ? table[new_slot] : -1;
     const bool ours = new_id >= 0 && new_id < p.n_pages;
-    const unsigned into = (unsigned)new_id * (unsigned)(p.page / 16) + (unsigned)((held - new_slot * p.page) / 16);
+    const unsigned into = (unsigned)new_id * (unsigned)(p.page / 16) + (unsigned)((at_new - new_slot * p.page) / 16);
     New nk{}, nv{};
     if (ours) {
       const unsigned to = l < DP / 8 ? 16u * (unsigned)l : kDropOffset;

@@ -333,7 +333,8 @@ hipError_t launch_attn_dkv(const AttnParams& p, hipStream_t stream);
 bool paged_dims_supported(int D);
 int kv_write_tokens();  // tokens a workgroup of the append copies
 hipError_t launch_kv_write(const AttnParams& p, hipStream_t stream);
-int decode_splits(long long N, long long Hkv, long long D, long long capacity);
+// (seen: keys of them that a token sees at most; eight: a cache in 8 bits)
+int decode_splits(long long N, long long Hkv, long long D, long long capacity, long long seen, bool eight);
 hipError_t launch_attn_decode(const AttnParams& p, hipStream_t stream);
 // the same of a cache in 8 bits
 int kv_write8_tokens();

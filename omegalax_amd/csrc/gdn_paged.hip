@@ -372,7 +372,7 @@ hipError_t launch_kv_write(const AttnParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-int decode_splits(long long N, long long Hkv, long long D, long long capacity) {
+int decode_splits(long long N, long long Hkv, long long D, long long capacity, long long seen, bool eight) {
   // One workgroup a sequence and key head where a sequence is so short that the join costs more than
   // it saves (B=1, 4 key heads of 128, calls one after the other: 611 keys 14.4 us in one launch, 18.5 in
   // two, 1,500 keys 21.8 and 18.0), and for more than 1,024 sequences, where each row's join sums up all
@@ -381,9 +381,23 @@ int decode_splits(long long N, long long Hkv, long long D, long long capacity) {
   // and 7,000 207 (230), 63 of 1,000 and one of 30,000 84 (380); 1,024 of 100 199 (196), with one of
   // 30,000 244 (532).  16/2 heads of 256, sequences of 75 to 525 keys: 512 98 (81), 1,024 182 (156),
   // 4,096 723 (579).
-  if (N > 1024 || capacity * D <= (1 << 17)) return 1;
+  // Of a cache in 8 bits, whose wavefronts pass twice the keys in a turn, twice the keys are short (1,200
+  // keys of 128: one sequence of 4 heads 14 us, shared 18, 64 of 2 heads 19 and 27; 4,800: 29 and 18, 56 and 44).
+  // With a window sequences are alike, and sharing only evens out the last round of workgroups, for some
+  // 11 us (the join, and a second sequence's start in most ranges): a key's bytes take a workgroup 19 ps each,
+  // or its part of 6.2 TB/s.  64 sequences of 8 heads of 128, two whole rounds, 1,024 keys: 63 us (70), in
+  // 8 bits 39 (49); 40 of 8, 3,000 keys: 115 us (102), 71 (66); one of 4, 2,048 keys: 28 us (17), 18 (17).
+  const int bytes = eight ? 1 : 2;
+  if (N > 1024) return 1;
+  if (seen < capacity) {
+    const long long groups = N * Hkv, rounds = (groups + kComputeUnits - 1) / kComputeUnits;
+    const double fill = (double)groups / (kComputeUnits * rounds), each = 2. * D * bytes * seen;
+    if (rounds * each * (fill < 0.46 ? 1.9e-5 : fill * 4.1e-5) * (1 - fill) < 11.) return 1;
+  } else if (capacity * D * bytes <= (1 << 18)) {
+    return 1;
+  }
   // stages are counted in 32 bits, and a range's end lies up to a range past the last
-  if (N * (capacity / 16 + 1) > INT_MAX / 2) return 1;
+  if (N * (seen / 16 + 1) > INT_MAX / 2) return 1;
   const long long s = kComputeUnits / Hkv;
   return (int)(s < 2 ? 1 : s);
 }
