@@ -96,16 +96,17 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   // the tile's keys: 0 .. last, in tiles of kBN, of which this split takes [kt0, kt1)
   const int keys = held + t0 + nt;
   int kt0 = 0, kt1 = (keys + kBN - 1) / kBN;
-  // With a window these tiles are counted without the `skip` ones between the sinks' and the first
-  // row's window, which no row sees: tile kt begins at key key0(kt).
-  int sink_tiles = 0, skip = 0, lo = 0;
+  // With a window these tiles are the sinks', and from the first row's window on, which starts one of
+  // its own (in a cache at a multiple of 16): `shift` keys between are left out.  Tile kt begins at key0(kt).
+  int sink_tiles = 0, shift = 0, lo = 0;
   if constexpr (WIN) {
     lo = held + t0 - p.window + 1;
     sink_tiles = (p.sinks + kBN - 1) / kBN;
-    skip = lo / kBN > sink_tiles ? lo / kBN - sink_tiles : 0;
-    kt1 -= skip;
+    const int from = PAGED ? lo & ~15 : lo;
+    shift = from > sink_tiles * kBN ? from - sink_tiles * kBN : 0;
+    kt1 = (keys - shift + kBN - 1) / kBN;
   }
-  auto key0 = [&](int kt) { return (WIN && kt >= sink_tiles ? kt + skip : kt) * kBN; };
+  auto key0 = [&](int kt) { return kt * kBN + (WIN && kt >= sink_tiles ? shift : 0); };
   if (PAGED && p.splits > 1) {
     const int each = (kt1 + p.splits - 1) / p.splits;
     kt0 = split * each < kt1 ? split * each : kt1;
@@ -140,7 +141,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   auto look = [&](int kt) {
     Pages x;
     x.have = 0;
-    if (WIN && kt == sink_tiles && skip > 0) {  // on from the sinks to the window
+    if (WIN && kt == sink_tiles && shift > 0) {  // on from the sinks to the window
       slot = key0(kt) / p.page;
       off = key0(kt) - slot * p.page;
     }
@@ -403,7 +404,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     }
     lds_barrier();
     // the wavefront's own last tile: rows of it see no keys of later ones
-    const int w_kt = w_hi / kBN - skip, last_kt = w_kt < kt1 - 1 ? w_kt : kt1 - 1;
+    const int w_kt = (w_hi - shift) / kBN, last_kt = w_kt < kt1 - 1 ? w_kt : kt1 - 1;
     int kt = kt0;
     if (kt <= last_kt) {
       f32x16 s0[2], s1[2];

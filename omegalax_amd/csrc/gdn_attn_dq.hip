@@ -47,15 +47,16 @@ void attn_dq_kernel(AttnParams p, int ranks) {
   const int pos = t0 + rt, w_lo = t0 + (32 * w) / G, w_hi = t0 + (32 * w + 31) / G;
 
   // fetches block kb's keys (and values) into its slot; blocks past the last have an empty range
-  // (with a window counted without the `skip` ones that no row sees: block kb begins at key0(kb))
-  int nb = (t0 + nt + kBN - 1) / kBN, sink_blocks = 0, skip = 0;
+  // (with a window these are the sinks' and from the first row's window on, `shift` keys later: block kb
+  // begins at key0(kb))
+  int nb = (t0 + nt + kBN - 1) / kBN, sink_blocks = 0, shift = 0;
   if constexpr (WIN) {
     const int lo = t0 - p.window + 1;
     sink_blocks = (p.sinks + kBN - 1) / kBN;
-    skip = lo / kBN > sink_blocks ? lo / kBN - sink_blocks : 0;
-    nb -= skip;
+    shift = lo > sink_blocks * kBN ? lo - sink_blocks * kBN : 0;
+    nb = (t0 + nt - shift + kBN - 1) / kBN;
   }
-  auto key0 = [&](int kb) { return (WIN && kb >= sink_blocks ? kb + skip : kb) * kBN; };
+  auto key0 = [&](int kb) { return kb * kBN + (WIN && kb >= sink_blocks ? shift : 0); };
   constexpr int kStep = 64 / (DP / 8) * kNW, NO = kStep % 16 ? 2 : 1;
   static_assert(NO * kStep % 16 == 0 && NO <= NJ, "rows whose swizzle repeats");
   const unsigned kld2 = (unsigned)(p.k_ld * 2), vld2 = (unsigned)(p.v_ld * 2);
@@ -184,7 +185,7 @@ void attn_dq_kernel(AttnParams p, int ranks) {
 #pragma unroll
   for (int t = 0; t < PF; ++t) f[t] = attn_frag<DP>(slot(0) + kVal, lane, 0, t);
   // the wavefront's own last block: rows of it see no keys of later ones
-  const int w_kb = w_hi / kBN - skip, last = w_kb < nb - 1 ? w_kb : nb - 1;
+  const int w_kb = (w_hi - shift) / kBN, last = w_kb < nb - 1 ? w_kb : nb - 1;
   int kb = 0;
   while (kb + 1 < last) {
     turn(Yes(), kb++, s0, s1);
