@@ -221,7 +221,7 @@ __global__ __launch_bounds__(kNT) void pages_release_one_kernel(PagesParams p) {
   typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
   __shared__ unsigned long long sWave[kNT / 64];
   __shared__ int sFrom[kLdsRows], sBehind[WIN ? kLdsRows : 1];
-  const int all = p.N * p.table_w, sinks = (p.sinks + p.page - 1) / p.page;
+  const int all = p.N * p.table_w, sinks = (int)(((unsigned)p.sinks + p.page - 1) / p.page);
   const int count = on_stack(p);
   for (int n = threadIdx.x; n < p.N; n += kNT) {
     const int keep = p.lengths[n];

@@ -112,6 +112,13 @@ def test_lengths_far_past_the_table():
     p.release([2 ** 31 - 1, 48, 7], window=2 ** 31 - 1)
 
 
+def test_sinks_past_every_position():
+    """More sinks than there are positions: nothing is behind the window, whatever the page's size."""
+    p = Pool([150000], 6, 4, 65536)
+    p.release([150000], window=10, sinks=2 ** 31 - 1)
+    p.release([150000], window=10, sinks=2)
+
+
 def test_more_tokens_than_the_others_sum():
     """Numbers whose sum passes 32 bits: the room decides."""
     p = Pool([0, 3, 9], 40, 10, 16)
