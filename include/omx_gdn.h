@@ -464,8 +464,9 @@ size_t omx_gdn_attn_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, in
  * within [-100, 120], and rounds each value to the nearest c.  A block that holds older tokens keeps its
  * exponent or raises it; then their numbers are divided by the power of two between and rounded again.
  * Values that are not finite become NaN and do not count for e; sizes above 1.875 2^127 are clamped to it.
- * What no token was written to may hold anything.  Other arguments as for omx_gdn_kv_write, and its
- * workspace size; less than 2^23 times 64 tokens of a key head.
+ * What no token was written to may hold anything.  Rows from cu_seqlens[N] on are left out (of other calls
+ * they are the last sequence's).  Other arguments as for omx_gdn_kv_write, and its workspace size; less than
+ * 2^23 times 64 tokens of a key head.
  */
 int omx_gdn_kv_write8(const void* k, const void* v, int64_t k_ld, int64_t v_ld,
                       const int32_t* cu_seqlens, int64_t N, void* k_pages, void* v_pages,
@@ -514,7 +515,9 @@ size_t omx_gdn_attn_decode_window_workspace_size(int64_t B, int64_t Hq, int64_t 
  * new_tokens[n] - 1 that name no page take one from the stack's top, in order of sequence and position;
  * entries that name one keep it.  lengths are not advanced.
  *   T            tokens that there is room for below; those past it, packed, get no place
- *   cu_seqlens   int32 [N + 1]: the packed new tokens' offsets, at most T
+ *   cu_seqlens   int32 [N + 1]: the packed new tokens' offsets, at most T.  Calls that are given more rows
+ *                than cu_seqlens[N] take the others for the last sequence's: where their results matter, a last
+ *                row of the table with a length below zero has them
  *   positions    int32 [T]: each packed token's position in its sequence; -1 from cu_seqlens[N] on
  *   slots        int64 [T]: page * page_size + row of each; -1 where there is no page, and from there on
  *   missing      int32 [1]: pages that the stack was short of; the last entries stay without one then

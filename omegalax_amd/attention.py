@@ -269,7 +269,7 @@ def kv_pages_write(k, v, k_pages, v_pages, block_table, lengths, *, cu_seqlens=N
     Token i of sequence n goes to position ``lengths[n] + i``; a position without a page is
     left out.  A page that is written to must stand once in all of ``block_table``.  With ``k_exps``
     and ``v_exps`` the cache is one in 8 bits, and a block's older tokens are rounded again when a new
-    one is larger than its exponent allows for.
+    one is larger than its exponent allows for; rows from ``cu_seqlens[N]`` on are then left out.
     """
     _no_grad_only("kv_pages_write", k, v, k_pages, v_pages)
     dev = _device(k, v)
@@ -364,7 +364,9 @@ def kv_pages_assign(block_table, lengths, new_tokens, free_pages, free_count, *,
     keep theirs.  ``tokens``: the most that there is room for, all sequences together.  Returns
     (cu_seqlens int32 [N + 1], positions int32 [tokens], slots int64 [tokens], missing int32 [1]): the packed
     tokens' offsets, their positions in their sequences, page * page_size + row of each (-1 past the last,
-    and where there is no page), and how many pages the stack was short of.
+    and where there is no page), and how many pages the stack was short of.  A batch padded to ``tokens`` rows
+    takes a last row of the table with a length of -1, as its rows behind the last token count as the last
+    sequence's.
     """
     dev, N, lengths = _pages(block_table, lengths, free_pages, free_count)
     _device(block_table, new_tokens)

@@ -78,7 +78,8 @@ __device__ __forceinline__ float exp_shift(int a, int b) { return a - b < -126 ?
 // Token i of sequence n goes to position held[n] + i, as in the cache of bf16.  A wavefront takes the
 // blocks that begin with one of its kSpan tokens (a block of a sequence's first new token among them),
 // whole and for one head's keys or values: a lane has 16 columns of every DP / 64-th group of rows.  The largest values
-// are found over the wavefront; the block's older tokens are written only if its exponent grows.
+// are found over the wavefront; the block's older tokens are written only if its exponent grows.  Rows from
+// the last offset on are no tokens: taken for the last sequence's they would raise the exponents of those it has.
 constexpr int kSpan = 16;
 
 template <int DP>
@@ -91,13 +92,17 @@ __global__ __launch_bounds__(256) void kv_write8_kernel(AttnParams p, int span) 
   uint8_t* pool = (uint8_t*)(value ? p.v_pages : p.k_pages);
   int8_t* exps = value ? p.v_exps : p.k_exps;
   const long long t0 = ((long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * span;
-  const long long t1 = t0 + span < p.tokens ? t0 + span : p.tokens;
   const bool lanes = p.cu && !p.plan;  // lane n holds sequence n's end
   int end = 0;
-  if (lanes) {
-    end = l + 1 < p.N ? p.cu[l + 1] : p.T;
+  long long t1 = t0 + span < p.tokens ? t0 + span : p.tokens;
+  if (p.cu) {
+    const int n = lanes ? l : p.N - 1;
+    end = n < p.N ? p.cu[n + 1] : 0;
     end = end < 0 ? 0 : (end > p.T ? p.T : end);
-    end = wave_scan_max(end);
+    if (lanes) end = wave_scan_max(end);
+    else end = end > p.cu_plan[n] ? end : p.cu_plan[n];
+    const int last = __builtin_amdgcn_readlane(end, 63);
+    t1 = last < t1 ? last : t1;
   }
   for (long long t = t0; t < t1;) {
     int seq;
@@ -114,7 +119,7 @@ __global__ __launch_bounds__(256) void kv_write8_kernel(AttnParams p, int span) 
       }
       seq = lo;
       start = p.cu_plan[lo];
-      stop = p.cu_plan[lo + 1];
+      stop = lo + 1 < p.N ? p.cu_plan[lo + 1] : end;
     } else {
       seq = (int)(t / p.T);
       start = (long long)seq * p.T;

@@ -61,6 +61,27 @@ def test_append_and_turn(held, new, page, Hq, Hkv, D):
     c.same()
 
 
+@pytest.mark.parametrize("N", [1, 3, 63, 64, 65, 100])
+@pytest.mark.parametrize("pads", [1, 70])
+def test_rows_behind_the_last_offset_are_left_out(N, pads):
+    """Large and infinite ones, which would raise the exponents of the last sequence's tokens."""
+    held, new = [5 * n % 37 for n in range(N)], [1 + n % 3 for n in range(N)]
+    c = Cache8(held, [80] * N, 16, 2, 64)
+    k, v = new_rows(c, new)
+    cu = torch.tensor(offsets(new), dtype=torch.int32, device="cuda")
+    more = torch.full((1, pads, 2, 64), 1e30, dtype=BF, device="cuda")
+    more[:, ::3] = INF
+    om.kv_pages_write(*(torch.cat([t, more], 1) for t in (k, v)), *c.args(), cu_seqlens=cu, **c.exps())
+    put_all(c, new, k, v)
+    c.same()
+    # offsets that are not in order count as their running maximum
+    bad = cu.clone()
+    bad[-1] = 0
+    om.kv_pages_write(*(torch.cat([t, more], 1) for t in (k, v)), *c.args(), cu_seqlens=bad, **c.exps())
+    put_all(c, new[:-1] + [0], k, v)
+    c.same()
+
+
 @pytest.mark.parametrize("held,T,page,Hkv,D", [([20, 0, 131], 50, 16, 2, 64), ([5, 16], 1, 32, 1, 256), ([0, 40, 9, 33], 17, 48, 3, 128)])
 def test_unpacked_rows(held, T, page, Hkv, D):
     B = len(held)

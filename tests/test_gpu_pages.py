@@ -219,6 +219,28 @@ def test_a_serving_loop_without_a_length_on_the_host(eight):
             assert int((table[0] >= 0).sum()) <= window // page + 3
 
 
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_padded_batch(eight):
+    """Room for more tokens than there are, whose rows a last row of the table takes: what the batch without them gives."""
+    Hq, Hkv, D, page, held, new, T = 4, 2, 64, 16, [20, 0, 45, -1], [7, 30, 1, 0], 60
+    pools = []
+    for tokens in (T, sum(new)):
+        p = Pool(held, 40, 6, page)
+        cache = [torch.zeros((40, page, Hkv, D), device="cuda").to(torch.float8_e4m3fn if eight else torch.bfloat16) for _ in range(2)]
+        exps = dict(zip(("k_exps", "v_exps"), torch.zeros((2, 40, 1, Hkv), dtype=torch.int8, device="cuda"))) if eight else {}
+        cu = p.assign(held, new, tokens)[0]
+        q, k, v = (draw(i, 1, T, h, D) for i, h in enumerate((Hq, Hkv, Hkv)))
+        k[:, sum(new):], v[:, sum(new):] = float("nan"), float("inf")
+        at = (*cache, p.t, ints(held))
+        om.kv_pages_write(k[:, :tokens], v[:, :tokens], *at, cu_seqlens=cu, **exps)
+        o = om.attention_prefill_paged(q[:, :tokens], *at, cu_seqlens=cu, window=30, sinks=2, **exps)
+        pools.append((cache, exps, o))
+    (a, ea, oa), (b, eb, ob) = pools
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+    assert all(torch.equal(ea[n], eb[n]) for n in ea)
+    assert torch.equal(oa[:, :sum(new)], ob) and not bool(oa[:, sum(new):].any())
+
+
 def test_refusals():
     p = Pool([40, 0], 20, 6, 16)
     l, n = ints([40, 0]), ints([1, 1])
