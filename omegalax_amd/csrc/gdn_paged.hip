@@ -208,7 +208,9 @@ void attn_decode_kernel(AttnParams p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = key0 + 16 * g + 4 * g4 + i;
-          if (!whole && (key >= keys || !((have >> g) & 1) || (WIN && key < seen.lo && key >= p.sinks))) s[g][i] = -INFINITY;
+          // (selects, not branches)
+          const bool no = (key >= keys) | !((have >> g) & 1) | (WIN & (key < seen.lo) & (key >= p.sinks));
+          s[g][i] = !whole & no ? -INFINITY : s[g][i];
           mx = fmaxf(mx, s[g][i]);
         }
       if (__any((mx - m[n]) * cs > 8.f)) {
