@@ -16,6 +16,16 @@
 // chip has places the longest one does: T=1,900 of 16/2 heads of 256, 238 tiles, 53 to 58 us, of which
 // the last tile's 30 tiles of keys take 47.  Sharing its keys between two workgroups cost as much
 // in partial sums and the join as it saved there (59 us and 12), at 1,000 tokens too (36 and 36).
+//
+// With a window a tile's keys are the sinks' tiles and those from its first row's window on, 18 of 64 for a
+// window of 1,024, however long the prompt: 12,000 tokens of 16/2 heads of 256 250 us (1.3 PFLOP/s in the
+// loop, a sixth of each workgroup's time before it), B=4 T=4,096 of
+// 32/8 heads of 128 310.  Which keys a row sees is one word of bits a tile (window_bits): compared key by
+// key, the rows' limits took 5,000 spilled registers.
+//
+// Of a cache in 8 bits a tile's codes come a tile ahead into registers, and go to LDS as bf16 beside the
+// products of the values: 700 new on 7,000 tokens each of 6 sequences of 32/8 heads of 128, with the append,
+// 1.04 of the time that the cache of bf16 takes (heads of 64 1.02, of 256 1.16).
 #include "gdn_attn.h"
 
 namespace omx {

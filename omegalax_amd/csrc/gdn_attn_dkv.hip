@@ -22,6 +22,9 @@ constexpr int kNW = 4, kNT = 64 * kNW;
 // behind all loads, two reads ahead (B=4 T=4,096 of 32/8 heads of 128: 1,690 us, now 1,150; the
 // MFMAs are busy for 56% of it, the clock falls to 1.9 GHz under them).  Stages lie in
 // a ring of six LDS buffers, filled from memory directly.
+// WIN: a tile's rows are those whose window reaches its keys; the first tiles' keys, which all rows see as
+// sinks, are summed in shares of their own (attn_dkv_window_plan).  Window 1,024 and 16 sinks at the same size:
+// 605 us, an eighth of it products of rows at both ends of the band that see none of a wavefront's keys.
 constexpr int kRows = 32;        // rows of a stage
 constexpr int kRing = 6;
 

@@ -19,7 +19,8 @@ struct No { static constexpr bool value = false; };
 // Bound by the MFMAs, three products a block: B=4 T=4,096 of 32/8 heads of 128 760 to 820 us (the
 // compiler's own order, tiles of 64 keys: 805 to 860); with few tiles by the longest and the loads
 // before it: 3,001 tokens in 5 sequences of 16/2 heads of 256 56 us (73).
-// WIN: as for the forward.
+// WIN: as for the forward, the blocks being the sinks' and those from the first row's window on; window 1,024
+// and 16 sinks at B=4 T=4,096 of 32/8 heads of 128 403 us.
 template <int DP, bool WIN>
 __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
 void attn_dq_kernel(AttnParams p, int ranks) {
