@@ -205,7 +205,17 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   // bf16, a half segment beside every other product of the values.
   constexpr int NR = DP / 64, kRows8 = 4096 / DP;  // rows of the workgroup's j-th load: kRows8 j ..
   struct Raw { u32x4 x[NR]; int e[NR]; };
-  const int row8 = tid / (DP / 16), seg8 = tid % (DP / 16);
+  // A lane's row of the first load and its segment.  Eight lanes' writes of a half of theirs fill the banks if
+  // four are of a row whose swizzle differs in its lowest bit, four further (with rows in order every write
+  // took twice its time).
+  int row8, seg8;
+  {
+    const int l = tid & 63, low = 4 * (l >> 2 & 1);
+    if constexpr (DP == 64) row8 = 16 * w + low + ((l >> 3 & 3) | (l >> 5) << 3);
+    else if constexpr (DP == 128) row8 = 8 * w + low + (l >> 4);
+    else row8 = 8 * (w >> 1) + 2 * (w & 1) + low + (l >> 5);
+    seg8 = (l & 3) + (DP == 64 ? 0 : 4 * (l >> 3 & (DP == 128 ? 1 : 3)));
+  }
   // (the wavefront's group of the j-th, by selects: an index into the pages would put them into memory)
   const unsigned zero8 = lane_zero();
   auto mine8 = [&](const Pages& x, int j) {

@@ -210,7 +210,7 @@ void attn_decode_kernel(AttnParams p) {
           const int key = key0 + 16 * g + 4 * g4 + i;
           // (selects, not branches)
           const bool no = (key >= keys) | !((have >> g) & 1) | (WIN & (key < seen.lo) & (key >= p.sinks));
-          s[g][i] = !whole & no ? -INFINITY : s[g][i];
+          s[g][i] = (!whole & no) ? -INFINITY : s[g][i];
           mx = fmaxf(mx, s[g][i]);
         }
       if (__any((mx - m[n]) * cs > 8.f)) {
