@@ -24,8 +24,9 @@
 // key, the rows' limits took 5,000 spilled registers.
 //
 // Of a cache in 8 bits a tile's codes come a tile ahead into registers, and go to LDS as bf16 beside the
-// products of the values: 700 new on 7,000 tokens each of 6 sequences of 32/8 heads of 128, with the append,
-// 1.04 of the time that the cache of bf16 takes (heads of 64 1.02, of 256 1.16).
+// products of the values.  Instructions bound it, 6 to 7 an MFMA at one or two wavefronts a SIMD: 700 new on
+// 7,000 tokens each of 6 sequences, 32/8 heads of 128 512 us (from a cache of bf16 500), 16/4 of 64 213
+// (212), 16/2 of 256 576 (503; 642 with a resource of its own for each exponent).
 #include "gdn_attn.h"
 
 namespace omx {
@@ -226,16 +227,19 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     const unsigned low = w & 1 ? b : a, high = w & 1 ? d : c;
     return w & 2 ? high : low;
   };
+  // (a block's offset in a pool is one product; exponents lie within 32 bits of their pool's first)
+  const unsigned blk_bytes = 16u * (unsigned)row_bytes, off8 = (unsigned)(row8 & 15) * (unsigned)row_bytes + 16u * (unsigned)seg8;
   auto load8 = [&](const Pages& x, const void* pool, const int8_t* exps) {
     Raw r;
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
       const bool there = (x.fetch >> (DP == 256 ? j : (DP == 128 ? 2 * j + w / 2 : w))) & 1;
-      const long long blk = (long long)mine8(x, j) * Hkv;
+      const unsigned blk = mine8(x, j);
       r.x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-          uniform_rsrc((const char*)pool + (blk * 16 + hk) * DP, there ? 15u * row_bytes + DP : 0u),
-          ((kRows8 * j + row8) & 15) * row_bytes + 16 * seg8, 0, 0));
-      r.e[j] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(uniform_rsrc(exps + blk + hk, there ? 1u : 0u), zero8, 0, 0);
+          uniform_rsrc((const char*)pool + hk * DP + (unsigned long long)blk * blk_bytes, there ? 15u * row_bytes + DP : 0u),
+          off8, 0, 0));
+      r.e[j] = (int8_t)__builtin_amdgcn_raw_buffer_load_b8(
+          uniform_rsrc(exps, kDropOffset), zero8 + (there ? blk * (unsigned)Hkv + (unsigned)hk : kDropOffset), 0, 0);
     }
     return r;
   };
