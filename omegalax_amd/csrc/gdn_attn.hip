@@ -25,8 +25,8 @@
 //
 // Of a cache in 8 bits a tile's codes come a tile ahead into registers, and go to LDS as bf16 beside the
 // products of the values.  Instructions bound it, 6 to 7 an MFMA at one or two wavefronts a SIMD: 700 new on
-// 7,000 tokens each of 6 sequences, 32/8 heads of 128 512 us (from a cache of bf16 500), 16/4 of 64 213
-// (212), 16/2 of 256 576 (503; 642 with a resource of its own for each exponent).
+// 7,000 tokens each of 6 sequences, 32/8 heads of 128 522 us (from a cache of bf16 516), 16/4 of 64 213
+// (212), 16/2 of 256 576 (515; 642 with a resource of its own for each exponent).
 #include "gdn_attn.h"
 
 namespace omx {
