@@ -139,38 +139,40 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     koff[n] = 8 * seg < D ? (unsigned)r * kld2 + 16u * (unsigned)seg : kDropOffset;
     voff[n] = 8 * seg < D ? (unsigned)r * vld2 + 16u * (unsigned)seg : kDropOffset;
   }
-  // The cache: page slot and offset of the next tile to look up, and a tile's pages, one for each
-  // of its four groups of 16 keys (a page is a multiple of 16 tokens), -1 where there is none.
-  // They are read a tile before they are used, through the scalar cache, whose wait does not touch
-  // the staging loads' counter.
+  // The cache: a tile's pages, one for each of its four groups of 16 keys (a page is a multiple of 16
+  // tokens).  Lane n asks for that of group n % 4, a tile before the answers are needed: with a scalar load for
+  // each group, each waited for, a turn took 3 (32/8 heads of 128) to 18% more (16/4 of 64).
   typedef const __attribute__((address_space(4))) int32_t const_i32;
   const_i32* table = PAGED ? (const_i32*)(p.table + (long long)it.seq * p.table_w) : nullptr;
-  int slot = 0, off = 0;
   const int row_bytes = EIGHT ? Hkv * D : Hkv * D * 2;
-  // (of bf16 the groups' byte offsets in a pool, of 8 bits the numbers of their blocks; none past the split)
-  struct Pages { long long at[EIGHT ? 1 : 4]; unsigned blk[EIGHT ? 4 : 1], have, fetch; };
-  auto look = [&](int kt) {
+  const unsigned blk_bytes = 16u * (unsigned)row_bytes;  // a group's, of a pool
+  struct Asked { int id, of; };                          // a page, and which of its blocks (-1: no key)
+  auto ask = [&](int kt) {
+    const int key = key0(kt) + 16 * (l & 3), slot = (int)(__umulhi((unsigned)key, p.page_mul) >> p.page_shift);
+    const bool in = (kt < kt1) & (key < keys) & (slot < p.table_w);
+    return Asked{(int)__builtin_amdgcn_raw_buffer_load_b32(uniform_rsrc((const void*)table, 4u * (unsigned)p.table_w),
+                                                           in ? 4u * (unsigned)slot : kDropOffset, 0, 0),
+                 in ? (key - slot * p.page) >> 4 : -1};
+  };
+  // Of each group whether there is a page, and of those that this wavefront stages the block's offset in a pool (of
+  // bf16) or its number (of 8 bits).
+  constexpr int NP = !PAGED ? 1 : (EIGHT ? DP / 64 : (DP == 64 ? 2 : 4));
+  struct Pages { long long at[EIGHT ? 1 : NP]; unsigned blk[EIGHT ? NP : 1], have; };
+  auto group = [&](int n) {  // of the wavefront's n-th
+    if constexpr (EIGHT) return DP == 256 ? n : (DP == 128 ? 2 * n + w / 2 : w);
+    return DP == 64 ? 2 * n + w / 2 : n;
+  };
+  auto told = [&](const Asked& y) {
     Pages x;
-    x.have = 0;
-    if (WIN && kt == sink_tiles && shift > 0) {  // on from the sinks to the window
-      slot = key0(kt) / p.page;
-      off = key0(kt) - slot * p.page;
-    }
+    const bool there = (y.of >= 0) & (y.id >= 0) & (y.id < p.n_pages);
+    const unsigned blk = there ? (unsigned)y.id * (unsigned)(p.page / 16) + (unsigned)y.of : 0u;
+    x.have = (unsigned)__ballot(there) & 15u;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const bool in = key0(kt) + 16 * g < keys && slot < p.table_w;
-      int id = in ? table[slot] : -1;
-      id = id >= p.n_pages ? -1 : id;
-      id = __builtin_amdgcn_readfirstlane(id);
-      if constexpr (EIGHT)
-        x.blk[g] = (unsigned)(id < 0 ? 0 : id) * (unsigned)(p.page / 16) + (unsigned)(off / 16);
-      else
-        x.at[g] = ((long long)(id < 0 ? 0 : id) * p.page + off) * row_bytes + 2 * hk * D;
-      x.have |= id >= 0 ? 1u << g : 0u;
-      off += 16;
-      if (off >= p.page) { off = 0; ++slot; }
+    for (int n = 0; n < NP; ++n) {
+      const unsigned b = (unsigned)__builtin_amdgcn_readlane((int)blk, group(n));
+      if constexpr (EIGHT) x.blk[n] = b;
+      else x.at[n] = (long long)((unsigned long long)b * blk_bytes) + 2 * hk * D;
     }
-    x.fetch = kt < kt1 ? x.have : 0u;
     return x;
   };
   // Fetches a share of a tile of keys (or values) into LDS: NL instructions from the j0-th on.  They
@@ -184,10 +186,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     if constexpr (PAGED) {
 #pragma unroll
       for (int j = j0; j < j0 + NL; ++j) {
-        const int g0 = kStep * j / 16;  // the group of the instruction's rows
-        const bool next = DP == 64 && w >= 2;
-        const long long at = next ? x.at[g0 + 1] : x.at[g0];
-        load_to_lds16(rsrc_words((const char*)pool + at, (x.fetch >> (next ? g0 + 1 : g0)) & 1 ? 16u * ld2 : 0),
+        const int n = DP == 64 ? j : kStep * j / 16;  // the wavefront's group of the instruction's rows
+        load_to_lds16(rsrc_words((const char*)pool + x.at[n], (x.have >> group(n)) & 1 ? 16u * ld2 : 0),
                       lds + 1024u * kNW * j, lane_off[j % NO]);
       }
     } else {
@@ -217,24 +217,15 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     else row8 = 8 * (w >> 1) + 2 * (w & 1) + low + (l >> 5);
     seg8 = (l & 3) + (DP == 64 ? 0 : 4 * (l >> 3 & (DP == 128 ? 1 : 3)));
   }
-  // (the wavefront's group of the j-th, by selects: an index into the pages would put them into memory)
   const unsigned zero8 = lane_zero();
-  auto mine8 = [&](const Pages& x, int j) {
-    const unsigned a = x.blk[0], b = x.blk[EIGHT ? 1 : 0], c = x.blk[EIGHT ? 2 : 0], d = x.blk[EIGHT ? 3 : 0];
-    if constexpr (DP == 256) return j == 0 ? a : (j == 1 ? b : (j == 2 ? c : d));
-    const unsigned even = w & 2 ? b : a, odd = w & 2 ? d : c;
-    if constexpr (DP == 128) return j == 0 ? even : odd;
-    const unsigned low = w & 1 ? b : a, high = w & 1 ? d : c;
-    return w & 2 ? high : low;
-  };
   // (a block's offset in a pool is one product; exponents lie within 32 bits of their pool's first)
-  const unsigned blk_bytes = 16u * (unsigned)row_bytes, off8 = (unsigned)(row8 & 15) * (unsigned)row_bytes + 16u * (unsigned)seg8;
+  const unsigned off8 = (unsigned)(row8 & 15) * (unsigned)row_bytes + 16u * (unsigned)seg8;
   auto load8 = [&](const Pages& x, const void* pool, const int8_t* exps) {
     Raw r;
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
-      const bool there = (x.fetch >> (DP == 256 ? j : (DP == 128 ? 2 * j + w / 2 : w))) & 1;
-      const unsigned blk = mine8(x, j);
+      const bool there = (x.have >> group(j)) & 1;
+      const unsigned blk = x.blk[j];
       r.x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
           uniform_rsrc((const char*)pool + hk * DP + (unsigned long long)blk * blk_bytes, there ? 15u * row_bytes + DP : 0u),
           off8, 0, 0));
@@ -263,6 +254,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   //   2: weighted values of this  | maximum of the next one's scores  | reads of v
   Pages pn, pk;  // of the tile whose values come next, and of the one after, whose keys do
   Pages pl;      // of the third, in 8 bits
+  Asked pa;      // and of the next but these
   u32x4 f[PF], pb[4];
   float mx = 0.f;
   auto kfrag = [&](const bf16_t* sk, AttnLane ln, int t) { return attn_frag<DP>(sk, ln, 32 * (t & 1), t / 2); };
@@ -391,9 +383,11 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       pn = pk;
       if constexpr (EIGHT) {
         pk = pl;
-        pl = look(kt + 4);
+        pl = told(pa);
+        pa = ask(kt + 5);
       } else {
-        pk = look(kt + 3);
+        pk = told(pa);
+        pa = ask(kt + 4);
       }
     }
   };
@@ -401,15 +395,16 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     Pages p0;
     p0.have = pn.have = pk.have = 15;
     if constexpr (PAGED) {
-      slot = key0(kt0) / p.page;
-      off = key0(kt0) - slot * p.page;
-      p0 = look(kt0);
-      pn = look(kt0 + 1);
-      pk = look(kt0 + 2);
+      const Asked a0 = ask(kt0), a1 = ask(kt0 + 1), a2 = ask(kt0 + 2);
+      pa = ask(kt0 + 3);
+      p0 = told(a0);
+      pn = told(a1);
+      pk = told(a2);
       have = p0.have;
     }
     if constexpr (EIGHT) {
-      pl = look(kt0 + 3);
+      pl = told(pa);
+      pa = ask(kt0 + 4);
       const Raw k0 = load8(p0, p.k_pages, p.k_exps), v0 = load8(p0, p.v_pages, p.v_exps);
       const Raw k1 = load8(pn, p.k_pages, p.k_exps);
       rv = load8(pn, p.v_pages, p.v_exps);

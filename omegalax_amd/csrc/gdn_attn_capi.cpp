@@ -479,6 +479,7 @@ int attn_paged(const char* fn, const void* q, int64_t q_ld, const int32_t* cu_se
   p.k_pages = const_cast<void*>(k_pages); p.v_pages = const_cast<void*>(v_pages);
   p.k_exps = const_cast<int8_t*>(k_exps); p.v_exps = const_cast<int8_t*>(v_exps);
   look_at(p, sight, table_width * page_size + T);
+  divide_by_page(p, page_size);
   p.table = block_table; p.held = lengths;
   p.table_w = (int)table_width; p.page = (int)page_size; p.n_pages = (int)n_pages;
   p.splits = ws.splits;
