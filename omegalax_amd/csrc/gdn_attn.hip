@@ -184,11 +184,16 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
                    const unsigned (&lane_off)[NO], const bf16_t* dst, int j0) {
     const unsigned lds = lds_address(dst + (kt & 1) * kTile) + 1024u * (unsigned)w;
     if constexpr (PAGED) {
+      // (of heads of 256 both instructions are of one group)
+      constexpr int NS = DP == 256 ? NL : 1;
 #pragma unroll
-      for (int j = j0; j < j0 + NL; ++j) {
+      for (int j = j0; j < j0 + NL; j += NS) {
         const int n = DP == 64 ? j : kStep * j / 16;  // the wavefront's group of the instruction's rows
-        load_to_lds16(rsrc_words((const char*)pool + x.at[n], (x.have >> group(n)) & 1 ? 16u * ld2 : 0),
-                      lds + 1024u * kNW * j, lane_off[j % NO]);
+        unsigned at[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) at[i] = lane_off[(j + i) % NO];
+        loads_to_lds16(rsrc_words((const char*)pool + x.at[n], (x.have >> group(n)) & 1 ? 16u * ld2 : 0),
+                       lds + 1024u * kNW * j, at);
       }
     } else {
       int left = it.len - key0(kt);  // rows past the sequence read as zeros
