@@ -107,17 +107,20 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   // the tile's keys: 0 .. last, in tiles of kBN, of which this split takes [kt0, kt1)
   const int keys = held + t0 + nt;
   int kt0 = 0, kt1 = (keys + kBN - 1) / kBN;
-  // With a window these tiles are the sinks', and from the first row's window on, which starts one of
-  // its own (in a cache at a multiple of 16): `shift` keys between are left out.  Tile kt begins at key0(kt).
-  int sink_tiles = 0, shift = 0, lo = 0;
+  // With a window the tiles are of a list: the sinks (in a cache whole groups of 16; more than a tile of a
+  // prompt's in whole tiles), then the keys from the first row's window on; `shift` keys between are left out.
+  // Tile `cut` holds the last of the sinks and the first of the window.
+  int sink_keys = 0, shift = 0, lo = 0, cut = -1;
   if constexpr (WIN) {
     lo = held + t0 - p.window + 1;
-    sink_tiles = (p.sinks + kBN - 1) / kBN;
+    sink_keys = PAGED ? (p.sinks + 15) & ~15 : (p.sinks <= kBN ? p.sinks : (p.sinks + kBN - 1) / kBN * kBN);
     const int from = PAGED ? lo & ~15 : lo;
-    shift = from > sink_tiles * kBN ? from - sink_tiles * kBN : 0;
+    shift = from > sink_keys ? from - sink_keys : 0;
+    if (shift > 0 && sink_keys % kBN != 0) cut = sink_keys / kBN;
     kt1 = (keys - shift + kBN - 1) / kBN;
   }
-  auto key0 = [&](int kt) { return kt * kBN + (WIN && kt >= sink_tiles ? shift : 0); };
+  auto place = [&](int x) { return x + (WIN && x >= sink_keys ? shift : 0); };  // the key at x
+  auto key0 = [&](int kt) { return place(kt * kBN); };
   if (PAGED && p.splits > 1) {
     const int each = (kt1 + p.splits - 1) / p.splits;
     kt0 = split * each < kt1 ? split * each : kt1;
@@ -148,7 +151,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   const unsigned blk_bytes = 16u * (unsigned)row_bytes;  // a group's, of a pool
   struct Asked { int id, of; };                          // a page, and which of its blocks (-1: no key)
   auto ask = [&](int kt) {
-    const int key = key0(kt) + 16 * (l & 3), slot = (int)(__umulhi((unsigned)key, p.page_mul) >> p.page_shift);
+    const int key = place(kt * kBN + 16 * (l & 3)), slot = (int)(__umulhi((unsigned)key, p.page_mul) >> p.page_shift);
     const bool in = (kt < kt1) & (key < keys) & (slot < p.table_w);
     return Asked{(int)__builtin_amdgcn_raw_buffer_load_b32(uniform_rsrc((const void*)table, 4u * (unsigned)p.table_w),
                                                            in ? 4u * (unsigned)slot : kDropOffset, 0, 0),
@@ -204,6 +207,20 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       loads_to_lds16(rsrc_words((const bf16_t*)rows + (it.start + key0(kt)) * ld + hk * D,
                                 kt < kt1 ? (unsigned)(left - 1) * ld2 + 2u * D : 0),
                      lds + 1024u * kNW * j0, at);
+    }
+  };
+  // the tile of a prompt that holds the sinks and the window's first: lanes with a row of each
+  auto fetch_cut = [&](const void* rows, long long ld, unsigned ld2, const unsigned (&lane_off)[NO], const bf16_t* dst) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int on = j / NO * NO * kStep, row = stage_row<DP, kNW>(w, j % NO) + on;
+      const unsigned lds = lds_address(dst) + 1024u * (unsigned)w + 1024u * kNW * (unsigned)j;
+      const bf16_t* at = (const bf16_t*)rows + it.start * ld + hk * D;
+      const int left = it.len - shift < kBN ? it.len - shift : kBN;
+      if (row < sink_keys)
+        load_to_lds16(rsrc_words(at, (unsigned)(sink_keys - 1) * ld2 + 2u * D), lds, lane_off[j % NO] + (unsigned)on * ld2);
+      else
+        load_to_lds16(rsrc_words(at + shift * ld, (unsigned)(left - 1) * ld2 + 2u * D), lds, lane_off[j % NO] + (unsigned)on * ld2);
     }
   };
   // Of a cache in 8 bits a thread loads NR segments of 16 numbers and their exponents into registers, two
@@ -277,6 +294,10 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     mx = -INFINITY;
     if constexpr (WIN) {
       unsigned long long see = window_bits(p, pos, key0(kt));
+      if (kt == cut) {
+        const unsigned long long sinks = keys_below(sink_keys - kt * kBN);
+        see = (sinks & keys_below(p.sinks - kt * kBN)) | (~sinks & window_bits(p, pos, kt * kBN + shift));
+      }
       if constexpr (PAGED)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
@@ -371,7 +392,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   auto clear = [&](int kt, bf16_t* sv, unsigned have) {
     for (int i = tid; i < kBN * DP / 8; i += kNT) {
       const int r = i / (DP / 8);
-      const int key = key0(kt) + r;
+      const int key = place(kt * kBN + r);
       if (key >= keys || !((have >> (r / 16)) & 1) || (WIN && key < lo && key >= p.sinks)) *(u32x4*)(sv + 8 * i) = u32x4{0, 0, 0, 0};
     }
   };
@@ -424,10 +445,17 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       store8_all(v0, sV + (kt0 & 1) * kTile);
       store8_all(k1, sK + ((kt0 + 1) & 1) * kTile);
     } else {
+      const bool both = WIN && !PAGED && cut == 0;
+      if (both) {
+        fetch_cut(p.k, p.k_ld, kld2, koff, sK);
+        fetch_cut(p.v, p.v_ld, vld2, voff, sV);
+      }
 #pragma unroll
       for (int j = 0; j < NF; ++j) {
-        fetch_k(kt0, p0, j);
-        fetch_v(kt0, p0, j);
+        if (!both) {
+          fetch_k(kt0, p0, j);
+          fetch_v(kt0, p0, j);
+        }
         fetch_k(kt0 + 1, pn, j);
       }
       wait_loads<0>();
@@ -500,7 +528,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       for (int e = 0; e < DP / 64; ++e) acc[e] = 0.f;
       static_assert(kBN == 64, "a key a lane");
       for (int kt = kt0; kt < kt1 && key0(kt) <= pos1; ++kt) {
-        const int key = key0(kt) + l;
+        const int key = place(kt * kBN + l);
         bool see = key <= pos1 && (!WIN || key > pos1 - p.window || key < p.sinks);
         long long at = (it.start + key) * p.k_ld + hk * D, av = (it.start + key) * p.v_ld + hk * D;
         if constexpr (PAGED) {
