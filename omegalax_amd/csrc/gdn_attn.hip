@@ -88,7 +88,7 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   const int w_hi = held + t0 + (32 * w + 31) / G;                 //   and last row's last key
 
   u32x4 q[KS];
-  {
+  auto load_q = [&]() __attribute__((always_inline)) {
     const bf16_t* qp = (const bf16_t*)p.q + tok * p.q_ld + (long long)(hk * G + rg) * D;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -96,7 +96,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       q[s] = u32x4{0, 0, 0, 0};
       if (live && d < D) q[s] = *(const u32x4*)(qp + d);
     }
-  }
+  };
+  if constexpr (!PAGED) load_q();
 
   f32x16 o[DB];
 #pragma unroll
@@ -143,7 +144,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     voff[n] = 8 * seg < D ? (unsigned)r * vld2 + 16u * (unsigned)seg : kDropOffset;
   }
   // The cache: a tile's pages, one for each of its four groups of 16 keys (a page is a multiple of 16
-  // tokens).  Lane n asks for that of group n % 4, a tile before the answers are needed: with a scalar load for
+  // tokens).  Lane n asks for that of group n % 4 of the n / 4-th tile, of four, a tile before the answers are
+  // needed (the first ones for three tiles at once): with a scalar load for
   // each group, each waited for, a turn took 3 (32/8 heads of 128) to 18% more (16/4 of 64).
   typedef const __attribute__((address_space(4))) int32_t const_i32;
   const_i32* table = PAGED ? (const_i32*)(p.table + (long long)it.seq * p.table_w) : nullptr;
@@ -151,8 +153,8 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
   const unsigned blk_bytes = 16u * (unsigned)row_bytes;  // a group's, of a pool
   struct Asked { int id, of; };                          // a page, and which of its blocks (-1: no key)
   auto ask = [&](int kt) {
-    const int key = place(kt * kBN + 16 * (l & 3)), slot = (int)(__umulhi((unsigned)key, p.page_mul) >> p.page_shift);
-    const bool in = (kt < kt1) & (key < keys) & (slot < p.table_w);
+    const int tile = kt + (l >> 2 & 3), key = place(tile * kBN + 16 * (l & 3)), slot = (int)(__umulhi((unsigned)key, p.page_mul) >> p.page_shift);
+    const bool in = (tile < kt1) & (key < keys) & (slot < p.table_w);
     return Asked{(int)__builtin_amdgcn_raw_buffer_load_b32(uniform_rsrc((const void*)table, 4u * (unsigned)p.table_w),
                                                            in ? 4u * (unsigned)slot : kDropOffset, 0, 0),
                  in ? (key - slot * p.page) >> 4 : -1};
@@ -165,14 +167,14 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     if constexpr (EIGHT) return DP == 256 ? n : (DP == 128 ? 2 * n + w / 2 : w);
     return DP == 64 ? 2 * n + w / 2 : n;
   };
-  auto told = [&](const Asked& y) {
+  auto told = [&](const Asked& y, int of_tile) {
     Pages x;
     const bool there = (y.of >= 0) & (y.id >= 0) & (y.id < p.n_pages);
     const unsigned blk = there ? (unsigned)y.id * (unsigned)(p.page / 16) + (unsigned)y.of : 0u;
-    x.have = (unsigned)__ballot(there) & 15u;
+    x.have = (unsigned)__ballot(there) >> 4 * of_tile & 15u;
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
-      const unsigned b = (unsigned)__builtin_amdgcn_readlane((int)blk, group(n));
+      const unsigned b = (unsigned)__builtin_amdgcn_readlane((int)blk, 4 * of_tile + group(n));
       if constexpr (EIGHT) x.blk[n] = b;
       else x.at[n] = (long long)((unsigned long long)b * blk_bytes) + 2 * hk * D;
     }
@@ -415,10 +417,10 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
       pn = pk;
       if constexpr (EIGHT) {
         pk = pl;
-        pl = told(pa);
+        pl = told(pa, 0);
         pa = ask(kt + 5);
       } else {
-        pk = told(pa);
+        pk = told(pa, 0);
         pa = ask(kt + 4);
       }
     }
@@ -427,16 +429,16 @@ void attn_fwd_kernel(AttnParams p, int ranks) {
     Pages p0;
     p0.have = pn.have = pk.have = 15;
     if constexpr (PAGED) {
-      const Asked a0 = ask(kt0), a1 = ask(kt0 + 1), a2 = ask(kt0 + 2);
-      pa = ask(kt0 + 3);
-      p0 = told(a0);
-      pn = told(a1);
-      pk = told(a2);
+      const Asked all = ask(kt0);
+      pa = ask(kt0 + (EIGHT ? 4 : 3));
+      load_q();  // (behind the pages, whose answers would wait for them)
+      p0 = told(all, 0);
+      pn = told(all, 1);
+      pk = told(all, 2);
+      if constexpr (EIGHT) pl = told(all, 3);
       have = p0.have;
     }
     if constexpr (EIGHT) {
-      pl = told(pa);
-      pa = ask(kt0 + 4);
       const Raw k0 = load8(p0, p.k_pages, p.k_exps), v0 = load8(p0, p.v_pages, p.v_exps);
       const Raw k1 = load8(pn, p.k_pages, p.k_exps);
       rv = load8(pn, p.v_pages, p.v_exps);
