@@ -248,11 +248,17 @@ def _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D, k_exps=None, 
     return block_table.contiguous(), lengths.contiguous(), shape[0], shape[1]
 
 
-def _variant(k_exps, v_exps, sight):
-    """(the entry points' suffix, its exponents' pointers, its window and sinks) of a call over a cache."""
+def _variant(call, k_exps, v_exps, sight):
+    """(the entry point, its workspace size's, its exponents' pointers, its window and sinks) of a call over a cache."""
     if k_exps is None and sight is None:
-        return "", (), ()
-    return "_window", (_ptr(k_exps), _ptr(v_exps)), sight or (0, 0)
+        return *_PLAIN[call], (), ()
+    return *_WINDOW[call], (_ptr(k_exps), _ptr(v_exps)), sight or (0, 0)
+
+
+_PLAIN = {"paged": ("omx_gdn_attn_paged", "omx_gdn_attn_paged_workspace_size"),
+          "decode": ("omx_gdn_attn_decode_step", "omx_gdn_attn_decode_workspace_size")}
+_WINDOW = {"paged": ("omx_gdn_attn_paged_window", "omx_gdn_attn_paged_window_workspace_size"),
+           "decode": ("omx_gdn_attn_decode_window", "omx_gdn_attn_decode_window_workspace_size")}
 
 
 def _no_grad_only(name, *ts):
@@ -305,13 +311,12 @@ def attention_prefill_paged(q, k_pages, v_pages, block_table, lengths, *, cu_seq
     Hkv = k_pages.shape[2] if k_pages.dim() == 4 else 0
     table, lengths, pages, page = _cache(dev, k_pages, v_pages, block_table, lengths, N, Hkv, D, k_exps, v_exps)
     o = torch.empty((B, T, Hq, D), dtype=torch.bfloat16, device=dev)
-    more, exps, sight = _variant(k_exps, v_exps, sight)
-    ws_bytes = _workspace_bytes(f"omx_gdn_attn_paged{more}_workspace_size", B, T, Hq, Hkv, D, N,
-                                int(cu_seqlens is not None), page, table.shape[1], *sight)
+    name, size, exps, sight = _variant("paged", k_exps, v_exps, sight)
+    ws_bytes = _workspace_bytes(size, B, T, Hq, Hkv, D, N, int(cu_seqlens is not None), page, table.shape[1], *sight)
     ws = _workspace(ws_bytes, dev)
-    _call(dev, "omx_gdn_attn_paged" + more, _ptr(q), q_ld, _ptr(cu_seqlens), N, _ptr(k_pages), _ptr(v_pages), *exps,
-          pages, page, _ptr(table), table.shape[1], _ptr(lengths), _ptr(o), B, T, Hq, Hkv, D, _scale(scale, D), *sight,
-          _ptr(ws), ws_bytes)
+    _call(dev, name, _ptr(q), q_ld, _ptr(cu_seqlens), N, _ptr(k_pages), _ptr(v_pages), *exps, pages, page,
+          _ptr(table), table.shape[1], _ptr(lengths), _ptr(o), B, T, Hq, Hkv, D, _scale(scale, D), *sight, _ptr(ws),
+          ws_bytes)
     return o
 
 
@@ -330,13 +335,12 @@ def attention_decode_step(q, k, v, k_pages, v_pages, block_table, lengths, *, sc
     Hkv = k.shape[1]
     table, lengths, pages, page = _cache(dev, k_pages, v_pages, block_table, lengths, B, Hkv, D, k_exps, v_exps)
     out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=dev)
-    more, exps, sight = _variant(k_exps, v_exps, sight)
-    ws_bytes = _workspace_bytes(f"omx_gdn_attn_decode{more}_workspace_size", B, Hq, Hkv, D, page, table.shape[1],
-                                *sight)
+    name, size, exps, sight = _variant("decode", k_exps, v_exps, sight)
+    ws_bytes = _workspace_bytes(size, B, Hq, Hkv, D, page, table.shape[1], *sight)
     ws = _workspace(ws_bytes, dev)
-    _call(dev, "omx_gdn_attn_decode" + (more or "_step"), _ptr(q), _ptr(k), _ptr(v), q_ld, k_ld, v_ld, _ptr(k_pages),
-          _ptr(v_pages), *exps, pages, page, _ptr(table), table.shape[1], _ptr(lengths), _ptr(out), B, Hq, Hkv, D,
-          _scale(scale, D), *sight, _ptr(ws), ws_bytes)
+    _call(dev, name, _ptr(q), _ptr(k), _ptr(v), q_ld, k_ld, v_ld, _ptr(k_pages), _ptr(v_pages), *exps, pages, page,
+          _ptr(table), table.shape[1], _ptr(lengths), _ptr(out), B, Hq, Hkv, D, _scale(scale, D), *sight, _ptr(ws),
+          ws_bytes)
     return out
 
 
