@@ -17,16 +17,14 @@
 // the last tile's 30 tiles of keys take 47.  Sharing its keys between two workgroups cost as much
 // in partial sums and the join as it saved there (59 us and 12), at 1,000 tokens too (36 and 36).
 //
-// With a window a tile's keys are the sinks' tiles and those from its first row's window on, 18 of 64 for a
-// window of 1,024, however long the prompt: 12,000 tokens of 16/2 heads of 256 250 us (1.3 PFLOP/s in the
-// loop, a sixth of each workgroup's time before it), B=4 T=4,096 of
-// 32/8 heads of 128 310.  Which keys a row sees is one word of bits a tile (window_bits): compared key by
-// key, the rows' limits took 5,000 spilled registers.
+// With a window a tile passes over the sinks and the keys from its first row's window on, 17 tiles of 64 for a
+// window of 1,024 and 4 sinks, however long the prompt: 12,000 tokens of 16/2 heads of 256 240 to 250 us (all
+// keys 1,090), B=4 T=4,096 of 32/8 heads of 128 290 to 310.  Which keys a row sees is one word of bits a tile
+// (window_bits): compared key by key, the rows' limits took 5,000 spilled registers.
 //
 // Of a cache in 8 bits a tile's codes come a tile ahead into registers, and go to LDS as bf16 beside the
-// products of the values.  Instructions bound it, 6 to 7 an MFMA at one or two wavefronts a SIMD: 700 new on
-// 7,000 tokens each of 6 sequences, 32/8 heads of 128 522 us (from a cache of bf16 516), 16/4 of 64 213
-// (212), 16/2 of 256 576 (515; 642 with a resource of its own for each exponent).
+// products of the values.  Instructions bound it, 11 to 12 an MFMA: 700 new on 7,000 tokens each of 6 sequences,
+// 32/8 heads of 128 498 us (from a cache of bf16 489), 16/4 of 64 183 (179), 16/2 of 256 533 (484).
 #include "gdn_attn.h"
 
 namespace omx {
