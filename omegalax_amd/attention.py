@@ -347,11 +347,12 @@ def attention_decode_step(q, k, v, k_pages, v_pages, block_table, lengths, *, sc
 def _pages(block_table, lengths, free_pages, free_count):
     """Checks of what deals pages; the table and the stack are changed where they lie."""
     dev = _device(block_table, lengths, free_pages, free_count)
-    N = lengths.shape[0] if lengths.dim() == 1 else -1
-    for name, t, ok, want in (
-            ("block_table", block_table, block_table.dim() == 2 and block_table.shape[0] == N, f"[{N}, width]"),
-            ("lengths", lengths, N >= 0, "[N]"), ("free_pages", free_pages, free_pages.dim() == 1, "[pages]"),
-            ("free_count", free_count, tuple(free_count.shape) == (1,), "[1]")):
+    rows, shape = lengths.shape, block_table.shape
+    N = rows[0] if len(rows) == 1 else -1
+    known = (("block_table", block_table, len(shape) == 2 and shape[0] == N, "[N, width]"),
+             ("lengths", lengths, N >= 0, "[N]"), ("free_pages", free_pages, len(free_pages.shape) == 1, "[pages]"),
+             ("free_count", free_count, free_count.shape == (1,), "[1]"))
+    for name, t, ok, want in known:
         if t.dtype is not torch.int32 or not ok:
             raise ValueError(f"{name} must be int32 {want} (got {t.dtype}, {tuple(t.shape)})")
         if t is not lengths and not t.is_contiguous():
@@ -380,10 +381,8 @@ def kv_pages_assign(block_table, lengths, new_tokens, free_pages, free_count, *,
     T = operator.index(tokens)
     if T < 0:
         raise ValueError(f"tokens must not be negative (got {T})")
-    cu = torch.empty(N + 1, dtype=torch.int32, device=dev)
-    positions = torch.empty(T, dtype=torch.int32, device=dev)
-    slots = torch.empty(T, dtype=torch.int64, device=dev)
-    missing = torch.empty(1, dtype=torch.int32, device=dev)
+    cu, positions, missing = lengths.new_empty(N + 1), lengths.new_empty(T), lengths.new_empty(1)
+    slots = lengths.new_empty(T, dtype=torch.int64)
     ws_bytes = _workspace_bytes("omx_gdn_pages_assign_workspace_size", N)
     ws = _workspace(ws_bytes, dev)
     _call(dev, "omx_gdn_pages_assign", _ptr(block_table), N, block_table.shape[1], _ptr(lengths), _ptr(new_tokens),

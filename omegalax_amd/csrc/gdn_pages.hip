@@ -5,8 +5,8 @@
 // all, the k-th goes to free[count + n - 1 - k], so that what is dealt and returned leaves the stack as it was.
 // Every place is a prefix sum, so the order of execution changes nothing.  Bound by latency: a few
 // dependent reads, and for many tokens the 12 bytes written for each.  One workgroup deals a whole batch, its
-// entries 16 a thread to one sum: 64 sequences of a token each 8.7 us, and 8.3 to return none; 512 prompts
-// of 300 on pages of 16 14.2, 4.4 for their tokens' slots and 11.8 to return them.  (With a sum for every turn's
+// entries 16 a thread to one sum: 64 sequences of a token each 8.1 us, and 8.3 to return none; 512 prompts
+// of 300 on pages of 16 14.0, 4.2 for their tokens' slots and 11.8 to return them.  (With a sum for every turn's
 // entry of a thread the calls took 37 and 50 us.)
 #include <climits>
 
@@ -63,10 +63,10 @@ __device__ __forceinline__ void map_token(const PagesParams& p, const S* cu, int
   long long slot = -1;
   if (t < used) {
     const int n = last_upto(cu, p.N, t);
-    const long long at = (long long)p.lengths[n] + (t - cu[n]), i = at / p.page;
+    const unsigned at = (unsigned)p.lengths[n] + (unsigned)(t - cu[n]), i = at / (unsigned)p.page;
     pos = at < INT_MAX ? (int)at : INT_MAX;
-    const int id = i < p.table_w ? p.table[(long long)n * p.table_w + i] : -1;
-    if (a_page(id, p.n_pages)) slot = (long long)id * p.page + (at - i * p.page);
+    const int id = i < (unsigned)p.table_w ? p.table[(long long)n * p.table_w + i] : -1;
+    if (a_page(id, p.n_pages)) slot = (long long)id * p.page + (at - i * (unsigned)p.page);
   }
   p.positions[t] = pos;
   p.slots[t] = slot;
@@ -129,11 +129,15 @@ __global__ __launch_bounds__(kNT) void pages_assign_kernel(PagesParams p, int ma
 #pragma unroll
     for (int j = 0; j < 4; ++j) {  // all reads before the sum
       const int f = f0 + 4 * (j * kNT + tid);
-      int n = f < all ? last_upto(first, p.N, f) : 0, upto = f < all ? first[n + 1] : 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         id[4 * j + i] = 0;
         at[4 * j + i] = nullptr;
+      }
+      if (f0 + 4 * j * kNT >= all) continue;  // uniform
+      int n = f < all ? last_upto(first, p.N, f) : 0, upto = f < all ? first[n + 1] : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         if (f + i >= all) continue;
         while (f + i >= upto) upto = first[++n + 1];  // (entries of a sequence that follows)
         const int slot = LDS ? sSlot[n] : p.lengths[n] / p.page;
@@ -148,6 +152,7 @@ __global__ __launch_bounds__(kNT) void pages_assign_kernel(PagesParams p, int ma
     const unsigned long long upto = block_scan<kNT>(mine, (unsigned long long*)sWave, total) - mine;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      if (f0 + 4 * j * kNT >= all) continue;
       int k = needed + field(upto, j);
 #pragma unroll
       for (int e = 4 * j; e < 4 * j + 4; ++e) {
@@ -276,6 +281,7 @@ __global__ __launch_bounds__(kNT) void pages_release_one_kernel(PagesParams p) {
   int done = 0;
 #pragma unroll
   for (int j = 0; j < kTurns; ++j) {
+    if (4 * j * kNT >= all) continue;
     give_back(p, 4 * (j * kNT + (int)threadIdx.x), id[j], mask[j], (long long)count + n - 1 - done - field(upto[j / 4], j % 4));
     done += field(total[j / 4], j % 4);
   }
