@@ -91,6 +91,18 @@ def test_rows_do_not_see_infinities_behind_their_window(Hq, Hkv, D, T, window, s
     assert bool(o[0, bad_at:past].isnan().all())
 
 
+@pytest.mark.parametrize("D", [64, 72, 128, 256])
+@pytest.mark.parametrize("sinks", [1, 31, 63, 64, 65, 100])
+def test_nothing_between_the_sinks_and_the_window_counts(D, sinks):
+    """Rows whose tile holds the sinks and the window's first keys, with no number between."""
+    T, first, window = 500, 300, 60
+    q, k, v = draw(1, 1, T, 6, D), draw(2, 1, T, 2, D), draw(3, 1, T, 2, D)
+    k[:, sinks:first - window + 1], v[:, sinks:first - window + 1] = NAN, float("inf")
+    o = om.attention_prefill(q, k, v, window=window, sinks=sinks)
+    val, tol = one_sequence(*(t[0].double() for t in (q[:, first:], k, v)), seen(T - first, T, first, window, sinks))
+    check("rows past them", o[0, first:], val["o"], tol["o"])
+
+
 def test_columns_of_one_projection():
     B, T, Hq, Hkv, D = 2, 190, 8, 2, 128
     qkv = draw(4, B, T, Hq + 2 * Hkv, D).requires_grad_(True)

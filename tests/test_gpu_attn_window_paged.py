@@ -74,6 +74,21 @@ def test_pages_behind_the_window_are_not_needed(D):
     assert torch.equal(want2, om.attention_prefill_paged(q[:, None], *c.args(), **sight))
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("sinks", [1, 15, 16, 17, 63, 64, 65, 100])
+def test_nothing_between_the_sinks_and_the_window_counts(D, sinks):
+    held, new, window = 500, 30, 60
+    c = Cache([held], [new], 32, 2, D)
+    bad = draw(5, 1, held - window + 1 - sinks, 2, D) * NAN
+    om.kv_pages_write(bad, bad, c.args()[0], c.args()[1], c.args()[2], torch.tensor([sinks], dtype=torch.int32, device="cuda"))
+    q, k, v = draw(7, 1, new, 6, D), draw(8, 1, new, 2, D), draw(9, 1, new, 2, D)
+    om.kv_pages_write(k, v, *c.args())
+    o = om.attention_prefill_paged(q, *c.args(), window=window, sinks=sinks)
+    val, tol = one_sequence(q[0].double(), torch.cat([c.keys[0], k[0]]).double(), torch.cat([c.values[0], v[0]]).double(),
+                            seen(new, held + new, held, window, sinks))
+    check("o", o[0], val["o"], tol["o"])
+
+
 def test_a_window_of_everything_is_no_window():
     c = Cache([300, 20], [5, 5], 16, 2, 128)
     q, k = draw(1, 2, 5, 8, 128), draw(2, 2, 5, 2, 128)
