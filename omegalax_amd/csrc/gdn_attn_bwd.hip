@@ -330,7 +330,7 @@ DkvPlan attn_dkv_plan(long long units, long long T, long long N, int G, long lon
 DkvPlan attn_dkv_window_plan(long long B, long long T, long long N, int Hkv, int G, int D, int window, int sinks) {
   DkvPlan plan{1, 1, 1};
   const long long seqs = N > 0 ? N : B;
-  if (N > 64 || T == 0 || seqs == 0) return plan;
+  if (N > 64 || B == 0 || T == 0) return plan;
   const long long longest = (T + kDkvKeys - 1) / kDkvKeys;
   long long nt = ((N > 0 ? T / N : T) + kDkvKeys - 1) / kDkvKeys;  // of sequences of equal length
   nt = nt < 1 ? 1 : nt;

@@ -68,3 +68,12 @@ def test_python_checks_before_the_library():
         om.attention_prefill(q, q, q, window=2.5)
     with pytest.raises(ValueError, match="GPU"):
         om.attention_prefill(q, q, q, window=5, sinks=1)
+
+
+@pytest.mark.parametrize("B,T,N", [(0, 100, 1), (0, 100, 64), (0, 100, 65), (0, 0, 3), (3, 0, 0), (1, 0, 2), (0, 100, 0), (0, 0, 0)])
+@pytest.mark.parametrize("window,sinks", [(10, 0), (10, 4), (1, 0)])
+def test_workspace_sizes_of_no_tokens(B, T, N, window, sinks):
+    """None of a batch's or a packed call's tokens: nothing to share, so what the attention without a window asks for."""
+    L = _lib.lib()
+    shape = [B, T, 8, 2, 64, N]
+    assert L.omx_gdn_attn_window_bwd_workspace_size(*shape, window, sinks) == L.omx_gdn_attn_bwd_workspace_size(*shape)
