@@ -85,7 +85,7 @@ __device__ __forceinline__ float exp_shift(int a, int b) { return a - b < -126 ?
 constexpr int kSpan = 16;
 
 template <int DP>
-__global__ __launch_bounds__(256) void kv_write8_kernel(AttnParams p, int span) {
+__global__ __launch_bounds__(256) void kv_write8_kernel(AttnParams p) {
   constexpr int NR = DP / 64, LR = DP / 16, RJ = 64 / LR;  // rows: NR loads of RJ, LR lanes each
   const int l = lane_id(), hk = (int)blockIdx.y >> 1, seg = l % LR;
   const bool value = blockIdx.y & 1;
@@ -93,10 +93,10 @@ __global__ __launch_bounds__(256) void kv_write8_kernel(AttnParams p, int span) 
   const long long src_ld = value ? p.v_ld : p.k_ld;
   uint8_t* pool = (uint8_t*)(value ? p.v_pages : p.k_pages);
   int8_t* exps = value ? p.v_exps : p.k_exps;
-  const long long t0 = ((long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * span;
+  const long long t0 = ((long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kSpan;
   const bool lanes = p.cu && !p.plan;  // lane n holds sequence n's end
   int end = 0;
-  long long t1 = t0 + span < p.tokens ? t0 + span : p.tokens;
+  long long t1 = t0 + kSpan < p.tokens ? t0 + kSpan : p.tokens;
   if (p.cu) {
     const int n = lanes ? l : p.N - 1;
     end = n < p.N ? p.cu[n + 1] : 0;
@@ -584,9 +584,9 @@ int kv_write8_tokens() { return 4 * kSpan; }
 
 hipError_t launch_kv_write8(const AttnParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)((p.tokens + 4 * kSpan - 1) / (4 * kSpan)), 2u * (unsigned)p.Hkv);
-  if (p.D == 64) kv_write8_kernel<64><<<grid, 256, 0, stream>>>(p, kSpan);
-  else if (p.D == 128) kv_write8_kernel<128><<<grid, 256, 0, stream>>>(p, kSpan);
-  else kv_write8_kernel<256><<<grid, 256, 0, stream>>>(p, kSpan);
+  if (p.D == 64) kv_write8_kernel<64><<<grid, 256, 0, stream>>>(p);
+  else if (p.D == 128) kv_write8_kernel<128><<<grid, 256, 0, stream>>>(p);
+  else kv_write8_kernel<256><<<grid, 256, 0, stream>>>(p);
   return hipGetLastError();
 }
 
