@@ -86,6 +86,20 @@ def test_dealt_and_returned(N, most_held, most_new, page, width, spare):
         p.release(held, **sight)
 
 
+@pytest.mark.parametrize("width", [1, 3])
+@pytest.mark.parametrize("N", [8191, 8192, 8193])
+def test_more_rows_than_one_workgroup_returns(N, width):
+    """Tables of few entries and many rows: the return's rows lie in LDS up to 8,192 of them."""
+    say(f"pages of {N} sequences, width {width}")
+    r = random.Random(N + width)
+    held = [r.choice([-1, 0, r.randrange(16 * width + 1)]) for _ in range(N)]
+    used = sum(-(-max(h, 0) // 16) for h in held)
+    for sight in (dict(), dict(window=9, sinks=3), dict(window=1)):
+        p = Pool(held, used + 40, width, 16, seed=N)
+        p.release([h if h < 0 else r.choice([h, 0, h // 2, -1]) for h in held], **sight)
+        p.release([0] * N, **sight)
+
+
 @pytest.mark.parametrize("count", [-4, 0, 3, 50, 1 << 30])
 def test_a_count_out_of_range_is_read_as_the_nearest(count):
     for what in ("assign", "release"):

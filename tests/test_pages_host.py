@@ -45,6 +45,15 @@ def test_workspaces():
         assert L.omx_gdn_pages_release_workspace_size(x, 10) == 0 and L.omx_gdn_pages_release_workspace_size(10, x) == 0
 
 
+def test_workspace_of_many_rows():
+    """One workgroup returns up to 8,192 rows, whatever their width: more take counts of 4,096 entries each."""
+    size = _lib.lib().omx_gdn_pages_release_workspace_size
+    for width in (0, 1, 2, 3, 4):
+        assert size(8191, width) == size(8192, width) == 0
+        entries = 8193 * width
+        assert size(8193, width) >= 4 * ((entries + 4095) // 4096 + 1)
+
+
 def test_an_empty_return_is_no_op():
     assert _run("omx_gdn_pages_release", RELEASE, dict(N=0, table=None, lengths=None))[0] == _lib.OK
     assert _run("omx_gdn_pages_release", RELEASE, dict(width=0, table=None))[0] == _lib.OK
