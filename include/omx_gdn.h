@@ -464,7 +464,9 @@ size_t omx_gdn_attn_decode_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, in
  * within [-100, 120], and rounds each value to the nearest c.  A block that holds older tokens keeps its
  * exponent or raises it; then their numbers are divided by the power of two between and rounded again.
  * Values that are not finite become NaN and do not count for e; sizes above 1.875 2^127 are clamped to it.
- * What no token was written to may hold anything.  Rows from cu_seqlens[N] on are left out (of other calls
+ * What no token was written to may hold anything.  A shorter length takes tokens back but not what they did to
+ * their block: its exponent stays, and its older numbers as they were rounded for it (a block that a later
+ * append begins anew forgets both).  Rows from cu_seqlens[N] on are left out (of other calls
  * they are the last sequence's).  Other arguments as for omx_gdn_kv_write, and its workspace size; less than
  * 2^23 times 64 tokens of a key head.
  */

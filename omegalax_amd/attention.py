@@ -275,7 +275,7 @@ def kv_pages_write(k, v, k_pages, v_pages, block_table, lengths, *, cu_seqlens=N
     Token i of sequence n goes to position ``lengths[n] + i``; a position without a page is
     left out.  A page that is written to must stand once in all of ``block_table``.  With ``k_exps``
     and ``v_exps`` the cache is one in 8 bits, and a block's older tokens are rounded again when a new
-    one is larger than its exponent allows for; rows from ``cu_seqlens[N]`` on are then left out.
+    one is larger than its exponent allows for, which shorter ``lengths`` do not undo; rows from ``cu_seqlens[N]`` on are then left out.
     """
     _no_grad_only("kv_pages_write", k, v, k_pages, v_pages)
     dev = _device(k, v)

@@ -386,6 +386,23 @@ def test_streams_at_once():
             assert all(torch.equal(a, b) for a, b in zip(w, r))
 
 
+@pytest.mark.parametrize("decode", [False, True])
+@pytest.mark.parametrize("kept", [16, 20])
+def test_a_draft_that_is_turned_down(decode, kept):
+    """Large tokens appended and taken back by a shorter length, then small ones in their place: the block that the
+    kept tokens end in stays as the draft left it, a block that begins anew forgets it."""
+    c = Cache8([kept], [20], 16, 2, 64)
+    for size, n in ((500.0, 3), (1.0, 2), (1e-3, 1)):
+        for i in range(n if decode else 1):
+            k, v = (c.rows(1 if decode else n, size).cuda() for _ in range(2))
+            if decode:
+                om.attention_decode_step(draw(i, 1, 4, 64), k, v, *c.args()[:3], c.lengths + i, **c.exps())
+            else:
+                om.kv_pages_write(k[None], v[None], *c.args(), **c.exps())
+            c.put(0, kept + i, k, v)
+        c.same()
+
+
 def test_refused_caches():
     c = Cache8([20], [5], 16, 2, 64)
     q, k = draw(1, 1, 5, 4, 64), draw(2, 1, 5, 2, 64)
