@@ -12,7 +12,7 @@
 //
 // Two wavefronts a SIMD for heads up to 128, one (two tiles of k and v fill the LDS) for 256.  The
 // MFMAs bound it where there are many tiles: B=4 T=4,096 of 32/8 heads of 128 525 to 547 us, 1,010 to
-// 1,050 TFLOP/s at about 1.9 GHz (a library product of 8,192 cubed reaches 1,254).  With fewer tiles than the
+// 1,050 TFLOP/s at about 1.9 GHz (a library product of 8,192 cubed reaches 1,204 to 1,254).  With fewer tiles than the
 // chip has places the longest one does: T=1,900 of 16/2 heads of 256, 238 tiles, 53 to 58 us, of which
 // the last tile's 30 tiles of keys take 47.  Sharing its keys between two workgroups cost as much
 // in partial sums and the join as it saved there (59 us and 12), at 1,000 tokens too (36 and 36).

@@ -326,7 +326,10 @@ DkvPlan attn_dkv_plan(long long units, long long T, long long N, int G, long lon
 // The same with a window, where a tile is seen by the rows of `reach` tiles at most, and one with sinks by
 // all behind it, and partial sums cost twice as much beside the fewer rows.  Of 1 to 16 shares that takes the
 // best within 2% in each of 12 layouts, lengths and windows (4,000 tokens of 16/2 heads of 256, window 1,000, both
-// passes: whole tiles 609 us, 332 in three shares, 370 in more).  The sums take 768 MiB at most.
+// passes: whole tiles 609 us, 332 in three shares, 370 in more).  The sums take 768 MiB at most.  More than 64
+// sequences have whole tiles, as without a window, and one with sinks then takes as long as its sequence: 20,000 tokens
+// and 63 documents of 16, 16/4 heads of 128, window 1,024, 4 sinks 730 us, with 64 documents 3,020 (without sinks
+// 690 and 730).
 DkvPlan attn_dkv_window_plan(long long B, long long T, long long N, int Hkv, int G, int D, int window, int sinks) {
   DkvPlan plan{1, 1, 1};
   const long long seqs = N > 0 ? N : B;

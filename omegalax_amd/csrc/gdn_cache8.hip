@@ -196,7 +196,9 @@ __global__ __launch_bounds__(256) void kv_write8_kernel(AttnParams p) {
 // ------------------------------------------------------------------------------------ decode
 // As for the cache of bf16 (gdn_paged.hip): equal ranges of all sequences' stages, a wavefront's stages in
 // turns, read once for all query heads of a key head.  A stage's numbers go from memory to LDS as they
-// are, two stages deep (128 KiB in flight a compute unit), and become bf16 on the way from there into a
+// are, into a wavefront's one slot, whose keys and values are refilled by turns: the next stage's keys once
+// this one's scores are formed, its values once these are added up (128 KiB a compute unit with eight
+// wavefronts, 64 with the four of more than 16 query heads a key head).  They become bf16 on the way from there into a
 // product, each once: keys by rows of 8, values by transposed reads of 8 keys, the 8 that a lane's weights
 // of two blocks stand for.  The wavefront whose stage holds the new token's block puts the token into it,
 // there and in the cache; it rounds it while its first stage is on its way (after it: 69 us where now 64).
@@ -425,7 +427,8 @@ void attn_decode8_kernel(AttnParams p) {
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
         if (!whole) {
-          // (as selects: of conditions that are evaluated in turn the compiler made branches, and lost one)
+          // (selects of whole conditions: of the three joined by || the compiler makes a branch of the last, and
+          // loses one element's write on it, which its assembly shows as an exec mask set and reset around nothing)
 #pragma unroll
           for (int g = 0; g < NG; ++g)
 #pragma unroll

@@ -208,7 +208,7 @@ void attn_decode_kernel(AttnParams p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = key0 + 16 * g + 4 * g4 + i;
-          // (selects, not branches)
+          // (selects: of the three joined by || the compiler may make branches, and lost a write so in gdn_cache8.hip)
           const bool no = (key >= keys) | !((have >> g) & 1) | (WIN & (key < seen.lo) & (key >= p.sinks));
           s[g][i] = (!whole & no) ? -INFINITY : s[g][i];
           mx = fmaxf(mx, s[g][i]);
@@ -385,10 +385,13 @@ int decode_splits(long long N, long long Hkv, long long D, long long capacity, l
   // 4,096 723 (579).
   // Of a cache in 8 bits, whose wavefronts pass twice the keys in a turn, twice the keys are short (1,200
   // keys of 128: one sequence of 4 heads 14 us, shared 18, 64 of 2 heads 19 and 27; 4,800: 29 and 18, 56 and 44).
-  // With a window sequences are alike, and sharing only evens out the last round of workgroups, for some
-  // 11 us (the join, and a second sequence's start in most ranges): a key's bytes take a workgroup 19 ps each,
-  // or its part of 6.2 TB/s.  64 sequences of 8 heads of 128, two whole rounds, 1,024 keys: 63 us (70), in
-  // 8 bits 39 (49); 40 of 8, 3,000 keys: 115 us (102), 71 (66); one of 4, 2,048 keys: 28 us (17), 18 (17).
+  // With a window sequences are taken for alike, as all that pass it are (lengths are not known here), and
+  // sharing only evens out the last round of workgroups, for some 11 us (the join, and a second sequence's start
+  // in most ranges): a key's bytes take a workgroup 19 ps each, or its part of 6.2 TB/s.  64 sequences of 8 heads
+  // of 128, two whole rounds, 1,024 keys: 63 us (70), in 8 bits 39 (49); 40 of 8, 3,000 keys: 115 us (102), 71
+  // (66); one of 4, 2,048 keys: 28 us (17), 18 (17).
+  // Where few sequences pass a long window theirs are the last workgroups: 63 of 1,000 to 1,400 tokens and one of
+  // 30,000, 32/8 heads of 128, window 1,024 62 us, 8,000 148, 20,000 293, and 94 without a window.
   const int bytes = eight ? 1 : 2;
   if (N > 1024) return 1;
   if (seen < capacity) {
